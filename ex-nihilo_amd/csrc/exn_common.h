@@ -283,6 +283,59 @@ hipError_t attend(hipStream_t s, const uint16_t* q, const uint16_t* k, const uin
                   int n, int q0, int p, int l, int64_t lcap, int b0, int b1, float scale, int of32 = 0,
                   int64_t qld = 0);
 
+// the prompt side's attention (packed.hip, kv8.hip).  A plan of packed sequences is lists of tiles:
+// tokens t0 .. t0 + tt - 1 (as far as len) of sequence seq, whose rows begin at row0 and are len
+#define SEQ_TT0 8   // tokens a tile of the first list; list i has SEQ_TT0 << i
+#define SEQ_TTS 5
+struct SeqTile {
+  int32_t row0, len, t0, seq;
+};
+hipError_t attend_packed(hipStream_t s, const SeqTile* const* tiles, const int64_t* ntiles, int bf16, int heads,
+                         int kv_heads, int head_dim, const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk,
+                         const uint16_t* v, int64_t ldv, float scale, uint16_t* out, int obf, int64_t ldo);
+// exn_kv8's arrays as the kernels take them
+struct Kv8 {
+  int bf16, kv_heads, head_dim, cols;
+  int64_t pages;
+  int8_t *k, *v;          // [page][kv head][64][dim], [page][kv head][dim][64]
+  float* scales;          // [page][kv head][2]
+  uint16_t *tk, *tv;      // [sequence][kv head][64][dim]
+  const int32_t* table;   // [sequence][cols]
+  int32_t* lens;          // tokens before the step
+};
+// a sequence's tokens before the step, and with its N new ones, as far as its table reaches
+__host__ __device__ inline int kv8_base(const Kv8& c, int seq) {
+  const int n = c.lens[seq], cap = c.cols * 64;
+  return n < 0 ? 0 : n > cap ? cap : n;
+}
+__host__ __device__ inline int kv8_total(const Kv8& c, int base, int n) {
+  const int cap = c.cols * 64;
+  return base + n > cap ? cap : base + n;
+}
+// the page of a sequence's block (below cols), or -1 where the table names none
+__host__ __device__ inline int64_t kv8_page(const Kv8& c, int seq, int block) {
+  const int64_t p = c.table[(int64_t)seq * c.cols + block];
+  return p >= 0 && p < c.pages ? p : -1;
+}
+// the scale of a block whose largest |x| has the bits TOP
+__host__ __device__ inline float kv8_scale(uint32_t top) {
+  if (top >= 0x7F800000u) top = 0x7FC00000u;
+  uint32_t d = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, top) / 127.f);
+  if (top < 0x7F800000u) d = (d + 0xFFFu) & ~0xFFFu;
+  return __builtin_bit_cast(float, d);
+}
+__host__ __device__ inline int8_t kv8_code(float x, float d) { return d > 0.f ? (int8_t)__builtin_rintf(x / d) : (int8_t)0; }
+hipError_t kv8_append(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, int longest, const uint16_t* k,
+                      int64_t ldk, const uint16_t* v, int64_t ldv);
+hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* tiles, int64_t n, int tt, uint16_t* k, int64_t ldk,
+                    uint16_t* v, int64_t ldv);
+hipError_t kv8_advance(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n);
+// floats of scratch with which kv8_attend splits the keys as far as it pays
+int64_t kv8_attend_part(int64_t rows, int seqs, int longest, int heads, int kv_heads, int head_dim, int cols);
+hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles, int64_t rows,
+                      int seqs, int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out,
+                      int obf, int64_t ldo, float* part, int64_t part_cap);
+
 // the VAE decoder (vae.hip).  vae_conv's outputs: fp32 (+ bias, + res when given), bf16 (+ bias,
 // + res when given), fp32 (+ bias) clamped to -1 .. 1, fp32 (+ bias, + DupUp3D of keep: kcin
 // channels at half size, frame ft - 1 of ft); taps 9 or 1; up 1: the input is the half-size

@@ -82,6 +82,16 @@ SIGNATURES = {
     "exn_qkv_prep": (c_int, [vp, vp, c_int64, vp, vp, vp, vp, vp, vp, c_int64, c_int64]),
     "exn_mm_qkv": (c_int, [vp, vp, vp, c_int64, vp, vp, vp, vp, vp, vp, c_int64, c_int64]),
     "exn_attend": (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, c_float]),
+    "exn_seqs_create": (c_int, [vp, vp, c_int, POINTER(vp)]),
+    "exn_seqs_info": (c_int, [vp, POINTER(c_int), POINTER(c_int64), POINTER(c_int)]),
+    "exn_seqs_free": (c_int, [vp]),
+    "exn_attend_packed": (c_int, [vp, vp, c_int, c_int, c_int, c_int, vp, c_int64, vp, c_int64, vp, c_int64, c_float, vp,
+                                  c_int, c_int64]),
+    "exn_kv8_append": (c_int, [vp, vp, vp, vp, c_int64, vp, c_int64]),
+    "exn_kv8_attend": (c_int, [vp, vp, vp, c_int, vp, c_int64, c_float, vp, c_int, c_int64, vp, c_int64]),
+    "exn_kv8_attend_part": (c_int, [vp, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
+    "exn_kv8_read": (c_int, [vp, vp, vp, vp, c_int64, vp, c_int64]),
+    "exn_kv8_advance": (c_int, [vp, vp, vp]),
     "exn_euler": (c_int, [vp, c_int64, vp, vp, c_float]),
     "exn_dit_create": (c_int, [vp, c_int, POINTER(vp)]),
     "exn_dit_set": (c_int, [vp, c_char_p, c_int, vp, c_int64, c_int64]),
@@ -312,6 +322,76 @@ class Weight:
             self.free()
         except Exception:
             pass
+
+
+# --- the prompt side's attention: packed prompts, the cache in 8 bits -----------------------
+
+class Seqs:
+    """A plan of packed sequences (exn_seqs_create): LENS tokens each, one after the other."""
+
+    def __init__(self, ctx: Context, lens):
+        a = np.ascontiguousarray(lens, dtype=np.int32).reshape(-1)
+        h = vp()
+        call("exn_seqs_create", ctx.h, ptr(a), len(a), ctypes.byref(h))
+        self.ctx, self.h = ctx, h
+        self.seqs, self.rows, self.longest = len(a), int(a.sum(dtype=np.int64)), int(a.max())
+
+    def free(self):
+        if getattr(self, "h", None):
+            call("exn_seqs_free", self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Kv8(ctypes.Structure):
+    """Keys and values of SEQS sequences in 8 bits (exn_kv8), in the caller's device arrays, given
+    as addresses: codes K, V, SCALES, the 16-bit tails TK, TV, the pages' TABLE and the LENS."""
+
+    _fields_ = [("dt", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("seqs", c_int), ("cols", c_int),
+                ("pages", c_int64), ("k", vp), ("v", vp), ("scales", vp), ("tk", vp), ("tv", vp), ("table", vp),
+                ("lens", vp)]
+
+    def __init__(self, dt, kv_heads, head_dim, pages, seqs, cols, k, v, scales, tk, tv, table, lens):
+        super().__init__(dt, kv_heads, head_dim, seqs, cols, pages, k, v, scales, tk, tv, table, lens)
+        self.ref = ctypes.addressof(self)
+
+
+def attend_packed(ctx: Context, seqs: Seqs, dt, heads, kv_heads, head_dim, q, ldq, k, ldk, v, ldv, scale, out, odt,
+                  ldo):
+    """Causal attention of each of SEQS over itself (exn_attend_packed), on device addresses."""
+    call("exn_attend_packed", ctx.h, seqs.h, dt, heads, kv_heads, head_dim, q, ldq, k, ldk, v, ldv, scale, out, odt, ldo)
+
+
+def kv8_append(ctx: Context, cache: Kv8, seqs: Seqs, k, ldk, v, ldv):
+    """A step's rows of keys and values into the cache (exn_kv8_append), on device addresses."""
+    call("exn_kv8_append", ctx.h, cache.ref, seqs.h, k, ldk, v, ldv)
+
+
+def kv8_attend_part(seqs: Seqs, heads, kv_heads, head_dim, cols) -> int:
+    """The floats of scratch that kv8_attend has a use for (exn_kv8_attend_part)."""
+    n = c_int64()
+    call("exn_kv8_attend_part", seqs.h, heads, kv_heads, head_dim, cols, ctypes.byref(n))
+    return n.value
+
+
+def kv8_attend(ctx: Context, cache: Kv8, seqs: Seqs, heads, q, ldq, scale, out, odt, ldo, part=None, part_cap=0):
+    """A step's rows over the cache that they were appended to (exn_kv8_attend), on device addresses."""
+    call("exn_kv8_attend", ctx.h, cache.ref, seqs.h, heads, q, ldq, scale, out, odt, ldo, part, part_cap)
+
+
+def kv8_read(ctx: Context, cache: Kv8, seqs: Seqs, k, ldk, v, ldv):
+    """A step's rows as the cache holds them (exn_kv8_read), into device arrays of its type."""
+    call("exn_kv8_read", ctx.h, cache.ref, seqs.h, k, ldk, v, ldv)
+
+
+def kv8_advance(ctx: Context, cache: Kv8, seqs: Seqs):
+    """The step's tokens counted into the cache's lengths (exn_kv8_advance)."""
+    call("exn_kv8_advance", ctx.h, cache.ref, seqs.h)
 
 
 # --- the backend trio (src/cuda-dit.lisp) -------------------------------------------------

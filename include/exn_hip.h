@@ -174,6 +174,62 @@ int exn_attend(exn_ctx* ctx, const uint16_t* q, const uint16_t* k, const uint16_
 /* the Euler update of generate's loop (src/generate.lisp:133-135): Z += DS * V */
 int exn_euler(exn_ctx* ctx, int64_t count, float* z, const float* v, float ds);
 
+/* --- the prompt side's attention: packed prompts, and a cache of keys and values in 8 bits (no
+ * reference counterpart: illatio runs one prompt at a time, src/encoder.lisp:143-183) ------------ */
+
+/* SEQS sequences of LENS tokens (host memory; 0 is allowed), packed one after the other in rows 0 ..
+ * sum - 1: the plan that the calls below take.  At most 2^16 sequences and 2^22 rows.  Made outside
+ * stream capture; freed when no work that reads it is left (exn_seqs_free waits for the device). */
+typedef struct exn_seqs exn_seqs;
+int exn_seqs_create(exn_ctx* ctx, const int32_t* lens, int seqs, exn_seqs** out);
+int exn_seqs_info(const exn_seqs* s, int* seqs, int64_t* rows, int* longest);
+int exn_seqs_free(exn_seqs* s);
+/* Causal attention of each sequence over itself: row i, head h of Q (rows LDQ values apart, HEADS
+ * heads of HEAD_DIM, 64 or 128) sees rows 0 .. i of its sequence in K and V (KV_HEADS heads, a
+ * divisor of HEADS; head h reads h / (HEADS / KV_HEADS)), softmax of SCALE q.k in fp32.  Q, K and V
+ * are EXN_DT_F16 or EXN_DT_BF16 (DT; the softmax's weights are rounded to that type for the second
+ * product, sums are fp32), OUT either (ODT).  All four 16-byte aligned, strides multiples of 8:
+ * they may be parts of one row (q | k | v).  OUT overlaps none of them. */
+int exn_attend_packed(exn_ctx* ctx, const exn_seqs* s, int dt, int heads, int kv_heads, int head_dim, const void* q,
+                      int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, float scale, void* out,
+                      int odt, int64_t ldo);
+
+/* Keys and values of SEQS sequences in 8 bits, in the caller's device arrays.  A page is a block of
+ * 64 tokens: int8 codes of keys K [page][kv head][64][dim] and values V [page][kv head][dim][64],
+ * and SCALES [page][kv head][2] (key, value): a block's largest |x| / 127 in fp32, rounded up to 12
+ * significant bits, the codes x / scale rounded to nearest even (a block with an infinity or a NaN
+ * has the scale NaN).  TABLE [sequence][COLS] names the page of each full block; an entry outside 0
+ * .. PAGES - 1 hides its keys.  A block that is not full is kept in 16 bits (DT) in its sequence's
+ * tail TK, TV [sequence][kv head][64][dim] until its last token, so that nothing is rounded twice.
+ * Sequences may share pages of full blocks (a common prefix, with a copy of its tail).  LENS
+ * [sequence]: the tokens before the step; a step's new tokens are a plan's rows.  Tokens past 64
+ * COLS are not kept. */
+typedef struct exn_kv8 {
+  int dt, kv_heads, head_dim, seqs, cols;
+  int64_t pages;
+  int8_t *k, *v;
+  float* scales;
+  void *tk, *tv;
+  const int32_t* table;
+  int32_t* lens;
+} exn_kv8;
+/* the plan's rows of K and V (DT, LDK and LDV values apart) after each sequence's LENS tokens */
+int exn_kv8_append(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const void* k, int64_t ldk, const void* v,
+                   int64_t ldv);
+/* attention of the plan's rows, after exn_kv8_append of the same rows: row i of a sequence sees its
+ * cache's tokens 0 .. LENS + i, as exn_kv8_read reads them (zeros where all are hidden).  HEADS, Q,
+ * SCALE, OUT as exn_attend_packed.  PART (PART_CAP floats, 16-byte aligned, or null and 0): scratch
+ * with which few rows' keys are split over the chip and joined in order; calls that may overlap take
+ * one each.  exn_kv8_attend_part (needs no GPU): how many floats are of use. */
+int exn_kv8_attend(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, int heads, const void* q, int64_t ldq,
+                   float scale, void* out, int odt, int64_t ldo, float* part, int64_t part_cap);
+int exn_kv8_attend_part(const exn_seqs* s, int heads, int kv_heads, int head_dim, int cols, int64_t* floats);
+/* the plan's rows as the cache holds them after exn_kv8_append, into K and V (DT; code x scale,
+ * rounded once; zeros where nothing is kept) */
+int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int64_t ldk, void* v, int64_t ldv);
+/* LENS += the plan's lengths, on the device: the step's last call */
+int exn_kv8_advance(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s);
+
 /* --- the model: the backend trio ----------------------------------------------------------------- */
 
 /* an empty DiT of LAYERS blocks (32 in the real model; fewer to look at part of a step, as
