@@ -213,7 +213,7 @@ int exn_kv8_attend_part(const exn_seqs* s, int heads, int kv_heads, int head_dim
   if (!s || !floats) FAIL(EXN_EINVAL, "kv8_attend_part: null pointer");
   TRY(check_heads(EXN_DT_F16, EXN_DT_F16, heads, kv_heads, head_dim));
   if (cols < 1 || cols > (1 << 20)) FAIL(EXN_EINVAL, "kv8_attend_part: %d columns", cols);
-  *floats = kv8_attend_part(s->rows, s->seqs, s->longest, heads, kv_heads, head_dim, cols);
+  *floats = kv8_attend_part(s->rows, s->ntiles, s->longest, heads, kv_heads, head_dim, cols);
   return EXN_OK;
 }
 
@@ -227,7 +227,7 @@ int exn_kv8_attend(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, int heads,
     FAIL(EXN_EINVAL, "kv8_attend: %lld floats of scratch at %p", (long long)part_cap, (const void*)part);
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
-  HIPCHK(kv8_attend(ctx->stream, kv8_of(c), s->tiles, s->ntiles, s->rows, s->seqs, s->longest, heads,
+  HIPCHK(kv8_attend(ctx->stream, kv8_of(c), s->tiles, s->ntiles, s->rows, s->longest, heads,
                     (const uint16_t*)q, ldq, scale, (uint16_t*)out, odt == EXN_DT_BF16, ldo, part, part_cap));
   return EXN_OK;
 }

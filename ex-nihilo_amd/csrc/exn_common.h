@@ -331,10 +331,10 @@ hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* tiles, int64_t n
                     uint16_t* v, int64_t ldv);
 hipError_t kv8_advance(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n);
 // floats of scratch with which kv8_attend splits the keys as far as it pays
-int64_t kv8_attend_part(int64_t rows, int seqs, int longest, int heads, int kv_heads, int head_dim, int cols);
+int64_t kv8_attend_part(int64_t rows, const int64_t* ntiles, int longest, int heads, int kv_heads, int head_dim, int cols);
 hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles, int64_t rows,
-                      int seqs, int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out,
-                      int obf, int64_t ldo, float* part, int64_t part_cap);
+                      int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out, int obf,
+                      int64_t ldo, float* part, int64_t part_cap);
 
 // the VAE decoder (vae.hip).  vae_conv's outputs: fp32 (+ bias, + res when given), bf16 (+ bias,
 // + res when given), fp32 (+ bias) clamped to -1 .. 1, fp32 (+ bias, + DupUp3D of keep: kcin

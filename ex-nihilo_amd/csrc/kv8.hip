@@ -9,6 +9,8 @@
 // NaN has the scale NaN: what is read of it is NaN.
 #include "exn_common.h"
 
+#include <type_traits>
+
 namespace exn {
 
 __device__ __forceinline__ float ld16(const uint16_t* p, int bf) { return bf ? bf16_to_f32(*p) : f16_to_f32(*p); }
@@ -110,63 +112,486 @@ hipError_t kv8_advance(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n) 
   return hipGetLastError();
 }
 
-// one wave a query row and head: 64 keys at a time, a score a lane, then a dim (two at 128) a lane
-template <int HD>
-__global__ void __launch_bounds__(64)
-k_kv8_attend(Kv8 c, const SeqTile* __restrict__ tiles, int group, const uint16_t* __restrict__ q, int64_t ldq,
-             float scale, uint16_t* __restrict__ out, int obf, int64_t ldo) {
-  __shared__ float qs[HD], ps[64];
-  const SeqTile t = tiles[blockIdx.x];
-  const int lane = threadIdx.x, h = blockIdx.y, kvh = h / group, i = t.t0 + blockIdx.z;
-  if (i >= t.len) return;
-  const int base = kv8_base(c, t.seq), total = kv8_total(c, base, t.len), lim = min(base + i + 1, total);
-  for (int d = lane; d < HD; d += 64) qs[d] = ld16(q + (int64_t)(t.row0 + i) * ldq + h * HD + d, c.bf16) * scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[HD / 64] = {};
-  for (int j0 = 0; j0 < lim; j0 += 64) {
-    const bool full = j0 + 64 <= total;
-    const int64_t page = full ? kv8_page(c, t.seq, j0 / 64) : 0;
-    if (page < 0) continue;
-    const int64_t ph = page * c.kv_heads + kvh, th = ((int64_t)t.seq * c.kv_heads + kvh) * 64 * HD;
-    const float kd = full ? c.scales[ph * 2] : 1.f, vd = full ? c.scales[ph * 2 + 1] : 1.f;
-    float s = -INFINITY;
-    if (j0 + lane < lim) {
-      s = 0.f;
-      for (int d = 0; d < HD; ++d)
-        s += qs[d] * (full ? (float)c.k[ph * 64 * HD + lane * HD + d] : ld16(c.tk + th + lane * HD + d, c.bf16));
-      s *= kd;
-    }
-    const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2f(m - mu), p = exp2f(s - mu);
-    l = l * a + wave_sum(p);
-    m = mn;
-    __syncthreads();
-    ps[lane] = p;
-    __syncthreads();
-    for (int e = 0; e < HD / 64; ++e) {
-      const int d = e * 64 + lane;
-      float acc = 0.f;
-      for (int j = 0; j < 64 && j0 + j < lim; ++j)
-        acc += ps[j] * (full ? (float)c.v[ph * 64 * HD + d * 64 + j] : ld16(c.tv + th + j * HD + d, c.bf16));
-      o[e] = o[e] * a + acc * vd;
-    }
-  }
-  for (int e = 0; e < HD / 64; ++e)
-    out[(int64_t)(t.row0 + i) * ldo + h * HD + e * 64 + lane] = st16(l > 0.f || l != l ? o[e] / l : 0.f, obf);
+// --- attention over the cache --------------------------------------------------------------------
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// four int8 codes as fp16: each byte, its sign bit flipped, under 0x64 is 1024 + 128 + code; as
+// bf16: the upper halves of the fp32 values (a code has 7 bits)
+__device__ __forceinline__ u32x2 codes_f16(uint32_t w) {
+  const uint32_t x = w ^ 0x80808080u;
+  const f16x2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+  const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + off;
+  const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + off;
+  return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+__device__ __forceinline__ u32x2 codes_bf16(uint32_t w) {
+  float f[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w >> (8 * e));
+  return u32x2{__builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302u),
+               __builtin_amdgcn_perm(__float_as_uint(f[3]), __float_as_uint(f[2]), 0x07060302u)};
+}
+template <int BF>
+__device__ __forceinline__ s16x8 codes8(uint32_t a, uint32_t b) {
+  const u32x2 x = BF ? codes_bf16(a) : codes_f16(a), y = BF ? codes_bf16(b) : codes_f16(b);
+  return __builtin_bit_cast(s16x8, u32x4{x[0], x[1], y[0], y[1]});
+}
+template <int BF>
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float max_groups(float v) {   // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  float a = v, b = v;
+  xswap16(a, b);
+  a = b = fmaxf(a, b);
+  xswap32(a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float sum_groups(float v) {
+  float a = v, b = v;
+  xswap16(a, b);
+  a = b = a + b;
+  xswap32(a, b);
+  return a + b;
 }
 
-int64_t kv8_attend_part(int64_t rows, int seqs, int longest, int heads, int kv_heads, int head_dim, int cols) { return 0; }
+struct Kv8Args {
+  Kv8 c;
+  const SeqTile* tiles;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t ldq, ldo;
+  float scale;            // times log2(e)
+  int heads, group;
+  int tt, hh, chunks;     // tokens and heads a workgroup; workgroups a key/value head's group
+  uint32_t magic;         // ceil(65536 / hh)
+  int obf, splits;
+  float* part;            // [split][row][head][dim], then [split][row][head][2]: the sums, their reference and weight
+  int64_t rows;
+};
+#define KV8_MIN 16   // blocks a split has at least, where the keys are split
+
+// the blocks of a sequence's NB that split I of S takes: [*lo, *hi); the number of splits with any
+__device__ __forceinline__ int kv8_split(int nb, int S, int i, int* lo, int* hi) {
+  const int per = max(KV8_MIN, (nb + S - 1) / S);
+  *lo = min(nb, i * per);
+  *hi = min(nb, (i + 1) * per);
+  return (nb + per - 1) / per;
+}
+
+#define MAX_SLACK 8.f
+
+// grid: splits x (tiles x chunks x kv_heads, the heads fastest); block 256.  RT row tiles of 16.
+template <int BF, int HD, int RT>
+__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
+k_kv8_attend(Kv8Args A) {
+  constexpr int NS = HD / 32, ND = HD / 16;   // k-steps of a score; 16-dim tiles of O
+  constexpr int KL = HD / 64;                 // 16-byte loads a lane, key tile and block of K
+  constexpr int LD = HD + 4;
+  __shared__ __align__(16) float obuf[4][16][LD];     // the waves' sums; the tail's V (64 rows of 16 bits) before that
+  __shared__ float mbuf[4][16], lbuf[4][16], pbuf[64][17];
+  const Kv8& c = A.c;
+  const int per = c.kv_heads * A.chunks;
+  const SeqTile T = A.tiles[blockIdx.x / per];
+  const int hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len), nfull = total / 64;
+  const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
+  const int nb = (min(base + T.t0 + live, total) + 63) / 64;   // blocks that some row here sees
+  int lo, hi;
+  const int active = max(1, kv8_split(nb, A.splits, blockIdx.y, &lo, &hi));
+  if ((int)blockIdx.y >= active) return;
+
+  int lim[RT];
+  s16x8 qf[RT][NS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rt * 16 + col, tok = min((int)(r * A.magic >> 16), live - 1);
+    const int head = min(r - (int)(r * A.magic >> 16) * A.hh, heads - 1);
+    lim[rt] = min(base + T.t0 + tok, total - 1);
+    // dims of k-step s: 16 g + 8 (s % 2) + 64 (s / 2) .., as the 16 bytes of codes a lane loads
+    const uint16_t* qr = A.q + (int64_t)(T.row0 + T.t0 + tok) * A.ldq +
+                         (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[rt][s] = *(const s16x8*)(qr + 8 * (s % 2) + 64 * (s / 2));
+  }
+  f32x4 o[RT][ND];
+  float mrun[RT], lrun[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{};
+    mrun[rt] = -INFINITY;
+    lrun[rt] = 0.f;
+  }
+  float s[RT][16];   // scores of keys 16 g + e of the block in hand
+  uint32_t pk[RT][8];
+
+  // from scores (log2 units, hidden ones -inf) to weights: the rows' references, sums and pk
+  auto weights = [&](int bf) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float mx = s[rt][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[rt][e]);
+      mx = max_groups(mx);
+      // a first reference (any above -inf), or one that has fallen behind
+      if (__ballot(mx > mrun[rt] + MAX_SLACK)) {
+        const float mn = mx > mrun[rt] + MAX_SLACK ? mx : mrun[rt];
+        const float a = mn == mrun[rt] ? 1.f : __builtin_amdgcn_exp2f(mrun[rt] - mn);
+        mrun[rt] = mn;
+        lrun[rt] *= a;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[rt][d] *= a;
+      }
+      const float ref = mrun[rt] == -INFINITY ? 0.f : mrun[rt];
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(s[rt][e] - ref), p1 = __builtin_amdgcn_exp2f(s[rt][e + 1] - ref);
+        pk[rt][e / 2] = bf ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+        lrun[rt] += p0;
+        lrun[rt] += p1;
+      }
+    }
+  };
+  auto pfrag = [&](int rt, int u) {
+    return __builtin_bit_cast(s16x8, u32x4{pk[rt][4 * u], pk[rt][4 * u + 1], pk[rt][4 * u + 2], pk[rt][4 * u + 3]});
+  };
+
+  // key of row r of key tile t: 16 (r / 4) + 4 t + r % 4, so that a lane's scores of the four tiles
+  // are 16 consecutive keys, the ones whose V codes it loads as 16 bytes
+  const int key0 = 16 * (col >> 2) + (col & 3);
+  const int its = (min(hi, nfull) - lo - wave + 3) >> 2;   // full blocks lo + wave + 4 it of this wave
+  int pages = 0;
+  float kds = 0.f, vds = 0.f;
+  // 64 blocks' pages and scales, a lane each
+  auto look = [&](int it) {
+    const int b = lo + wave + 4 * (it + lane);
+    int64_t p = b < min(hi, nfull) ? kv8_page(c, T.seq, b) : -1;
+    pages = (int)p;
+    p = p < 0 ? 0 : p;
+    const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
+    kds = d[0];
+    vds = d[1];
+  };
+  u32x4 kr[4][KL], vr[ND];
+  auto load_k = [&](int page) {
+    const int8_t* p = c.k + ((int64_t)max(page, 0) * c.kv_heads + kvh) * 64 * HD;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < KL; ++e) kr[t][e] = *(const u32x4*)(p + (key0 + 4 * t) * HD + 16 * g + 64 * e);
+  };
+  auto load_v = [&](int page) {
+    const int8_t* p = c.v + ((int64_t)max(page, 0) * c.kv_heads + kvh) * 64 * HD;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) vr[d] = *(const u32x4*)(p + (16 * d + col) * 64 + 16 * g);
+  };
+  if (its > 0) {
+    look(0);
+    load_k(__builtin_amdgcn_readlane(pages, 0));
+    load_v(__builtin_amdgcn_readlane(pages, 0));
+  }
+  for (int it = 0; it < its; ++it) {
+    const int page = __builtin_amdgcn_readlane(pages, it & 63);
+    const float kd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kds), it & 63)) * A.scale;
+    const float vd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vds), it & 63));
+    if ((it & 63) == 63 && it + 1 < its) look(it + 1);
+    const int next = it + 1 < its ? __builtin_amdgcn_readlane(pages, (it + 1) & 63) : 0;
+    const int k0 = (lo + wave + 4 * it) * 64;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f32x4 a[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) a[rt] = f32x4{};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        const u32x4 w = kr[t][ks / 2];
+        const s16x8 kf = codes8<BF>(w[2 * (ks % 2)], w[2 * (ks % 2) + 1]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) a[rt] = mfma16<BF>(kf, qf[rt][ks], a[rt]);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[rt][4 * t + i] = a[rt][i] * kd;
+    }
+    if (it + 1 < its) load_k(next);
+    float vdl[RT];   // a row that sees nothing of the block takes nothing of its scale, which may be NaN
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      vdl[rt] = page >= 0 && k0 <= lim[rt] ? vd : 0.f;
+      if (page < 0 || k0 + 63 > base + T.t0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (page < 0 || k0 + 16 * g + e > lim[rt]) s[rt][e] = -INFINITY;
+      }
+    }
+    weights(0);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const s16x8 v0 = codes8<0>(vr[d][0], vr[d][1]), v1 = codes8<0>(vr[d][2], vr[d][3]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const f32x4 a = mfma16<0>(v1, pfrag(rt, 1), mfma16<0>(v0, pfrag(rt, 0), f32x4{}));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[rt][d][i] = __builtin_fmaf(a[i], vdl[rt], o[rt][d][i]);
+      }
+    }
+    if (it + 1 < its) load_v(next);
+  }
+
+  // the tail, in 16 bits, by the wave whose turn it is
+  if (nfull < hi && nfull >= lo && ((nfull - lo) & 3) == wave) {
+    const int left = total - nfull * 64;
+    const int64_t at = ((int64_t)T.seq * c.kv_heads + kvh) * 64 * HD;
+    uint16_t* vt = (uint16_t*)obuf;
+#pragma unroll
+    for (int e = 0; e < HD / 8; ++e) {   // V's rows into LDS, those past the last token as zeros
+      const int i = (e * 64 + lane) * 8, key = i / HD;
+      u32x4 x = {};
+      if (key < left) x = *(const u32x4*)(c.tv + at + i);
+      *(u32x4*)(vt + i) = x;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f32x4 a[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) a[rt] = f32x4{};
+#pragma unroll
+      for (int ks = 0; ks < NS; ++ks) {
+        s16x8 kf = {};
+        if (key0 + 4 * t < left)
+          kf = *(const s16x8*)(c.tk + at + (key0 + 4 * t) * HD + 16 * g + 8 * (ks % 2) + 64 * (ks / 2));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) a[rt] = mfma16<BF>(kf, qf[rt][ks], a[rt]);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[rt][4 * t + i] = nfull * 64 + 16 * g + 4 * t + i > lim[rt] ? -INFINITY : a[rt][i] * A.scale;
+    }
+    weights(BF);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's V rows are in LDS
+    asm volatile("" ::: "memory");
+    typedef __attribute__((address_space(3))) s16x4 lds_s4;
+    // lane i of 16 addresses key i / 4's dims 4 (i % 4) .. and gets dim i of the 4 keys
+    uint16_t* vl = vt + (16 * g + (col >> 2)) * HD + 4 * (col & 3);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      f32x4 a[ND];
+      uint32_t bad = 0;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        s16x8 v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vl + 8 * u * HD + 16 * d));
+          const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vl + (8 * u + 4) * HD + 16 * d));
+          v[u] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        a[d] = mfma16<BF>(v[1], pfrag(rt, 1), mfma16<BF>(v[0], pfrag(rt, 0), f32x4{}));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= (__float_as_uint(a[d][i]) & 0x7F800000u) == 0x7F800000u;
+      }
+      if (__ballot(bad)) {
+        // an infinity or a NaN among the values: again, each row over the keys it sees only
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pbuf[16 * g + e][col] = __builtin_amdgcn_exp2f(s[rt][e] - (mrun[rt] == -INFINITY ? 0.f : mrun[rt]));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int d = 0; d < ND; ++d) a[d] = f32x4{};
+        for (int j = 0; j < left && nfull * 64 + j <= lim[rt]; ++j) {
+          const float p = pbuf[j][col];
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[d][i] += p * ld16(vt + j * HD + 16 * d + 4 * g + i, BF);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[rt][d] += a[d];
+    }
+  }
+
+  // the four waves' sums of a row tile through LDS, 16 threads a row
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *(f32x4*)&obuf[wave][col][16 * d + 4 * g] = o[rt][d];
+    const float l = sum_groups(lrun[rt]);
+    if (g == 0) {
+      mbuf[wave][col] = mrun[rt];
+      lbuf[wave][col] = l;
+    }
+    __syncthreads();
+    const int rr = tid >> 4, r = rt * 16 + rr, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
+    if (tok >= live || head >= heads) continue;
+    const float m = fmaxf(fmaxf(mbuf[0][rr], mbuf[1][rr]), fmaxf(mbuf[2][rr], mbuf[3][rr]));
+    float w[4], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = mbuf[k][rr] == -INFINITY ? 0.f : mbuf[k][rr] == m ? 1.f : __builtin_amdgcn_exp2f(mbuf[k][rr] - m);
+      sum += mbuf[k][rr] == -INFINITY ? lbuf[k][rr] : w[k] * lbuf[k][rr];   // no reference: 0, or NaN
+    }
+    const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + kvh * A.group + chunk * A.hh + head;
+    const float inv = active > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    constexpr int E = HD / 16;   // dims a thread
+    const int d0 = (tid & 15) * E;
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      y[e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (w[k] > 0.f) y[e] = __builtin_fmaf(w[k], obuf[k][rr][d0 + e], y[e]);
+      y[e] *= inv;
+    }
+    if (active > 1) {
+      const int64_t n = A.rows * A.heads, at = blockIdx.y * n + rowhead;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + at * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+      if ((tid & 15) == 0) *(f32x2*)(A.part + A.splits * n * HD + at * 2) = f32x2{m, sum};
+    } else {
+      uint32_t x[E / 2];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) x[e / 2] = A.obf ? pack_bf16x2(y[e], y[e + 1]) : pack_f16x2(y[e], y[e + 1]);
+      uint16_t* po = A.out + (rowhead / A.heads) * A.ldo + (rowhead % A.heads) * HD + d0;
+      if constexpr (E == 8)
+        *(u32x4*)po = u32x4{x[0], x[1], x[2], x[3]};
+      else
+        *(u32x2*)po = u32x2{x[0], x[1]};
+    }
+  }
+}
+
+// the splits' sums of each row and head, in order; rows whose keys were not split are done
+template <int HD>
+__global__ void __launch_bounds__(256)
+k_kv8_join(Kv8Args A) {
+  const Kv8& c = A.c;
+  const SeqTile T = A.tiles[blockIdx.x];
+  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len);
+  const int live = min(A.tt, T.len - T.t0);
+  int lo, hi;
+  const int active = kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, 0, &lo, &hi);
+  if (active < 2) return;
+  constexpr int TH = HD / 4;   // threads a row and head
+  const int i = blockIdx.y * (256 / TH) + threadIdx.x / TH, d = threadIdx.x % TH * 4;
+  if (i >= live * A.heads) return;
+  const int64_t rowhead = (int64_t)(T.row0 + T.t0) * A.heads + i, n = A.rows * A.heads;
+  const float* ml = A.part + A.splits * n * HD + rowhead * 2;
+  float m = -INFINITY;
+  for (int z = 0; z < active; ++z) m = fmaxf(m, ml[z * n * 2]);
+  float sum = 0.f;
+  f32x4 y = {};
+  for (int z = 0; z < active; ++z) {
+    const f32x2 p = *(const f32x2*)(ml + z * n * 2);
+    const float w = p[0] == -INFINITY ? 0.f : p[0] == m ? 1.f : __builtin_amdgcn_exp2f(p[0] - m);
+    sum += p[0] == -INFINITY ? p[1] : w * p[1];
+    if (w > 0.f) y += w * *(const f32x4*)(A.part + (z * n + rowhead) * HD + d);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* po = A.out + (rowhead / A.heads) * A.ldo + (rowhead % A.heads) * HD + d;
+  *(u32x2*)po = A.obf ? u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)}
+                      : u32x2{pack_f16x2(y[0] * inv, y[1] * inv), pack_f16x2(y[2] * inv, y[3] * inv)};
+}
+
+namespace {
+
+struct Kv8Way {
+  int rt, z, hh, chunks, splits;   // row tiles a workgroup; the tiles' list; heads a workgroup, workgroups a group; splits
+};
+Kv8Way kv8_way(int longest, int heads, int kv_heads, int head_dim, int cols, const int64_t* ntiles) {
+  Kv8Way w;
+  const int group = heads / kv_heads;
+  w.hh = group < 16 ? group : 16;
+  w.z = 0;
+  if (longest * w.hh <= 32) {
+    w.rt = longest * w.hh <= 16 ? 1 : 2;
+    while ((SEQ_TT0 << w.z) < longest) ++w.z;
+  } else {
+    w.rt = head_dim == 128 ? 2 : 4;
+    const int most = 16 * w.rt / SEQ_TT0;
+    w.hh = group < most ? group : most;
+    while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 16 * w.rt) ++w.z;
+  }
+  w.chunks = (group + w.hh - 1) / w.hh;
+  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, s = groups > 0 ? 4096 / groups : 1;
+  const int64_t most = (cols + KV8_MIN - 1) / KV8_MIN;
+  w.splits = (int)(s < 1 ? 1 : s > most ? most : s);
+  return w;
+}
+
+}  // namespace
+
+int64_t kv8_attend_part(int64_t rows, const int64_t* ntiles, int longest, int heads, int kv_heads, int head_dim, int cols) {
+  const Kv8Way w = kv8_way(longest, heads, kv_heads, head_dim, cols, ntiles);
+  return w.splits > 1 ? w.splits * rows * heads * (head_dim + 2) : 0;
+}
 
 hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles, int64_t rows,
-                      int seqs, int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out,
-                      int obf, int64_t ldo, float* part, int64_t part_cap) {
+                      int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out, int obf,
+                      int64_t ldo, float* part, int64_t part_cap) {
   if (ntiles[0] == 0) return hipSuccess;
-  const dim3 grid((unsigned)ntiles[0], heads, SEQ_TT0);
-  const float sc = scale * 1.4426950408889634f;
+  Kv8Way w = kv8_way(longest, heads, c.kv_heads, c.head_dim, c.cols, ntiles);
+  const int64_t fit = part_cap / (rows * heads * (c.head_dim + 2));
+  if (w.splits > fit) w.splits = fit < 1 ? 1 : (int)fit;
+  Kv8Args a;
+  a.c = c;
+  a.tiles = tiles[w.z];
+  a.q = q;
+  a.out = out;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.scale = scale * 1.4426950408889634f;
+  a.heads = heads;
+  a.group = heads / c.kv_heads;
+  a.tt = SEQ_TT0 << w.z;
+  a.hh = w.hh;
+  a.chunks = w.chunks;
+  a.magic = (65536 + w.hh - 1) / w.hh;
+  a.obf = obf;
+  a.splits = w.splits;
+  a.part = part;
+  a.rows = rows;
+  const int64_t groups = ntiles[w.z] * w.chunks * c.kv_heads;
+  if (groups > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)groups, w.splits);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
+  auto rts = [&](auto bf, auto hd) {
+    constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
+    if constexpr (HD == 64)
+      if (w.rt == 4) return go(k_kv8_attend<BF, HD, 4>);
+    w.rt == 1 ? go(k_kv8_attend<BF, HD, 1>) : go(k_kv8_attend<BF, HD, 2>);
+  };
+  typedef std::integral_constant<int, 0> I0;
+  typedef std::integral_constant<int, 1> I1;
+  typedef std::integral_constant<int, 64> I64;
+  typedef std::integral_constant<int, 128> I128;
   if (c.head_dim == 128)
-    hipLaunchKernelGGL(k_kv8_attend<128>, grid, dim3(64), 0, s, c, tiles[0], heads / c.kv_heads, q, ldq, sc, out, obf, ldo);
+    c.bf16 ? rts(I1(), I128()) : rts(I0(), I128());
   else
-    hipLaunchKernelGGL(k_kv8_attend<64>, grid, dim3(64), 0, s, c, tiles[0], heads / c.kv_heads, q, ldq, sc, out, obf, ldo);
+    c.bf16 ? rts(I1(), I64()) : rts(I0(), I64());
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || w.splits < 2) return e;
+  const int each = 256 / (c.head_dim / 4), most = a.tt < longest ? a.tt : longest;
+  const dim3 jg((unsigned)ntiles[w.z], (most * heads + each - 1) / each);
+  if (c.head_dim == 128)
+    hipLaunchKernelGGL(k_kv8_join<128>, jg, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_kv8_join<64>, jg, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

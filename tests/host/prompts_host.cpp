@@ -40,8 +40,8 @@ hipError_t kv8_read(hipStream_t, const Kv8&, const SeqTile*, int64_t, int, uint1
   return note("read");
 }
 hipError_t kv8_advance(hipStream_t, const Kv8&, const SeqTile*, int) { return note("advance"); }
-int64_t kv8_attend_part(int64_t, int, int, int, int, int, int) { return 12; }
-hipError_t kv8_attend(hipStream_t, const Kv8&, const SeqTile* const*, const int64_t*, int64_t, int, int, int,
+int64_t kv8_attend_part(int64_t, const int64_t*, int, int, int, int, int) { return 12; }
+hipError_t kv8_attend(hipStream_t, const Kv8&, const SeqTile* const*, const int64_t*, int64_t, int, int,
                       const uint16_t*, int64_t, float, uint16_t*, int, int64_t, float*, int64_t) {
   return note("attend");
 }
