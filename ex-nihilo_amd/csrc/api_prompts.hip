@@ -197,7 +197,7 @@ int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int
   TRY(check_rows("kv8_read v", v, ldv, (int64_t)c->kv_heads * c->head_dim));
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
-  HIPCHK(kv8_read(ctx->stream, kv8_of(c), s->tiles[0], s->ntiles[0], SEQ_TT0, (uint16_t*)k, ldk, (uint16_t*)v, ldv));
+  HIPCHK(kv8_read(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (uint16_t*)k, ldk, (uint16_t*)v, ldv));
   return EXN_OK;
 }
 

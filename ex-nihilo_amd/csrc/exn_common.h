@@ -327,7 +327,7 @@ __host__ __device__ inline float kv8_scale(uint32_t top) {
 __host__ __device__ inline int8_t kv8_code(float x, float d) { return d > 0.f ? (int8_t)__builtin_rintf(x / d) : (int8_t)0; }
 hipError_t kv8_append(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, int longest, const uint16_t* k,
                       int64_t ldk, const uint16_t* v, int64_t ldv);
-hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* tiles, int64_t n, int tt, uint16_t* k, int64_t ldk,
+hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, int longest, uint16_t* k, int64_t ldk,
                     uint16_t* v, int64_t ldv);
 hipError_t kv8_advance(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n);
 // floats of scratch with which kv8_attend splits the keys as far as it pays

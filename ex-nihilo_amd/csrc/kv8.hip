@@ -14,50 +14,113 @@
 namespace exn {
 
 __device__ __forceinline__ float ld16(const uint16_t* p, int bf) { return bf ? bf16_to_f32(*p) : f16_to_f32(*p); }
-__device__ __forceinline__ uint16_t st16(float v, int bf) {
-  return bf ? __builtin_bit_cast(uint16_t, (__bf16)v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+// HD / 16 consecutive 16-bit values
+template <int HD>
+struct Piece {
+  uint32_t w[HD / 32];
+};
+template <int HD>
+__device__ __forceinline__ Piece<HD> load_piece(const uint16_t* p) {
+  if constexpr (HD == 128) {
+    const u32x4 x = *(const u32x4*)p;
+    return Piece<HD>{{x[0], x[1], x[2], x[3]}};
+  } else {
+    const u32x2 x = *(const u32x2*)p;
+    return Piece<HD>{{x[0], x[1]}};
+  }
+}
+template <int HD>
+__device__ __forceinline__ void store_piece(uint16_t* p, const Piece<HD>& x) {
+  if constexpr (HD == 128)
+    *(u32x4*)p = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+  else
+    *(u32x2*)p = u32x2{x.w[0], x.w[1]};
+}
+__device__ __forceinline__ float half_of(uint32_t w, int e, int bf) {
+  return bf ? (e & 1 ? bf16_hi(w) : bf16_lo(w)) : (e & 1 ? f16_hi(w) : f16_lo(w));
 }
 
-// One workgroup a (sequence, key/value head, block the step can touch, keys or values).  Block 0's
-// also writes the tail, after it has read the old one: the one slot serves the block that fills and
-// the block begun after it.
+// One workgroup a (sequence and key/value head, block the step can touch, keys or values): bytes are
+// what it costs.  A thread has 4 tokens x HD / 16 dims of a block in registers, from the tail or the
+// new rows, between the block's largest |x| and its codes; values leave through LDS, where four
+// tokens' codes of a dim are a dword.  Block 0's workgroup also writes the tail, after it has read the
+// old one: the one slot serves the block that fills and the block begun after it.
+template <int HD>
 __global__ void __launch_bounds__(256)
 k_kv8_append(Kv8 c, const SeqTile* __restrict__ seqs, const uint16_t* __restrict__ k, int64_t ldk,
              const uint16_t* __restrict__ v, int64_t ldv) {
-  __shared__ uint32_t tops[4];
+  constexpr int E = HD / 16, LD = 17;   // dims a thread; dwords a dim's row in LDS
+  __shared__ uint32_t tops[4], cols[HD * LD];
   const SeqTile t = seqs[blockIdx.x / c.kv_heads];
-  const int h = blockIdx.x % c.kv_heads, isv = blockIdx.z, hd = c.head_dim, tid = threadIdx.x;
+  const int h = blockIdx.x % c.kv_heads, isv = blockIdx.z, tid = threadIdx.x;
   const int base = kv8_base(c, t.seq), total = kv8_total(c, base, t.len);
   const int first = base / 64, b = first + blockIdx.y;
   if (t.len == 0 || total <= base) return;
   const int64_t ld = isv ? ldv : ldk;
-  const uint16_t* x = (isv ? v : k) + (int64_t)t.row0 * ld + h * hd;
-  uint16_t* tail = (isv ? c.tv : c.tk) + ((int64_t)t.seq * c.kv_heads + h) * 64 * hd;
+  const uint16_t* x = (isv ? v : k) + (int64_t)t.row0 * ld + h * HD;
+  uint16_t* tail = (isv ? c.tv : c.tk) + ((int64_t)t.seq * c.kv_heads + h) * 64 * HD;
+  const int d0 = (tid & 15) * E, quad = tid >> 4;
   if ((b + 1) * 64 <= total) {   // the block is full now
-    auto at = [&](int e) {
-      const int pos = b * 64 + e / hd;
-      return ld16(pos < base ? tail + e : x + (pos - base) * ld + e % hd, c.bf16);
-    };
+    const int64_t page = kv8_page(c, t.seq, b);
+    Piece<HD> r[4];
     uint32_t top = 0;
-    for (int e = tid; e < 64 * hd; e += 256) top = max(top, __float_as_uint(at(e)) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int pos = b * 64 + 4 * quad + i;
+      r[i] = load_piece<HD>(pos < base ? tail + pos % 64 * HD + d0 : x + (int64_t)(pos - base) * ld + d0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(half_of(r[i].w[e / 2], e, c.bf16)) & 0x7FFFFFFFu);
     for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     if (tid % 64 == 0) tops[tid / 64] = top;
     __syncthreads();
     const float d = kv8_scale(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
-    const int64_t page = kv8_page(c, t.seq, b);
     if (page >= 0) {
-      int8_t* dst = (isv ? c.v : c.k) + (page * c.kv_heads + h) * 64 * hd;
-      for (int e = tid; e < 64 * hd; e += 256) dst[isv ? e % hd * 64 + e / hd : e] = kv8_code(at(e), d);
+      int8_t* dst = (isv ? c.v : c.k) + (page * c.kv_heads + h) * 64 * HD;
+      uint32_t code[4][E / 4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e4 = 0; e4 < E / 4; ++e4) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w |= (uint32_t)(uint8_t)kv8_code(half_of(r[i].w[2 * e4 + e / 2], e, c.bf16), d) << (8 * e);
+          code[i][e4] = w;
+        }
+      if (isv) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w |= (code[i][e / 4] >> (8 * (e % 4)) & 0xFFu) << (8 * i);
+          cols[(d0 + e) * LD + quad] = w;
+        }
+        __syncthreads();
+        for (int i = tid; i < HD * 4; i += 256) {
+          const uint32_t* p = cols + i / 4 * LD + i % 4 * 4;
+          *(u32x4*)(dst + i * 16) = u32x4{p[0], p[1], p[2], p[3]};
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          int8_t* p = dst + (4 * quad + i) * HD + d0;
+          if constexpr (HD == 128)
+            *(u32x2*)p = u32x2{code[i][0], code[i][1]};
+          else
+            *(uint32_t*)p = code[i][0];
+        }
+      }
       if (tid == 0) c.scales[(page * c.kv_heads + h) * 2 + isv] = d;
     }
   }
   if (blockIdx.y == 0 && total % 64) {
     __syncthreads();   // the old tail has been read
     const int from = max(base, total / 64 * 64);
-    for (int e = tid; e < (total - from) * hd; e += 256) {
-      const int pos = from + e / hd;
-      tail[pos % 64 * hd + e % hd] = x[(pos - base) * ld + e % hd];
-    }
+    for (int pos = from + quad; pos < total; pos += 16)
+      store_piece<HD>(tail + pos % 64 * HD + d0, load_piece<HD>(x + (int64_t)(pos - base) * ld + d0));
   }
 }
 
@@ -65,39 +128,96 @@ hipError_t kv8_append(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, i
                       int64_t ldk, const uint16_t* v, int64_t ldv) {
   if (n == 0 || longest == 0) return hipSuccess;
   const dim3 grid(n * c.kv_heads, (62 + longest) / 64 + 1, 2);
-  hipLaunchKernelGGL(k_kv8_append, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
+  if (c.head_dim == 128)
+    hipLaunchKernelGGL(k_kv8_append<128>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
+  else
+    hipLaunchKernelGGL(k_kv8_append<64>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
   return hipGetLastError();
 }
 
-// the step's rows as the cache holds them, 16 bits (code x d rounded once); a place past the
-// table, or on a page that is none, reads zeros
+// the step's rows as the cache holds them, 16 bits (code x d rounded once): workgroups and threads as
+// in the append; a place past the table, or on a page that is none, reads zeros
+template <int HD>
 __global__ void __launch_bounds__(256)
-k_kv8_read(Kv8 c, const SeqTile* __restrict__ tiles, int tt, uint16_t* __restrict__ k, int64_t ldk,
-           uint16_t* __restrict__ v, int64_t ldv) {
-  const SeqTile t = tiles[blockIdx.x];
-  const int h = blockIdx.y, isv = blockIdx.z, hd = c.head_dim;
+k_kv8_read(Kv8 c, const SeqTile* __restrict__ seqs, uint16_t* __restrict__ k, int64_t ldk, uint16_t* __restrict__ v,
+           int64_t ldv) {
+  constexpr int E = HD / 16, LD = 17;
+  __shared__ uint32_t cols[HD * LD];
+  const SeqTile t = seqs[blockIdx.x / c.kv_heads];
+  const int h = blockIdx.x % c.kv_heads, isv = blockIdx.z, tid = threadIdx.x;
   const int base = kv8_base(c, t.seq), total = kv8_total(c, base, t.len);
-  for (int e = threadIdx.x; e < min(tt, t.len - t.t0) * hd; e += 256) {
-    const int i = t.t0 + e / hd, d = e % hd, pos = base + i;
-    uint16_t y = 0;
-    if (pos < total / 64 * 64) {
-      const int64_t page = kv8_page(c, t.seq, pos / 64);
-      if (page >= 0) {
-        const int64_t ph = page * c.kv_heads + h;
-        const int8_t q = (isv ? c.v + ph * 64 * hd + d * 64 + pos % 64 : c.k + ph * 64 * hd + pos % 64 * hd + d)[0];
-        y = st16((float)q * c.scales[ph * 2 + isv], c.bf16);
+  const int b = base / 64 + blockIdx.y, end = base + t.len;   // the last places may be past the table
+  if (t.len == 0 || b * 64 >= end) return;
+  const int64_t ld = isv ? ldv : ldk;
+  uint16_t* y = (isv ? v : k) + (int64_t)t.row0 * ld + h * HD;
+  const int d0 = (tid & 15) * E, quad = tid >> 4;
+  Piece<HD> r[4] = {};
+  if ((b + 1) * 64 <= total) {
+    const int64_t page = kv8_page(c, t.seq, b);
+    if (page >= 0) {
+      const int64_t ph = page * c.kv_heads + h;
+      const float d = c.scales[ph * 2 + isv];
+      const int8_t* src = (isv ? c.v : c.k) + ph * 64 * HD;
+      uint32_t code[4][E / 4] = {};
+      if (isv) {
+        for (int i = tid; i < HD * 4; i += 256) {
+          const u32x4 w = *(const u32x4*)(src + i * 16);
+          uint32_t* p = cols + i / 4 * LD + i % 4 * 4;
+          p[0] = w[0];
+          p[1] = w[1];
+          p[2] = w[2];
+          p[3] = w[3];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t w = cols[(d0 + e) * LD + quad];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) code[i][e / 4] |= (w >> (8 * i) & 0xFFu) << (8 * (e % 4));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int8_t* p = src + (4 * quad + i) * HD + d0;
+          if constexpr (HD == 128) {
+            const u32x2 w = *(const u32x2*)p;
+            code[i][0] = w[0];
+            code[i][1] = w[1];
+          } else {
+            code[i][0] = *(const uint32_t*)p;
+          }
+        }
       }
-    } else if (pos < total) {
-      y = (isv ? c.tv : c.tk)[(((int64_t)t.seq * c.kv_heads + h) * 64 + pos % 64) * hd + d];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float a = d * (float)(int8_t)(code[i][e / 4] >> (8 * (e % 4)));
+          const float z = d * (float)(int8_t)(code[i][e / 4] >> (8 * (e % 4) + 8));
+          r[i].w[e / 2] = c.bf16 ? pack_bf16x2(a, z) : pack_f16x2(a, z);
+        }
     }
-    (isv ? v : k)[(int64_t)(t.row0 + i) * (isv ? ldv : ldk) + h * hd + d] = y;
+  } else {
+    const uint16_t* tail = (isv ? c.tv : c.tk) + ((int64_t)t.seq * c.kv_heads + h) * 64 * HD;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (b * 64 + 4 * quad + i < total) r[i] = load_piece<HD>(tail + (4 * quad + i) * HD + d0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int pos = b * 64 + 4 * quad + i;
+    if (pos >= base && pos < end) store_piece<HD>(y + (int64_t)(pos - base) * ld + d0, r[i]);
   }
 }
 
-hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* tiles, int64_t n, int tt, uint16_t* k, int64_t ldk,
+hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, int longest, uint16_t* k, int64_t ldk,
                     uint16_t* v, int64_t ldv) {
-  if (n == 0) return hipSuccess;
-  hipLaunchKernelGGL(k_kv8_read, dim3((unsigned)n, c.kv_heads, 2), dim3(256), 0, s, c, tiles, tt, k, ldk, v, ldv);
+  if (n == 0 || longest == 0) return hipSuccess;
+  const dim3 grid(n * c.kv_heads, (62 + longest) / 64 + 1, 2);
+  if (c.head_dim == 128)
+    hipLaunchKernelGGL(k_kv8_read<128>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
+  else
+    hipLaunchKernelGGL(k_kv8_read<64>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
   return hipGetLastError();
 }
 
@@ -476,31 +596,48 @@ k_kv8_attend(Kv8Args A) {
   }
 }
 
-// the splits' sums of each row and head, in order; rows whose keys were not split are done
+// The splits' sums of one row and head (a workgroup), in a fixed order: 256 / (HD / 4) shares of the
+// splits, then the shares.  Rows whose keys were not split are done.
 template <int HD>
 __global__ void __launch_bounds__(256)
 k_kv8_join(Kv8Args A) {
+  constexpr int TH = HD / 4, SH = 256 / TH;   // threads a share; shares
+  __shared__ __align__(16) float ys[SH][HD];
+  __shared__ float ss[SH], ms[4];
   const Kv8& c = A.c;
   const SeqTile T = A.tiles[blockIdx.x];
   const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len);
   const int live = min(A.tt, T.len - T.t0);
   int lo, hi;
   const int active = kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, 0, &lo, &hi);
-  if (active < 2) return;
-  constexpr int TH = HD / 4;   // threads a row and head
-  const int i = blockIdx.y * (256 / TH) + threadIdx.x / TH, d = threadIdx.x % TH * 4;
-  if (i >= live * A.heads) return;
-  const int64_t rowhead = (int64_t)(T.row0 + T.t0) * A.heads + i, n = A.rows * A.heads;
+  if (active < 2 || (int)blockIdx.y >= live * A.heads) return;
+  const int tid = threadIdx.x, sh = tid / TH, d = tid % TH * 4;
+  const int64_t rowhead = (int64_t)(T.row0 + T.t0) * A.heads + blockIdx.y, n = A.rows * A.heads;
   const float* ml = A.part + A.splits * n * HD + rowhead * 2;
   float m = -INFINITY;
-  for (int z = 0; z < active; ++z) m = fmaxf(m, ml[z * n * 2]);
+  for (int z = tid; z < active; z += 256) m = fmaxf(m, ml[z * n * 2]);
+  m = wave_max(m);
+  if (tid % 64 == 0) ms[tid / 64] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
   float sum = 0.f;
   f32x4 y = {};
-  for (int z = 0; z < active; ++z) {
+#pragma unroll 4
+  for (int z = sh; z < active; z += SH) {
     const f32x2 p = *(const f32x2*)(ml + z * n * 2);
+    const f32x4 x = *(const f32x4*)(A.part + (z * n + rowhead) * HD + d);
     const float w = p[0] == -INFINITY ? 0.f : p[0] == m ? 1.f : __builtin_amdgcn_exp2f(p[0] - m);
-    sum += p[0] == -INFINITY ? p[1] : w * p[1];
-    if (w > 0.f) y += w * *(const f32x4*)(A.part + (z * n + rowhead) * HD + d);
+    sum += p[0] == -INFINITY ? p[1] : w * p[1];   // no reference: 0, or NaN
+    if (w > 0.f) y += w * x;
+  }
+  *(f32x4*)&ys[sh][d] = y;
+  if (d == 0) ss[sh] = sum;
+  __syncthreads();
+  if (sh) return;
+#pragma unroll
+  for (int k = 1; k < SH; ++k) {
+    y += *(const f32x4*)&ys[k][d];
+    sum += ss[k];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* po = A.out + (rowhead / A.heads) * A.ldo + (rowhead % A.heads) * HD + d;
@@ -586,8 +723,7 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
     c.bf16 ? rts(I1(), I64()) : rts(I0(), I64());
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.splits < 2) return e;
-  const int each = 256 / (c.head_dim / 4), most = a.tt < longest ? a.tt : longest;
-  const dim3 jg((unsigned)ntiles[w.z], (most * heads + each - 1) / each);
+  const dim3 jg((unsigned)ntiles[w.z], (a.tt < longest ? a.tt : longest) * heads);
   if (c.head_dim == 128)
     hipLaunchKernelGGL(k_kv8_join<128>, jg, dim3(256), 0, s, a);
   else

@@ -36,7 +36,7 @@ hipError_t attend_packed(hipStream_t, const SeqTile* const* tiles, const int64_t
 hipError_t kv8_append(hipStream_t, const Kv8&, const SeqTile*, int, int, const uint16_t*, int64_t, const uint16_t*, int64_t) {
   return note("append");
 }
-hipError_t kv8_read(hipStream_t, const Kv8&, const SeqTile*, int64_t, int, uint16_t*, int64_t, uint16_t*, int64_t) {
+hipError_t kv8_read(hipStream_t, const Kv8&, const SeqTile*, int, int, uint16_t*, int64_t, uint16_t*, int64_t) {
   return note("read");
 }
 hipError_t kv8_advance(hipStream_t, const Kv8&, const SeqTile*, int) { return note("advance"); }
