@@ -127,13 +127,6 @@ k_attend_packed(PackedArgs A) {
   const int lim = T.t0 + min(tok, live - 1);
   const int h = kvh * A.group + chunk * A.hh + min(head, heads - 1);
 
-  // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
-  s16x8 qf[NS];
-  {
-    const uint16_t* qr = A.q + (int64_t)(T.row0 + lim) * A.ldq + (int64_t)h * HD + 8 * hi;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s);
-  }
   const int tiles = (T.t0 + live - 1) / PK + 1;
   const int minlim = T.t0 + (int)(wave * 32 * A.magic >> 16);     // the wave's first token
 
@@ -161,6 +154,17 @@ k_attend_packed(PackedArgs A) {
   auto dma_k = [&](int t) { dma(kbase, A.ldk, koff, t, smem + (t & 1) * STAGE); };
   auto dma_v = [&](int t) { dma(vbase, A.ldv, voff, t, smem + (2 + (t & 1)) * STAGE); };
 
+  dma_k(0);
+
+  // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
+  s16x8 qf[NS];
+  {
+    const uint16_t* qr = A.q + (int64_t)(T.row0 + lim) * A.ldq + (int64_t)h * HD + 8 * hi;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s);
+  }
+  dma_v(0);
+  if (tiles > 1) dma_k(1);
   // per-lane LDS offsets: K row 32b + lo, chunk 2s + hi; V key 16u + 8e + 4 hi + i / 4 (i the lane of
   // its 16), dims 32d + 16 (lane / 16 % 2) + 4 (i % 4) ..: u, e, b and the stage are immediates
   int kofs[NS], vofs[ND];
@@ -306,14 +310,14 @@ k_attend_packed(PackedArgs A) {
     asm volatile("" : "+v"(lrun));
   };
 
-  // prologue: K of tile 0, then S of tile 0 while V 0 and K 1 move
-  dma_k(0);
+  // S of tile 0 once its K has landed: V 0 and K 1, asked for after it (and after Q), still move
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((0x7 << 4) | (0x0 << 8));
+  if (tiles > 1)
+    __builtin_amdgcn_s_waitcnt(0xF70 | 2 * DI);
+  else
+    __builtin_amdgcn_s_waitcnt(0xF70 | DI);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  dma_v(0);
-  if (tiles > 1) dma_k(1);
   sc[0] = f32x16{};
   sc[1] = f32x16{};
 #pragma unroll
@@ -335,24 +339,30 @@ k_attend_packed(PackedArgs A) {
     step(S0(), Last(), t);
   }
 
+  // the wave's rows through its share of K's stages, which nobody reads in the last step, so that 16
+  // bytes a lane leave in whole rows: HD / 8 lanes a row
   const float inv = 1.f / psum32(lrun);
-  uint32_t bad = 0;
+  float zero = lrun * 0.f;   // not zero where a sum is not finite
+  uint8_t* mem = smem + wave * 32 * ROWB;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      o[d][r] *= inv;
-      bad |= (__float_as_uint(o[d][r]) & 0x7F800000u) == 0x7F800000u;
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const int c = 4 * d + r4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(o[d][4 * r4 + e], 0.f, zero);
+      *(u32x2*)(mem + lo * ROWB + ((c ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4) + 8 * hi) =
+          u32x2{pack16(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, A.obf),
+                pack16(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv, A.obf)};
     }
-  if (mine) {
-    uint16_t* po = A.out + (int64_t)(T.row0 + lim) * A.ldo + (int64_t)h * HD + 4 * hi;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4)
-        *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack16(o[d][4 * r4], o[d][4 * r4 + 1], A.obf),
-                                                pack16(o[d][4 * r4 + 2], o[d][4 * r4 + 3], A.obf)};
+  for (int i = 0; i < 32 / RI; ++i) {
+    const int r = i * RI + lane / CH, c = lane % CH, gr = wave * 32 + r, rt = (int)(gr * A.magic >> 16), rh = gr - rt * A.hh;
+    const u32x4 x = *(const u32x4*)(mem + r * ROWB + ((c ^ (HD == 128 ? r & 15 : (r >> 1) & 7)) << 4));
+    if (rt < live && rh < heads)
+      *(u32x4*)(A.out + (int64_t)(T.row0 + T.t0 + rt) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + rh) * HD + 8 * c) = x;
   }
+  const bool bad = !(zero == 0.f);
   uint64_t redo = __ballot(bad && mine);
   for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1) {
     const int r = wave * 32 + __builtin_ctz(rows), rt = (int)(r * A.magic >> 16);
