@@ -114,7 +114,7 @@ k_attend_packed(PackedArgs A) {
   // tile t+1 and V of tile t.  K rows: 16-byte chunk c at c ^ (row % 16) (HD 64: c ^ (row / 2 % 8)),
   // so that 32 rows' same chunk meets every bank once; V rows: c ^ 4 (row % 4) (HD 64: c ^ 4 (row / 2
   // % 2)), so that the transposing read's 4 rows of 64 bytes do.
-  __shared__ __align__(1024) uint8_t smem[4 * STAGE];
+  __shared__ __align__(1024) uint8_t smem[5 * STAGE];
   const int per = A.kv_heads * A.chunks;
   const SeqTile T = A.tiles[blockIdx.x / per];
   const int hc = blockIdx.x % per, kvh = hc % A.kv_heads, chunk = hc / A.kv_heads;
@@ -125,7 +125,6 @@ k_attend_packed(PackedArgs A) {
   const int row = wave * 32 + lo, tok = (int)(row * A.magic >> 16), head = row - tok * A.hh;
   const bool mine = tok < live && head < heads;
   const int lim = T.t0 + min(tok, live - 1);
-  const int h = kvh * A.group + chunk * A.hh + min(head, heads - 1);
 
   const int tiles = (T.t0 + live - 1) / PK + 1;
   const int minlim = T.t0 + (int)(wave * 32 * A.magic >> 16);     // the wave's first token
@@ -139,8 +138,8 @@ k_attend_packed(PackedArgs A) {
   for (int i = 0; i < DI; ++i) {
     const int r = (4 * i + wave) * RI + lane / CH, c = lane % CH;
     const int kc = HD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7), vc = HD == 128 ? c ^ (4 * (r & 3)) : c ^ (4 * ((r >> 1) & 1));
-    koff[i] = (uint32_t)(r * A.ldk + 8 * kc) * 2u;
-    voff[i] = (uint32_t)(r * A.ldv + 8 * vc) * 2u;
+    koff[i] = (r * (uint32_t)A.ldk + 8 * kc) * 2u;
+    voff[i] = (r * (uint32_t)A.ldv + 8 * vc) * 2u;
   }
   auto dma = [&](const uint16_t* base, int64_t ld, const uint32_t* off, int t, uint8_t* dst) {
     const int64_t ext = ((int64_t)(T.len - t * PK - 1) * ld + HD) * 2;
@@ -156,17 +155,23 @@ k_attend_packed(PackedArgs A) {
 
   dma_k(0);
 
-  // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
-  s16x8 qf[NS];
-  {
-    const uint16_t* qr = A.q + (int64_t)(T.row0 + lim) * A.ldq + (int64_t)h * HD + 8 * hi;
+  // The wave's rows of Q by DMA too, into V's stage 1 and the stage after it, which nobody needs yet:
+  // whole rows of memory at a time, where reading the operand's 16-byte pieces of 32 rows a load keeps
+  // the address unit busy several times as long.
+  uint8_t* qmem = smem + 3 * STAGE + wave * 32 * ROWB;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s);
+  for (int i = 0; i < 32 / RI; ++i) {
+    const int r = i * RI + lane / CH, gr = wave * 32 + r, rt = (int)(gr * A.magic >> 16);
+    const int c = lane % CH ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
+    const uint16_t* qr = A.q + (int64_t)(T.row0 + T.t0 + min(rt, live - 1)) * A.ldq +
+                         (int64_t)(kvh * A.group + chunk * A.hh + min(gr - rt * A.hh, heads - 1)) * HD + 8 * c;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)qr, (lds_void*)(qmem + i * 1024), 16, 0, 0);
   }
   dma_v(0);
   if (tiles > 1) dma_k(1);
   // per-lane LDS offsets: K row 32b + lo, chunk 2s + hi; V key 16u + 8e + 4 hi + i / 4 (i the lane of
-  // its 16), dims 32d + 16 (lane / 16 % 2) + 4 (i % 4) ..: u, e, b and the stage are immediates
+  // its 16), dims 32d + 16 (lane / 16 % 2) + 4 (i % 4) ..: u, e and b are immediates, the
+  // stage is toggled (one body for both keeps the accumulators in one place)
   int kofs[NS], vofs[ND];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
@@ -181,17 +186,16 @@ k_attend_packed(PackedArgs A) {
   }
   // S product i = 2s + b: K fragment of 32-key block b, k-step s; O product j = ND u + d: V^T
   // fragment of dims 32d .., keys 16u ..
-  auto kfrag = [&](auto st, int i) {
-    return *(const s16x8*)(smem + kofs[i / 2] + (decltype(st)::value * STAGE + (i % 2) * 32 * ROWB));
-  };
-  auto vfrag = [&](auto st, int j) {
+  auto kfrag = [&](int i) { return *(const s16x8*)(smem + kofs[i / 2] + (i % 2) * 32 * ROWB); };
+  auto vfrag = [&](int j) {
     typedef __attribute__((address_space(3))) s16x4 lds_s4;
-    uint8_t* p = smem + vofs[j % ND] + (decltype(st)::value * STAGE + (j / ND) * 16 * ROWB);
+    uint8_t* p = smem + vofs[j % ND] + (j / ND) * 16 * ROWB;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * ROWB));
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   };
 
+  s16x8 qf[NS];   // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
   f32x16 o[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x16{};
@@ -200,8 +204,7 @@ k_attend_packed(PackedArgs A) {
 
   // Step t: the softmax of tile t, the S product of tile t+1 interleaved with tile t's exp2, then
   // O^T += V^T P^T of tile t.
-  auto step = [&](auto st_c, auto last_c, int t) {
-    constexpr int ST = decltype(st_c)::value;
+  auto step = [&](auto last_c, int t) __attribute__((always_inline)) {
     constexpr bool LAST = decltype(last_c)::value;
     // K of tile t+1 and V of tile t have landed for every wave, and every wave is done with K of
     // tile t and V of tile t-1
@@ -266,19 +269,19 @@ k_attend_packed(PackedArgs A) {
       sn[0] = f32x16{};
       sn[1] = f32x16{};
 #pragma unroll
-      for (int i = 0; i < KD; ++i) kq[i] = kfrag(std::integral_constant<int, ST ^ 1>(), i);
+      for (int i = 0; i < KD; ++i) kq[i] = kfrag(i);
     }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       if constexpr (!LAST) {
         s16x8 kn = {};
-        if (i + KD < NI) kn = kfrag(std::integral_constant<int, ST ^ 1>(), i + KD);
+        if (i + KD < NI) kn = kfrag(i + KD);
         sn[i % 2] = mfma32<BF>(kq[0], qf[i / 2], sn[i % 2]);
 #pragma unroll
         for (int d = 0; d + 1 < KD; ++d) kq[d] = kq[d + 1];
         kq[KD - 1] = kn;
       }
-      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(std::integral_constant<int, ST>(), i - (NI - KD));
+      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(i - (NI - KD));
 #pragma unroll
       for (int e = 0; e < PS; ++e) {
         const int pi = PS * i + e, b = pi / 8, r = 2 * (pi % 8);
@@ -294,7 +297,7 @@ k_attend_packed(PackedArgs A) {
 #pragma unroll
     for (int j = 0; j < 4 * ND; ++j) {
       s16x8 vn = {};
-      if (j + KD < 4 * ND) vn = vfrag(std::integral_constant<int, ST>(), j + KD);
+      if (j + KD < 4 * ND) vn = vfrag(j + KD);
       const int u = j / ND;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
       o[j % ND] = mfma32<BF>(vq[0], pb, o[j % ND]);
@@ -318,43 +321,50 @@ k_attend_packed(PackedArgs A) {
     __builtin_amdgcn_s_waitcnt(0xF70 | DI);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qmem + kofs[s]);
   sc[0] = f32x16{};
   sc[1] = f32x16{};
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i) sc[i % 2] = mfma32<BF>(kfrag(std::integral_constant<int, 0>(), i), qf[i / 2], sc[i % 2]);
+  for (int i = 0; i < 2 * NS; ++i) {
+    sc[i % 2] = mfma32<BF>(kfrag(i), qf[i / 2], sc[i % 2]);
+    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+  }
 
-  typedef std::integral_constant<int, 0> S0;
-  typedef std::integral_constant<int, 1> S1;
-  typedef std::integral_constant<bool, false> More;
-  typedef std::integral_constant<bool, true> Last;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) kofs[s] ^= STAGE;
   int t = 0;
-  for (; t + 2 < tiles; t += 2) {
-    step(S0(), More(), t);
-    step(S1(), More(), t + 1);
+  for (; t + 1 < tiles; ++t) {
+    step(std::integral_constant<bool, false>(), t);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) kofs[s] ^= STAGE;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) vofs[d] ^= STAGE;
   }
-  if (t + 1 < tiles) {
-    step(S0(), More(), t);
-    step(S1(), Last(), t + 1);
-  } else {
-    step(S0(), Last(), t);
-  }
+  step(std::integral_constant<bool, true>(), t);
 
   // the wave's rows through its share of K's stages, which nobody reads in the last step, so that 16
   // bytes a lane leave in whole rows: HD / 8 lanes a row
   const float inv = 1.f / psum32(lrun);
-  float zero = lrun * 0.f;   // not zero where a sum is not finite
+  float zero[4] = {lrun * 0.f};   // not zero where a sum is not finite
   uint8_t* mem = smem + wave * 32 * ROWB;
+  auto leave = [&](auto obf) __attribute__((always_inline)) {
 #pragma unroll
-  for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int c = 4 * d + r4;
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int c = 4 * d + r4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(o[d][4 * r4 + e], 0.f, zero);
-      *(u32x2*)(mem + lo * ROWB + ((c ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4) + 8 * hi) =
-          u32x2{pack16(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, A.obf),
-                pack16(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv, A.obf)};
-    }
+        for (int e = 0; e < 4; ++e) zero[e] = __builtin_fmaf(o[d][4 * r4 + e], 0.f, zero[e]);
+        *(u32x2*)(mem + lo * ROWB + ((c ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4) + 8 * hi) =
+            u32x2{pack16(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, decltype(obf)::value),
+                  pack16(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv, decltype(obf)::value)};
+      }
+  };
+  if (A.obf)
+    leave(std::integral_constant<int, 1>());
+  else
+    leave(std::integral_constant<int, 0>());
 #pragma unroll
   for (int i = 0; i < 32 / RI; ++i) {
     const int r = i * RI + lane / CH, c = lane % CH, gr = wave * 32 + r, rt = (int)(gr * A.magic >> 16), rh = gr - rt * A.hh;
@@ -362,7 +372,7 @@ k_attend_packed(PackedArgs A) {
     if (rt < live && rh < heads)
       *(u32x4*)(A.out + (int64_t)(T.row0 + T.t0 + rt) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + rh) * HD + 8 * c) = x;
   }
-  const bool bad = !(zero == 0.f);
+  const bool bad = !(zero[0] + zero[1] + zero[2] + zero[3] == 0.f);
   uint64_t redo = __ballot(bad && mine);
   for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1) {
     const int r = wave * 32 + __builtin_ctz(rows), rt = (int)(r * A.magic >> 16);
