@@ -102,7 +102,7 @@ struct PackedArgs {
 
 // grid: tiles x chunks x kv_heads, the heads fastest; block 256
 template <int BF, int HD>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, HD == 64 ? 3 : 2)
 k_attend_packed(PackedArgs A) {
   constexpr int ROWB = HD * 2, STAGE = PK * ROWB;   // bytes of a key's row; of a tile
   constexpr int CH = HD / 8;                        // 16-byte chunks a row
