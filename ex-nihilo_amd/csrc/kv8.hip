@@ -280,6 +280,12 @@ __device__ __forceinline__ float sum_groups(float v) {
   return a + b;
 }
 
+// codes: a step of few rows reads each page once, past the caches
+template <int RT>
+__device__ __forceinline__ u32x4 kv8_load(const int8_t* p) {
+  return RT == 1 ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
+}
+
 struct Kv8Args {
   Kv8 c;
   const SeqTile* tiles;
@@ -291,14 +297,13 @@ struct Kv8Args {
   int tt, hh, chunks;     // tokens and heads a workgroup; workgroups a key/value head's group
   uint32_t magic;         // ceil(65536 / hh)
   int obf, splits;
+  int least;              // blocks a split has at least, where the keys are split
   float* part;            // [split][row][head][dim], then [split][row][head][2]: the sums, their reference and weight
   int64_t rows;
 };
-#define KV8_MIN 16   // blocks a split has at least, where the keys are split
-
 // the blocks of a sequence's NB that split I of S takes: [*lo, *hi); the number of splits with any
-__device__ __forceinline__ int kv8_split(int nb, int S, int i, int* lo, int* hi) {
-  const int per = max(KV8_MIN, (nb + S - 1) / S);
+__device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* lo, int* hi) {
+  const int per = max(least, (nb + S - 1) / S);
   *lo = min(nb, i * per);
   *hi = min(nb, (i + 1) * per);
   return (nb + per - 1) / per;
@@ -325,7 +330,7 @@ k_kv8_attend(Kv8Args A) {
   const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
   const int nb = (min(base + T.t0 + live, total) + 63) / 64;   // blocks that some row here sees
   int lo, hi;
-  const int active = max(1, kv8_split(nb, A.splits, blockIdx.y, &lo, &hi));
+  const int active = max(1, kv8_split(nb, A.splits, A.least, blockIdx.y, &lo, &hi));
   if ((int)blockIdx.y >= active) return;
 
   int lim[RT];
@@ -406,12 +411,12 @@ k_kv8_attend(Kv8Args A) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int e = 0; e < KL; ++e) kr[t][e] = *(const u32x4*)(p + (key0 + 4 * t) * HD + 16 * g + 64 * e);
+      for (int e = 0; e < KL; ++e) kr[t][e] = kv8_load<RT>(p + (key0 + 4 * t) * HD + 16 * g + 64 * e);
   };
   auto load_v = [&](int page) {
     const int8_t* p = c.v + ((int64_t)max(page, 0) * c.kv_heads + kvh) * 64 * HD;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) vr[d] = *(const u32x4*)(p + (16 * d + col) * 64 + 16 * g);
+    for (int d = 0; d < ND; ++d) vr[d] = kv8_load<RT>(p + (16 * d + col) * 64 + 16 * g);
   };
   if (its > 0) {
     look(0);
@@ -596,30 +601,459 @@ k_kv8_attend(Kv8Args A) {
   }
 }
 
-// The splits' sums of one row and head (a workgroup), in a fixed order: 256 / (HD / 4) shares of the
-// splits, then the shares.  Rows whose keys were not split are done.
-template <int HD>
+// --- many rows: 128 a workgroup -------------------------------------------------------------------
+//
+// packed.hip's arrangement (32 rows a wave, S^T = K Q^T, O^T += V^T P^T, the S product of the next
+// block interleaved with this one's exp2), with each block's codes made 16 bits on the way into LDS: a
+// wave converts a quarter of a block for all four, 96 VALU instructions of about 300 a block, and the
+// next codes are asked for a block ahead.  Codes are whole numbers: K's scale goes into the scores'
+// factor, V's into the weights' exponent, p vd 2^-E with E the largest exponent of a scale so far, so that
+// fp16 weights of blocks of small values keep their bits; a block's sum of them times 1 / (vd 2^-E) is
+// its share of the row's weight.
+typedef __attribute__((address_space(3))) void lds_void;
+template <int BF>
+__device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// SUM plus a pair of weights as the second product takes them
+template <int BF>
+__device__ __forceinline__ float weight_sum(uint32_t pair, float sum) {
+  if constexpr (BF)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
+}
+
+// One row by a whole wave, blocks [lo, hi), nothing that it does not see multiplied: for rows whose
+// sums came out not finite (a hidden value of the tail that is not, times a weight of zero)
+template <int BF, int HD>
+__device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int total, int lim, const uint16_t* q,
+                        float scale, float* m_, float* l_, float* o) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY, l = 0.f;
+  for (int e = 0; e < HD / 64; ++e) o[e] = 0.f;
+#pragma unroll 1
+  for (int b = lo; b < hi && b * 64 <= lim; ++b) {
+    const bool full = b * 64 + 64 <= total;
+    const int64_t page = full ? kv8_page(c, seq, b) : 0;
+    if (page < 0) continue;
+    const int64_t ph = (page * c.kv_heads + kvh), th = ((int64_t)seq * c.kv_heads + kvh) * 64 * HD;
+    const float kd = full ? c.scales[ph * 2] : 1.f, vd = full ? c.scales[ph * 2 + 1] : 1.f;
+    float s = -INFINITY;
+    if (b * 64 + lane <= lim) {
+      s = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < HD; ++d)
+        s += ld16(q + d, BF) * (full ? (float)c.k[ph * 64 * HD + lane * HD + d] : ld16(c.tk + th + lane * HD + d, BF));
+      s *= scale * kd;
+    }
+    const float mn = fmaxf(m, wave_max(s)), mu = mn == -INFINITY ? 0.f : mn;
+    const float a = exp2f(m - mu), p = exp2f(s - mu);
+    l = l * a + wave_sum(p);
+    m = mn;
+    for (int e = 0; e < HD / 64; ++e) o[e] *= a;
+#pragma unroll 1
+    for (int j = 0; j < 64 && b * 64 + j <= lim; ++j) {
+      const float pj = __shfl(p, j, 64);
+      for (int e = 0; e < HD / 64; ++e) {
+        const int d = e * 64 + lane;
+        o[e] += pj * (full ? (float)c.v[ph * 64 * HD + d * 64 + j] * vd : ld16(c.tv + th + j * HD + d, BF));
+      }
+    }
+  }
+  *m_ = m;
+  *l_ = l;
+}
+
+template <int BF, int HD>
+__global__ void __launch_bounds__(256, 2)
+k_kv8_chunk(Kv8Args A) {
+  constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
+  constexpr int NS = HD / 16, ND = HD / 32;
+  constexpr int CI = HD / 64;                       // 16-byte loads of codes a thread and block
+  // K stage s at s STAGE: rows of keys, 16-byte chunk c at c ^ (key % 16) (HD 64: c ^ (key / 2 % 8)).
+  // V^T stage s at (2 + s) STAGE: rows of dims of 128 bytes, chunk c at c ^ (dim / 2 % 8); a row's
+  // keys in vt_pos's order, the one in which a lane's weights lie.
+  __shared__ __align__(1024) uint8_t smem[4 * STAGE];
+  const Kv8& c = A.c;
+  const int per = c.kv_heads * A.chunks;
+  const SeqTile T = A.tiles[blockIdx.x / per];
+  const int hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, lo = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len), nfull = total / 64;
+  const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
+  int b0, b1;   // the blocks taken here
+  const int active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, blockIdx.y, &b0, &b1));
+  if ((int)blockIdx.y >= active) return;
+  const int row = wave * 32 + lo, tok = (int)(row * A.magic >> 16), head = row - tok * A.hh;
+  const bool mine = tok < live && head < heads;
+  const int ctok = min(tok, live - 1), chead = kvh * A.group + chunk * A.hh + min(head, heads - 1);
+  const int lim = min(base + T.t0 + ctok, total - 1);
+  const int minlim = min(base + T.t0 + min((int)(wave * 32 * A.magic >> 16), live - 1), total - 1);
+  const uint16_t* qr = A.q + (int64_t)(T.row0 + T.t0 + ctok) * A.ldq + (int64_t)chead * HD;
+  s16x8 qf[NS];   // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s + 8 * hi);
+
+  // 64 blocks' pages and scales from block B on, a lane each
+  int pages = 0;
+  float kds = 1.f, vds = 1.f;
+  auto look = [&](int b) __attribute__((always_inline)) {
+    int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, T.seq, b + lane) : -1;
+    pages = (int)p;
+    p = p < 0 ? 0 : p;
+    const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
+    kds = b + lane < nfull ? d[0] : 1.f;
+    vds = b + lane < nfull ? d[1] : 1.f;
+  };
+  // a block's page and scales: the looked-up 64 are replaced once its last is asked for by FETCH, three
+  // blocks ahead of its use, so each block's facts ride along
+  struct Facts {
+    int page;
+    float kd, vd;
+  };
+  auto facts = [&](int b) __attribute__((always_inline)) {
+    const int i = (b - b0) & 63;
+    if (i == 0) look(b);
+    return Facts{__builtin_amdgcn_readlane(pages, i), __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kds), i)),
+                 __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vds), i))};
+  };
+  struct Codes {
+    u32x4 w[CI];
+  };
+  auto fetch = [&](const int8_t* all, int page) __attribute__((always_inline)) {
+    const int8_t* p = all + ((int64_t)max(page, 0) * c.kv_heads + kvh) * 64 * HD;
+    Codes x;
+#pragma unroll
+    for (int i = 0; i < CI; ++i) x.w[i] = *(const u32x4*)(p + (tid + 256 * i) * 16);
+    return x;
+  };
+  const int64_t th = ((int64_t)T.seq * c.kv_heads + kvh) * 64 * HD;
+  // block B's K (codes in KC, or the tail's rows; those past its last token as zeros) into a stage
+  auto fill_k = [&](int b, int st, const Codes& x) __attribute__((always_inline)) {
+    uint8_t* p = smem + st * STAGE;
+    if (b < nfull) {
+#pragma unroll
+      for (int i = 0; i < CI; ++i) {
+        const int ci = tid + 256 * i, key = ci / (HD / 16), c2 = ci % (HD / 16) * 2;
+        const int z = HD == 128 ? key & 15 : (key >> 1) & 7;
+        *(s16x8*)(p + key * ROWB + ((c2 ^ z) << 4)) = codes8<BF>(x.w[i][0], x.w[i][1]);
+        *(s16x8*)(p + key * ROWB + (((c2 + 1) ^ z) << 4)) = codes8<BF>(x.w[i][2], x.w[i][3]);
+      }
+    } else {
+      for (int ci = tid; ci < 64 * HD / 8; ci += 256) {
+        const int key = ci / (HD / 8), cc = ci % (HD / 8), z = HD == 128 ? key & 15 : (key >> 1) & 7;
+        u32x4 w = {};
+        if (b * 64 + key < total) w = *(const u32x4*)(c.tk + th + ci * 8);
+        *(u32x4*)(p + key * ROWB + ((cc ^ z) << 4)) = w;
+      }
+    }
+  };
+  auto fill_v = [&](int b, int st, const Codes& x) __attribute__((always_inline)) {
+    uint8_t* p = smem + (2 + st) * STAGE;
+    if (b < nfull) {
+#pragma unroll
+      for (int i = 0; i < CI; ++i) {
+        const int ci = tid + 256 * i, dim = ci >> 2, c2 = 2 * (ci & 3), z = (dim >> 1) & 7;
+        *(s16x8*)(p + dim * 128 + ((c2 ^ z) << 4)) = codes8<BF>(x.w[i][0], x.w[i][2]);
+        *(s16x8*)(p + dim * 128 + (((c2 + 1) ^ z) << 4)) = codes8<BF>(x.w[i][1], x.w[i][3]);
+      }
+    } else {
+      for (int ci = tid; ci < 64 * HD / 8; ci += 256) {
+        const int key = ci / (HD / 8), d0 = ci % (HD / 8) * 8, pos = (int)vt_pos(key);
+        u32x4 w = {};
+        if (b * 64 + key < total) w = *(const u32x4*)(c.tv + th + ci * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *(uint16_t*)(p + (d0 + e) * 128 + (((pos >> 3) ^ ((d0 + e) >> 1 & 7)) << 4) + (pos & 7) * 2) =
+              (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+      }
+    }
+  };
+  int kofs[NS], vofs[4];   // K row lo, chunk 2s + hi; V^T row lo, chunk 2u + hi
+#pragma unroll
+  for (int s = 0; s < NS; ++s) kofs[s] = lo * ROWB + (((2 * s + hi) ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) vofs[u] = 2 * STAGE + lo * 128 + (((2 * u + hi) ^ ((lo >> 1) & 7)) << 4);
+  auto kfrag = [&](int i) { return *(const s16x8*)(smem + kofs[i / 2] + (i % 2) * 32 * ROWB); };
+  auto vfrag = [&](int j) { return *(const s16x8*)(smem + vofs[j / ND] + (j % ND) * 32 * 128); };
+
+  f32x16 o[ND], sc[2];
+  float mrun = 0.f, lrun = 0.f;
+  bool set = false;          // the row has a reference
+  int top = -1000;           // E: the sums are in units of 2^E
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f32x16{};
+  auto barrier = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+
+  // Block B of facts F: its softmax, the S product of block b+1 interleaved with its exp2, O^T += V^T P^T
+  auto step = [&](auto last_c, int b, const Facts& F) __attribute__((always_inline)) {
+    constexpr bool LAST = decltype(last_c)::value;
+    const int k0 = b * 64;
+    const float factor = F.kd * A.scale;
+    const bool gone = F.page < 0 && b < nfull;
+    // V's scale, in units of 2^E and not under 2^-100 of them, goes into the weights' exponent; a row
+    // that sees nothing of the block takes nothing of it, NaN or not
+    const int e = (int)((__float_as_uint(F.vd) >> 23) & 0xFF) - 127;
+    if (e > top && e < 128) {
+      const float f = top == -1000 ? 1.f : __builtin_ldexpf(1.f, top - e);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+      top = e;
+    }
+    const float vd = __builtin_ldexpf(F.vd, top == -1000 ? 0 : -top);
+    const float lv = gone || k0 > lim || F.vd == 0.f ? 0.f : __builtin_amdgcn_logf(vd < 0x1p-100f ? 0x1p-100f : vd);
+    const float from = lv - mrun;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[h][r] = __builtin_fmaf(sc[h][r], factor, from);
+    if (gone || k0 + 63 > minlim) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = k0 + 32 * h + 8 * (r >> 2) + 4 * hi + (r & 3);
+          if (gone || key > lim) sc[h][r] = -INFINITY;
+        }
+    }
+    float m4[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int h = q / 2, r0 = (q % 2) * 8;
+      float m = max3(sc[h][r0], sc[h][r0 + 1], sc[h][r0 + 2]);
+      m = max3(m, sc[h][r0 + 3], sc[h][r0 + 4]);
+      m = max3(m, sc[h][r0 + 5], sc[h][r0 + 6]);
+      m4[q] = fmaxf(m, sc[h][r0 + 7]);
+    }
+    float ma = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), mb = ma;
+    xswap32(ma, mb);
+    const float mx = fmaxf(ma, mb) - lv;
+    const bool move = set ? mx > MAX_SLACK : mx > -INFINITY;
+    if (__ballot(move)) {
+      const float shift = move ? mx : 0.f;
+      const float alpha = set ? __builtin_amdgcn_exp2f(-shift) : 1.f;   // without a reference the sums are 0, or NaN
+      lrun *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      mrun += shift;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[h][r] -= shift;
+      set = set || move;
+    }
+    constexpr int KD = 3, NI = 2 * NS, PS = 16 / NI;
+    f32x16 sn[2];
+    uint32_t pk[16];
+    float ls[2] = {};
+    s16x8 kq[KD], vq[KD];
+    if constexpr (!LAST) {
+      sn[0] = f32x16{};
+      sn[1] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < KD; ++i) kq[i] = kfrag(i);
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if constexpr (!LAST) {
+        s16x8 kn = {};
+        if (i + KD < NI) kn = kfrag(i + KD);
+        sn[i % 2] = mfma32<BF>(kq[0], qf[i / 2], sn[i % 2]);
+#pragma unroll
+        for (int d = 0; d + 1 < KD; ++d) kq[d] = kq[d + 1];
+        kq[KD - 1] = kn;
+      }
+      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(i - (NI - KD));
+#pragma unroll
+      for (int z = 0; z < PS; ++z) {
+        const int pi = PS * i + z, h = pi / 8, r = 2 * (pi % 8);
+        const float p0 = __builtin_amdgcn_exp2f(sc[h][r]), p1 = __builtin_amdgcn_exp2f(sc[h][r + 1]);
+        pk[pi] = BF ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+        ls[pi % 2] = weight_sum<BF>(pk[pi], ls[pi % 2]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    lrun = __builtin_fmaf(ls[0] + ls[1], __builtin_amdgcn_exp2f(-lv), lrun);
+    if (F.vd == 0.f) {   // whatever the codes, the values are 0
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pk[i] = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4 * ND; ++j) {
+      s16x8 vn = {};
+      if (j + KD < 4 * ND) vn = vfrag(j + KD);
+      const int u = j / ND;
+      const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
+      o[j % ND] = mfma32<BF>(vq[0], pb, o[j % ND]);
+#pragma unroll
+      for (int d = 0; d + 1 < KD; ++d) vq[d] = vq[d + 1];
+      vq[KD - 1] = vn;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!LAST) {
+      sc[0] = sn[0];
+      sc[1] = sn[1];
+    }
+    asm volatile("" : "+v"(lrun));
+  };
+
+  // block b's K is filled two steps ahead of its softmax, its V one; codes are asked for one step
+  // before they are filled
+  Facts F0 = facts(b0), F1 = F0, F2 = F0;
+  Codes kc = fetch(c.k, F0.page), vc = fetch(c.v, F0.page), kn = kc;
+  if (b0 + 1 < b1) {
+    F1 = facts(b0 + 1);
+    kn = fetch(c.k, F1.page);
+  }
+  fill_k(b0, 0, kc);
+  barrier();
+  sc[0] = f32x16{};
+  sc[1] = f32x16{};
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i) {
+    sc[i % 2] = mfma32<BF>(kfrag(i), qf[i / 2], sc[i % 2]);
+    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+  }
+  fill_v(b0, 0, vc);
+  if (b0 + 1 < b1) {
+    vc = fetch(c.v, F1.page);
+    if (b0 + 2 < b1) {
+      F2 = facts(b0 + 2);
+      kc = fetch(c.k, F2.page);
+    }
+    fill_k(b0 + 1, 1, kn);
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) kofs[s] ^= STAGE;
+  int b = b0;
+  for (; b + 1 < b1; ++b) {
+    barrier();   // K of block b+1 and V of block b are filled; K of b and V of b-1 are done with
+    fill_v(b + 1, (b + 1 - b0) & 1, vc);
+    if (b + 2 < b1) {
+      fill_k(b + 2, (b - b0) & 1, kc);
+      vc = fetch(c.v, F2.page);
+    }
+    Facts F3 = F2;
+    if (b + 3 < b1) {
+      F3 = facts(b + 3);
+      kc = fetch(c.k, F3.page);
+    }
+    step(std::integral_constant<bool, false>(), b, F0);
+    F0 = F1;
+    F1 = F2;
+    F2 = F3;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) kofs[s] ^= STAGE;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) vofs[u] ^= STAGE;
+  }
+  barrier();
+  step(std::integral_constant<bool, true>(), b, F0);
+
+  float la = lrun, lb = lrun;
+  xswap32(la, lb);
+  const float sum = la + lb, unit = top == -1000 ? 1.f : __builtin_ldexpf(1.f, top);
+  const float mul = active > 1 ? unit : sum == 0.f ? 0.f : unit / sum;
+  float zero[4] = {sum * 0.f};
+  const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = A.rows * A.heads;
+  auto leave = [&](auto obf) __attribute__((always_inline)) {
+    uint16_t* po = A.out + (int64_t)(T.row0 + T.t0 + tok) * A.ldo + (int64_t)chead * HD + 4 * hi;
+    float* pp = A.part + ((int64_t)blockIdx.y * n + rowhead) * HD + 4 * hi;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        float y[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          zero[z] = __builtin_fmaf(o[d][4 * r4 + z], 0.f, zero[z]);
+          y[z] = o[d][4 * r4 + z] * mul;
+        }
+        if (!mine) continue;
+        if constexpr (decltype(obf)::value == 2)
+          *(f32x4*)(pp + 32 * d + 8 * r4) = f32x4{y[0], y[1], y[2], y[3]};
+        else if constexpr (decltype(obf)::value == 1)
+          *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        else
+          *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3])};
+      }
+  };
+  if (active > 1) {
+    leave(std::integral_constant<int, 2>());
+    if (mine && hi == 0)
+      *(f32x2*)(A.part + A.splits * n * HD + ((int64_t)blockIdx.y * n + rowhead) * 2) = f32x2{set ? mrun : -INFINITY, sum};
+  } else if (A.obf) {
+    leave(std::integral_constant<int, 1>());
+  } else {
+    leave(std::integral_constant<int, 0>());
+  }
+  const uint64_t redo = __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.f) && mine);
+#pragma unroll 1
+  for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1) {
+    const int r = wave * 32 + __builtin_ctz(rows), rt = (int)(r * A.magic >> 16);
+    const int64_t rh = kvh * A.group + chunk * A.hh + r - rt * A.hh, at = T.row0 + T.t0 + rt;
+    float m, l, y[HD / 64];
+    kv8_row<BF, HD>(c, T.seq, kvh, b0, b1, total, min(base + T.t0 + rt, total - 1), A.q + at * A.ldq + rh * HD, A.scale, &m, &l, y);
+    const int64_t slot = (int64_t)blockIdx.y * n + at * A.heads + rh;
+    for (int z = 0; z < HD / 64; ++z) {
+      const float w = active > 1 ? y[z] : l == 0.f ? 0.f : y[z] / l;
+      if (active > 1)
+        A.part[slot * HD + z * 64 + lane] = w;
+      else
+        A.out[at * A.ldo + rh * HD + z * 64 + lane] = (uint16_t)(A.obf ? pack_bf16x2(w, 0.f) : pack_f16x2(w, 0.f));
+    }
+    if (active > 1 && lane == 0) *(f32x2*)(A.part + A.splits * n * HD + slot * 2) = f32x2{m, l};
+  }
+}
+
+// The splits' sums of each row and head, in a fixed order: HD / 4 threads take one's dims in each of SH
+// shares of the splits (all 256 threads of a workgroup for few rows and many splits, SH 1 for many rows),
+// then the shares are summed.  Rows whose keys were not split are done.
+template <int HD, int SH>
 __global__ void __launch_bounds__(256)
 k_kv8_join(Kv8Args A) {
-  constexpr int TH = HD / 4, SH = 256 / TH;   // threads a share; shares
-  __shared__ __align__(16) float ys[SH][HD];
-  __shared__ float ss[SH], ms[4];
+  constexpr int TH = HD / 4, RW = 256 / TH / SH;   // threads a row and share; rows a workgroup
+  __shared__ __align__(16) float ys[256 / TH][HD];
+  __shared__ float ss[256 / TH], ms[256 / TH];
   const Kv8& c = A.c;
   const SeqTile T = A.tiles[blockIdx.x];
   const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len);
   const int live = min(A.tt, T.len - T.t0);
   int lo, hi;
-  const int active = kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, 0, &lo, &hi);
-  if (active < 2 || (int)blockIdx.y >= live * A.heads) return;
-  const int tid = threadIdx.x, sh = tid / TH, d = tid % TH * 4;
-  const int64_t rowhead = (int64_t)(T.row0 + T.t0) * A.heads + blockIdx.y, n = A.rows * A.heads;
+  const int active = kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, 0, &lo, &hi);
+  if (active < 2 || (int)blockIdx.y * RW >= live * A.heads) return;
+  const int tid = threadIdx.x, sh = tid / TH % SH, r = tid / TH / SH, d = tid % TH * 4;
+  const int i = min((int)blockIdx.y * RW + r, live * A.heads - 1);
+  const int64_t rowhead = (int64_t)(T.row0 + T.t0) * A.heads + i, n = A.rows * A.heads;
   const float* ml = A.part + A.splits * n * HD + rowhead * 2;
   float m = -INFINITY;
-  for (int z = tid; z < active; z += 256) m = fmaxf(m, ml[z * n * 2]);
-  m = wave_max(m);
-  if (tid % 64 == 0) ms[tid / 64] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+  for (int z = sh; z < active; z += SH) m = fmaxf(m, ml[z * n * 2]);
+  if constexpr (SH > 1) {
+    if (d == 0) ms[tid / TH] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SH; ++k) m = fmaxf(m, ms[r * SH + k]);
+  }
   float sum = 0.f;
   f32x4 y = {};
 #pragma unroll 4
@@ -630,15 +1064,18 @@ k_kv8_join(Kv8Args A) {
     sum += p[0] == -INFINITY ? p[1] : w * p[1];   // no reference: 0, or NaN
     if (w > 0.f) y += w * x;
   }
-  *(f32x4*)&ys[sh][d] = y;
-  if (d == 0) ss[sh] = sum;
-  __syncthreads();
-  if (sh) return;
+  if constexpr (SH > 1) {
+    *(f32x4*)&ys[tid / TH][d] = y;
+    if (d == 0) ss[tid / TH] = sum;
+    __syncthreads();
+    if (sh) return;
 #pragma unroll
-  for (int k = 1; k < SH; ++k) {
-    y += *(const f32x4*)&ys[k][d];
-    sum += ss[k];
+    for (int k = 1; k < SH; ++k) {
+      y += *(const f32x4*)&ys[r * SH + k][d];
+      sum += ss[r * SH + k];
+    }
   }
+  if ((int)blockIdx.y * RW + r >= live * A.heads) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* po = A.out + (rowhead / A.heads) * A.ldo + (rowhead % A.heads) * HD + d;
   *(u32x2*)po = A.obf ? u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)}
@@ -648,7 +1085,9 @@ k_kv8_join(Kv8Args A) {
 namespace {
 
 struct Kv8Way {
-  int rt, z, hh, chunks, splits;   // row tiles a workgroup; the tiles' list; heads a workgroup, workgroups a group; splits
+  int rt;                  // row tiles of 16 a workgroup (1 or 2), or 0: k_kv8_chunk's 128 rows
+  int z, hh, chunks;       // the tiles' list; heads a workgroup, workgroups a group
+  int splits, least;
 };
 Kv8Way kv8_way(int longest, int heads, int kv_heads, int head_dim, int cols, const int64_t* ntiles) {
   Kv8Way w;
@@ -658,15 +1097,16 @@ Kv8Way kv8_way(int longest, int heads, int kv_heads, int head_dim, int cols, con
   if (longest * w.hh <= 32) {
     w.rt = longest * w.hh <= 16 ? 1 : 2;
     while ((SEQ_TT0 << w.z) < longest) ++w.z;
+    w.least = 32;
   } else {
-    w.rt = head_dim == 128 ? 2 : 4;
-    const int most = 16 * w.rt / SEQ_TT0;
-    w.hh = group < most ? group : most;
-    while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 16 * w.rt) ++w.z;
+    w.rt = 0;
+    w.hh = group < 8 ? group : 8;
+    while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
+    w.least = 2;
   }
   w.chunks = (group + w.hh - 1) / w.hh;
-  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, s = groups > 0 ? 4096 / groups : 1;
-  const int64_t most = (cols + KV8_MIN - 1) / KV8_MIN;
+  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, s = groups > 0 ? (w.rt ? 4096 : 512) / groups : 1;
+  const int64_t most = (cols + w.least - 1) / w.least;
   w.splits = (int)(s < 1 ? 1 : s > most ? most : s);
   return w;
 }
@@ -701,6 +1141,7 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   a.magic = (65536 + w.hh - 1) / w.hh;
   a.obf = obf;
   a.splits = w.splits;
+  a.least = w.least;
   a.part = part;
   a.rows = rows;
   const int64_t groups = ntiles[w.z] * w.chunks * c.kv_heads;
@@ -709,9 +1150,7 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-    if constexpr (HD == 64)
-      if (w.rt == 4) return go(k_kv8_attend<BF, HD, 4>);
-    w.rt == 1 ? go(k_kv8_attend<BF, HD, 1>) : go(k_kv8_attend<BF, HD, 2>);
+    w.rt == 0 ? go(k_kv8_chunk<BF, HD>) : w.rt == 1 ? go(k_kv8_attend<BF, HD, 1>) : go(k_kv8_attend<BF, HD, 2>);
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
@@ -723,11 +1162,15 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
     c.bf16 ? rts(I1(), I64()) : rts(I0(), I64());
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.splits < 2) return e;
-  const dim3 jg((unsigned)ntiles[w.z], (a.tt < longest ? a.tt : longest) * heads);
+  const int th = c.head_dim / 4, most = (a.tt < longest ? a.tt : longest) * heads;   // a tile's rows and heads
+  const bool few = w.splits > 4;
+  const int each = few ? 1 : 256 / th;
+  const dim3 jg((unsigned)ntiles[w.z], (most + each - 1) / each);
+  auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jg, dim3(256), 0, s, a); };
   if (c.head_dim == 128)
-    hipLaunchKernelGGL(k_kv8_join<128>, jg, dim3(256), 0, s, a);
+    few ? join(k_kv8_join<128, 8>) : join(k_kv8_join<128, 1>);
   else
-    hipLaunchKernelGGL(k_kv8_join<64>, jg, dim3(256), 0, s, a);
+    few ? join(k_kv8_join<64, 16>) : join(k_kv8_join<64, 1>);
   return hipGetLastError();
 }
 
