@@ -235,6 +235,7 @@ hipError_t kv8_advance(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n) 
 // --- attention over the cache --------------------------------------------------------------------
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // four int8 codes as fp16: each byte, its sign bit flipped, under 0x64 is 1024 + 128 + code; as
@@ -247,6 +248,7 @@ __device__ __forceinline__ u32x2 codes_f16(uint32_t w) {
   return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 __device__ __forceinline__ u32x2 codes_bf16(uint32_t w) {
+  asm("" : "+v"(w));   // taken apart here: not byte by byte where it was loaded, in four registers
   float f[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w >> (8 * e));
@@ -280,15 +282,10 @@ __device__ __forceinline__ float sum_groups(float v) {
   return a + b;
 }
 
-// codes: a step of few rows reads each page once, past the caches
-template <int RT>
-__device__ __forceinline__ u32x4 kv8_load(const int8_t* p) {
-  return RT == 1 ? __builtin_nontemporal_load((const u32x4*)p) : *(const u32x4*)p;
-}
-
 struct Kv8Args {
   Kv8 c;
   const SeqTile* tiles;
+  int ntiles;
   const uint16_t* q;
   uint16_t* out;
   int64_t ldq, ldo;
@@ -296,12 +293,18 @@ struct Kv8Args {
   int heads, group;
   int tt, hh, chunks;     // tokens and heads a workgroup; workgroups a key/value head's group
   uint32_t magic;         // ceil(65536 / hh)
-  int obf, splits;
-  int least;              // blocks a split has at least, where the keys are split
-  float* part;            // [split][row][head][dim], then [split][row][head][2]: the sums, their reference and weight
+  int obf;
+  // k_kv8_few: workgroups that share the sequences' blocks evenly, 0: one a sequence.
+  // k_kv8_chunk: splits of each tile's blocks
+  int splits;
+  int least;              // blocks a workgroup takes at least, where they are shared or split
+  // k_kv8_few: [workgroup and head][2][16 RT rows][dim], then [..][2][16 RT rows][2]; k_kv8_chunk: [split][row][head][dim],
+  // then [split][row][head][2]: the sums, their reference and weight
+  float* part;
   int64_t rows;
 };
-// the blocks of a sequence's NB that split I of S takes: [*lo, *hi); the number of splits with any
+
+// the blocks of a tile's NB that split I of S takes: [*lo, *hi); the number of splits with any
 __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* lo, int* hi) {
   const int per = max(least, (nb + S - 1) / S);
   *lo = min(nb, i * per);
@@ -309,96 +312,110 @@ __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* l
   return (nb + per - 1) / per;
 }
 
+// a sequence's blocks after its new tokens
+__device__ __forceinline__ int kv8_blocks(const Kv8& c, const SeqTile& t) {
+  return (kv8_total(c, kv8_base(c, t.seq), t.len) + 63) >> 6;
+}
+// by a wave: the blocks of tiles 0 .. n-1; *FIRST, if not null, where tile I's begin
+__device__ __forceinline__ int kv8_sum_blocks(const Kv8Args& A, int n, int i, int* first) {
+  const int lane = threadIdx.x & 63;
+  int all = 0, before = 0;
+  for (int t = lane; t < n; t += 64) {
+    const int nb = kv8_blocks(A.c, A.tiles[t]);
+    all += nb;
+    before += t < i ? nb : 0;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    all += __shfl_xor(all, o, 64);
+    before += __shfl_xor(before, o, 64);
+  }
+  if (first) *first = before;
+  return all;
+}
+
 #define MAX_SLACK 8.f
 
-// grid: splits x (tiles x chunks x kv_heads, the heads fastest); block 256.  RT row tiles of 16.
-template <int BF, int HD, int RT>
-__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
-k_kv8_attend(Kv8Args A) {
+// --- few rows ------------------------------------------------------------------------------------
+//
+// The cache's bytes are the cost.  A key/value head's blocks of all sequences, one after the other, are
+// shared evenly by the workgroups of that head, however long each sequence is: the loop reads at the
+// memory's rate, and what a workgroup takes to begin (four loads that wait for each other, microseconds
+// next to that many reads) and to end is paid once.  A workgroup whose share ends within a sequence
+// leaves its sums to k_kv8_join_few.  Waves take a sequence's blocks in turn, each with sums of its own,
+// which meet in LDS.  RT row tiles of 16 (rows: tokens times a group's heads).
+//
+// Grid: workgroups x kv_heads x chunks, the heads fastest; WV waves.
+template <int BF, int HD, int RT, int WV>
+__global__ void __launch_bounds__(64 * WV, RT == 1 ? 2 : 1)
+k_kv8_few(Kv8Args A) {
   constexpr int NS = HD / 32, ND = HD / 16;   // k-steps of a score; 16-dim tiles of O
   constexpr int KL = HD / 64;                 // 16-byte loads a lane, key tile and block of K
-  constexpr int LD = HD + 4;
-  __shared__ __align__(16) float obuf[4][16][LD];     // the waves' sums; the tail's V (64 rows of 16 bits) before that
-  __shared__ float mbuf[4][16], lbuf[4][16], pbuf[64][17];
+  constexpr int LD = HD + 4, ROWB = HD * 2, CH = HD / 8;
+  __shared__ __align__(16) float obuf[WV][16][LD];
+  __shared__ __align__(1024) uint8_t tbuf[2][64 * ROWB];   // the tail's K and V
+  __shared__ float mbuf[WV][16], lbuf[WV][16], pbuf[64][17];
   const Kv8& c = A.c;
   const int per = c.kv_heads * A.chunks;
-  const SeqTile T = A.tiles[blockIdx.x / per];
-  const int hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
+  const int w = blockIdx.x / per, hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len), nfull = total / 64;
-  const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
-  const int nb = (min(base + T.t0 + live, total) + 63) / 64;   // blocks that some row here sees
-  int lo, hi;
-  const int active = max(1, kv8_split(nb, A.splits, A.least, blockIdx.y, &lo, &hi));
-  if ((int)blockIdx.y >= active) return;
-
-  int lim[RT];
-  s16x8 qf[RT][NS];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = rt * 16 + col, tok = min((int)(r * A.magic >> 16), live - 1);
-    const int head = min(r - (int)(r * A.magic >> 16) * A.hh, heads - 1);
-    lim[rt] = min(base + T.t0 + tok, total - 1);
-    // dims of k-step s: 16 g + 8 (s % 2) + 64 (s / 2) .., as the 16 bytes of codes a lane loads
-    const uint16_t* qr = A.q + (int64_t)(T.row0 + T.t0 + tok) * A.ldq +
-                         (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) qf[rt][s] = *(const s16x8*)(qr + 8 * (s % 2) + 64 * (s / 2));
-  }
-  f32x4 o[RT][ND];
-  float mrun[RT], lrun[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{};
-    mrun[rt] = -INFINITY;
-    lrun[rt] = 0.f;
-  }
-  float s[RT][16];   // scores of keys 16 g + e of the block in hand
-  uint32_t pk[RT][8];
-
-  // from scores (log2 units, hidden ones -inf) to weights: the rows' references, sums and pk
-  auto weights = [&](int bf) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float mx = s[rt][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[rt][e]);
-      mx = max_groups(mx);
-      // a first reference (any above -inf), or one that has fallen behind
-      if (__ballot(mx > mrun[rt] + MAX_SLACK)) {
-        const float mn = mx > mrun[rt] + MAX_SLACK ? mx : mrun[rt];
-        const float a = mn == mrun[rt] ? 1.f : __builtin_amdgcn_exp2f(mrun[rt] - mn);
-        mrun[rt] = mn;
-        lrun[rt] *= a;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[rt][d] *= a;
-      }
-      const float ref = mrun[rt] == -INFINITY ? 0.f : mrun[rt];
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(s[rt][e] - ref), p1 = __builtin_amdgcn_exp2f(s[rt][e + 1] - ref);
-        pk[rt][e / 2] = bf ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
-        lrun[rt] += p0;
-        lrun[rt] += p1;
-      }
-    }
-  };
-  auto pfrag = [&](int rt, int u) {
-    return __builtin_bit_cast(s16x8, u32x4{pk[rt][4 * u], pk[rt][4 * u + 1], pk[rt][4 * u + 2], pk[rt][4 * u + 3]});
-  };
-
+  const int heads = min(A.hh, A.group - chunk * A.hh);
   // key of row r of key tile t: 16 (r / 4) + 4 t + r % 4, so that a lane's scores of the four tiles
   // are 16 consecutive keys, the ones whose V codes it loads as 16 bytes
   const int key0 = 16 * (col >> 2) + (col & 3);
-  const int its = (min(hi, nfull) - lo - wave + 3) >> 2;   // full blocks lo + wave + 4 it of this wave
+
+  // this workgroup's share: blocks [from, to) of the run of all tiles' blocks; tile I's begin at AT
+  int i = w, at = 0, from = 0, to = 0x7FFFFFFF;
+  if (A.splits) {
+    const int all = __builtin_amdgcn_readfirstlane(kv8_sum_blocks(A, A.ntiles, 0, nullptr));
+    const int share = max(A.least, (all + A.splits - 1) / A.splits);
+    from = w * share;
+    to = min(all, from + share);
+    if (from >= to) return;
+    i = 0;
+    for (int t0 = 0; t0 < A.ntiles; t0 += 64) {   // the tile in which FROM lies
+      const int nb = t0 + lane < A.ntiles ? kv8_blocks(c, A.tiles[t0 + lane]) : 0;
+      int upto = nb;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(upto, o, 64);
+        upto += lane >= o ? x : 0;
+      }
+      const uint64_t past = __ballot(at + upto > from);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        i = t0 + l;
+        at += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(nb, l);
+        break;
+      }
+      at += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+
+  // a tile's part of the share
+  struct Seg {
+    SeqTile T;
+    int base, total, nfull, nb, lo, hi, its;
+  };
+  auto segment = [&](int i, int at) __attribute__((always_inline)) {
+    Seg s;
+    s.T = A.tiles[i];
+    s.base = kv8_base(c, s.T.seq);
+    s.total = kv8_total(c, s.base, s.T.len);
+    s.nfull = s.total / 64;
+    s.nb = (s.total + 63) / 64;
+    s.lo = max(0, from - at);
+    s.hi = min(s.nb, to - at);
+    s.its = (min(s.hi, s.nfull) - s.lo - wave + WV - 1) / WV;   // full blocks lo + wave + WV it of this wave
+    return s;
+  };
   int pages = 0;
   float kds = 0.f, vds = 0.f;
-  // 64 blocks' pages and scales, a lane each
-  auto look = [&](int it) {
-    const int b = lo + wave + 4 * (it + lane);
-    int64_t p = b < min(hi, nfull) ? kv8_page(c, T.seq, b) : -1;
+  // 64 of the wave's blocks' pages and scales, a lane each
+  auto look = [&](const Seg& s, int it) __attribute__((always_inline)) {
+    const int b = s.lo + wave + WV * (it + lane);
+    int64_t p = b < min(s.hi, s.nfull) ? kv8_page(c, s.T.seq, b) : -1;
     pages = (int)p;
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
@@ -406,199 +423,358 @@ k_kv8_attend(Kv8Args A) {
     vds = d[1];
   };
   u32x4 kr[4][KL], vr[ND];
-  auto load_k = [&](int page) {
+  // the codes are read once: past the caches
+  auto load_k = [&](int page) __attribute__((always_inline)) {
     const int8_t* p = c.k + ((int64_t)max(page, 0) * c.kv_heads + kvh) * 64 * HD;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int e = 0; e < KL; ++e) kr[t][e] = kv8_load<RT>(p + (key0 + 4 * t) * HD + 16 * g + 64 * e);
+      for (int e = 0; e < KL; ++e)
+        kr[t][e] = __builtin_nontemporal_load((const u32x4*)(p + (key0 + 4 * t) * HD + 16 * g + 64 * e));
   };
-  auto load_v = [&](int page) {
+  auto load_v = [&](int page) __attribute__((always_inline)) {
     const int8_t* p = c.v + ((int64_t)max(page, 0) * c.kv_heads + kvh) * 64 * HD;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) vr[d] = kv8_load<RT>(p + (16 * d + col) * 64 + 16 * g);
+    for (int d = 0; d < ND; ++d) vr[d] = __builtin_nontemporal_load((const u32x4*)(p + (16 * d + col) * 64 + 16 * g));
   };
-  if (its > 0) {
-    look(0);
-    load_k(__builtin_amdgcn_readlane(pages, 0));
-    load_v(__builtin_amdgcn_readlane(pages, 0));
-  }
-  for (int it = 0; it < its; ++it) {
-    const int page = __builtin_amdgcn_readlane(pages, it & 63);
-    const float kd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kds), it & 63)) * A.scale;
-    const float vd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vds), it & 63));
-    if ((it & 63) == 63 && it + 1 < its) look(it + 1);
-    const int next = it + 1 < its ? __builtin_amdgcn_readlane(pages, (it + 1) & 63) : 0;
-    const int k0 = (lo + wave + 4 * it) * 64;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 a[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) a[rt] = f32x4{};
-#pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {
-        const u32x4 w = kr[t][ks / 2];
-        const s16x8 kf = codes8<BF>(w[2 * (ks % 2)], w[2 * (ks % 2) + 1]);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) a[rt] = mfma16<BF>(kf, qf[rt][ks], a[rt]);
-      }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[rt][4 * t + i] = a[rt][i] * kd;
+  auto has_tail = [&](const Seg& s) { return s.nfull < s.hi && s.nfull >= s.lo && (s.nfull - s.lo) % WV == wave; };
+  // the first loads of a tile's part: its first block's codes, and its tail into LDS (the wave that
+  // takes it): 16-byte chunk x of row r at x ^ (r % 16) (HD 64: x ^ (r / 2 % 8)) for K, at
+  // x ^ 4 (r % 4) (HD 64: x ^ 4 (r / 2 % 2)) for V
+  auto begin = [&](const Seg& s) __attribute__((always_inline)) {
+    if (s.its > 0) {
+      look(s, 0);
+      load_k(__builtin_amdgcn_readlane(pages, 0));
+      load_v(__builtin_amdgcn_readlane(pages, 0));
     }
-    if (it + 1 < its) load_k(next);
-    float vdl[RT];   // a row that sees nothing of the block takes nothing of its scale, which may be NaN
+    if (has_tail(s)) {
+      const int64_t th = ((int64_t)s.T.seq * c.kv_heads + kvh) * 64 * HD;
+#pragma unroll 1
+      for (int e = 0; e < CH; ++e) {
+        const int r = (64 / CH) * e + lane / CH, x = lane % CH;
+        const int kx = x ^ (HD == 128 ? r & 15 : (r >> 1) & 7), vx = x ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1));
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(c.tk + th + r * HD + 8 * kx),
+                                         (lds_void*)(tbuf[0] + e * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(c.tv + th + r * HD + 8 * vx),
+                                         (lds_void*)(tbuf[1] + e * 1024), 16, 0, 0);
+      }
+    }
+  };
+
+  Seg S = segment(i, at);
+  begin(S);
+  for (;;) {
+    const SeqTile T = S.T;
+    const int live = T.len, base = S.base;
+    int lim[RT];
+    s16x8 qf[RT][NS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      vdl[rt] = page >= 0 && k0 <= lim[rt] ? vd : 0.f;
-      if (page < 0 || k0 + 63 > base + T.t0) {
+      const int r = rt * 16 + col, tok = min((int)(r * A.magic >> 16), live - 1);
+      const int head = min(r - (int)(r * A.magic >> 16) * A.hh, heads - 1);
+      lim[rt] = min(base + tok, S.total - 1);
+      // dims of k-step s: 16 g + 8 (s % 2) + 64 (s / 2) .., as the 16 bytes of codes a lane loads
+      const uint16_t* qr = A.q + (int64_t)(T.row0 + tok) * A.ldq + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (page < 0 || k0 + 16 * g + e > lim[rt]) s[rt][e] = -INFINITY;
-      }
+      for (int s = 0; s < NS; ++s) qf[rt][s] = *(const s16x8*)(qr + 8 * (s % 2) + 64 * (s / 2));
     }
-    weights(0);
+    f32x4 o[RT][ND];
+    float mrun[RT], lrun[RT];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      const s16x8 v0 = codes8<0>(vr[d][0], vr[d][1]), v1 = codes8<0>(vr[d][2], vr[d][3]);
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[rt][d] = f32x4{};
+      mrun[rt] = -INFINITY;
+      lrun[rt] = 0.f;
+    }
+    float s[RT][16];   // scores of keys 16 g + e of the block in hand
+    uint32_t pk[RT][8];
+
+    // from scores (log2 units, hidden ones -inf) to weights: the rows' references, sums and pk
+    auto weights = [&](auto bf_c) __attribute__((always_inline)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const f32x4 a = mfma16<0>(v1, pfrag(rt, 1), mfma16<0>(v0, pfrag(rt, 0), f32x4{}));
+        float mx = s[rt][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[rt][d][i] = __builtin_fmaf(a[i], vdl[rt], o[rt][d][i]);
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[rt][e]);
+        mx = max_groups(mx);
+        // a first reference (any above -inf), or one that has fallen behind
+        if (__ballot(mx > mrun[rt] + MAX_SLACK)) {
+          const float mn = mx > mrun[rt] + MAX_SLACK ? mx : mrun[rt];
+          const float a = mn == mrun[rt] ? 1.f : __builtin_amdgcn_exp2f(mrun[rt] - mn);
+          mrun[rt] = mn;
+          lrun[rt] *= a;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[rt][d] *= a;
+        }
+        const float ref = mrun[rt] == -INFINITY ? 0.f : mrun[rt];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(s[rt][e] - ref), p1 = __builtin_amdgcn_exp2f(s[rt][e + 1] - ref);
+          pk[rt][e / 2] = decltype(bf_c)::value ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+          lrun[rt] += p0;
+          lrun[rt] += p1;
+        }
       }
-    }
-    if (it + 1 < its) load_v(next);
-  }
+    };
+    auto pfrag = [&](int rt, int u) {
+      return __builtin_bit_cast(s16x8, u32x4{pk[rt][4 * u], pk[rt][4 * u + 1], pk[rt][4 * u + 2], pk[rt][4 * u + 3]});
+    };
 
-  // the tail, in 16 bits, by the wave whose turn it is
-  if (nfull < hi && nfull >= lo && ((nfull - lo) & 3) == wave) {
-    const int left = total - nfull * 64;
-    const int64_t at = ((int64_t)T.seq * c.kv_heads + kvh) * 64 * HD;
-    uint16_t* vt = (uint16_t*)obuf;
+    for (int it = 0; it < S.its; ++it) {
+      const int page = __builtin_amdgcn_readlane(pages, it & 63);
+      const float kd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kds), it & 63)) * A.scale;
+      const float vd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vds), it & 63));
+      if ((it & 63) == 63 && it + 1 < S.its) look(S, it + 1);
+      const int next = it + 1 < S.its ? __builtin_amdgcn_readlane(pages, (it + 1) & 63) : 0;
+      const int k0 = (S.lo + wave + WV * it) * 64;
 #pragma unroll
-    for (int e = 0; e < HD / 8; ++e) {   // V's rows into LDS, those past the last token as zeros
-      const int i = (e * 64 + lane) * 8, key = i / HD;
-      u32x4 x = {};
-      if (key < left) x = *(const u32x4*)(c.tv + at + i);
-      *(u32x4*)(vt + i) = x;
-    }
+      for (int t = 0; t < 4; ++t) {
+        f32x4 a[RT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 a[RT];
+        for (int rt = 0; rt < RT; ++rt) a[rt] = f32x4{};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) a[rt] = f32x4{};
+        for (int ks = 0; ks < NS; ++ks) {
+          const u32x4 x = kr[t][ks / 2];
+          const s16x8 kf = codes8<BF>(x[2 * (ks % 2)], x[2 * (ks % 2) + 1]);
 #pragma unroll
-      for (int ks = 0; ks < NS; ++ks) {
-        s16x8 kf = {};
-        if (key0 + 4 * t < left)
-          kf = *(const s16x8*)(c.tk + at + (key0 + 4 * t) * HD + 16 * g + 8 * (ks % 2) + 64 * (ks / 2));
+          for (int rt = 0; rt < RT; ++rt) a[rt] = mfma16<BF>(kf, qf[rt][ks], a[rt]);
+        }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) a[rt] = mfma16<BF>(kf, qf[rt][ks], a[rt]);
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[rt][4 * t + e] = a[rt][e] * kd;
+        __builtin_amdgcn_sched_barrier(0);
       }
+      if (it + 1 < S.its) load_k(next);
+      float vdl[RT];   // a row that sees nothing of the block takes nothing of its scale, which may be NaN
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int rt = 0; rt < RT; ++rt) {
+        vdl[rt] = page >= 0 && k0 <= lim[rt] ? vd : 0.f;
+        if (page < 0 || k0 + 63 > base) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[rt][4 * t + i] = nfull * 64 + 16 * g + 4 * t + i > lim[rt] ? -INFINITY : a[rt][i] * A.scale;
-    }
-    weights(BF);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's V rows are in LDS
-    asm volatile("" ::: "memory");
-    typedef __attribute__((address_space(3))) s16x4 lds_s4;
-    // lane i of 16 addresses key i / 4's dims 4 (i % 4) .. and gets dim i of the 4 keys
-    uint16_t* vl = vt + (16 * g + (col >> 2)) * HD + 4 * (col & 3);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      f32x4 a[ND];
-      uint32_t bad = 0;
+          for (int e = 0; e < 16; ++e)
+            if (page < 0 || k0 + 16 * g + e > lim[rt]) s[rt][e] = -INFINITY;
+        }
+      }
+      weights(std::integral_constant<int, 0>());
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        s16x8 v[2];
+        const s16x8 v0 = codes8<0>(vr[d][0], vr[d][1]), v1 = codes8<0>(vr[d][2], vr[d][3]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vl + 8 * u * HD + 16 * d));
-          const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(vl + (8 * u + 4) * HD + 16 * d));
-          v[u] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int rt = 0; rt < RT; ++rt) {
+          const f32x4 a = mfma16<0>(v1, pfrag(rt, 1), mfma16<0>(v0, pfrag(rt, 0), f32x4{}));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[rt][d][e] = __builtin_fmaf(a[e], vdl[rt], o[rt][d][e]);
         }
-        a[d] = mfma16<BF>(v[1], pfrag(rt, 1), mfma16<BF>(v[0], pfrag(rt, 0), f32x4{}));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= (__float_as_uint(a[d][i]) & 0x7F800000u) == 0x7F800000u;
+        if (d % 2) __builtin_amdgcn_sched_barrier(0);
       }
-      if (__ballot(bad)) {
-        // an infinity or a NaN among the values: again, each row over the keys it sees only
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pbuf[16 * g + e][col] = __builtin_amdgcn_exp2f(s[rt][e] - (mrun[rt] == -INFINITY ? 0.f : mrun[rt]));
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0xC07F);
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int d = 0; d < ND; ++d) a[d] = f32x4{};
-        for (int j = 0; j < left && nfull * 64 + j <= lim[rt]; ++j) {
-          const float p = pbuf[j][col];
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[d][i] += p * ld16(vt + j * HD + 16 * d + 4 * g + i, BF);
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[rt][d] += a[d];
+      if (it + 1 < S.its) load_v(next);
     }
-  }
 
-  // the four waves' sums of a row tile through LDS, 16 threads a row
+    // the tail, in 16 bits, by the wave whose turn it is
+    if (has_tail(S)) {
+      const int left = S.total - S.nfull * 64, t0 = S.nfull * 64;
+      int l = lane;
+      asm volatile("" : "+v"(l));   // its addresses are made here, not kept through the loop above
+      const int col = l & 15, g = l >> 4, key0 = 16 * (col >> 2) + (col & 3);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): its rows are in LDS
+      asm volatile("" ::: "memory");
+      // V's rows past the last token may hold anything: zeros
+      for (int e = left * CH + lane; e < 64 * CH; e += 64) *(u32x4*)(tbuf[1] + e * 16) = u32x4{};
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    __syncthreads();
+      for (int t = 0; t < 4; ++t) {
+        f32x4 a[RT];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *(f32x4*)&obuf[wave][col][16 * d + 4 * g] = o[rt][d];
-    const float l = sum_groups(lrun[rt]);
-    if (g == 0) {
-      mbuf[wave][col] = mrun[rt];
-      lbuf[wave][col] = l;
+        for (int rt = 0; rt < RT; ++rt) a[rt] = f32x4{};
+#pragma unroll
+        for (int ks = 0; ks < NS; ++ks) {
+          const int r = key0 + 4 * t, x = 2 * g + ks % 2 + 8 * (ks / 2);
+          const s16x8 kf = *(const s16x8*)(tbuf[0] + r * ROWB + ((x ^ (HD == 128 ? r & 15 : (r >> 1) & 7)) << 4));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) a[rt] = mfma16<BF>(kf, qf[rt][ks], a[rt]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[rt][4 * t + e] = t0 + 16 * g + 4 * t + e > lim[rt] ? -INFINITY : a[rt][e] * A.scale;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      weights(std::integral_constant<int, BF>());
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): the zeros are in LDS
+      asm volatile("" ::: "memory");
+      typedef __attribute__((address_space(3))) s16x4 lds_s4;
+      // lane l of 16 addresses key l / 4's dims 4 (l % 4) .. and gets dim l of the 4 keys
+      auto v4 = [&](int key, int d) {
+        const int r = key + (col >> 2), x = 2 * d + ((col & 3) >> 1);
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s4*)(tbuf[1] + r * ROWB + ((x ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))) << 4) + 8 * (col & 1)));
+      };
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x4 a[ND];
+        uint32_t bad = 0;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          s16x8 v[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            v[u] = __builtin_shufflevector(v4(16 * g + 8 * u, d), v4(16 * g + 8 * u + 4, d), 0, 1, 2, 3, 4, 5, 6, 7);
+          a[d] = mfma16<BF>(v[1], pfrag(rt, 1), mfma16<BF>(v[0], pfrag(rt, 0), f32x4{}));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(a[d][e]) & 0x7F800000u) == 0x7F800000u;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__ballot(bad)) {
+          // an infinity or a NaN among the values: again, each row over the keys it sees only
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            pbuf[16 * g + e][col] = __builtin_amdgcn_exp2f(s[rt][e] - (mrun[rt] == -INFINITY ? 0.f : mrun[rt]));
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_waitcnt(0xC07F);
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int d = 0; d < ND; ++d) a[d] = f32x4{};
+#pragma unroll 1
+          for (int j = 0; j < left && t0 + j <= lim[rt]; ++j) {
+            const float p = pbuf[j][col];
+            const int z = HD == 128 ? 4 * (j & 3) : 4 * ((j >> 1) & 1);
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                a[d][e] += p * ld16((const uint16_t*)(tbuf[1] + j * ROWB + (((2 * d + (g >> 1)) ^ z) << 4)) + 4 * (g & 1) + e, BF);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[rt][d] += a[d];
+      }
     }
-    __syncthreads();
-    const int rr = tid >> 4, r = rt * 16 + rr, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
-    if (tok >= live || head >= heads) continue;
-    const float m = fmaxf(fmaxf(mbuf[0][rr], mbuf[1][rr]), fmaxf(mbuf[2][rr], mbuf[3][rr]));
-    float w[4], sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = mbuf[k][rr] == -INFINITY ? 0.f : mbuf[k][rr] == m ? 1.f : __builtin_amdgcn_exp2f(mbuf[k][rr] - m);
-      sum += mbuf[k][rr] == -INFINITY ? lbuf[k][rr] : w[k] * lbuf[k][rr];   // no reference: 0, or NaN
+
+    int mt = tid;
+    asm volatile("" : "+v"(mt));   // as above
+    // the next tile's first loads, then this one's sums meet: 16 threads a row, all waves' sums of it
+    const bool whole = S.lo == 0 && S.hi == S.nb, more = at + S.nb < to && i + 1 < A.ntiles && A.splits;
+    const int nb = S.nb, lo = S.lo;
+    if (more) {
+      at += nb;
+      ++i;
+      S = segment(i, at);
+      __syncthreads();   // the tail in LDS is done with
+      begin(S);
     }
-    const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + kvh * A.group + chunk * A.hh + head;
-    const float inv = active > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-    constexpr int E = HD / 16;   // dims a thread
-    const int d0 = (tid & 15) * E;
-    float y[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      y[e] = 0.f;
+    for (int rt = 0; rt < RT; ++rt) {
+      __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (w[k] > 0.f) y[e] = __builtin_fmaf(w[k], obuf[k][rr][d0 + e], y[e]);
-      y[e] *= inv;
+      for (int d = 0; d < ND; ++d) *(f32x4*)&obuf[wave][col][16 * d + 4 * g] = o[rt][d];
+      const float l = sum_groups(lrun[rt]);
+      if (g == 0) {
+        mbuf[wave][col] = mrun[rt];
+        lbuf[wave][col] = l;
+      }
+      __syncthreads();
+      const int rr = mt >> 4, r = rt * 16 + rr, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
+      if (rr >= 16 || tok >= live || head >= heads) continue;
+      float m = mbuf[0][rr];
+#pragma unroll
+      for (int k = 1; k < WV; ++k) m = fmaxf(m, mbuf[k][rr]);
+      float wt[WV], sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < WV; ++k) {
+        wt[k] = mbuf[k][rr] == -INFINITY ? 0.f : mbuf[k][rr] == m ? 1.f : __builtin_amdgcn_exp2f(mbuf[k][rr] - m);
+        sum += mbuf[k][rr] == -INFINITY ? lbuf[k][rr] : wt[k] * lbuf[k][rr];   // no reference: 0, or NaN
+      }
+      const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      constexpr int E = HD / 16;   // dims a thread
+      const int d0 = (mt & 15) * E;
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        y[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < WV; ++k)
+          if (wt[k] > 0.f) y[e] = __builtin_fmaf(wt[k], obuf[k][rr][d0 + e], y[e]);
+        y[e] *= inv;
+      }
+      if (!whole) {   // the share's own first part (0) or the one begun in it (1)
+        const int64_t slot = ((int64_t)blockIdx.x * 2 + (lo == 0)) * 16 * RT + r;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + slot * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        if ((mt & 15) == 0) *(f32x2*)(A.part + (int64_t)A.splits * per * 32 * RT * HD + slot * 2) = f32x2{m, sum};
+      } else {
+        uint32_t x[E / 2];
+        if (A.obf) {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) x[e / 2] = pack_bf16x2(y[e], y[e + 1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) x[e / 2] = pack_f16x2(y[e], y[e + 1]);
+        }
+        uint16_t* po = A.out + (int64_t)(T.row0 + tok) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + d0;
+        if constexpr (E == 8)
+          *(u32x4*)po = u32x4{x[0], x[1], x[2], x[3]};
+        else
+          *(u32x2*)po = u32x2{x[0], x[1]};
+      }
     }
-    if (active > 1) {
-      const int64_t n = A.rows * A.heads, at = blockIdx.y * n + rowhead;
-#pragma unroll
-      for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + at * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
-      if ((tid & 15) == 0) *(f32x2*)(A.part + A.splits * n * HD + at * 2) = f32x2{m, sum};
-    } else {
-      uint32_t x[E / 2];
-#pragma unroll
-      for (int e = 0; e < E; e += 2) x[e / 2] = A.obf ? pack_bf16x2(y[e], y[e + 1]) : pack_f16x2(y[e], y[e + 1]);
-      uint16_t* po = A.out + (rowhead / A.heads) * A.ldo + (rowhead % A.heads) * HD + d0;
-      if constexpr (E == 8)
-        *(u32x4*)po = u32x4{x[0], x[1], x[2], x[3]};
-      else
-        *(u32x2*)po = u32x2{x[0], x[1]};
-    }
+    if (!more) return;
   }
+}
+
+// The sums of k_kv8_few's workgroups of each tile that more than one had a part of: a workgroup a row and
+// key/value head (blockIdx.y: the row), HD / 4 threads a share of them, in a fixed order.
+template <int HD, int RT>
+__global__ void __launch_bounds__(256)
+k_kv8_join_few(Kv8Args A) {
+  constexpr int TH = HD / 4, SH = 256 / TH;   // threads a share; shares
+  __shared__ __align__(16) float ys[SH][HD];
+  __shared__ float ss[SH], ms[SH];
+  const int per = A.c.kv_heads * A.chunks;
+  const int i = blockIdx.x / per, hc = blockIdx.x % per, kvh = hc % A.c.kv_heads, chunk = hc / A.c.kv_heads;
+  const int r = blockIdx.y, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
+  const SeqTile T = A.tiles[i];
+  if (tok >= T.len || head >= min(A.hh, A.group - chunk * A.hh)) return;
+  int first;
+  const int all = kv8_sum_blocks(A, A.ntiles, i, &first);
+  const int nb = kv8_blocks(A.c, T), share = max(A.least, (all + A.splits - 1) / A.splits);
+  const int w0 = first / share, w1 = (first + nb - 1) / share;   // the workgroups that had a part
+  if (w0 == w1) return;
+  const int tid = threadIdx.x, sh = tid / TH, d = tid % TH * 4;
+  const float* ml = A.part + (int64_t)A.splits * per * 32 * RT * HD;
+  auto slot = [&](int w) { return (((int64_t)w * per + hc) * 2 + (w == w0)) * 16 * RT + r; };
+  float m = -INFINITY;
+  for (int w = w0 + sh; w <= w1; w += SH) m = fmaxf(m, ml[slot(w) * 2]);
+  if (d == 0) ms[sh] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < SH; ++k) m = fmaxf(m, ms[k]);
+  float sum = 0.f;
+  f32x4 y = {};
+#pragma unroll 4
+  for (int w = w0 + sh; w <= w1; w += SH) {
+    const f32x2 p = *(const f32x2*)(ml + slot(w) * 2);
+    const f32x4 x = *(const f32x4*)(A.part + slot(w) * HD + d);
+    const float f = p[0] == -INFINITY ? 0.f : p[0] == m ? 1.f : __builtin_amdgcn_exp2f(p[0] - m);
+    sum += p[0] == -INFINITY ? p[1] : f * p[1];   // no reference: 0, or NaN
+    if (f > 0.f) y += f * x;
+  }
+  *(f32x4*)&ys[sh][d] = y;
+  if (d == 0) ss[sh] = sum;
+  __syncthreads();
+  if (sh) return;
+#pragma unroll
+  for (int k = 1; k < SH; ++k) {
+    y += *(const f32x4*)&ys[k][d];
+    sum += ss[k];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* po = A.out + (int64_t)(T.row0 + tok) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + d;
+  *(u32x2*)po = A.obf ? u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)}
+                      : u32x2{pack_f16x2(y[0] * inv, y[1] * inv), pack_f16x2(y[2] * inv, y[3] * inv)};
 }
 
 // --- many rows: 128 a workgroup -------------------------------------------------------------------
@@ -610,7 +786,6 @@ k_kv8_attend(Kv8Args A) {
 // factor, V's into the weights' exponent, p vd 2^-E with E the largest exponent of a scale so far, so that
 // fp16 weights of blocks of small values keep their bits; a block's sum of them times 1 / (vd 2^-E) is
 // its share of the row's weight.
-typedef __attribute__((address_space(3))) void lds_void;
 template <int BF>
 __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
   if constexpr (BF)
@@ -1086,48 +1261,70 @@ namespace {
 
 struct Kv8Way {
   int rt;                  // row tiles of 16 a workgroup (1 or 2), or 0: k_kv8_chunk's 128 rows
+  int wv;                  // waves a workgroup
   int z, hh, chunks;       // the tiles' list; heads a workgroup, workgroups a group
   int splits, least;
+  int64_t floats;          // of scratch that the splits take
 };
-Kv8Way kv8_way(int longest, int heads, int kv_heads, int head_dim, int cols, const int64_t* ntiles) {
+// at most SPLITS of them (as far as the caller's scratch goes)
+Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim, int cols, const int64_t* ntiles,
+               int64_t part_cap) {
   Kv8Way w;
   const int group = heads / kv_heads;
   w.hh = group < 16 ? group : 16;
   w.z = 0;
+  w.splits = 0;
+  w.floats = 0;
+  w.wv = 4;
   if (longest * w.hh <= 32) {
     w.rt = longest * w.hh <= 16 ? 1 : 2;
     while ((SEQ_TT0 << w.z) < longest) ++w.z;
-    w.least = 32;
-  } else {
-    w.rt = 0;
-    w.hh = group < 8 ? group : 8;
-    while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
-    w.least = 2;
+    w.chunks = (group + w.hh - 1) / w.hh;
+    const int per = kv_heads * w.chunks;
+    // as many workgroups as the chip holds at once
+    const int slots = 256 * (w.rt == 1 ? (head_dim == 64 ? 4 : 2) : (head_dim == 64 ? 2 : 1));
+    int64_t s = slots / per > 0 ? slots / per : 1;
+    const int64_t each = (int64_t)per * 32 * w.rt * (head_dim + 2);
+    if (s * each > part_cap) s = part_cap / each;
+    w.least = 16;
+    if (cols > 16 && s > 1 && ntiles[w.z] <= 4096) {
+      w.splits = (int)s;
+      w.floats = s * each;
+    } else if (w.rt == 1 && ntiles[w.z] * per <= 256) {
+      w.wv = 8;
+    }
+    return w;
   }
+  w.rt = 0;
+  w.hh = group < 8 ? group : 8;
+  while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
+  w.least = 2;
   w.chunks = (group + w.hh - 1) / w.hh;
-  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, s = groups > 0 ? (w.rt ? 4096 : 512) / groups : 1;
-  const int64_t most = (cols + w.least - 1) / w.least;
-  w.splits = (int)(s < 1 ? 1 : s > most ? most : s);
+  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, most = (cols + w.least - 1) / w.least;
+  const int64_t each = rows * heads * (head_dim + 2);
+  int64_t s = groups > 0 ? 512 / groups : 1;
+  if (s > most) s = most;
+  if (each > 0 && s * each > part_cap) s = part_cap / each;
+  w.splits = s < 1 ? 1 : (int)s;
+  w.floats = w.splits > 1 ? w.splits * each : 0;
   return w;
 }
 
 }  // namespace
 
 int64_t kv8_attend_part(int64_t rows, const int64_t* ntiles, int longest, int heads, int kv_heads, int head_dim, int cols) {
-  const Kv8Way w = kv8_way(longest, heads, kv_heads, head_dim, cols, ntiles);
-  return w.splits > 1 ? w.splits * rows * heads * (head_dim + 2) : 0;
+  return rows == 0 ? 0 : kv8_way(rows, longest, heads, kv_heads, head_dim, cols, ntiles, INT64_MAX).floats;
 }
 
 hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles, int64_t rows,
                       int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out, int obf,
                       int64_t ldo, float* part, int64_t part_cap) {
   if (ntiles[0] == 0) return hipSuccess;
-  Kv8Way w = kv8_way(longest, heads, c.kv_heads, c.head_dim, c.cols, ntiles);
-  const int64_t fit = part_cap / (rows * heads * (c.head_dim + 2));
-  if (w.splits > fit) w.splits = fit < 1 ? 1 : (int)fit;
+  const Kv8Way w = kv8_way(rows, longest, heads, c.kv_heads, c.head_dim, c.cols, ntiles, part_cap);
   Kv8Args a;
   a.c = c;
   a.tiles = tiles[w.z];
+  a.ntiles = (int)ntiles[w.z];
   a.q = q;
   a.out = out;
   a.ldq = ldq;
@@ -1144,13 +1341,15 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   a.least = w.least;
   a.part = part;
   a.rows = rows;
-  const int64_t groups = ntiles[w.z] * w.chunks * c.kv_heads;
-  if (groups > INT32_MAX) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)groups, w.splits);
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
+  const int64_t groups = (w.rt && w.splits ? w.splits : ntiles[w.z]) * w.chunks * c.kv_heads;
+  const int64_t joins = ntiles[w.z] * w.chunks * c.kv_heads;
+  if (groups > INT32_MAX || joins > INT32_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)groups, w.rt ? 1 : w.splits);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * w.wv), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-    w.rt == 0 ? go(k_kv8_chunk<BF, HD>) : w.rt == 1 ? go(k_kv8_attend<BF, HD, 1>) : go(k_kv8_attend<BF, HD, 2>);
+    w.rt == 0 ? go(k_kv8_chunk<BF, HD>) : w.rt == 2 ? go(k_kv8_few<BF, HD, 2, 4>)
+    : w.wv == 8 ? go(k_kv8_few<BF, HD, 1, 8>) : go(k_kv8_few<BF, HD, 1, 4>);
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
@@ -1162,6 +1361,14 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
     c.bf16 ? rts(I1(), I64()) : rts(I0(), I64());
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.splits < 2) return e;
+  if (w.rt) {
+    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins, longest * w.hh), dim3(256), 0, s, a); };
+    if (c.head_dim == 128)
+      w.rt == 1 ? join(k_kv8_join_few<128, 1>) : join(k_kv8_join_few<128, 2>);
+    else
+      w.rt == 1 ? join(k_kv8_join_few<64, 1>) : join(k_kv8_join_few<64, 2>);
+    return hipGetLastError();
+  }
   const int th = c.head_dim / 4, most = (a.tt < longest ? a.tt : longest) * heads;   // a tile's rows and heads
   const bool few = w.splits > 4;
   const int each = few ? 1 : 256 / th;
