@@ -36,8 +36,22 @@ __device__ __forceinline__ void store_piece(uint16_t* p, const Piece<HD>& x) {
   else
     *(u32x2*)p = u32x2{x.w[0], x.w[1]};
 }
-__device__ __forceinline__ float half_of(uint32_t w, int e, int bf) {
-  return bf ? (e & 1 ? bf16_hi(w) : bf16_lo(w)) : (e & 1 ? f16_hi(w) : f16_lo(w));
+template <int BF>
+__device__ __forceinline__ float half_of(uint32_t w, int e) {
+  return BF ? (e & 1 ? bf16_hi(w) : bf16_lo(w)) : (e & 1 ? f16_hi(w) : f16_lo(w));
+}
+// kv8_code of four values, a byte each; R = 1 / d to an ulp, d of at least 2^-100.  One correction makes
+// a quotient that is exactly between two codes exact, and any other is further from there than it is
+// off; adding 1.5 x 2^23 rounds it to the nearest even whole number, in the low bits.
+__device__ __forceinline__ uint32_t kv8_codes4(const float* x, float d, float r) {
+  uint32_t u[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float q = x[e] * r;
+    u[e] = __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, d, x[e]), r, q) + 12582912.f);
+  }
+  const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), b = __builtin_amdgcn_perm(u[3], u[2], 0x0C0C0400u);
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
 
 // One workgroup a (sequence and key/value head, block the step can touch, keys or values): bytes are
@@ -45,7 +59,7 @@ __device__ __forceinline__ float half_of(uint32_t w, int e, int bf) {
 // new rows, between the block's largest |x| and its codes; values leave through LDS, where four
 // tokens' codes of a dim are a dword.  Block 0's workgroup also writes the tail, after it has read the
 // old one: the one slot serves the block that fills and the block begun after it.
-template <int HD>
+template <int BF, int HD>
 __global__ void __launch_bounds__(256)
 k_kv8_append(Kv8 c, const SeqTile* __restrict__ seqs, const uint16_t* __restrict__ k, int64_t ldk,
              const uint16_t* __restrict__ v, int64_t ldv) {
@@ -72,7 +86,7 @@ k_kv8_append(Kv8 c, const SeqTile* __restrict__ seqs, const uint16_t* __restrict
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(half_of(r[i].w[e / 2], e, c.bf16)) & 0x7FFFFFFFu);
+      for (int e = 0; e < E; ++e) top = max(top, __float_as_uint(half_of<BF>(r[i].w[e / 2], e)) & 0x7FFFFFFFu);
     for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     if (tid % 64 == 0) tops[tid / 64] = top;
     __syncthreads();
@@ -80,16 +94,29 @@ k_kv8_append(Kv8 c, const SeqTile* __restrict__ seqs, const uint16_t* __restrict
     if (page >= 0) {
       int8_t* dst = (isv ? c.v : c.k) + (page * c.kv_heads + h) * 64 * HD;
       uint32_t code[4][E / 4];
+      const bool plain = d >= 0x1p-100f;   // else zeros, values next to nothing, or not finite ones
+      const float rd = __builtin_amdgcn_rcpf(d);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e4 = 0; e4 < E / 4; ++e4) {
-          uint32_t w = 0;
+          float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w |= (uint32_t)(uint8_t)kv8_code(half_of(r[i].w[2 * e4 + e / 2], e, c.bf16), d) << (8 * e);
-          code[i][e4] = w;
+          for (int e = 0; e < 4; ++e) y[e] = half_of<BF>(r[i].w[2 * e4 + e / 2], e);
+          code[i][e4] = kv8_codes4(y, d, rd);
         }
+      if (!plain) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e4 = 0; e4 < E / 4; ++e4) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w |= (uint32_t)(uint8_t)kv8_code(half_of<BF>(r[i].w[2 * e4 + e / 2], e), d) << (8 * e);
+            code[i][e4] = w;
+          }
+      }
       if (isv) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -128,10 +155,11 @@ hipError_t kv8_append(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, i
                       int64_t ldk, const uint16_t* v, int64_t ldv) {
   if (n == 0 || longest == 0) return hipSuccess;
   const dim3 grid(n * c.kv_heads, (62 + longest) / 64 + 1, 2);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv); };
   if (c.head_dim == 128)
-    hipLaunchKernelGGL(k_kv8_append<128>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
+    c.bf16 ? go(k_kv8_append<1, 128>) : go(k_kv8_append<0, 128>);
   else
-    hipLaunchKernelGGL(k_kv8_append<64>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
+    c.bf16 ? go(k_kv8_append<1, 64>) : go(k_kv8_append<0, 64>);
   return hipGetLastError();
 }
 

@@ -281,6 +281,34 @@ def test_one_by_one_is_all_at_once(ctx, dt):
     d.same()
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("power", [-20, -8, 0, 9])
+def test_codes_on_and_next_to_ties(ctx, dt, power):
+    """Blocks of values exactly between two codes, and next to there; the smallest and largest ones."""
+    rng = np.random.default_rng([20, power + 40])
+    kv, hd, rows = 4, 128, 128
+    x = (2.0 ** power * rng.standard_normal((rows, kv, hd))).astype(np.float32)
+    x[0] = x[64] = 0
+    x[0, :, 0] = x[64, :, 0] = 2.0 ** power * rng.choice([4.0, 5.0625, 6.5, 7.984375], kv)
+    x = pm.rounded(np.clip(x, -4 * 2.0 ** power, 4 * 2.0 ** power), dt)
+    for b in range(2):
+        for h in range(kv):
+            d = np.float64(pm.scale_of(x[64 * b:64 * b + 64, h]))
+            tie = (rng.integers(-64, 64, (63, hd)) + 0.5) * d
+            x[64 * b + 1:64 * b + 64, h] = pm.rounded(tie.astype(np.float32), dt)
+    if power == -20:      # the second block: values of the type's smallest
+        x[64:] = pm.rounded((2.0 ** (-23 if dt == "fp16" else -132) * rng.standard_normal((64, kv, hd))).astype(np.float32), dt)
+    if power == 9:        # and of its largest
+        x[64:] = pm.rounded((x[64:] / 4096 * (65000 if dt == "fp16" else 3e38)).astype(np.float32), dt)
+    say("ties", dt, power)
+    b = pm.bits(x, dt)
+    m, d = cache_of(ctx, dt, 1, kv, hd, 2, rng)
+    db = X.DevBuf.of(ctx, b)
+    X.kv8_append(ctx, d.h, X.Seqs(ctx, [rows]), db.h, kv * hd, db.h, kv * hd)
+    m.append(b, b, [rows])
+    d.same([rows])
+
+
 def test_cache_edges(ctx):
     """Rows past the table's end, pages that are none, lengths out of range: hidden, never written."""
     rng = np.random.default_rng(13)
