@@ -1,6 +1,8 @@
 // api_encoder.hip -- the prompt encoder's text model (src/encoder.lisp): weights and driver.
 #include "api_host.h"
 
+#include <new>
+
 // --- the prompt encoder (replaces illatio's qwen3 forward under src/encoder.lisp) -------------
 
 namespace {
@@ -53,6 +55,7 @@ struct EncLayer {
 
 struct exn_enc {
   exn_ctx* ctx = nullptr;
+  int caches = 0;            // exn_enc_cache objects made and not freed
   int layers = 36;
   double base = 5e6;
   int64_t vocab = 0;
@@ -65,6 +68,38 @@ struct exn_enc {
   std::map<int, int32_t*> maps;  // device row maps by slot
   bool bf16 = true;           // the matrices run from resident bf16 expansions (exn_enc_resident)
 };
+
+// kept keys and values of SEQS sequences through every layer, in 8 bits (exn_kv8's layout, a run of PAGES
+// pages a layer): the host counts tokens and pages, the device has a copy of both for a step
+struct exn_enc_cache {
+  exn_enc* e = nullptr;
+  int seqs = 0, cols = 0, pages = 0;
+  std::vector<int32_t> lens, table;   // table [seqs][cols], -1 where no full block is
+  std::vector<int32_t> refs, spare;   // sequences that name a page; pages that none names
+  int8_t *k = nullptr, *v = nullptr;
+  float* scales = nullptr;
+  uint16_t *tk = nullptr, *tv = nullptr;
+  int32_t *d_table = nullptr, *d_lens = nullptr;
+  size_t block = (size_t)8 * 64 * EXN_HD;   // values of a page's keys, or values; of a tail's
+};
+
+// layer IL's part of a cache
+static Kv8 cache_layer(const exn_enc_cache* c, int il) {
+  Kv8 r;
+  r.bf16 = 0;
+  r.kv_heads = 8;
+  r.head_dim = EXN_HD;
+  r.cols = c->cols;
+  r.pages = c->pages;
+  r.k = c->k + (size_t)il * c->pages * c->block;
+  r.v = c->v + (size_t)il * c->pages * c->block;
+  r.scales = c->scales + (size_t)il * c->pages * 16;
+  r.tk = c->tk + (size_t)il * c->seqs * c->block;
+  r.tv = c->tv + (size_t)il * c->seqs * c->block;
+  r.table = c->d_table;
+  r.lens = c->d_lens;
+  return r;
+}
 
 static int enc_buf(exn_enc* e, const char* key, size_t bytes, void** out, bool zero = false) {
   Buf& b = e->bufs[key];
@@ -155,6 +190,7 @@ int exn_enc_release(exn_enc* e) {
 
 int exn_enc_destroy(exn_enc* e) {
   if (!e) return EXN_OK;
+  if (e->caches) FAIL(EXN_ESTATE, "encoder: %d caches of it are not freed", e->caches);
   TRY(exn_enc_release(e));
   for (auto& L : e->L) {
     exn_weight_free(L.qkv);
@@ -334,8 +370,10 @@ int exn_enc_rope_table(const int32_t* pos, int n, double base, float* cs) {
 // encoder-states on the device: IDS (n, validated), CS (n x 128, exn_enc_rope_table's), the
 // picture's rows PIC0 .. PIC0 + M - 1 taking MERGED after the embedding and DEEP[j] (3 x M x
 // 4096) after layer j; OUT n x 4096
+// With PLAN its rows are several sequences' (packed, n in all), each seeing itself alone, or with CACHE too
+// what the cache has of it before them.
 static int enc_states(exn_enc* e, const int32_t* ids, int n, const float* cs, int pic0, int m, const float* merged,
-                      const float* deep, float* out) {
+                      const float* deep, float* out, const exn_seqs* plan = nullptr, const exn_enc_cache* cache = nullptr) {
   hipStream_t s = e->ctx->stream;
   // expansions made (or remade after a set) once a prompt reads them, then kept: a prompt of at
   // most 256 tokens takes every product from the Q8_0 codes (wop_n) and leaves them unmade
@@ -344,14 +382,22 @@ static int enc_states(exn_enc* e, const int32_t* ids, int n, const float* cs, in
       for (exn_w* w : {L.qkv, L.out, L.gate_up, L.down}) TRY(w_resident(w, true));
   const int64_t lcap = ((int64_t)n + 63) / 64 * 64;
   float* x;
-  uint16_t *y, *att, *ff, *q, *kc, *vt, *qkv;
+  uint16_t *y, *att, *ff, *q = nullptr, *kc = nullptr, *vt = nullptr, *qkv;
   TRY(enc_buf(e, "x", (size_t)n * EXN_W * 4, (void**)&x));
   TRY(enc_buf(e, "y", (size_t)n * EXN_W * 2, (void**)&y));
   TRY(enc_buf(e, "att", (size_t)n * EXN_W * 2, (void**)&att));
   TRY(enc_buf(e, "ff", (size_t)n * EXN_F * 2, (void**)&ff));
-  TRY(enc_buf(e, "q", (size_t)n * EXN_W * 2, (void**)&q));
-  TRY(enc_buf(e, "kc", (size_t)lcap * EXN_W * 2, (void**)&kc, true));
-  TRY(enc_buf(e, "vt", (size_t)lcap * EXN_W * 2, (void**)&vt, true));
+  if (!plan) {
+    TRY(enc_buf(e, "q", (size_t)n * EXN_W * 2, (void**)&q));
+    TRY(enc_buf(e, "kc", (size_t)lcap * EXN_W * 2, (void**)&kc, true));
+    TRY(enc_buf(e, "vt", (size_t)lcap * EXN_W * 2, (void**)&vt, true));
+  }
+  float* joins = nullptr;   // the cached attention's scratch
+  int64_t njoins = 0;
+  if (cache) {
+    njoins = kv8_attend_part(plan->rows, plan->ntiles, plan->longest, EXN_H, 8, EXN_HD, cache->cols);
+    TRY(enc_buf(e, "joins", (size_t)njoins * 4, (void**)&joins));
+  }
   TRY(enc_buf(e, "qkv", (size_t)n * (EXN_W + 2 * kEncKV) * 2, (void**)&qkv));
   // a prompt of at most 1024 tokens is about one row of 256-row tiles: its products split K
   // over the chip (the DiT's prompt-row path), the partial sums then added in order; a longer
@@ -396,11 +442,25 @@ static int enc_states(exn_enc* e, const int32_t* ids, int n, const float* cs, in
     ea.ldy = EXN_W + 2 * kEncKV;
     int ns = 0;
     HIPCHK(mm(L.qkv, y, EXN_W, EPI_F16, ea, &ns));
-    if (ns > 0)
+    if (plan) {
+      const int64_t ld = EXN_W + 2 * kEncKV;
+      const uint16_t *pk = qkv + EXN_W, *pv = pk + kEncKV;
+      const float scale = 0.08838834764831845f;   // 1 / sqrt(128)
+      HIPCHK(enc_qkv_rows(s, qkv, part, ns, n, L.vec[E_QNORM], L.vec[E_KNORM], cs));
+      if (cache) {
+        const Kv8 kv = cache_layer(cache, il);
+        HIPCHK(kv8_append(s, kv, plan->whole, plan->seqs, plan->longest, pk, ld, pv, ld));
+        HIPCHK(kv8_attend(s, kv, plan->tiles, plan->ntiles, plan->rows, plan->longest, EXN_H, qkv, ld, scale, att, 1,
+                          EXN_W, joins, njoins));
+      } else {
+        HIPCHK(attend_packed(s, plan->tiles, plan->ntiles, 0, EXN_H, 8, EXN_HD, qkv, ld, pk, ld, pv, ld, scale, att, 1,
+                             EXN_W));
+      }
+    } else if (ns > 0)
       HIPCHK(qkv_prep_part(s, part, ns, n, L.vec[E_QNORM], L.vec[E_KNORM], cs, q, kc, vt, 0, lcap, n, kEncGroup));
     else
       HIPCHK(qkv_prep(s, qkv, n, L.vec[E_QNORM], L.vec[E_KNORM], cs, q, kc, vt, 0, lcap, n, kEncGroup));
-    HIPCHK(attend(s, q, kc, vt, att, n, 0, n, n, lcap, 0, 0, 1.f));
+    if (!plan) HIPCHK(attend(s, q, kc, vt, att, n, 0, n, n, lcap, 0, 0, 1.f));
     ea = EpiArgs{};
     ea.resid = x;
     ea.ldy = EXN_W;
@@ -442,13 +502,10 @@ int exn_enc_states_dev(exn_enc* e, const int32_t* ids, int n, const float* cs, i
   return enc_states(e, ids, n, cs, pic0, m, merged, deep, out);
 }
 
-int exn_enc_states(exn_enc* e, const int32_t* ids, int n, const int32_t* pos, int pic0, int m, const float* merged,
-                   const float* deep, float* out) {
-  if (!e) FAIL(EXN_EINVAL, "null encoder");
-  TRY(use(e->ctx));
-  if (!ids || !out || n < 1 || n > 65536 || m < 0 || (m > 0 && (!merged || pic0 < 0 || pic0 + m > n)))
-    FAIL(EXN_EINVAL, "encoder states: n %d, picture rows %d at %d", n, m, pic0);
-  TRY(exn_enc_check(e));
+// the host-array form of a pass over n rows: ids checked, everything to the device and back
+static int enc_states_host(exn_enc* e, const int32_t* ids, int n, const int32_t* pos, int pic0, int m, const float* merged,
+                           const float* deep, float* out, const exn_seqs* plan = nullptr,
+                           const exn_enc_cache* cache = nullptr) {
   for (int t = 0; t < n; ++t)
     if (ids[t] < 0 || ids[t] >= e->vocab) FAIL(EXN_EINVAL, "encoder states: token %d is %d (vocab %lld)", t, ids[t], (long long)e->vocab);
   std::vector<float> cs((size_t)n * 128);
@@ -466,8 +523,225 @@ int exn_enc_states(exn_enc* e, const int32_t* ids, int n, const int32_t* pos, in
   }
   HIPCHK(hipMemcpyAsync(dids, ids, (size_t)n * 4, hipMemcpyHostToDevice, s));
   HIPCHK(hipMemcpyAsync(dcs, cs.data(), cs.size() * 4, hipMemcpyHostToDevice, s));
-  TRY(enc_states(e, dids, n, dcs, pic0, m, dpic, deep && m > 0 ? dpic + (int64_t)m * EXN_W : nullptr, dout));
+  TRY(enc_states(e, dids, n, dcs, pic0, m, dpic, deep && m > 0 ? dpic + (int64_t)m * EXN_W : nullptr, dout, plan, cache));
   HIPCHK(hipMemcpyAsync(out, dout, (size_t)n * EXN_W * 4, hipMemcpyDeviceToHost, s));
   HIPCHK(hipStreamSynchronize(s));
   return EXN_OK;
+}
+
+int exn_enc_states(exn_enc* e, const int32_t* ids, int n, const int32_t* pos, int pic0, int m, const float* merged,
+                   const float* deep, float* out) {
+  if (!e) FAIL(EXN_EINVAL, "null encoder");
+  TRY(use(e->ctx));
+  if (!ids || !out || n < 1 || n > 65536 || m < 0 || (m > 0 && (!merged || pic0 < 0 || pic0 + m > n)))
+    FAIL(EXN_EINVAL, "encoder states: n %d, picture rows %d at %d", n, m, pic0);
+  TRY(exn_enc_check(e));
+  return enc_states_host(e, ids, n, pos, pic0, m, merged, deep, out);
+}
+
+// --- several prompts in a pass -------------------------------------------------------------------
+
+int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s, const float* cs, float* out) {
+  if (!e || !s) FAIL(EXN_EINVAL, "null encoder or sequences");
+  TRY(use(e->ctx));
+  if (s->device != e->ctx->device) FAIL(EXN_EINVAL, "sequences planned on device %d, the encoder's is %d", s->device, e->ctx->device);
+  if (!ids || !cs || !out || s->rows < 1 || s->rows > 65536)
+    FAIL(EXN_EINVAL, "encoder states: %lld rows (1 to 65536), or a null pointer", (long long)s->rows);
+  TRY(exn_enc_check(e));
+  return enc_states(e, ids, (int)s->rows, cs, 0, 0, nullptr, nullptr, out, s);
+}
+
+namespace {
+// a plan that goes with its scope, after the work that reads it
+struct Plan {
+  exn_seqs* s = nullptr;
+  ~Plan() { exn_seqs_free(s); }
+};
+// the rows of SEQS lengths, or -1
+int64_t rows_of(const int32_t* lens, int seqs) {
+  int64_t n = 0;
+  for (int i = 0; i < seqs; ++i) {
+    if (lens[i] < 0) return -1;
+    n += lens[i];
+  }
+  return n;
+}
+// text positions of each sequence's new tokens, from START on (null: 0)
+std::vector<int32_t> text_positions(const int32_t* lens, const int32_t* start, int seqs, int64_t n) {
+  std::vector<int32_t> pos;
+  pos.reserve((size_t)n * 3);
+  for (int i = 0; i < seqs; ++i)
+    for (int t = 0; t < lens[i]; ++t) pos.insert(pos.end(), 3, (start ? start[i] : 0) + t);
+  return pos;
+}
+}  // namespace
+
+int exn_enc_states_packed(exn_enc* e, const int32_t* ids, const int32_t* lens, int seqs, const int32_t* pos, float* out) {
+  if (!e) FAIL(EXN_EINVAL, "null encoder");
+  if (!ids || !lens || !out || seqs < 1 || seqs > 65536) FAIL(EXN_EINVAL, "encoder states: %d prompts, or a null pointer", seqs);
+  const int64_t n = rows_of(lens, seqs);
+  if (n < 1 || n > 65536) FAIL(EXN_EINVAL, "encoder states: prompts of %lld tokens in all (1 to 65536), none negative", (long long)n);
+  TRY(use(e->ctx));
+  TRY(exn_enc_check(e));
+  try {
+    std::vector<int32_t> text;
+    if (!pos) {
+      text = text_positions(lens, nullptr, seqs, n);
+      pos = text.data();
+    }
+    Plan p;
+    TRY(exn_seqs_create(e->ctx, lens, seqs, &p.s));
+    return enc_states_host(e, ids, (int)n, pos, 0, 0, nullptr, nullptr, out, p.s);
+  } catch (const std::bad_alloc&) {
+    FAIL(EXN_ENOMEM, "encoder states: host memory");
+  }
+}
+
+// --- kept prompts, continued ----------------------------------------------------------------------
+
+int exn_enc_cache_create(exn_enc* e, int seqs, int tokens, exn_enc_cache** out) {
+  if (!out) FAIL(EXN_EINVAL, "null output");
+  *out = nullptr;
+  if (!e) FAIL(EXN_EINVAL, "null encoder");
+  if (seqs < 1 || seqs > 4096 || tokens < 1 || tokens > (1 << 20))
+    FAIL(EXN_EINVAL, "encoder cache: %d sequences (1 to 4096) of %d tokens (1 to 2^20)", seqs, tokens);
+  TRY(use(e->ctx));
+  exn_enc_cache* c = nullptr;
+  try {
+    c = new exn_enc_cache();
+    c->e = e;
+    c->seqs = seqs;
+    c->cols = (tokens + 63) / 64;
+    c->pages = seqs * c->cols;
+    c->lens.assign((size_t)seqs, 0);
+    c->table.assign((size_t)seqs * c->cols, -1);
+    c->refs.assign((size_t)c->pages, 0);
+    for (int p = c->pages; p-- > 0;) c->spare.push_back(p);
+  } catch (const std::bad_alloc&) {
+    delete c;
+    FAIL(EXN_ENOMEM, "encoder cache: host memory");
+  }
+  const size_t L = (size_t)e->layers, pg = (size_t)c->pages, codes = L * pg * c->block, tails = L * seqs * c->block * 2;
+  int r = dev_alloc((void**)&c->k, codes);
+  if (r == EXN_OK) r = dev_alloc((void**)&c->v, codes);
+  if (r == EXN_OK) r = dev_alloc((void**)&c->scales, L * pg * 16 * 4);
+  if (r == EXN_OK) r = dev_alloc((void**)&c->tk, tails);
+  if (r == EXN_OK) r = dev_alloc((void**)&c->tv, tails);
+  if (r == EXN_OK) r = dev_alloc((void**)&c->d_table, c->table.size() * 4);
+  if (r == EXN_OK) r = dev_alloc((void**)&c->d_lens, c->lens.size() * 4);
+  ++e->caches;
+  if (r != EXN_OK) {
+    exn_enc_cache_destroy(c);
+    return r;
+  }
+  *out = c;
+  return EXN_OK;
+}
+
+int exn_enc_cache_destroy(exn_enc_cache* c) {
+  if (!c) return EXN_OK;
+  TRY(use(c->e->ctx));
+  HIPCHK(hipStreamSynchronize(c->e->ctx->stream));
+  for (void* p : {(void*)c->k, (void*)c->v, (void*)c->scales, (void*)c->tk, (void*)c->tv, (void*)c->d_table, (void*)c->d_lens})
+    dev_free(p);
+  --c->e->caches;
+  delete c;
+  return EXN_OK;
+}
+
+int exn_enc_cache_lens(const exn_enc_cache* c, int32_t* lens, int seqs) {
+  if (!c || !lens || seqs != c->seqs) FAIL(EXN_EINVAL, "encoder cache lens: null pointer, or %d sequences", seqs);
+  for (int i = 0; i < seqs; ++i) lens[i] = c->lens[(size_t)i];
+  return EXN_OK;
+}
+
+// sequence I names no page from block B on
+static void cache_drop(exn_enc_cache* c, int i, int b) {
+  for (; b < c->cols; ++b) {
+    int32_t& p = c->table[(size_t)i * c->cols + b];
+    if (p >= 0 && --c->refs[(size_t)p] == 0) c->spare.push_back(p);
+    p = -1;
+  }
+}
+
+int exn_enc_cache_reset(exn_enc_cache* c, int seq) {
+  if (!c || seq < 0 || seq >= c->seqs) FAIL(EXN_EINVAL, "encoder cache reset: sequence %d", seq);
+  cache_drop(c, seq, 0);
+  c->lens[(size_t)seq] = 0;
+  return EXN_OK;
+}
+
+int exn_enc_cache_fork(exn_enc_cache* c, int from, int to) {
+  if (!c || from < 0 || from >= c->seqs || to < 0 || to >= c->seqs)
+    FAIL(EXN_EINVAL, "encoder cache fork: sequence %d to %d of %d", from, to, c ? c->seqs : 0);
+  if (from == to) return EXN_OK;
+  TRY(use(c->e->ctx));
+  // the tails of all layers: a strided copy of one sequence's share of each
+  if (c->lens[(size_t)from] % 64) {
+    const size_t each = c->block * 2, pitch = each * (size_t)c->seqs;
+    for (uint16_t* t : {c->tk, c->tv})
+      HIPCHK(hipMemcpy2DAsync((char*)t + (size_t)to * each, pitch, (const char*)t + (size_t)from * each, pitch, each,
+                              (size_t)c->e->layers, hipMemcpyDeviceToDevice, c->e->ctx->stream));
+  }
+  cache_drop(c, to, 0);
+  for (int b = 0; b < c->cols; ++b) {
+    const int32_t p = c->table[(size_t)from * c->cols + b];
+    c->table[(size_t)to * c->cols + b] = p;
+    if (p >= 0) ++c->refs[(size_t)p];
+  }
+  c->lens[(size_t)to] = c->lens[(size_t)from];
+  return EXN_OK;
+}
+
+int exn_enc_cache_extend(exn_enc_cache* c, const int32_t* ids, const int32_t* lens, int seqs, const int32_t* pos, int pic0,
+                         int m, const float* merged, const float* deep, float* out) {
+  if (!c) FAIL(EXN_EINVAL, "null cache");
+  if (!ids || !lens || !out || seqs != c->seqs) FAIL(EXN_EINVAL, "encoder cache extend: %d sequences of %d, or a null pointer", seqs, c->seqs);
+  const int64_t n = rows_of(lens, seqs);
+  if (n < 1 || n > 65536 || m < 0 || (m > 0 && (!merged || pic0 < 0 || (int64_t)pic0 + m > n)))
+    FAIL(EXN_EINVAL, "encoder cache extend: %lld new tokens (1 to 65536, none negative), picture rows %d at %d", (long long)n, m, pic0);
+  for (int i = 0; i < seqs; ++i)
+    if ((int64_t)c->lens[(size_t)i] + lens[i] > (int64_t)c->cols * 64)
+      FAIL(EXN_EINVAL, "encoder cache extend: sequence %d has %d tokens and gets %d, the cache holds %d", i,
+           c->lens[(size_t)i], lens[i], c->cols * 64);
+  exn_enc* e = c->e;
+  TRY(use(e->ctx));
+  TRY(exn_enc_check(e));
+  for (int64_t t = 0; t < n; ++t)
+    if (ids[t] < 0 || ids[t] >= e->vocab)
+      FAIL(EXN_EINVAL, "encoder cache extend: token %lld is %d (vocab %lld)", (long long)t, ids[t], (long long)e->vocab);
+  try {
+    std::vector<int32_t> text;
+    if (!pos) {
+      text = text_positions(lens, c->lens.data(), seqs, n);
+      pos = text.data();
+    }
+    Plan p;
+    TRY(exn_seqs_create(e->ctx, lens, seqs, &p.s));
+    // a page for each block that fills: sequences name COLS pages each at most, and there are as many
+    for (int i = 0; i < seqs; ++i)
+      for (int b = c->lens[(size_t)i] / 64; b < (c->lens[(size_t)i] + lens[i]) / 64; ++b) {
+        const int32_t page = c->spare.back();
+        c->spare.pop_back();
+        c->refs[(size_t)page] = 1;
+        c->table[(size_t)i * c->cols + b] = page;
+      }
+    hipStream_t s = e->ctx->stream;
+    int r = EXN_OK;
+    hipError_t h = hipMemcpyAsync(c->d_table, c->table.data(), c->table.size() * 4, hipMemcpyHostToDevice, s);
+    if (h == hipSuccess) h = hipMemcpyAsync(c->d_lens, c->lens.data(), c->lens.size() * 4, hipMemcpyHostToDevice, s);
+    if (h == hipSuccess) h = hipStreamSynchronize(s);
+    if (h != hipSuccess) {
+      exn::set_error("encoder cache extend: %s", hipGetErrorString(h));
+      r = EXN_EHIP;
+    }
+    if (r == EXN_OK) r = enc_states_host(e, ids, (int)n, pos, pic0, m, merged, deep, out, p.s, c);
+    for (int i = 0; i < seqs; ++i) {
+      if (r == EXN_OK) c->lens[(size_t)i] += lens[i];
+      else if (lens[i]) exn_enc_cache_reset(c, i);   // its last block may be half overwritten
+    }
+    return r;
+  } catch (const std::bad_alloc&) {
+    FAIL(EXN_ENOMEM, "encoder cache extend: host memory");
+  }
 }

@@ -66,6 +66,18 @@ struct exn_w {
   bool view = false;       // rows inside another allocation (not freed here)
 };
 
+// a plan of packed sequences (api_prompts.hip)
+struct exn_seqs {
+  int device = 0;
+  int seqs = 0, longest = 0;
+  int64_t rows = 0;
+  std::vector<int32_t> lens;
+  void* mem = nullptr;                    // the tile lists, then the sequences
+  const SeqTile* tiles[SEQ_TTS] = {};     // the sequences' tiles of SEQ_TT0 << i tokens, the costliest (causal) first
+  int64_t ntiles[SEQ_TTS] = {};
+  const SeqTile* whole = nullptr;         // one entry a sequence, in order
+};
+
 struct Buf {
   void* p = nullptr;
   size_t bytes = 0;

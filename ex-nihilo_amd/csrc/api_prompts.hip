@@ -5,17 +5,6 @@
 #include <new>
 #include <numeric>
 
-struct exn_seqs {
-  int device = 0;
-  int seqs = 0, longest = 0;
-  int64_t rows = 0;
-  std::vector<int32_t> lens;
-  void* mem = nullptr;                    // the tile lists, then the sequences
-  const SeqTile* tiles[SEQ_TTS] = {};     // the sequences' tiles of SEQ_TT0 << i tokens, the costliest (causal) first
-  int64_t ntiles[SEQ_TTS] = {};
-  const SeqTile* whole = nullptr;         // one entry a sequence, in order
-};
-
 constexpr int kSeqsMax = 1 << 16;
 constexpr int64_t kSeqRowsMax = 1 << 22;
 

@@ -423,5 +423,8 @@ hipError_t vis_attend_s(hipStream_t s, int n, int np, int heads, const uint16_t*
 // the prompt encoder (encoder.hip): the token embedding's rows, Q8_0 (qs, d) or fp32 (f32)
 hipError_t enc_embed(hipStream_t s, const int32_t* ids, int n, int64_t vocab, const int8_t* qs, const uint16_t* d,
                      const float* f32, int width, float* out);
+// q | k | v rows (n x 6144 fp16) with the q/k norms and the rotary, in place (S 0) or from S partial sums (S <= 8)
+hipError_t enc_qkv_rows(hipStream_t s, uint16_t* qkv, const float* part, int S, int64_t n, const float* wq,
+                        const float* wk, const float* cs);
 
 }  // namespace exn

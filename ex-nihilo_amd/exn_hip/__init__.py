@@ -160,6 +160,14 @@ SIGNATURES = {
     "exn_enc_check": (c_int, [vp]),
     "exn_enc_states": (c_int, [vp, vp, c_int, vp, c_int, c_int, vp, vp, vp]),
     "exn_enc_states_dev": (c_int, [vp, vp, c_int, vp, c_int, c_int, vp, vp, vp]),
+    "exn_enc_states_packed": (c_int, [vp, vp, vp, c_int, vp, vp]),
+    "exn_enc_states_packed_dev": (c_int, [vp, vp, vp, vp, vp]),
+    "exn_enc_cache_create": (c_int, [vp, c_int, c_int, POINTER(vp)]),
+    "exn_enc_cache_extend": (c_int, [vp, vp, vp, c_int, vp, c_int, c_int, vp, vp, vp]),
+    "exn_enc_cache_fork": (c_int, [vp, c_int, c_int]),
+    "exn_enc_cache_reset": (c_int, [vp, c_int]),
+    "exn_enc_cache_lens": (c_int, [vp, vp, c_int]),
+    "exn_enc_cache_destroy": (c_int, [vp]),
     "exn_enc_rope_table": (c_int, [vp, c_int, c_double, vp]),
     "exn_enc_release": (c_int, [vp]),
     "exn_enc_destroy": (c_int, [vp]),
@@ -809,6 +817,77 @@ def encoder_states(e: Encoder, ids, pos=None, picture=None):
         call("exn_enc_states", e.h, ptr(ids), n, None if p is None else ptr(p), a0, len(mg), ptr(mg),
              None if dp is None else ptr(dp), ptr(out))
     return out
+
+
+def _packed(rows, width, dtype):
+    """Per-prompt arrays as one, and their lengths."""
+    a = [np.ascontiguousarray(r, dtype=dtype).reshape((-1, width) if width else -1) for r in rows]
+    return np.concatenate(a) if a else np.zeros((0, width) if width else 0, dtype), np.array([len(x) for x in a], np.int32)
+
+
+def encoder_states_packed(e: Encoder, prompts, pos=None):
+    """encoder_states of several prompts (lists of token ids) in one pass: a list of (n, 4096).
+    POS: each prompt's (n, 3) positions, or None (text 0..n-1 each)."""
+    ids, lens = _packed(prompts, 0, np.int32)
+    p = None
+    if pos is not None:
+        p, pl = _packed(pos, 3, np.int32)
+        if not np.array_equal(pl, lens):
+            raise ExnError(EINVAL, "positions of %s tokens for prompts of %s" % (pl.tolist(), lens.tolist()))
+    out = np.empty((len(ids), WIDTH), np.float32)
+    call("exn_enc_states_packed", e.h, ptr(ids), ptr(lens), len(lens), None if p is None else ptr(p), ptr(out))
+    return np.split(out, np.cumsum(lens)[:-1])
+
+
+class EncoderCache:
+    """Prompts kept and continued: SEQS sequences of up to TOKENS tokens (exn_enc_cache_create)."""
+
+    def __init__(self, e: Encoder, seqs: int, tokens: int):
+        h = vp()
+        call("exn_enc_cache_create", e.h, seqs, tokens, ctypes.byref(h))
+        self.e, self.h, self.seqs = e, h, seqs
+
+    def extend(self, new, pos=None, picture=None):
+        """NEW: {sequence: token ids}; the new tokens' states, {sequence: (n, 4096)}.  POS:
+        {sequence: (n, 3)} or None (text, on from the sequence's tokens); PICTURE: (sequence, a0, merged,
+        deep or None), the picture's rows from that sequence's new row a0 on."""
+        if any(s < 0 or s >= self.seqs for s in new):
+            raise ExnError(EINVAL, "sequences %s of %d" % (sorted(new), self.seqs))
+        ids, lens = _packed([new.get(s, ()) for s in range(self.seqs)], 0, np.int32)
+        p = None
+        if pos is not None:
+            p, pl = _packed([pos.get(s, ()) for s in range(self.seqs)], 3, np.int32)
+            if not np.array_equal(pl, lens):
+                raise ExnError(EINVAL, "positions of %s tokens for new ones of %s" % (pl.tolist(), lens.tolist()))
+        out = np.empty((len(ids), WIDTH), np.float32)
+        starts = np.concatenate([[0], np.cumsum(lens)])
+        pic = (0, 0, None, None)
+        if picture is not None:
+            s, a0, merged, deep = picture
+            mg = np.ascontiguousarray(merged, dtype=np.float32)
+            dp = None if deep is None else np.ascontiguousarray(deep, dtype=np.float32)
+            if a0 < 0 or a0 + len(mg) > lens[s]:
+                raise ExnError(EINVAL, "picture rows %d at %d of %d new tokens" % (len(mg), a0, lens[s]))
+            pic = (int(starts[s]) + a0, len(mg), ptr(mg), None if dp is None else ptr(dp))
+        call("exn_enc_cache_extend", self.h, ptr(ids), ptr(lens), self.seqs, None if p is None else ptr(p), *pic, ptr(out))
+        return {s: out[starts[s]:starts[s + 1]] for s in new}
+
+    def fork(self, src: int, dst: int):
+        """Sequence DST becomes SRC as it stands, sharing the pages of its full blocks."""
+        call("exn_enc_cache_fork", self.h, src, dst)
+
+    def reset(self, seq: int):
+        call("exn_enc_cache_reset", self.h, seq)
+
+    def lens(self):
+        a = np.empty(self.seqs, np.int32)
+        call("exn_enc_cache_lens", self.h, ptr(a), self.seqs)
+        return a
+
+    def destroy(self):
+        if self.h:
+            call("exn_enc_cache_destroy", self.h)
+            self.h = None
 
 
 def enc_rope_table(n: int, pos=None, base: float = ENC_ROPE_BASE):

@@ -490,6 +490,31 @@ int exn_enc_states_dev(exn_enc* e, const int32_t* ids, int n, const float* cs, i
  * by its position on axis j mod 3 (t, h, w) below 60, by t above, at BASE^(-2j/128); the cos and
  * sin of pair j at CS[128 t + 2j] and [128 t + 2j + 1] (rotate_half's dims j and j + 64). */
 int exn_enc_rope_table(const int32_t* pos, int n, double base, float* cs);
+/* exn_enc_states of SEQS prompts in one pass (no reference counterpart: illatio runs them one by
+ * one): LENS tokens each (host memory; 0 is allowed), IDS, POS and OUT's rows one prompt after the
+ * other, at most 65536 in all; POS NULL gives each text positions from 0.  A prompt's states do not
+ * depend on the others'.  _dev: a plan of the prompts (exn_seqs_create) and device arrays, CS the rows'
+ * rotary table. */
+int exn_enc_states_packed(exn_enc* e, const int32_t* ids, const int32_t* lens, int seqs, const int32_t* pos, float* out);
+int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s, const float* cs, float* out);
+/* Prompts kept and continued (no reference counterpart): keys and values of SEQS sequences of up to
+ * TOKENS tokens (rounded up to 64) through every layer, as exn_kv8 holds them, 74 kB a token at 36
+ * layers (147 kB in 16 bits) and 9.4 MB of tails a sequence.  exn_enc_cache_extend: LENS new tokens of
+ * each sequence (SEQS lengths, 0 for those that wait), packed as in exn_enc_states_packed; POS NULL
+ * goes on from the sequence's tokens so far; the picture's rows as in exn_enc_states, among the new
+ * rows; OUT the new rows' states.  A full block is seen in 8 bits, by the tokens that filled it too.
+ * exn_enc_cache_fork: sequence TO becomes FROM as it stands, sharing the pages of its full blocks (a
+ * template and a picture's rows encoded once, continued by several instructions).  A refused call
+ * changes nothing; one that fails on the GPU empties the sequences it was to extend.  An encoder is
+ * destroyed after its caches (EXN_ESTATE before). */
+typedef struct exn_enc_cache exn_enc_cache;
+int exn_enc_cache_create(exn_enc* e, int seqs, int tokens, exn_enc_cache** out);
+int exn_enc_cache_extend(exn_enc_cache* c, const int32_t* ids, const int32_t* lens, int seqs, const int32_t* pos, int pic0,
+                         int m, const float* merged, const float* deep, float* out);
+int exn_enc_cache_fork(exn_enc_cache* c, int from, int to);
+int exn_enc_cache_reset(exn_enc_cache* c, int seq);
+int exn_enc_cache_lens(const exn_enc_cache* c, int32_t* lens, int seqs);
+int exn_enc_cache_destroy(exn_enc_cache* c);
 /* scratch freed, weights kept; destroy frees both */
 int exn_enc_release(exn_enc* e);
 int exn_enc_destroy(exn_enc* e);
