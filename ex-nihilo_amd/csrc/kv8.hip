@@ -344,22 +344,33 @@ __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* l
 __device__ __forceinline__ int kv8_blocks(const Kv8& c, const SeqTile& t) {
   return (kv8_total(c, kv8_base(c, t.seq), t.len) + 63) >> 6;
 }
-// by a wave: the blocks of tiles 0 .. n-1; *FIRST, if not null, where tile I's begin
-__device__ __forceinline__ int kv8_sum_blocks(const Kv8Args& A, int n, int i, int* first) {
+// How k_kv8_few's workgroups share the blocks of all tiles, one after the other (a wave finds it out).
+// SHARE consecutive ones each; or, where there is a workgroup for every tile and none has over 16, a
+// tile each: then nothing is left to be joined.
+struct Kv8Share {
+  int all, share;   // share 0: a tile each
+  int first;        // where tile I's blocks begin
+};
+__device__ __forceinline__ Kv8Share kv8_share(const Kv8Args& A, int i) {
   const int lane = threadIdx.x & 63;
-  int all = 0, before = 0;
-  for (int t = lane; t < n; t += 64) {
+  int all = 0, first = 0, most = 0;
+#pragma unroll 4
+  for (int t = lane; t < A.ntiles; t += 64) {
     const int nb = kv8_blocks(A.c, A.tiles[t]);
     all += nb;
-    before += t < i ? nb : 0;
+    first += t < i ? nb : 0;
+    most = max(most, nb);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     all += __shfl_xor(all, o, 64);
-    before += __shfl_xor(before, o, 64);
+    first += __shfl_xor(first, o, 64);
+    most = max(most, __shfl_xor(most, o, 64));
   }
-  if (first) *first = before;
-  return all;
+  const bool each = A.ntiles <= A.splits && most <= 16;
+  return Kv8Share{__builtin_amdgcn_readfirstlane(all),
+                  each ? 0 : __builtin_amdgcn_readfirstlane(max(A.least, (all + A.splits - 1) / A.splits)),
+                  __builtin_amdgcn_readfirstlane(first)};
 }
 
 #define MAX_SLACK 8.f
@@ -395,11 +406,11 @@ k_kv8_few(Kv8Args A) {
 
   // this workgroup's share: blocks [from, to) of the run of all tiles' blocks; tile I's begin at AT
   int i = w, at = 0, from = 0, to = 0x7FFFFFFF;
-  if (A.splits) {
-    const int all = __builtin_amdgcn_readfirstlane(kv8_sum_blocks(A, A.ntiles, 0, nullptr));
-    const int share = max(A.least, (all + A.splits - 1) / A.splits);
-    from = w * share;
-    to = min(all, from + share);
+  const Kv8Share sh = A.splits ? kv8_share(A, 0) : Kv8Share{0, 0, 0};
+  if (i >= A.ntiles && sh.share == 0) return;
+  if (sh.share) {
+    from = w * sh.share;
+    to = min(sh.all, from + sh.share);
     if (from >= to) return;
     i = 0;
     for (int t0 = 0; t0 < A.ntiles; t0 += 64) {   // the tile in which FROM lies
@@ -516,7 +527,7 @@ k_kv8_few(Kv8Args A) {
       lrun[rt] = 0.f;
     }
     float s[RT][16];   // scores of keys 16 g + e of the block in hand
-    uint32_t pk[RT][8];
+    uint32_t pk[RT][8], pl[RT][BF ? 8 : 1];   // weights; the tail's, in bf16, as two parts
 
     // from scores (log2 units, hidden ones -inf) to weights: the rows' references, sums and pk
     auto weights = [&](auto bf_c) __attribute__((always_inline)) {
@@ -540,6 +551,8 @@ k_kv8_few(Kv8Args A) {
         for (int e = 0; e < 16; e += 2) {
           const float p0 = __builtin_amdgcn_exp2f(s[rt][e] - ref), p1 = __builtin_amdgcn_exp2f(s[rt][e + 1] - ref);
           pk[rt][e / 2] = decltype(bf_c)::value ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+          if constexpr (decltype(bf_c)::value)
+            pl[rt][e / 2] = pack_bf16x2(p0 - bf16_lo(pk[rt][e / 2]), p1 - bf16_hi(pk[rt][e / 2]));
           lrun[rt] += p0;
           lrun[rt] += p1;
         }
@@ -652,6 +665,11 @@ k_kv8_few(Kv8Args A) {
           for (int u = 0; u < 2; ++u)
             v[u] = __builtin_shufflevector(v4(16 * g + 8 * u, d), v4(16 * g + 8 * u + 4, d), 0, 1, 2, 3, 4, 5, 6, 7);
           a[d] = mfma16<BF>(v[1], pfrag(rt, 1), mfma16<BF>(v[0], pfrag(rt, 0), f32x4{}));
+          if constexpr (BF) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              a[d] = mfma16<BF>(v[u], __builtin_bit_cast(s16x8, u32x4{pl[rt][4 * u], pl[rt][4 * u + 1], pl[rt][4 * u + 2], pl[rt][4 * u + 3]}), a[d]);
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(a[d][e]) & 0x7F800000u) == 0x7F800000u;
           __builtin_amdgcn_sched_barrier(0);
@@ -685,7 +703,7 @@ k_kv8_few(Kv8Args A) {
     int mt = tid;
     asm volatile("" : "+v"(mt));   // as above
     // the next tile's first loads, then this one's sums meet: 16 threads a row, all waves' sums of it
-    const bool whole = S.lo == 0 && S.hi == S.nb, more = at + S.nb < to && i + 1 < A.ntiles && A.splits;
+    const bool whole = S.lo == 0 && S.hi == S.nb, more = sh.share && at + S.nb < to;
     const int nb = S.nb, lo = S.lo;
     if (more) {
       at += nb;
@@ -766,10 +784,9 @@ k_kv8_join_few(Kv8Args A) {
   const int r = blockIdx.y, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
   const SeqTile T = A.tiles[i];
   if (tok >= T.len || head >= min(A.hh, A.group - chunk * A.hh)) return;
-  int first;
-  const int all = kv8_sum_blocks(A, A.ntiles, i, &first);
-  const int nb = kv8_blocks(A.c, T), share = max(A.least, (all + A.splits - 1) / A.splits);
-  const int w0 = first / share, w1 = (first + nb - 1) / share;   // the workgroups that had a part
+  const Kv8Share s = kv8_share(A, i);
+  if (s.share == 0) return;
+  const int w0 = s.first / s.share, w1 = (s.first + kv8_blocks(A.c, T) - 1) / s.share;   // the workgroups that had a part
   if (w0 == w1) return;
   const int tid = threadIdx.x, sh = tid / TH, d = tid % TH * 4;
   const float* ml = A.part + (int64_t)A.splits * per * 32 * RT * HD;
@@ -877,7 +894,8 @@ __device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int tota
   *l_ = l;
 }
 
-template <int BF, int HD>
+// LO: weights as two bf16 parts, where a bf16 cache gives fp16 rows
+template <int BF, int HD, int LO>
 __global__ void __launch_bounds__(256, 2)
 k_kv8_chunk(Kv8Args A) {
   constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
@@ -1067,7 +1085,7 @@ k_kv8_chunk(Kv8Args A) {
     }
     constexpr int KD = 3, NI = 2 * NS, PS = 16 / NI;
     f32x16 sn[2];
-    uint32_t pk[16];
+    uint32_t pk[16], pl[LO ? 16 : 1];
     float ls[2] = {};
     s16x8 kq[KD], vq[KD];
     if constexpr (!LAST) {
@@ -1093,13 +1111,17 @@ k_kv8_chunk(Kv8Args A) {
         const float p0 = __builtin_amdgcn_exp2f(sc[h][r]), p1 = __builtin_amdgcn_exp2f(sc[h][r + 1]);
         pk[pi] = BF ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
         ls[pi % 2] = weight_sum<BF>(pk[pi], ls[pi % 2]);
+        if constexpr (LO) {
+          pl[pi] = pack_bf16x2(p0 - bf16_lo(pk[pi]), p1 - bf16_hi(pk[pi]));
+          ls[pi % 2] = weight_sum<BF>(pl[pi], ls[pi % 2]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     lrun = __builtin_fmaf(ls[0] + ls[1], __builtin_amdgcn_exp2f(-lv), lrun);
     if (F.vd == 0.f) {   // whatever the codes, the values are 0
 #pragma unroll
-      for (int i = 0; i < 16; ++i) pk[i] = 0;
+      for (int i = 0; i < 16; ++i) pk[i] = pl[LO ? i : 0] = 0;
     }
 #pragma unroll
     for (int j = 0; j < 4 * ND; ++j) {
@@ -1108,6 +1130,9 @@ k_kv8_chunk(Kv8Args A) {
       const int u = j / ND;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
       o[j % ND] = mfma32<BF>(vq[0], pb, o[j % ND]);
+      if constexpr (LO)
+        o[j % ND] = mfma32<BF>(vq[0], __builtin_bit_cast(s16x8, u32x4{pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]}),
+                               o[j % ND]);
 #pragma unroll
       for (int d = 0; d + 1 < KD; ++d) vq[d] = vq[d + 1];
       vq[KD - 1] = vn;
@@ -1315,7 +1340,7 @@ Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim,
     const int64_t each = (int64_t)per * 32 * w.rt * (head_dim + 2);
     if (s * each > part_cap) s = part_cap / each;
     w.least = 16;
-    if (cols > 16 && s > 1 && ntiles[w.z] <= 4096) {
+    if (cols > 16 && s > 1 && ntiles[w.z] * per <= 4 * slots) {
       w.splits = (int)s;
       w.floats = s * each;
     } else if (w.rt == 1 && ntiles[w.z] * per <= 256) {
@@ -1376,7 +1401,8 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * w.wv), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-    w.rt == 0 ? go(k_kv8_chunk<BF, HD>) : w.rt == 2 ? go(k_kv8_few<BF, HD, 2, 4>)
+    if (w.rt == 0) return BF && !obf ? go(k_kv8_chunk<BF, HD, BF>) : go(k_kv8_chunk<BF, HD, 0>);
+    w.rt == 2 ? go(k_kv8_few<BF, HD, 2, 4>)
     : w.wv == 8 ? go(k_kv8_few<BF, HD, 1, 8>) : go(k_kv8_few<BF, HD, 1, 4>);
   };
   typedef std::integral_constant<int, 0> I0;

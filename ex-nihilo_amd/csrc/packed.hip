@@ -100,8 +100,9 @@ struct PackedArgs {
   int obf;
 };
 
-// grid: tiles x chunks x kv_heads, the heads fastest; block 256
-template <int BF, int HD>
+// grid: tiles x chunks x kv_heads, the heads fastest; block 256.  LO: weights as two bf16 parts, where
+// bf16 inputs give fp16 rows: one part's half step, 2^-9, would be eight of the output's.
+template <int BF, int HD, int LO>
 __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2)
 k_attend_packed(PackedArgs A) {
   constexpr int ROWB = HD * 2, STAGE = PK * ROWB;   // bytes of a key's row; of a tile
@@ -263,7 +264,7 @@ k_attend_packed(PackedArgs A) {
     // slots of the S product.  A slot of the S product takes its share of the tile's 16 pairs of p.
     constexpr int KD = 3, NI = 2 * NS, PS = 16 / NI;
     f32x16 sn[2];
-    uint32_t pk[16];   // pair i: keys of S element (i / 8, 2 (i % 8)) and the next
+    uint32_t pk[16], pl[LO ? 16 : 1];   // pair i: keys of S element (i / 8, 2 (i % 8)) and the next
     s16x8 kq[KD], vq[KD];
     if constexpr (!LAST) {
       sn[0] = f32x16{};
@@ -287,6 +288,7 @@ k_attend_packed(PackedArgs A) {
         const int pi = PS * i + e, b = pi / 8, r = 2 * (pi % 8);
         const float p0 = __builtin_amdgcn_exp2f(sc[b][r]), p1 = __builtin_amdgcn_exp2f(sc[b][r + 1]);
         pk[pi] = pack16(p0, p1, BF);
+        if constexpr (LO) pl[pi] = pack_bf16x2(p0 - bf16_lo(pk[pi]), p1 - bf16_hi(pk[pi]));
         lrun += p0;
         lrun += p1;
       }
@@ -301,6 +303,9 @@ k_attend_packed(PackedArgs A) {
       const int u = j / ND;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
       o[j % ND] = mfma32<BF>(vq[0], pb, o[j % ND]);
+      if constexpr (LO)
+        o[j % ND] = mfma32<BF>(vq[0], __builtin_bit_cast(s16x8, u32x4{pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]}),
+                               o[j % ND]);
 #pragma unroll
       for (int d = 0; d + 1 < KD; ++d) vq[d] = vq[d + 1];
       vq[KD - 1] = vn;
@@ -409,10 +414,12 @@ hipError_t attend_packed(hipStream_t s, const SeqTile* const* tiles, const int64
   const int64_t groups = ntiles[z] * a.chunks * kv_heads;
   if (groups > INT32_MAX) return hipErrorInvalidValue;
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, s, a); };
-  if (bf16)
-    head_dim == 128 ? go(k_attend_packed<1, 128>) : go(k_attend_packed<1, 64>);
+  if (bf16 && obf)
+    head_dim == 128 ? go(k_attend_packed<1, 128, 0>) : go(k_attend_packed<1, 64, 0>);
+  else if (bf16)
+    head_dim == 128 ? go(k_attend_packed<1, 128, 1>) : go(k_attend_packed<1, 64, 1>);
   else
-    head_dim == 128 ? go(k_attend_packed<0, 128>) : go(k_attend_packed<0, 64>);
+    head_dim == 128 ? go(k_attend_packed<0, 128, 0>) : go(k_attend_packed<0, 64, 0>);
   return hipGetLastError();
 }
 

@@ -28,12 +28,13 @@ def rounded(x, t):
     return np.where(np.isnan(x), np.nan, r)
 
 
-def attend(q, k, v, seen, scale, dt, odt):
+def attend(q, k, v, seen, scale, dt, odt, codes=False):
     """One head: q [n][hd] over k, v [m][hd], row i seeing the keys of seen [n][m]; zeros where it
     sees none.  The values and how far a kernel may be off them, element by element:
     - a weight p (at most 2^8 times the running largest: the sum of p is at least 1) is rounded to
       DT: half a step of p, and 2^-25 where fp16 has no smaller step; and, on the sum's side, the
-      same again at most
+      same again at most.  For bf16 in and fp16 out it is held as two bf16 parts: 2^-16 (CODES: a
+      cache's codes of either type may take fp16 weights)
     - a score is a sum of hd products in fp32, off by at most hd 2^-24 sum |q k|, scaled (and
       SCALE log2(e) rounded: 2^-23 of it); p is off by as much times ln 2, plus 2^-22 of exp2 itself
     - the sums over m keys are off by at most m 2^-24 of the sum of |p v|
@@ -51,9 +52,10 @@ def attend(q, k, v, seen, scale, dt, odt):
     o = p @ v / l
     m, hd = k.shape
     top = np.where(seen, abs(scale) * (abs(q) @ abs(k).T), 0).max(1, keepdims=True, initial=0)
-    c = 2 * HALF[dt] + 2 * m * 2.0 ** -24 + 2 * (top * (hd + 3) * 2.0 ** -24 + 2.0 ** -22)
+    held = HALF[dt] if dt == odt or odt == "bf16" else HALF["fp16"] if codes else 2.0 ** -16
+    c = 2 * held + 2 * m * 2.0 ** -24 + 2 * (top * (hd + 3) * 2.0 ** -24 + 2.0 ** -22)
     size = p @ abs(v) / l
-    low = m * 2.0 ** -25 * abs(v).max(initial=0) if dt == "fp16" else 0.0
+    low = m * 2.0 ** -25 * abs(v).max(initial=0) if dt == "fp16" or codes else 0.0
     tol = 1.01 * (size * c + low) + HALF[odt] * (abs(o) + size * c + low) + (2.0 ** -25 if odt == "fp16" else 1e-38)
     return o, tol
 
@@ -162,7 +164,7 @@ class Cache:
                 seen = (np.arange(len(k)) <= place[:, None]) & there
                 for h in range(q.shape[1]):
                     o[r:r + n, h], tol[r:r + n, h] = attend(q[r:r + n, h], k[:, h // group], v[:, h // group], seen,
-                                                            scale, self.dt, odt)
+                                                            scale, self.dt, odt, True)
             r += n
         return o, tol
 
