@@ -903,7 +903,8 @@ k_kv8_chunk(Kv8Args A) {
   constexpr int CI = HD / 64;                       // 16-byte loads of codes a thread and block
   // K stage s at s STAGE: rows of keys, 16-byte chunk c at c ^ (key % 16) (HD 64: c ^ (key / 2 % 8)).
   // V^T stage s at (2 + s) STAGE: rows of dims of 128 bytes, chunk c at c ^ (dim / 2 % 8); a row's
-  // keys in vt_pos's order, the one in which a lane's weights lie.
+  // keys in vt_pos's order, the one in which a lane's weights lie.  The tail's V is as in memory, rows
+  // of keys, chunk c at c ^ 4 (key % 4) (HD 64: c ^ 4 (key / 2 % 2)), and is turned when it is read.
   __shared__ __align__(1024) uint8_t smem[4 * STAGE];
   const Kv8& c = A.c;
   const int per = c.kv_heads * A.chunks;
@@ -960,7 +961,16 @@ k_kv8_chunk(Kv8Args A) {
     return x;
   };
   const int64_t th = ((int64_t)T.seq * c.kv_heads + kvh) * 64 * HD;
-  // block B's K (codes in KC, or the tail's rows; those past its last token as zeros) into a stage
+  // the tail's 64 rows by DMA; those past its last token hold anything
+  auto tail = [&](const uint16_t* all, uint8_t* p, auto swizzle) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int e = wave; e < 64 * ROWB / 1024; e += 4) {
+      const int r = e * (1024 / ROWB) + lane / (HD / 8), x = lane % (HD / 8) ^ swizzle(r);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(all + th + r * HD + 8 * x),
+                                       (lds_void*)(p + e * 1024), 16, 0, 0);
+    }
+  };
+  // block B's K, the codes X or the tail's rows, into a stage
   auto fill_k = [&](int b, int st, const Codes& x) __attribute__((always_inline)) {
     uint8_t* p = smem + st * STAGE;
     if (b < nfull) {
@@ -972,12 +982,7 @@ k_kv8_chunk(Kv8Args A) {
         *(s16x8*)(p + key * ROWB + (((c2 + 1) ^ z) << 4)) = codes8<BF>(x.w[i][2], x.w[i][3]);
       }
     } else {
-      for (int ci = tid; ci < 64 * HD / 8; ci += 256) {
-        const int key = ci / (HD / 8), cc = ci % (HD / 8), z = HD == 128 ? key & 15 : (key >> 1) & 7;
-        u32x4 w = {};
-        if (b * 64 + key < total) w = *(const u32x4*)(c.tk + th + ci * 8);
-        *(u32x4*)(p + key * ROWB + ((cc ^ z) << 4)) = w;
-      }
+      tail(c.tk, p, [&](int r) { return HD == 128 ? r & 15 : (r >> 1) & 7; });
     }
   };
   auto fill_v = [&](int b, int st, const Codes& x) __attribute__((always_inline)) {
@@ -990,15 +995,7 @@ k_kv8_chunk(Kv8Args A) {
         *(s16x8*)(p + dim * 128 + (((c2 + 1) ^ z) << 4)) = codes8<BF>(x.w[i][1], x.w[i][3]);
       }
     } else {
-      for (int ci = tid; ci < 64 * HD / 8; ci += 256) {
-        const int key = ci / (HD / 8), d0 = ci % (HD / 8) * 8, pos = (int)vt_pos(key);
-        u32x4 w = {};
-        if (b * 64 + key < total) w = *(const u32x4*)(c.tv + th + ci * 8);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *(uint16_t*)(p + (d0 + e) * 128 + (((pos >> 3) ^ ((d0 + e) >> 1 & 7)) << 4) + (pos & 7) * 2) =
-              (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-      }
+      tail(c.tv, p, [&](int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); });
     }
   };
   int kofs[NS], vofs[4];   // K row lo, chunk 2s + hi; V^T row lo, chunk 2u + hi
@@ -1007,7 +1004,18 @@ k_kv8_chunk(Kv8Args A) {
 #pragma unroll
   for (int u = 0; u < 4; ++u) vofs[u] = 2 * STAGE + lo * 128 + (((2 * u + hi) ^ ((lo >> 1) & 7)) << 4);
   auto kfrag = [&](int i) { return *(const s16x8*)(smem + kofs[i / 2] + (i % 2) * 32 * ROWB); };
-  auto vfrag = [&](int j) { return *(const s16x8*)(smem + vofs[j / ND] + (j % ND) * 32 * 128); };
+  auto vfrag = [&](auto tail_c, int j) __attribute__((always_inline)) {
+    if constexpr (decltype(tail_c)::value) {
+      typedef __attribute__((address_space(3))) s16x4 lds_s4;
+      const int r = 4 * hi + ((lane & 15) >> 2), x = 4 * (j % ND) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      uint8_t* p = smem + ((vofs[0] & ~(STAGE - 1)) + (16 * (j / ND) + r) * ROWB +
+                           ((x ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))) << 4) + 8 * (lane & 1));
+      return __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p),
+                                     __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * ROWB)), 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return *(const s16x8*)(smem + vofs[j / ND] + (j % ND) * 32 * 128);
+    }
+  };
 
   f32x16 o[ND], sc[2];
   float mrun = 0.f, lrun = 0.f;
@@ -1015,15 +1023,16 @@ k_kv8_chunk(Kv8Args A) {
   int top = -1000;           // E: the sums are in units of 2^E
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x16{};
-  auto barrier = [&]() __attribute__((always_inline)) {
+  auto barrier = [&](bool dma) __attribute__((always_inline)) {   // DMA: with the tail's rows asked for before it
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    if (dma) __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0xC07F);            // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
 
   // Block B of facts F: its softmax, the S product of block b+1 interleaved with its exp2, O^T += V^T P^T
-  auto step = [&](auto last_c, int b, const Facts& F) __attribute__((always_inline)) {
+  auto step = [&](auto last_c, auto tail_c, int b, const Facts& F) __attribute__((always_inline)) {
     constexpr bool LAST = decltype(last_c)::value;
     const int k0 = b * 64;
     const float factor = F.kd * A.scale;
@@ -1104,7 +1113,7 @@ k_kv8_chunk(Kv8Args A) {
         for (int d = 0; d + 1 < KD; ++d) kq[d] = kq[d + 1];
         kq[KD - 1] = kn;
       }
-      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(i - (NI - KD));
+      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(tail_c, i - (NI - KD));
 #pragma unroll
       for (int z = 0; z < PS; ++z) {
         const int pi = PS * i + z, h = pi / 8, r = 2 * (pi % 8);
@@ -1126,7 +1135,7 @@ k_kv8_chunk(Kv8Args A) {
 #pragma unroll
     for (int j = 0; j < 4 * ND; ++j) {
       s16x8 vn = {};
-      if (j + KD < 4 * ND) vn = vfrag(j + KD);
+      if (j + KD < 4 * ND) vn = vfrag(tail_c, j + KD);
       const int u = j / ND;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
       o[j % ND] = mfma32<BF>(vq[0], pb, o[j % ND]);
@@ -1154,7 +1163,7 @@ k_kv8_chunk(Kv8Args A) {
     kn = fetch(c.k, F1.page);
   }
   fill_k(b0, 0, kc);
-  barrier();
+  barrier(b0 == nfull);
   sc[0] = f32x16{};
   sc[1] = f32x16{};
 #pragma unroll
@@ -1175,7 +1184,8 @@ k_kv8_chunk(Kv8Args A) {
   for (int s = 0; s < NS; ++s) kofs[s] ^= STAGE;
   int b = b0;
   for (; b + 1 < b1; ++b) {
-    barrier();   // K of block b+1 and V of block b are filled; K of b and V of b-1 are done with
+    // K of block b+1 and V of block b are filled; K of b and V of b-1 are done with
+    barrier(b + 1 == nfull);
     fill_v(b + 1, (b + 1 - b0) & 1, vc);
     if (b + 2 < b1) {
       fill_k(b + 2, (b - b0) & 1, kc);
@@ -1186,7 +1196,7 @@ k_kv8_chunk(Kv8Args A) {
       F3 = facts(b + 3);
       kc = fetch(c.k, F3.page);
     }
-    step(std::integral_constant<bool, false>(), b, F0);
+    step(std::integral_constant<bool, false>(), std::integral_constant<bool, false>(), b, F0);
     F0 = F1;
     F1 = F2;
     F2 = F3;
@@ -1195,8 +1205,15 @@ k_kv8_chunk(Kv8Args A) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) vofs[u] ^= STAGE;
   }
-  barrier();
-  step(std::integral_constant<bool, true>(), b, F0);
+  barrier(b == nfull);
+  if (b < nfull) {
+    step(std::integral_constant<bool, true>(), std::integral_constant<bool, false>(), b, F0);
+  } else {
+    uint8_t* p = smem + (2 + ((b - b0) & 1)) * STAGE;   // V's rows past the last token: zeros
+    for (int e = (total - b * 64) * (HD / 8) + tid; e < 64 * HD / 8; e += 256) *(u32x4*)(p + e * 16) = u32x4{};
+    barrier(false);
+    step(std::integral_constant<bool, true>(), std::integral_constant<bool, true>(), b, F0);
+  }
 
   float la = lrun, lb = lrun;
   xswap32(la, lb);
