@@ -58,7 +58,9 @@ __device__ __forceinline__ uint32_t kv8_codes4(const float* x, float d, float r)
 // what it costs.  A thread has 4 tokens x HD / 16 dims of a block in registers, from the tail or the
 // new rows, between the block's largest |x| and its codes; values leave through LDS, where four
 // tokens' codes of a dim are a dword.  Block 0's workgroup also writes the tail, after it has read the
-// old one: the one slot serves the block that fills and the block begun after it.
+// old one: the one slot serves the block that fills and the block begun after it.  With the read below,
+// 8 x 1100 tokens (8 heads of 128, bf16) 22.1 us, 4.9 TB/s of what a copy's 5.1 allow; 64 x 1 token
+// 10 us, two launches' time.
 template <int BF, int HD>
 __global__ void __launch_bounds__(256)
 k_kv8_append(Kv8 c, const SeqTile* __restrict__ seqs, const uint16_t* __restrict__ k, int64_t ldk,
@@ -163,7 +165,7 @@ hipError_t kv8_append(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, i
   return hipGetLastError();
 }
 
-// the step's rows as the cache holds them, 16 bits (code x d rounded once): workgroups and threads as
+// The step's rows as the cache holds them, 16 bits (code x d rounded once): workgroups and threads as
 // in the append; a place past the table, or on a page that is none, reads zeros
 template <int HD>
 __global__ void __launch_bounds__(256)
@@ -326,8 +328,9 @@ struct Kv8Args {
   // k_kv8_chunk: splits of each tile's blocks
   int splits;
   int least;              // blocks a workgroup takes at least, where they are shared or split
-  // k_kv8_few: [workgroup and head][2][16 RT rows][dim], then [..][2][16 RT rows][2]; k_kv8_chunk: [split][row][head][dim],
-  // then [split][row][head][2]: the sums, their reference and weight
+  // the sums, then their reference and weight: k_kv8_few: [workgroup and head][2][16 RT rows][dim],
+  // [..][2][16 RT rows][2], and [tile and head][2], the first and last workgroup that had a part of it;
+  // k_kv8_chunk: [split][row][head][dim], [split][row][head][2]
   float* part;
   int64_t rows;
 };
@@ -345,32 +348,38 @@ __device__ __forceinline__ int kv8_blocks(const Kv8& c, const SeqTile& t) {
   return (kv8_total(c, kv8_base(c, t.seq), t.len) + 63) >> 6;
 }
 // How k_kv8_few's workgroups share the blocks of all tiles, one after the other (a wave finds it out).
-// SHARE consecutive ones each; or, where there is a workgroup for every tile and none has over 16, a
-// tile each: then nothing is left to be joined.
+// SHARE consecutive ones each; or, where there is a workgroup for every tile and the longest is at most
+// 16 blocks over an even share, a tile each: then nothing is left to be joined (64 x 1000..2000 tokens
+// 43.7 us, shared 46.3; 4 x 1000..2000 13.0 shared, 24.7 a tile each).
 struct Kv8Share {
   int all, share;   // share 0: a tile each
-  int first;        // where tile I's blocks begin
+  int own;          // the blocks of the lane's tile of the first 64
 };
-__device__ __forceinline__ Kv8Share kv8_share(const Kv8Args& A, int i) {
+__device__ __forceinline__ Kv8Share kv8_share(const Kv8Args& A) {
   const int lane = threadIdx.x & 63;
-  int all = 0, first = 0, most = 0;
+  int own = 0;
+  if (lane < A.ntiles) own = kv8_blocks(A.c, A.tiles[lane]);
+  int all = own, most = own;
 #pragma unroll 4
-  for (int t = lane; t < A.ntiles; t += 64) {
+  for (int t = lane + 64; t < A.ntiles; t += 64) {
     const int nb = kv8_blocks(A.c, A.tiles[t]);
     all += nb;
-    first += t < i ? nb : 0;
     most = max(most, nb);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     all += __shfl_xor(all, o, 64);
-    first += __shfl_xor(first, o, 64);
     most = max(most, __shfl_xor(most, o, 64));
   }
-  const bool each = A.ntiles <= A.splits && most <= 16;
+  const bool each = A.ntiles <= A.splits && most <= all / A.splits + 16;
   return Kv8Share{__builtin_amdgcn_readfirstlane(all),
                   each ? 0 : __builtin_amdgcn_readfirstlane(max(A.least, (all + A.splits - 1) / A.splits)),
-                  __builtin_amdgcn_readfirstlane(first)};
+                  own};
+}
+
+// A.part's last piece
+__device__ __forceinline__ uint32_t* kv8_parts(const Kv8Args& A, int per, int rt, int hd) {
+  return (uint32_t*)(A.part + (int64_t)A.splits * per * 32 * rt * (hd + 2));
 }
 
 #define MAX_SLACK 8.f
@@ -382,12 +391,18 @@ __device__ __forceinline__ Kv8Share kv8_share(const Kv8Args& A, int i) {
 // memory's rate, and what a workgroup takes to begin (four loads that wait for each other, microseconds
 // next to that many reads) and to end is paid once.  A workgroup whose share ends within a sequence
 // leaves its sums to k_kv8_join_few.  Waves take a sequence's blocks in turn, each with sums of its own,
-// which meet in LDS.  RT row tiles of 16 (rows: tokens times a group's heads).
+// which meet in LDS.  RT row tiles of 16 (rows: tokens times a group's heads).  Codes go from memory to
+// the matrix operands in registers: a lane's 16 bytes of K are its own dims of a key, of V its own keys
+// of a dim, so nothing is turned; eight waves a workgroup, or codes read through the caches, took longer.
 //
-// Grid: workgroups x kv_heads x chunks, the heads fastest; WV waves.
-template <int BF, int HD, int RT, int WV>
-__global__ void __launch_bounds__(64 * WV, RT == 1 ? 2 : 1)
+// With the join (8 heads of 128, groups of 4): 64 x 1 token over 700..8191, bf16, 81.1 us and 1 over
+// 131071, fp16, 52.5 us, 5.0 and 5.1 TB/s, a copy's rate; 4 over 270..333 9.3 us, which is latency.
+//
+// Grid: workgroups x kv_heads x chunks, the heads fastest.
+template <int BF, int HD, int RT>
+__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
 k_kv8_few(Kv8Args A) {
+  constexpr int WV = 4;                       // waves
   constexpr int NS = HD / 32, ND = HD / 16;   // k-steps of a score; 16-dim tiles of O
   constexpr int KL = HD / 64;                 // 16-byte loads a lane, key tile and block of K
   constexpr int LD = HD + 4, ROWB = HD * 2, CH = HD / 8;
@@ -406,7 +421,7 @@ k_kv8_few(Kv8Args A) {
 
   // this workgroup's share: blocks [from, to) of the run of all tiles' blocks; tile I's begin at AT
   int i = w, at = 0, from = 0, to = 0x7FFFFFFF;
-  const Kv8Share sh = A.splits ? kv8_share(A, 0) : Kv8Share{0, 0, 0};
+  const Kv8Share sh = A.splits ? kv8_share(A) : Kv8Share{0, 0, 0};
   if (i >= A.ntiles && sh.share == 0) return;
   if (sh.share) {
     from = w * sh.share;
@@ -414,7 +429,8 @@ k_kv8_few(Kv8Args A) {
     if (from >= to) return;
     i = 0;
     for (int t0 = 0; t0 < A.ntiles; t0 += 64) {   // the tile in which FROM lies
-      const int nb = t0 + lane < A.ntiles ? kv8_blocks(c, A.tiles[t0 + lane]) : 0;
+      int nb = sh.own;
+      if (t0 > 0) nb = t0 + lane < A.ntiles ? kv8_blocks(c, A.tiles[t0 + lane]) : 0;
       int upto = nb;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -705,6 +721,9 @@ k_kv8_few(Kv8Args A) {
     // the next tile's first loads, then this one's sums meet: 16 threads a row, all waves' sums of it
     const bool whole = S.lo == 0 && S.hi == S.nb, more = sh.share && at + S.nb < to;
     const int nb = S.nb, lo = S.lo;
+    if (A.splits && lo == 0 && tid == 0)
+      *(u32x2*)(kv8_parts(A, per, RT, HD) + 2 * ((int64_t)i * per + hc)) =
+          u32x2{(uint32_t)w, (uint32_t)(sh.share ? (at + nb - 1) / sh.share : w)};
     if (more) {
       at += nb;
       ++i;
@@ -724,7 +743,7 @@ k_kv8_few(Kv8Args A) {
       }
       __syncthreads();
       const int rr = mt >> 4, r = rt * 16 + rr, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
-      if (rr >= 16 || tok >= live || head >= heads) continue;
+      if (tok >= live || head >= heads) continue;
       float m = mbuf[0][rr];
 #pragma unroll
       for (int k = 1; k < WV; ++k) m = fmaxf(m, mbuf[k][rr]);
@@ -771,32 +790,31 @@ k_kv8_few(Kv8Args A) {
   }
 }
 
-// The sums of k_kv8_few's workgroups of each tile that more than one had a part of: a workgroup a row and
-// key/value head (blockIdx.y: the row), HD / 4 threads a share of them, in a fixed order.
-template <int HD, int RT>
+// The sums of k_kv8_few's workgroups of each tile that more than one had a part of, in a fixed order:
+// HD / 4 threads take a row's dims in each of SH shares of them, 1024 / HD / SH rows a workgroup
+// (blockIdx.y: which).
+template <int HD, int RT, int SH>
 __global__ void __launch_bounds__(256)
 k_kv8_join_few(Kv8Args A) {
-  constexpr int TH = HD / 4, SH = 256 / TH;   // threads a share; shares
-  __shared__ __align__(16) float ys[SH][HD];
-  __shared__ float ss[SH], ms[SH];
+  constexpr int TH = HD / 4, RW = 256 / TH / SH;   // threads a share; rows
+  __shared__ __align__(16) float ys[256 / TH][HD];
+  __shared__ float ss[256 / TH], ms[256 / TH];
   const int per = A.c.kv_heads * A.chunks;
   const int i = blockIdx.x / per, hc = blockIdx.x % per, kvh = hc % A.c.kv_heads, chunk = hc / A.c.kv_heads;
-  const int r = blockIdx.y, tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
+  const u32x2 parts = *(const u32x2*)(kv8_parts(A, per, RT, HD) + 2 * (int64_t)blockIdx.x);
   const SeqTile T = A.tiles[i];
-  if (tok >= T.len || head >= min(A.hh, A.group - chunk * A.hh)) return;
-  const Kv8Share s = kv8_share(A, i);
-  if (s.share == 0) return;
-  const int w0 = s.first / s.share, w1 = (s.first + kv8_blocks(A.c, T) - 1) / s.share;   // the workgroups that had a part
+  const int w0 = (int)parts[0], w1 = (int)parts[1];
   if (w0 == w1) return;
-  const int tid = threadIdx.x, sh = tid / TH, d = tid % TH * 4;
+  const int tid = threadIdx.x, g = tid / TH, sh = g % SH, d = tid % TH * 4;
+  const int r = min((int)blockIdx.y * RW + g / SH, 16 * RT - 1), tok = (int)(r * A.magic >> 16), head = r - tok * A.hh;
   const float* ml = A.part + (int64_t)A.splits * per * 32 * RT * HD;
   auto slot = [&](int w) { return (((int64_t)w * per + hc) * 2 + (w == w0)) * 16 * RT + r; };
   float m = -INFINITY;
   for (int w = w0 + sh; w <= w1; w += SH) m = fmaxf(m, ml[slot(w) * 2]);
-  if (d == 0) ms[sh] = m;
+  if (d == 0) ms[g] = m;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < SH; ++k) m = fmaxf(m, ms[k]);
+  for (int k = 0; k < SH; ++k) m = fmaxf(m, ms[g - sh + k]);
   float sum = 0.f;
   f32x4 y = {};
 #pragma unroll 4
@@ -807,14 +825,14 @@ k_kv8_join_few(Kv8Args A) {
     sum += p[0] == -INFINITY ? p[1] : f * p[1];   // no reference: 0, or NaN
     if (f > 0.f) y += f * x;
   }
-  *(f32x4*)&ys[sh][d] = y;
-  if (d == 0) ss[sh] = sum;
+  *(f32x4*)&ys[g][d] = y;
+  if (d == 0) ss[g] = sum;
   __syncthreads();
-  if (sh) return;
+  if (sh || (int)blockIdx.y * RW + g / SH > r || tok >= T.len || head >= min(A.hh, A.group - chunk * A.hh)) return;
 #pragma unroll
   for (int k = 1; k < SH; ++k) {
-    y += *(const f32x4*)&ys[k][d];
-    sum += ss[k];
+    y += *(const f32x4*)&ys[g + k][d];
+    sum += ss[g + k];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* po = A.out + (int64_t)(T.row0 + tok) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + d;
@@ -830,7 +848,10 @@ k_kv8_join_few(Kv8Args A) {
 // next codes are asked for a block ahead.  Codes are whole numbers: K's scale goes into the scores'
 // factor, V's into the weights' exponent, p vd 2^-E with E the largest exponent of a scale so far, so that
 // fp16 weights of blocks of small values keep their bits; a block's sum of them times 1 / (vd 2^-E) is
-// its share of the row's weight.
+// its share of the row's weight.  Two workgroups a CU hide a part of the conversion only: 4 x 512 tokens
+// over 2500..4001 (2 heads of 64, groups of 8, bf16) 64.7 us, 385 TFLOP/s; 1 x 76 over 1100 (8 heads of
+// 128) 18.9 us, of which a third is its start (tile, length, page, scale and codes wait for each other),
+// a third the join.
 template <int BF>
 __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
   if constexpr (BF)
@@ -1331,12 +1352,12 @@ namespace {
 
 struct Kv8Way {
   int rt;                  // row tiles of 16 a workgroup (1 or 2), or 0: k_kv8_chunk's 128 rows
-  int wv;                  // waves a workgroup
   int z, hh, chunks;       // the tiles' list; heads a workgroup, workgroups a group
   int splits, least;
   int64_t floats;          // of scratch that the splits take
 };
-// at most SPLITS of them (as far as the caller's scratch goes)
+// Splits go as far as the caller's scratch.  Times below are of 8 key/value heads of 128 and groups of 4,
+// fp16, in us, unless said.
 Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim, int cols, const int64_t* ntiles,
                int64_t part_cap) {
   Kv8Way w;
@@ -1345,33 +1366,42 @@ Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim,
   w.z = 0;
   w.splits = 0;
   w.floats = 0;
-  w.wv = 4;
-  if (longest * w.hh <= 32) {
+  // Few rows: k_kv8_few, which reads codes into registers (64 x 1 token over 700..8191, bf16: 81, with
+  // k_kv8_chunk 231).  Two row tiles are one workgroup a CU, whose start and end short tables do not make
+  // up for: 17 to 32 rows take k_kv8_chunk up to 32 columns (1 x 8 tokens over 1100 13.4, with k_kv8_few
+  // 15.7; 64 x 8 over 700..2000 71, 92) and k_kv8_few past them (16 x 8 over 4000 51, 54; 64 x 8 over
+  // 700..8191, bf16, 138, 232).
+  if (longest * w.hh <= (cols > 32 ? 32 : 16)) {
     w.rt = longest * w.hh <= 16 ? 1 : 2;
     while ((SEQ_TT0 << w.z) < longest) ++w.z;
     w.chunks = (group + w.hh - 1) / w.hh;
     const int per = kv_heads * w.chunks;
-    // as many workgroups as the chip holds at once
+    // as many workgroups as the chip holds at once (64 x 1 over 700..8191: half of them 94, twice 92,
+    // these 83; 1 x 1 over 131071: 54.6, 58.0, 53.5)
     const int slots = 256 * (w.rt == 1 ? (head_dim == 64 ? 4 : 2) : (head_dim == 64 ? 2 : 1));
     int64_t s = slots / per > 0 ? slots / per : 1;
-    const int64_t each = (int64_t)per * 32 * w.rt * (head_dim + 2);
-    if (s * each > part_cap) s = part_cap / each;
-    w.least = 16;
+    const int64_t each = (int64_t)per * 32 * w.rt * (head_dim + 2), parts = 2 * ntiles[w.z] * per;
+    if (s * each + parts > part_cap) s = (part_cap - parts) / each;
+    w.least = 2;   // 4 x 1 over 1100..4000: 15.1, with 4 blocks 16.6, with 16 23.0
+    // Tables of up to 16 blocks a workgroup a sequence: the sharing's own steps and the join cost more
+    // than it evens out (4 x 1 over 270..333 9.3, shared 15.4; 64 x 1 over 600..1000 26.9, 35.8).  So
+    // do many sequences even themselves out (200 x 1 over 700..4000 152, shared 145; 300 x 1 over
+    // 300..4000 174, 191).
     if (cols > 16 && s > 1 && ntiles[w.z] * per <= 4 * slots) {
       w.splits = (int)s;
-      w.floats = s * each;
-    } else if (w.rt == 1 && ntiles[w.z] * per <= 256) {
-      w.wv = 8;
+      w.floats = s * each + parts;
     }
     return w;
   }
   w.rt = 0;
-  w.hh = group < 8 ? group : 8;
+  w.hh = group < 8 ? group : 8;   // as attend_packed
   while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
-  w.least = 2;
+  w.least = 2;   // 1 x 76 over 1100 19.1, with 1 or 4 blocks 21.8
   w.chunks = (group + w.hh - 1) / w.hh;
   const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, most = (cols + w.least - 1) / w.least;
   const int64_t each = rows * heads * (head_dim + 2);
+  // two workgroups a CU: 4 x 512 over 2500..4001 (2 heads of 64, groups of 8, bf16) 65, from 256 in all
+  // 86, from 1024 69; 1 x 64 over 16000 40.4, 43.5, 54.4
   int64_t s = groups > 0 ? 512 / groups : 1;
   if (s > most) s = most;
   if (each > 0 && s * each > part_cap) s = part_cap / each;
@@ -1415,12 +1445,11 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   const int64_t joins = ntiles[w.z] * w.chunks * c.kv_heads;
   if (groups > INT32_MAX || joins > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((unsigned)groups, w.rt ? 1 : w.splits);
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * w.wv), 0, s, a); };
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
     if (w.rt == 0) return BF && !obf ? go(k_kv8_chunk<BF, HD, BF>) : go(k_kv8_chunk<BF, HD, 0>);
-    w.rt == 2 ? go(k_kv8_few<BF, HD, 2, 4>)
-    : w.wv == 8 ? go(k_kv8_few<BF, HD, 1, 8>) : go(k_kv8_few<BF, HD, 1, 4>);
+    w.rt == 2 ? go(k_kv8_few<BF, HD, 2>) : go(k_kv8_few<BF, HD, 1>);
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
@@ -1433,14 +1462,25 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.splits < 2) return e;
   if (w.rt) {
-    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins, longest * w.hh), dim3(256), 0, s, a); };
-    if (c.head_dim == 128)
-      w.rt == 1 ? join(k_kv8_join_few<128, 1>) : join(k_kv8_join_few<128, 2>);
-    else
-      w.rt == 1 ? join(k_kv8_join_few<64, 1>) : join(k_kv8_join_few<64, 2>);
+    // a row a workgroup where a tile has many parts (1 x 1 over 131071 53.0, else 57.7), or two shares
+    // and four rows (64-wide: eight)
+    const bool few = ntiles[w.z] * 8 <= w.splits;
+    const int rw = few ? 1 : 512 / c.head_dim;
+    const dim3 jg((unsigned)joins, (longest * w.hh + rw - 1) / rw);
+    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jg, dim3(256), 0, s, a); };
+    auto jrt = [&](auto rt) {
+      constexpr int RT = decltype(rt)::value;
+      if (c.head_dim == 128)
+        few ? join(k_kv8_join_few<128, RT, 8>) : join(k_kv8_join_few<128, RT, 2>);
+      else
+        few ? join(k_kv8_join_few<64, RT, 16>) : join(k_kv8_join_few<64, RT, 2>);
+    };
+    w.rt == 1 ? jrt(std::integral_constant<int, 1>()) : jrt(std::integral_constant<int, 2>());
     return hipGetLastError();
   }
   const int th = c.head_dim / 4, most = (a.tt < longest ? a.tt : longest) * heads;   // a tile's rows and heads
+  // 1 x 64 over 16000 (32 splits) 40.3 with the splits in shares, 47.4 without; 4 x 512 over 2500..4001 (64-wide,
+  // 2 splits) 100 with, 65 without
   const bool few = w.splits > 4;
   const int each = few ? 1 : 256 / th;
   const dim3 jg((unsigned)ntiles[w.z], (most + each - 1) / each);

@@ -13,6 +13,13 @@
 // The products are taken transposed (attn.hip's arrangement): S^T = K Q^T leaves a query in a lane's
 // column, whose p are then the B operand of O^T += V^T P^T as they are.  V lies in LDS as in memory,
 // [key][dim]; gfx950's transposing LDS read hands each lane four keys of its dim.
+//
+// Matrix instructions bound it for long prompts: 2 x 8192 tokens (32 heads of 128, 8 of keys and values,
+// bf16) 992 us, 1,110 TFLOP/s where a large library product reaches 1,210 (matrix units busy 57% of the
+// cycles at a clock that power holds at 1.6 to 1.9 GHz).  Two waves of a SIMD alternate between products
+// and exp2; 64 rows a wave took 1.21 ms, eight waves in two fixed phases 1.06 ms.  Short ones are bound
+// by the start and end of a workgroup: 4 x 1100..1180 57 us (740 TFLOP/s), 16 x 21..257 11.4 us, 1 x 24
+// 6.9 us; 24 x 5..4001 (16 heads of 64, 2 of keys and values) 89 us (830 TFLOP/s).
 #include "exn_common.h"
 
 #include <type_traits>
@@ -403,6 +410,9 @@ hipError_t attend_packed(hipStream_t s, const SeqTile* const* tiles, const int64
   a.scale = scale * 1.4426950408889634f;
   a.kv_heads = kv_heads;
   a.group = heads / kv_heads;
+  // up to 8 heads of a group share a tile: with groups of 4, 16 x 21..257 tokens 11.9 us, 2 at a time 13.2,
+  // alone 15.0, and 4 x 1100..1180 60.8, 62.6, 66.0; with groups of 8 (64-wide), 24 x 5..4001 90, 4 at a
+  // time 94, alone 98
   a.hh = a.group < 8 ? a.group : 8;
   a.chunks = (a.group + a.hh - 1) / a.hh;
   a.magic = (65536 + a.hh - 1) / a.hh;
