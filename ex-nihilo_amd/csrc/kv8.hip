@@ -846,9 +846,9 @@ k_kv8_join_few(Kv8Args A) {
 // block interleaved with this one's exp2), with each block's codes made 16 bits on the way into LDS: a
 // wave converts a quarter of a block for all four, 96 VALU instructions of about 300 a block, and the
 // next codes are asked for a block ahead.  Codes are whole numbers: K's scale goes into the scores'
-// factor, V's into the weights' exponent, p vd 2^-E with E the largest exponent of a scale so far, so that
-// fp16 weights of blocks of small values keep their bits; a block's sum of them times 1 / (vd 2^-E) is
-// its share of the row's weight.  Two workgroups a CU hide a part of the conversion only: 4 x 512 tokens
+// factor, and a block's products of weights (fp16) and V codes meet the sums under V's scale.  (The scale
+// in the weights' exponent saves those multiply-adds, but then a value 2^17 times the others, seen or
+// not, takes the others' weights below fp16's least.)  Two workgroups a CU hide a part of the conversion only: 4 x 512 tokens
 // over 2500..4001 (2 heads of 64, groups of 8, bf16) 64.7 us, 385 TFLOP/s; 1 x 76 over 1100 (8 heads of
 // 128) 18.9 us, of which a third is its start (tile, length, page, scale and codes wait for each other),
 // a third the join.
@@ -863,15 +863,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
-}
-
-// SUM plus a pair of weights as the second product takes them
-template <int BF>
-__device__ __forceinline__ float weight_sum(uint32_t pair, float sum) {
-  if constexpr (BF)
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
-  else
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair), f16x2{(_Float16)1.f, (_Float16)1.f}, sum, false);
 }
 
 // One row by a whole wave, blocks [lo, hi), nothing that it does not see multiplied: for rows whose
@@ -915,8 +906,7 @@ __device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int tota
   *l_ = l;
 }
 
-// LO: weights as two bf16 parts, where a bf16 cache gives fp16 rows
-template <int BF, int HD, int LO>
+template <int BF, int HD>
 __global__ void __launch_bounds__(256, 2)
 k_kv8_chunk(Kv8Args A) {
   constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
@@ -1012,8 +1002,8 @@ k_kv8_chunk(Kv8Args A) {
 #pragma unroll
       for (int i = 0; i < CI; ++i) {
         const int ci = tid + 256 * i, dim = ci >> 2, c2 = 2 * (ci & 3), z = (dim >> 1) & 7;
-        *(s16x8*)(p + dim * 128 + ((c2 ^ z) << 4)) = codes8<BF>(x.w[i][0], x.w[i][2]);
-        *(s16x8*)(p + dim * 128 + (((c2 + 1) ^ z) << 4)) = codes8<BF>(x.w[i][1], x.w[i][3]);
+        *(s16x8*)(p + dim * 128 + ((c2 ^ z) << 4)) = codes8<0>(x.w[i][0], x.w[i][2]);
+        *(s16x8*)(p + dim * 128 + (((c2 + 1) ^ z) << 4)) = codes8<0>(x.w[i][1], x.w[i][3]);
       }
     } else {
       tail(c.tv, p, [&](int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); });
@@ -1025,23 +1015,22 @@ k_kv8_chunk(Kv8Args A) {
 #pragma unroll
   for (int u = 0; u < 4; ++u) vofs[u] = 2 * STAGE + lo * 128 + (((2 * u + hi) ^ ((lo >> 1) & 7)) << 4);
   auto kfrag = [&](int i) { return *(const s16x8*)(smem + kofs[i / 2] + (i % 2) * 32 * ROWB); };
-  auto vfrag = [&](auto tail_c, int j) __attribute__((always_inline)) {
+  auto vfrag = [&](auto tail_c, int u, int d) __attribute__((always_inline)) {
     if constexpr (decltype(tail_c)::value) {
       typedef __attribute__((address_space(3))) s16x4 lds_s4;
-      const int r = 4 * hi + ((lane & 15) >> 2), x = 4 * (j % ND) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      uint8_t* p = smem + ((vofs[0] & ~(STAGE - 1)) + (16 * (j / ND) + r) * ROWB +
+      const int r = 4 * hi + ((lane & 15) >> 2), x = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      uint8_t* p = smem + ((vofs[0] & ~(STAGE - 1)) + (16 * u + r) * ROWB +
                            ((x ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))) << 4) + 8 * (lane & 1));
       return __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p),
                                      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * ROWB)), 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      return *(const s16x8*)(smem + vofs[j / ND] + (j % ND) * 32 * 128);
+      return *(const s16x8*)(smem + vofs[u] + d * 32 * 128);
     }
   };
 
   f32x16 o[ND], sc[2];
   float mrun = 0.f, lrun = 0.f;
   bool set = false;          // the row has a reference
-  int top = -1000;           // E: the sums are in units of 2^E
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x16{};
   auto barrier = [&](bool dma) __attribute__((always_inline)) {   // DMA: with the tail's rows asked for before it
@@ -1054,28 +1043,15 @@ k_kv8_chunk(Kv8Args A) {
 
   // Block B of facts F: its softmax, the S product of block b+1 interleaved with its exp2, O^T += V^T P^T
   auto step = [&](auto last_c, auto tail_c, int b, const Facts& F) __attribute__((always_inline)) {
-    constexpr bool LAST = decltype(last_c)::value;
+    constexpr bool LAST = decltype(last_c)::value, TAIL = decltype(tail_c)::value;
+    constexpr int WB = TAIL && BF;   // weights: fp16, or with values in bf16 two bf16 parts
     const int k0 = b * 64;
     const float factor = F.kd * A.scale;
     const bool gone = F.page < 0 && b < nfull;
-    // V's scale, in units of 2^E and not under 2^-100 of them, goes into the weights' exponent; a row
-    // that sees nothing of the block takes nothing of it, NaN or not
-    const int e = (int)((__float_as_uint(F.vd) >> 23) & 0xFF) - 127;
-    if (e > top && e < 128) {
-      const float f = top == -1000 ? 1.f : __builtin_ldexpf(1.f, top - e);
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= f;
-      top = e;
-    }
-    const float vd = __builtin_ldexpf(F.vd, top == -1000 ? 0 : -top);
-    const float lv = gone || k0 > lim || F.vd == 0.f ? 0.f : __builtin_amdgcn_logf(vd < 0x1p-100f ? 0x1p-100f : vd);
-    const float from = lv - mrun;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[h][r] = __builtin_fmaf(sc[h][r], factor, from);
+      for (int r = 0; r < 16; ++r) sc[h][r] = __builtin_fmaf(sc[h][r], factor, -mrun);
     if (gone || k0 + 63 > minlim) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -1096,7 +1072,7 @@ k_kv8_chunk(Kv8Args A) {
     }
     float ma = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), mb = ma;
     xswap32(ma, mb);
-    const float mx = fmaxf(ma, mb) - lv;
+    const float mx = fmaxf(ma, mb);
     const bool move = set ? mx > MAX_SLACK : mx > -INFINITY;
     if (__ballot(move)) {
       const float shift = move ? mx : 0.f;
@@ -1115,8 +1091,8 @@ k_kv8_chunk(Kv8Args A) {
     }
     constexpr int KD = 3, NI = 2 * NS, PS = 16 / NI;
     f32x16 sn[2];
-    uint32_t pk[16], pl[LO ? 16 : 1];
-    float ls[2] = {};
+    uint32_t pk[16], pl[WB ? 16 : 1];
+    float ls[2] = {lrun, 0.f};
     s16x8 kq[KD], vq[KD];
     if constexpr (!LAST) {
       sn[0] = f32x16{};
@@ -1134,39 +1110,48 @@ k_kv8_chunk(Kv8Args A) {
         for (int d = 0; d + 1 < KD; ++d) kq[d] = kq[d + 1];
         kq[KD - 1] = kn;
       }
-      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(tail_c, i - (NI - KD));
+      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(tail_c, (i - (NI - KD)) % 4, (i - (NI - KD)) / 4);
 #pragma unroll
       for (int z = 0; z < PS; ++z) {
         const int pi = PS * i + z, h = pi / 8, r = 2 * (pi % 8);
         const float p0 = __builtin_amdgcn_exp2f(sc[h][r]), p1 = __builtin_amdgcn_exp2f(sc[h][r + 1]);
-        pk[pi] = BF ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
-        ls[pi % 2] = weight_sum<BF>(pk[pi], ls[pi % 2]);
-        if constexpr (LO) {
-          pl[pi] = pack_bf16x2(p0 - bf16_lo(pk[pi]), p1 - bf16_hi(pk[pi]));
-          ls[pi % 2] = weight_sum<BF>(pl[pi], ls[pi % 2]);
-        }
+        pk[pi] = WB ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+        if constexpr (WB) pl[pi] = pack_bf16x2(p0 - bf16_lo(pk[pi]), p1 - bf16_hi(pk[pi]));
+        ls[0] += p0;
+        ls[1] += p1;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    lrun = __builtin_fmaf(ls[0] + ls[1], __builtin_amdgcn_exp2f(-lv), lrun);
-    if (F.vd == 0.f) {   // whatever the codes, the values are 0
-#pragma unroll
-      for (int i = 0; i < 16; ++i) pk[i] = pl[LO ? i : 0] = 0;
-    }
+    lrun = ls[0] + ls[1];
+    // a block's products of codes, then its scale; a row that sees nothing of it takes nothing of the scale,
+    // which may be NaN
+    const float vd = gone || k0 > lim ? 0.f : F.vd;
+    f32x16 t[2];
 #pragma unroll
     for (int j = 0; j < 4 * ND; ++j) {
       s16x8 vn = {};
-      if (j + KD < 4 * ND) vn = vfrag(tail_c, j + KD);
-      const int u = j / ND;
+      if (j + KD < 4 * ND) vn = vfrag(tail_c, (j + KD) % 4, (j + KD) / 4);
+      const int u = j % 4, d = j / 4;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
-      o[j % ND] = mfma32<BF>(vq[0], pb, o[j % ND]);
-      if constexpr (LO)
-        o[j % ND] = mfma32<BF>(vq[0], __builtin_bit_cast(s16x8, u32x4{pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]}),
-                               o[j % ND]);
+      if constexpr (TAIL) {
+        o[d] = mfma32<BF>(vq[0], pb, o[d]);
+        if constexpr (WB)
+          o[d] = mfma32<BF>(vq[0], __builtin_bit_cast(s16x8, u32x4{pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]}), o[d]);
+      } else {
+        t[d % 2] = mfma32<0>(vq[0], pb, u == 0 ? f32x16{} : t[d % 2]);
+        if (d > 0) {
+#pragma unroll
+          for (int r = 4 * u; r < 4 * u + 4; ++r) o[d - 1][r] = __builtin_fmaf(t[(d - 1) % 2][r], vd, o[d - 1][r]);
+        }
+      }
 #pragma unroll
       for (int d = 0; d + 1 < KD; ++d) vq[d] = vq[d + 1];
       vq[KD - 1] = vn;
       __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!TAIL) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[ND - 1][r] = __builtin_fmaf(t[(ND - 1) % 2][r], vd, o[ND - 1][r]);
     }
     if constexpr (!LAST) {
       sc[0] = sn[0];
@@ -1238,8 +1223,7 @@ k_kv8_chunk(Kv8Args A) {
 
   float la = lrun, lb = lrun;
   xswap32(la, lb);
-  const float sum = la + lb, unit = top == -1000 ? 1.f : __builtin_ldexpf(1.f, top);
-  const float mul = active > 1 ? unit : sum == 0.f ? 0.f : unit / sum;
+  const float sum = la + lb, mul = active > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   float zero[4] = {sum * 0.f};
   const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = A.rows * A.heads;
   auto leave = [&](auto obf) __attribute__((always_inline)) {
@@ -1448,7 +1432,7 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-    if (w.rt == 0) return BF && !obf ? go(k_kv8_chunk<BF, HD, BF>) : go(k_kv8_chunk<BF, HD, 0>);
+    if (w.rt == 0) return go(k_kv8_chunk<BF, HD>);
     w.rt == 2 ? go(k_kv8_few<BF, HD, 2>) : go(k_kv8_few<BF, HD, 1>);
   };
   typedef std::integral_constant<int, 0> I0;
