@@ -433,6 +433,128 @@ def test_two_runs_are_bit_identical(ctx):
     assert (outs[0] == outs[1]).all() and (outs[0] == outs[2]).all()
 
 
+def filled(ctx, dt, lens, kv, hd, cols, rng, pages=None, table=None):
+    """A cache as many steps would leave it: random codes, scales and tails."""
+    m, d = cache_of(ctx, dt, len(lens), kv, hd, cols, rng, pages, table)
+    m.scales[:] = (rng.uniform(0.5, 2, m.scales.shape) / 64).astype(np.float32)
+    for n in ("tk", "tv"):
+        getattr(m, n)[:] = normal(rng, getattr(m, n).shape, dt)[0]
+    m.lens[:] = lens
+    for n in ("scales", "tk", "tv", "lens"):
+        d.b[n].upload(getattr(m, n))
+    return m, d
+
+
+def attended(ctx, d, q, new, heads, odt, scale, floats=None):
+    """kv8_attend alone, over the cache as it is: its rows' values."""
+    m = d.m
+    s = X.Seqs(ctx, new)
+    dq = X.DevBuf.of(ctx, q)
+    o = X.DevBuf.of(ctx, np.full((sum(new) + 1, heads, m.hd), 0x1234, np.uint16))
+    n = X.kv8_attend_part(s, heads, m.kv, m.hd, m.cols)
+    n = n if floats is None else floats(n)
+    part = X.DevBuf.of(ctx, np.full(n + 4, np.nan, np.float32))
+    X.kv8_attend(ctx, d.h, s, heads, dq.h, heads * m.hd, scale, o.h, DT[odt], heads * m.hd, part.h if n else None, n)
+    got = o.get()
+    assert (got[-1] == 0x1234).all()
+    assert np.isnan(part.get()[n:]).all()
+    return pm.value(got[:-1], odt)
+
+
+@pytest.mark.parametrize("dt,odt", [("fp16", "fp16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("n,top,cols", [(3, 1000, 40), (70, 300, 40), (70, 2500, 40), (5, 2500, 40), (200, 900, 15),
+                                        (150, 1100, 18)])
+def test_cache_many_sequences(ctx, n, top, cols, dt, odt):
+    """Single tokens over lengths from none to TOP, in tables that are larger: shares that begin and
+    end within sequences, a workgroup a sequence, more sequences than lanes or workgroups."""
+    rng = np.random.default_rng([n, top])
+    say("many sequences", n, top, dt)
+    lens = rng.integers(0, top, n)
+    lens[:3] = [0, top - 1, 63]
+    pages = 300                                     # sequences share pages
+    kv, hd, heads = 8, 64, 8
+    m, d = filled(ctx, dt, lens, kv, hd, cols, rng, pages, rng.integers(0, pages, (n, cols)))
+    qb, q = normal(rng, (n, heads, hd), dt)
+    want, tol = m.attend(q, [1] * n, 0.125, odt)
+    assert off(attended(ctx, d, qb, [1] * n, heads, odt, 0.125), want, tol) <= 1
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cols", [30, 45])
+@pytest.mark.parametrize("new", [[8, 5, 1], [4, 2], [1, 1, 1], [20, 33]], ids=str)
+def test_cache_any_scratch(ctx, new, cols, hd):
+    """All the scratch asked for, less of it, too little for any split, none; one to 132 rows a
+    sequence and head, over tables on both sides of the few-row kernel's bound."""
+    rng = np.random.default_rng([sum(new), cols, hd])
+    say("any scratch", new, cols, hd)
+    lens = rng.integers(cols * 40, cols * 60, len(new))
+    kv, heads = 2, 8
+    m, d = filled(ctx, "bf16", lens, kv, hd, cols, rng)
+    qb, q = normal(rng, (sum(new), heads, hd), "bf16")
+    want, tol = m.attend(q, new, 0.125, "fp16")
+    for floats in (lambda n: n, lambda n: n // 2, lambda n: n // 7, lambda n: min(n, 100), lambda n: 0):
+        assert off(attended(ctx, d, qb, new, heads, "fp16", 0.125, floats), want, tol) <= 1
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", [1, 8, 40])
+def test_cache_values_of_very_different_sizes(ctx, new, dt):
+    """A block whose values are 2^17 times the others' and whose keys weigh nothing (scores of
+    -100, over 100 under each row's largest: e^-100 2^17 is 2^-127 of a value) is as if it were not there."""
+    rng = np.random.default_rng(new)
+    say("very different sizes", new, dt)
+    lens, kv, hd, heads, cols = [1500, 700], 2, 64, 8, 40
+    m, d = filled(ctx, dt, lens, kv, hd, cols, rng)
+    qb, q = normal(rng, (2 * new, heads, hd), dt)
+    qb[:, :, 0], q[:, :, 0] = pm.bits(np.float32(16), dt), 16.0
+    for s in range(2):
+        for p in m.table[s]:
+            m.k[p, :, :, 0] = 0
+        p = m.table[s, 5]
+        m.k[p] = 0
+        m.k[p, :, :, 0] = -100                       # q of 16 x -100 x 1 / 16
+        m.scales[p] = [1 / 16, m.scales[p, 0, 1] * 2.0 ** 17]
+    m.tk[:, :, :, 0] = 0
+    for n in ("k", "scales", "tk"):
+        d.b[n].upload(getattr(m, n))
+    got = attended(ctx, d, qb, [new, new], heads, dt, 1.0)
+    m.table = m.table.copy()
+    m.table[:, 5] = -1
+    want, tol = m.attend(q, [new, new], 1.0, dt)
+    assert off(got, want, tol) <= 1
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("cols", [12, 40])
+@pytest.mark.parametrize("new", [1, 8, 40])
+def test_cache_not_finite_in_each_kernel(ctx, new, cols, dt):
+    """A block that is not finite makes its sequence's rows NaN and nobody else's; a value of the tail
+    its dim only; a page that is none hides a scale of NaN."""
+    rng = np.random.default_rng([new, cols])
+    say("not finite", new, cols, dt)
+    lens, kv, hd, heads = [cols * 32, cols * 50, cols * 40 // 64 * 64 + 5], 1, 128, 4
+    m, d = filled(ctx, dt, lens, kv, hd, cols, rng)
+    qb, q = normal(rng, (3 * new, heads, hd), dt)
+    want, tol = m.attend(q, [new] * 3, 0.1, dt)
+    nan = m.table[0, 2]
+    m.scales[nan, 0, rng.integers(2)] = np.nan
+    m.tv[2, 0, 3, 9] = pm.bits(np.float32(np.inf), dt)[0]
+    for n in ("scales", "tv"):
+        d.b[n].upload(getattr(m, n))
+    got = attended(ctx, d, qb, [new] * 3, heads, dt, 0.1)
+    assert np.isnan(got[:new]).all()
+    assert (got[2 * new:, :, 9] == np.inf).all()
+    same = np.ones(got.shape, bool)
+    same[:new] = same[2 * new:, :, 9] = False
+    assert (abs(got - want)[same] <= tol[same]).all()
+    m.table[0, 2] = -1
+    d.b["table"].upload(m.table)
+    m.tv[2, 0, 3, 9] = 0
+    d.b["tv"].upload(m.tv)
+    want, tol = m.attend(q, [new] * 3, 0.1, dt)
+    assert off(attended(ctx, d, qb, [new] * 3, heads, dt, 0.1), want, tol) <= 1
+
+
 # --- a run of them under a graph, on another stream ---------------------------------------------
 
 
