@@ -1463,16 +1463,16 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
     return hipGetLastError();
   }
   const int th = c.head_dim / 4, most = (a.tt < longest ? a.tt : longest) * heads;   // a tile's rows and heads
-  // 1 x 64 over 16000 (32 splits) 40.3 with the splits in shares, 47.4 without; 4 x 512 over 2500..4001 (64-wide,
-  // 2 splits) 100 with, 65 without
-  const bool few = w.splits > 4;
-  const int each = few ? 1 : 256 / th;
-  const dim3 jg((unsigned)ntiles[w.z], (most + each - 1) / each);
+  // The splits in as many shares as leave a row a workgroup, in half as many, or in one: 1 x 64 over 16000
+  // (32 splits) 40.7, 42.8, 47.4; 1 x 76 over 1100 (10) 18.8, 17.8, 19.3; 4 x 512 over 2500..4001 (64-wide, 2
+  // splits) 100, -, 65
+  const int rw = w.splits > 16 ? 1 : w.splits > 4 ? 2 : 256 / th;
+  const dim3 jg((unsigned)ntiles[w.z], (most + rw - 1) / rw);
   auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jg, dim3(256), 0, s, a); };
   if (c.head_dim == 128)
-    few ? join(k_kv8_join<128, 8>) : join(k_kv8_join<128, 1>);
+    rw == 1 ? join(k_kv8_join<128, 8>) : rw == 2 ? join(k_kv8_join<128, 4>) : join(k_kv8_join<128, 1>);
   else
-    few ? join(k_kv8_join<64, 16>) : join(k_kv8_join<64, 1>);
+    rw == 1 ? join(k_kv8_join<64, 16>) : rw == 2 ? join(k_kv8_join<64, 8>) : join(k_kv8_join<64, 1>);
   return hipGetLastError();
 }
 
