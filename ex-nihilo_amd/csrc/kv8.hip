@@ -849,8 +849,8 @@ k_kv8_join_few(Kv8Args A) {
 // factor, and a block's products of weights (fp16) and V codes meet the sums under V's scale.  (The scale
 // in the weights' exponent saves those multiply-adds, but then a value 2^17 times the others, seen or
 // not, takes the others' weights below fp16's least.)  Two workgroups a CU hide a part of the conversion only: 4 x 512 tokens
-// over 2500..4001 (2 heads of 64, groups of 8, bf16) 64.7 us, 385 TFLOP/s; 1 x 76 over 1100 (8 heads of
-// 128) 18.9 us, of which a third is its start (tile, length, page, scale and codes wait for each other),
+// over 2500..4001 (2 heads of 64, groups of 8, bf16) 63.0 us, 390 TFLOP/s; 1 x 76 over 1100 (8 heads of
+// 128) 17.6 us, of which a third is its start (tile, length, page, scale and codes wait for each other),
 // a third the join.
 template <int BF>
 __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
@@ -1384,8 +1384,8 @@ Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim,
   w.chunks = (group + w.hh - 1) / w.hh;
   const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, most = (cols + w.least - 1) / w.least;
   const int64_t each = rows * heads * (head_dim + 2);
-  // two workgroups a CU: 4 x 512 over 2500..4001 (2 heads of 64, groups of 8, bf16) 65, from 256 in all
-  // 86, from 1024 69; 1 x 64 over 16000 40.4, 43.5, 54.4
+  // two workgroups a CU: 4 x 512 over 2500..4001 (2 heads of 64, groups of 8, bf16) 65, with 256 in all
+  // 86, with 1024 69; 1 x 64 over 16000 40.4, 43.5, 54.4
   int64_t s = groups > 0 ? 512 / groups : 1;
   if (s > most) s = most;
   if (each > 0 && s * each > part_cap) s = part_cap / each;

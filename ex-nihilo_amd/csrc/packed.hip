@@ -15,11 +15,11 @@
 // [key][dim]; gfx950's transposing LDS read hands each lane four keys of its dim.
 //
 // Matrix instructions bound it for long prompts: 2 x 8192 tokens (32 heads of 128, 8 of keys and values,
-// bf16) 992 us, 1,110 TFLOP/s where a large library product reaches 1,210 (matrix units busy 57% of the
+// bf16) 998 us, 1,100 TFLOP/s where a large library product reaches 1,210 (matrix units busy 57% of the
 // cycles at a clock that power holds at 1.6 to 1.9 GHz).  Two waves of a SIMD alternate between products
 // and exp2; 64 rows a wave took 1.21 ms, eight waves in two fixed phases 1.06 ms.  Short ones are bound
-// by the start and end of a workgroup: 4 x 1100..1180 57 us (740 TFLOP/s), 16 x 21..257 11.4 us, 1 x 24
-// 6.9 us; 24 x 5..4001 (16 heads of 64, 2 of keys and values) 89 us (830 TFLOP/s).
+// by the start and end of a workgroup: 4 x 1100..1180 57 us (740 TFLOP/s), 16 x 21..257 11.7 us, 1 x 24
+// 6.9 us; 24 x 5..4001 (16 heads of 64, 2 of keys and values) 91 us (820 TFLOP/s).
 #include "exn_common.h"
 
 #include <type_traits>

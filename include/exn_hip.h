@@ -188,7 +188,7 @@ int exn_seqs_free(exn_seqs* s);
  * heads of HEAD_DIM, 64 or 128) sees rows 0 .. i of its sequence in K and V (KV_HEADS heads, a
  * divisor of HEADS; head h reads h / (HEADS / KV_HEADS)), softmax of SCALE q.k in fp32.  Q, K and V
  * are EXN_DT_F16 or EXN_DT_BF16 (DT; the softmax's weights are rounded to that type for the second
- * product, sums are fp32), OUT either (ODT).  All four 16-byte aligned, strides multiples of 8:
+ * product, from bf16 to fp16 rows in two parts; sums are fp32), OUT either (ODT).  All four 16-byte aligned, strides multiples of 8:
  * they may be parts of one row (q | k | v).  OUT overlaps none of them. */
 int exn_attend_packed(exn_ctx* ctx, const exn_seqs* s, int dt, int heads, int kv_heads, int head_dim, const void* q,
                       int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, float scale, void* out,
@@ -218,9 +218,9 @@ int exn_kv8_append(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const void
                    int64_t ldv);
 /* attention of the plan's rows, after exn_kv8_append of the same rows: row i of a sequence sees its
  * cache's tokens 0 .. LENS + i, as exn_kv8_read reads them (zeros where all are hidden).  HEADS, Q,
- * SCALE, OUT as exn_attend_packed.  PART (PART_CAP floats, 16-byte aligned, or null and 0): scratch
- * with which few rows' keys are split over the chip and joined in order; calls that may overlap take
- * one each.  exn_kv8_attend_part (needs no GPU): how many floats are of use. */
+ * SCALE, OUT as exn_attend_packed; the weights of codes are rounded to fp16, whatever DT is.  PART
+ * (PART_CAP floats, 16-byte aligned, or null and 0): scratch with which a sequence's keys are split
+ * over the chip and joined in order; calls that may overlap take one each.  exn_kv8_attend_part (needs no GPU): how many floats are of use. */
 int exn_kv8_attend(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, int heads, const void* q, int64_t ldq,
                    float scale, void* out, int odt, int64_t ldo, float* part, int64_t part_cap);
 int exn_kv8_attend_part(const exn_seqs* s, int heads, int kv_heads, int head_dim, int cols, int64_t* floats);
