@@ -548,7 +548,11 @@ int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s,
   if (!ids || !cs || !out || s->rows < 1 || s->rows > 65536)
     FAIL(EXN_EINVAL, "encoder states: %lld rows (1 to 65536), or a null pointer", (long long)s->rows);
   TRY(exn_enc_check(e));
-  return enc_states(e, ids, (int)s->rows, cs, 0, 0, nullptr, nullptr, out, s);
+  try {
+    return enc_states(e, ids, (int)s->rows, cs, 0, 0, nullptr, nullptr, out, s);
+  } catch (const std::bad_alloc&) {
+    FAIL(EXN_ENOMEM, "encoder states: host memory");
+  }
 }
 
 namespace {
@@ -676,6 +680,7 @@ int exn_enc_cache_fork(exn_enc_cache* c, int from, int to) {
     FAIL(EXN_EINVAL, "encoder cache fork: sequence %d to %d of %d", from, to, c ? c->seqs : 0);
   if (from == to) return EXN_OK;
   TRY(use(c->e->ctx));
+  TRY(exn_enc_cache_reset(c, to));   // it stays empty if a copy fails
   // the tails of all layers: a strided copy of one sequence's share of each
   if (c->lens[(size_t)from] % 64) {
     const size_t each = c->block * 2, pitch = each * (size_t)c->seqs;
@@ -683,7 +688,6 @@ int exn_enc_cache_fork(exn_enc_cache* c, int from, int to) {
       HIPCHK(hipMemcpy2DAsync((char*)t + (size_t)to * each, pitch, (const char*)t + (size_t)from * each, pitch, each,
                               (size_t)c->e->layers, hipMemcpyDeviceToDevice, c->e->ctx->stream));
   }
-  cache_drop(c, to, 0);
   for (int b = 0; b < c->cols; ++b) {
     const int32_t p = c->table[(size_t)from * c->cols + b];
     c->table[(size_t)to * c->cols + b] = p;
@@ -735,7 +739,12 @@ int exn_enc_cache_extend(exn_enc_cache* c, const int32_t* ids, const int32_t* le
       exn::set_error("encoder cache extend: %s", hipGetErrorString(h));
       r = EXN_EHIP;
     }
-    if (r == EXN_OK) r = enc_states_host(e, ids, (int)n, pos, pic0, m, merged, deep, out, p.s, c);
+    try {
+      if (r == EXN_OK) r = enc_states_host(e, ids, (int)n, pos, pic0, m, merged, deep, out, p.s, c);
+    } catch (const std::bad_alloc&) {
+      exn::set_error("encoder cache extend: host memory");
+      r = EXN_ENOMEM;
+    }
     for (int i = 0; i < seqs; ++i) {
       if (r == EXN_OK) c->lens[(size_t)i] += lens[i];
       else if (lens[i]) exn_enc_cache_reset(c, i);   // its last block may be half overwritten

@@ -505,8 +505,8 @@ int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s,
  * rows; OUT the new rows' states.  A full block is seen in 8 bits, by the tokens that filled it too.
  * exn_enc_cache_fork: sequence TO becomes FROM as it stands, sharing the pages of its full blocks (a
  * template and a picture's rows encoded once, continued by several instructions).  A refused call
- * changes nothing; one that fails on the GPU empties the sequences it was to extend.  An encoder is
- * destroyed after its caches (EXN_ESTATE before). */
+ * changes nothing; one that fails on the GPU, or for want of memory in its pass, empties the sequences it
+ * was to extend (a fork, TO).  An encoder is destroyed after its caches (EXN_ESTATE before). */
 typedef struct exn_enc_cache exn_enc_cache;
 int exn_enc_cache_create(exn_enc* e, int seqs, int tokens, exn_enc_cache** out);
 int exn_enc_cache_extend(exn_enc_cache* c, const int32_t* ids, const int32_t* lens, int seqs, const int32_t* pos, int pic0,
