@@ -7,6 +7,7 @@
 
 constexpr int kSeqsMax = 1 << 16;
 constexpr int64_t kSeqRowsMax = 1 << 22;
+constexpr int kNewMax = 1 << 21;   // new tokens of a sequence: its blocks are a grid's second axis
 
 int exn_seqs_create(exn_ctx* ctx, const int32_t* lens, int seqs, exn_seqs** out) {
   if (!out) FAIL(EXN_EINVAL, "null output");
@@ -174,6 +175,7 @@ int exn_kv8_append(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const void
   TRY(check_kv8(c, s));
   TRY(check_rows("kv8_append k", k, ldk, (int64_t)c->kv_heads * c->head_dim));
   TRY(check_rows("kv8_append v", v, ldv, (int64_t)c->kv_heads * c->head_dim));
+  if (s->longest > kNewMax) FAIL(EXN_EINVAL, "kv8_append: %d new tokens of a sequence (at most %d)", s->longest, kNewMax);
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
   HIPCHK(kv8_append(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (const uint16_t*)k, ldk, (const uint16_t*)v, ldv));
@@ -184,6 +186,7 @@ int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int
   TRY(check_kv8(c, s));
   TRY(check_rows("kv8_read k", k, ldk, (int64_t)c->kv_heads * c->head_dim));
   TRY(check_rows("kv8_read v", v, ldv, (int64_t)c->kv_heads * c->head_dim));
+  if (s->longest > kNewMax) FAIL(EXN_EINVAL, "kv8_read: %d new tokens of a sequence (at most %d)", s->longest, kNewMax);
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
   HIPCHK(kv8_read(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (uint16_t*)k, ldk, (uint16_t*)v, ldv));

@@ -1371,7 +1371,7 @@ Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim,
     // than it evens out (4 x 1 over 270..333 9.3, shared 15.4; 64 x 1 over 600..1000 26.9, 35.8).  So
     // do many sequences even themselves out (200 x 1 over 700..4000 152, shared 145; 300 x 1 over
     // 300..4000 174, 191).
-    if (cols > 16 && s > 1 && ntiles[w.z] * per <= 4 * slots) {
+    if (cols > 16 && s > 1 && ntiles[w.z] * per <= 4 * slots && ntiles[w.z] * cols <= INT32_MAX) {
       w.splits = (int)s;
       w.floats = s * each + parts;
     }

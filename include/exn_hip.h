@@ -213,7 +213,8 @@ typedef struct exn_kv8 {
   const int32_t* table;
   int32_t* lens;
 } exn_kv8;
-/* the plan's rows of K and V (DT, LDK and LDV values apart) after each sequence's LENS tokens */
+/* the plan's rows of K and V (DT, LDK and LDV values apart) after each sequence's LENS tokens; at most
+ * 2^21 of a sequence in a step */
 int exn_kv8_append(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const void* k, int64_t ldk, const void* v,
                    int64_t ldv);
 /* attention of the plan's rows, after exn_kv8_append of the same rows: row i of a sequence sees its
@@ -493,7 +494,7 @@ int exn_enc_rope_table(const int32_t* pos, int n, double base, float* cs);
 /* exn_enc_states of SEQS prompts in one pass (no reference counterpart: illatio runs them one by
  * one): LENS tokens each (host memory; 0 is allowed), IDS, POS and OUT's rows one prompt after the
  * other, at most 65536 in all; POS NULL gives each text positions from 0.  A prompt's states do not
- * depend on the others'.  _dev: a plan of the prompts (exn_seqs_create) and device arrays, CS the rows'
+ * depend on the others' tokens (how the rows in all are tiled may change a rounding).  _dev: a plan of the prompts (exn_seqs_create) and device arrays, CS the rows'
  * rotary table. */
 int exn_enc_states_packed(exn_enc* e, const int32_t* ids, const int32_t* lens, int seqs, const int32_t* pos, float* out);
 int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s, const float* cs, float* out);

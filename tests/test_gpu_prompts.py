@@ -614,3 +614,52 @@ def test_captured_steps(ctx):
     for b in (*d.b.values(), part, dk, dv, dq, o):
         b.free()
     c2.close()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_captured_splits(ctx, new):
+    """Calls that split keys over workgroups and join them, captured and replayed over lengths that
+    change, with eager calls of other sizes on the same scratch between."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    rng = np.random.default_rng([19, new])
+    kv, hd, heads, cols = 2, 128, 8, 60
+    say("captured splits", new)
+    c2 = X.Context(0)
+    st = ctypes.c_void_p()
+    assert hip.hipStreamCreateWithFlags(ctypes.byref(st), 1) == 0
+    X.call("exn_set_stream", c2.h, st)
+    m, d = filled(c2, "fp16", [3000, 10, 900], kv, hd, cols, rng)
+    plans = [X.Seqs(c2, [new] * 3), X.Seqs(c2, [2, 0, 17])]
+    floats = max(X.kv8_attend_part(s, heads, kv, hd, cols) for s in plans)
+    part = X.DevBuf.of(c2, np.zeros(floats + 4, np.float32))
+    dq, o = (X.DevBuf(c2, (3 * max(new, 7), heads, hd), np.uint16) for _ in range(2))
+
+    def once(s):
+        X.kv8_attend(c2, d.h, s, heads, dq.h, heads * hd, 0.1, o.h, X.DT_BF16, heads * hd, part.h, floats)
+
+    graph, ex = ctypes.c_void_p(), ctypes.c_void_p()
+    c2.sync()
+    assert hip.hipStreamBeginCapture(st, 2) == 0
+    once(plans[0])
+    assert hip.hipStreamEndCapture(st, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(ex), graph, None, None, 0) == 0
+    for lens in ([3000, 10, 900], [64, 3700, 0], [1, 2, 3], [3800, 3800, 3800]):
+        m.lens[:] = lens
+        d.b["lens"].upload(m.lens)
+        qb, q = normal(rng, (3 * max(new, 7), heads, hd), "fp16")
+        dq.upload(qb)
+        for s, lens in ((plans[0], [new] * 3), (plans[1], [2, 0, 17])):
+            if s is plans[0]:
+                assert hip.hipGraphLaunch(ex, st) == 0
+            else:
+                once(s)
+            c2.sync()
+            n = sum(lens)
+            want, tol = m.attend(q[:n], lens, 0.1, "bf16")
+            assert off(pm.value(o.get()[:n], "bf16"), want, tol) <= 1
+    assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
+    X.call("exn_set_stream", c2.h, None)
+    assert hip.hipStreamDestroy(st) == 0
+    for b in (*d.b.values(), part, dq, o):
+        b.free()
+    c2.close()

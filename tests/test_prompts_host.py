@@ -208,3 +208,13 @@ def test_scales_and_codes(L, dt):
         d = L.ph_block(x.ctypes.data_as(vp), 4, c.ctypes.data_as(vp))
         assert np.isfinite(d) and abs(c[0]) <= 127
         assert abs(float(x[0]) - float(d) * c[0]) <= max(abs(float(x[0])) * 2.0 ** -8, 2.0 ** -138)
+
+
+def test_steps_of_too_many_tokens_are_refused(L):
+    for n, ok in ((1 << 21, True), ((1 << 21) + 1, False)):
+        r, h = seqs(L, [5, n])
+        assert r == X.OK
+        c = cache(2)
+        for f in (L.exn_kv8_append, L.exn_kv8_read):
+            assert f(L.ph_ctx(), ctypes.byref(c), h, AT, 128, AT, 128) == (X.OK if ok else X.EINVAL)
+        L.exn_seqs_free(h)
