@@ -11,6 +11,7 @@
 ;;;; rows go to the forward as arguments instead of through il::*after-embed* /
 ;;;; il::*after-layer*.  Loads after hip-dit.lisp and hip-vision.lisp, whose shared object,
 ;;;; status check and %exn-open it uses; listed in ex-nihilo.asd after them and encoder.lisp.
+;;;; It adds encoder-states-packed and the encoder-cache-* functions, which the reference lacks.
 
 (in-package #:ex-nihilo)
 
@@ -142,3 +143,90 @@
 (defun encoder-release (model)
   "MODEL's scratch freed (the weights stay)."
   (exn-check (%exn-enc-release (cdr (gethash model *hip-encoders*)))))
+
+;;; Several prompts in a pass, and prompts kept in 8 bits and continued: the reference has neither
+;;; (encoder-states takes one prompt, src/encoder.lisp:143); a host that serves several calls these.
+
+(sb-alien:define-alien-routine ("exn_enc_states_packed" %exn-enc-states-packed) sb-alien:int
+  (e sb-sys:system-area-pointer) (ids sb-sys:system-area-pointer) (lens sb-sys:system-area-pointer)
+  (seqs sb-alien:int) (pos sb-sys:system-area-pointer) (out sb-sys:system-area-pointer))
+(sb-alien:define-alien-routine ("exn_enc_cache_create" %exn-enc-cache-create) sb-alien:int
+  (e sb-sys:system-area-pointer) (seqs sb-alien:int) (tokens sb-alien:int) (out sb-sys:system-area-pointer))
+(sb-alien:define-alien-routine ("exn_enc_cache_extend" %exn-enc-cache-extend) sb-alien:int
+  (c sb-sys:system-area-pointer) (ids sb-sys:system-area-pointer) (lens sb-sys:system-area-pointer)
+  (seqs sb-alien:int) (pos sb-sys:system-area-pointer) (pic0 sb-alien:int) (m sb-alien:int)
+  (merged sb-sys:system-area-pointer) (deep sb-sys:system-area-pointer) (out sb-sys:system-area-pointer))
+(sb-alien:define-alien-routine ("exn_enc_cache_fork" %exn-enc-cache-fork) sb-alien:int
+  (c sb-sys:system-area-pointer) (from sb-alien:int) (to sb-alien:int))
+(sb-alien:define-alien-routine ("exn_enc_cache_reset" %exn-enc-cache-reset) sb-alien:int
+  (c sb-sys:system-area-pointer) (seq sb-alien:int))
+(sb-alien:define-alien-routine ("exn_enc_cache_destroy" %exn-enc-cache-destroy) sb-alien:int
+  (c sb-sys:system-area-pointer))
+
+(defun gpu-encoder (model)
+  "The library's encoder of MODEL, its weights' expansions as *hip-resident* says."
+  (let ((e (cdr (or (gethash model *hip-encoders*) (error "not a GPU encoder: ~A" model)))))
+    (exn-check (%exn-enc-resident e (if *hip-resident* 1 0)))
+    e))
+
+(defun int32s (numbers)
+  (let ((l (coerce numbers 'list)))
+    (make-array (length l) :element-type '(signed-byte 32) :initial-contents l)))
+
+(defun states-by-length (out lens)
+  "OUT's rows of 4096 floats, LENS of them each: a list of vectors."
+  (let ((at 0))
+    (mapcar (lambda (n) (prog1 (subseq out (* 4096 at) (* 4096 (+ at n))) (incf at n))) lens)))
+
+(defun encoder-states-packed (model prompts)
+  "encoder-states of each of PROMPTS (sequences of ids, at their text positions), in one pass: a list
+   in their order."
+  (let* ((e (gpu-encoder model)) (lens (mapcar #'length prompts)) (n (reduce #'+ lens))
+         (ids (int32s (mapcan (lambda (p) (coerce (copy-seq p) 'list)) prompts)))
+         (lv (int32s lens)) (out (f32vec (* n 4096))))
+    (sb-sys:with-pinned-objects (ids lv out)
+      (exn-check (%exn-enc-states-packed e (sb-sys:vector-sap ids) (sb-sys:vector-sap lv) (length lens)
+                                         (sb-sys:int-sap 0) (sb-sys:vector-sap out))))
+    (states-by-length out lens)))
+
+(defstruct (encoder-cache (:constructor %make-encoder-cache)) handle model seqs)
+
+(defun make-encoder-cache (model seqs tokens)
+  "A cache of SEQS prompts of up to TOKENS tokens each."
+  (%make-encoder-cache :handle (exn-out-pointer #'%exn-enc-cache-create (gpu-encoder model) seqs tokens)
+                       :model model :seqs seqs))
+
+(defun encoder-cache-extend (cache new &key pos picture)
+  "NEW: a list of (sequence . ids), each sequence at most once; their new tokens' states, a list of
+   (sequence . states) by sequence.  POS: the new tokens' (t h w), one list for all in the sequences'
+   order, or NIL (text, on from each sequence's tokens).  PICTURE: (row merged deep), the picture's
+   rows from new row ROW on (DEEP a list of three, or NIL), or NIL."
+  (gpu-encoder (encoder-cache-model cache))
+  (let* ((new (sort (copy-list new) #'< :key #'car))
+         (lens (loop for s below (encoder-cache-seqs cache) collect (length (cdr (assoc s new)))))
+         (n (reduce #'+ lens))
+         (ids (int32s (mapcan (lambda (p) (coerce (copy-seq (cdr p)) 'list)) new)))
+         (lv (int32s lens)) (out (f32vec (* n 4096)))
+         (pv (and pos (int32s (reduce #'append pos :from-end t))))
+         (merged (second picture))
+         (deep (and (third picture) (apply #'concatenate '(simple-array single-float (*)) (third picture)))))
+    (unless (and (= n (length ids)) (or (null pos) (= (length pv) (* 3 n))))
+      (error "sequences ~S of a cache of ~D, positions of ~D tokens" (mapcar #'car new) (encoder-cache-seqs cache)
+             (length pos)))
+    (sb-sys:with-pinned-objects (ids lv out pv merged deep)
+      (flet ((sap (v) (if v (sb-sys:vector-sap v) (sb-sys:int-sap 0))))
+        (exn-check (%exn-enc-cache-extend (encoder-cache-handle cache) (sap ids) (sap lv) (length lens) (sap pv)
+                                          (if picture (first picture) 0) (if merged (floor (length merged) 4096) 0)
+                                          (sap merged) (sap deep) (sap out)))))
+    (mapcar #'cons (mapcar #'car new) (states-by-length out (mapcar (lambda (p) (length (cdr p))) new)))))
+
+(defun encoder-cache-fork (cache from to)
+  "Sequence TO of CACHE becomes FROM as it stands."
+  (exn-check (%exn-enc-cache-fork (encoder-cache-handle cache) from to)))
+
+(defun encoder-cache-reset (cache seq)
+  (exn-check (%exn-enc-cache-reset (encoder-cache-handle cache) seq)))
+
+(defun encoder-cache-free (cache)
+  (exn-check (%exn-enc-cache-destroy (encoder-cache-handle cache)))
+  (setf (encoder-cache-handle cache) nil))
