@@ -108,7 +108,8 @@ struct PackedArgs {
 };
 
 // grid: tiles x chunks x kv_heads, the heads fastest; block 256.  LO: weights as two bf16 parts, where
-// bf16 inputs give fp16 rows: one part's half step, 2^-9, would be eight of the output's.
+// bf16 inputs give fp16 rows: one part's half step, 2^-9, would be eight of the output's (4 x 1100..1180
+// tokens 73 us where bf16 rows take 56; 2.2e-4 from the exact values, in one part 1.2e-3).
 template <int BF, int HD, int LO>
 __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2)
 k_attend_packed(PackedArgs A) {

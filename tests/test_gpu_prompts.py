@@ -555,6 +555,29 @@ def test_cache_not_finite_in_each_kernel(ctx, new, cols, dt):
     assert off(attended(ctx, d, qb, [new] * 3, heads, dt, 0.1), want, tol) <= 1
 
 
+@pytest.mark.parametrize("heads,kv", [(1024, 1), (1024, 1024), (96, 6), (17, 1), (1, 1), (1000, 8)])
+def test_any_number_of_heads(ctx, heads, kv):
+    """As many heads as are taken, groups of 1 to 1024 that do not divide a workgroup's rows: packed
+    prompts, and a cache of short and long tables."""
+    rng = np.random.default_rng([heads, kv])
+    hd, lens = 64, [3, 0, 70]
+    say("heads", heads, kv)
+    rows = sum(lens)
+    qb, q = normal(rng, (rows, heads, hd), "bf16")
+    kb, k = normal(rng, (rows, kv, hd), "bf16")
+    vb, v = normal(rng, (rows, kv, hd), "bf16")
+    dq, dk, dv = (X.DevBuf.of(ctx, b) for b in (qb, kb, vb))
+    o = X.DevBuf(ctx, (rows, heads, hd), np.uint16)
+    X.attend_packed(ctx, X.Seqs(ctx, lens), X.DT_BF16, heads, kv, hd, dq.h, heads * hd, dk.h, kv * hd, dv.h, kv * hd, 0.125,
+                    o.h, X.DT_BF16, heads * hd)
+    want, tol = pm.packed(q, k, v, lens, 0.125, "bf16", "bf16")
+    assert off(pm.value(o.get(), "bf16"), want, tol) <= 1
+    for cols in (3, 33):
+        m, d = cache_of(ctx, "bf16", 3, kv, hd, cols, rng)
+        for new in ([100, 70, 1], [1, 1, 1], [2, 0, 1], [9, 3, 0]):
+            assert step(ctx, m, d, new, heads, "bf16", rng) <= 1
+
+
 # --- a run of them under a graph, on another stream ---------------------------------------------
 
 
