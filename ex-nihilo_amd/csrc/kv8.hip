@@ -382,7 +382,16 @@ __device__ __forceinline__ uint32_t* kv8_parts(const Kv8Args& A, int per, int rt
   return (uint32_t*)(A.part + (int64_t)A.splits * per * 32 * rt * (hd + 2));
 }
 
+// Weights are 2^(score - reference), the reference at most MAX_SLACK under the row's largest score, and
+// fp16 for codes of either type.  fp16 has none under 2^-24, which the many small ones beside one that
+// takes nearly all would be: they are held 2^LIFT higher (up to 2^15), and what is lost is under 2^-32
+// of a row's largest.  A key of no value with 0.999 of the weight before 8,100 others, fp16 rows: 2.3e-4
+// off (relative L2), which is their rounding, and unlifted 1.4e-2 (k_kv8_chunk).  Sums of weights are kept
+// as high, sums of weights and values are not (a block's scale takes the 2^-LIFT, exactly: it has 12
+// significant bits or is a multiple of 2^-137).
 #define MAX_SLACK 8.f
+#define LIFT 7.f
+#define LIFT2 128.f   // 2^LIFT
 
 // --- few rows ------------------------------------------------------------------------------------
 //
@@ -475,7 +484,7 @@ k_kv8_few(Kv8Args A) {
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
     kds = d[0];
-    vds = d[1];
+    vds = d[1] * (1.f / LIFT2);
   };
   u32x4 kr[4][KL], vr[ND];
   // the codes are read once: past the caches
@@ -554,20 +563,21 @@ k_kv8_few(Kv8Args A) {
         for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[rt][e]);
         mx = max_groups(mx);
         // a first reference (any above -inf), or one that has fallen behind
-        if (__ballot(mx > mrun[rt] + MAX_SLACK)) {
-          const float mn = mx > mrun[rt] + MAX_SLACK ? mx : mrun[rt];
+        if (__ballot(mx > mrun[rt] + (MAX_SLACK + LIFT))) {
+          const float mn = mx > mrun[rt] + (MAX_SLACK + LIFT) ? mx - LIFT : mrun[rt];
           const float a = mn == mrun[rt] ? 1.f : __builtin_amdgcn_exp2f(mrun[rt] - mn);
           mrun[rt] = mn;
           lrun[rt] *= a;
 #pragma unroll
           for (int d = 0; d < ND; ++d) o[rt][d] *= a;
         }
+        constexpr bool WB = decltype(bf_c)::value;
         const float ref = mrun[rt] == -INFINITY ? 0.f : mrun[rt];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
           const float p0 = __builtin_amdgcn_exp2f(s[rt][e] - ref), p1 = __builtin_amdgcn_exp2f(s[rt][e + 1] - ref);
-          pk[rt][e / 2] = decltype(bf_c)::value ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
-          if constexpr (decltype(bf_c)::value)
+          pk[rt][e / 2] = WB ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+          if constexpr (WB)
             pl[rt][e / 2] = pack_bf16x2(p0 - bf16_lo(pk[rt][e / 2]), p1 - bf16_hi(pk[rt][e / 2]));
           lrun[rt] += p0;
           lrun[rt] += p1;
@@ -690,11 +700,14 @@ k_kv8_few(Kv8Args A) {
           for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(a[d][e]) & 0x7F800000u) == 0x7F800000u;
           __builtin_amdgcn_sched_barrier(0);
         }
+        float down = 1.f / LIFT2;
         if (__ballot(bad)) {
-          // an infinity or a NaN among the values: again, each row over the keys it sees only
+          // an infinity or a NaN among the values, or a sum past fp32's largest: again, each row over the
+          // keys it sees only, with weights that are not lifted
+          down = 1.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            pbuf[16 * g + e][col] = __builtin_amdgcn_exp2f(s[rt][e] - (mrun[rt] == -INFINITY ? 0.f : mrun[rt]));
+            pbuf[16 * g + e][col] = __builtin_amdgcn_exp2f(s[rt][e] - (mrun[rt] == -INFINITY ? 0.f : mrun[rt])) * (1.f / LIFT2);
           asm volatile("" ::: "memory");
           __builtin_amdgcn_s_waitcnt(0xC07F);
           asm volatile("" ::: "memory");
@@ -712,7 +725,7 @@ k_kv8_few(Kv8Args A) {
           }
         }
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[rt][d] += a[d];
+        for (int d = 0; d < ND; ++d) o[rt][d] += a[d] * down;
       }
     }
 
@@ -736,9 +749,9 @@ k_kv8_few(Kv8Args A) {
       __syncthreads();
 #pragma unroll
       for (int d = 0; d < ND; ++d) *(f32x4*)&obuf[wave][col][16 * d + 4 * g] = o[rt][d];
-      const float l = sum_groups(lrun[rt]);
+      const float l = sum_groups(lrun[rt]) * (1.f / LIFT2);
       if (g == 0) {
-        mbuf[wave][col] = mrun[rt];
+        mbuf[wave][col] = mrun[rt] + LIFT;
         lbuf[wave][col] = l;
       }
       __syncthreads();
@@ -1045,13 +1058,14 @@ k_kv8_chunk(Kv8Args A) {
   auto step = [&](auto last_c, auto tail_c, int b, const Facts& F) __attribute__((always_inline)) {
     constexpr bool LAST = decltype(last_c)::value, TAIL = decltype(tail_c)::value;
     constexpr int WB = TAIL && BF;   // weights: fp16, or with values in bf16 two bf16 parts
+    constexpr float UP = WB ? 0.f : LIFT;
     const int k0 = b * 64;
     const float factor = F.kd * A.scale;
     const bool gone = F.page < 0 && b < nfull;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[h][r] = __builtin_fmaf(sc[h][r], factor, -mrun);
+      for (int r = 0; r < 16; ++r) sc[h][r] = __builtin_fmaf(sc[h][r], factor, UP - mrun);
     if (gone || k0 + 63 > minlim) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -1073,9 +1087,9 @@ k_kv8_chunk(Kv8Args A) {
     float ma = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), mb = ma;
     xswap32(ma, mb);
     const float mx = fmaxf(ma, mb);
-    const bool move = set ? mx > MAX_SLACK : mx > -INFINITY;
+    const bool move = set ? mx > MAX_SLACK + UP : mx > -INFINITY;
     if (__ballot(move)) {
-      const float shift = move ? mx : 0.f;
+      const float shift = move ? mx - UP : 0.f;
       const float alpha = set ? __builtin_amdgcn_exp2f(-shift) : 1.f;   // without a reference the sums are 0, or NaN
       lrun *= alpha;
 #pragma unroll
@@ -1117,15 +1131,15 @@ k_kv8_chunk(Kv8Args A) {
         const float p0 = __builtin_amdgcn_exp2f(sc[h][r]), p1 = __builtin_amdgcn_exp2f(sc[h][r + 1]);
         pk[pi] = WB ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
         if constexpr (WB) pl[pi] = pack_bf16x2(p0 - bf16_lo(pk[pi]), p1 - bf16_hi(pk[pi]));
-        ls[0] += p0;
-        ls[1] += p1;
+        ls[0] += WB ? p0 * LIFT2 : p0;
+        ls[1] += WB ? p1 * LIFT2 : p1;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
     lrun = ls[0] + ls[1];
     // a block's products of codes, then its scale; a row that sees nothing of it takes nothing of the scale,
     // which may be NaN
-    const float vd = gone || k0 > lim ? 0.f : F.vd;
+    const float vd = gone || k0 > lim ? 0.f : (TAIL ? 1.f : F.vd) * (1.f / LIFT2);
     f32x16 t[2];
 #pragma unroll
     for (int j = 0; j < 4 * ND; ++j) {
@@ -1133,10 +1147,9 @@ k_kv8_chunk(Kv8Args A) {
       if (j + KD < 4 * ND) vn = vfrag(tail_c, (j + KD) % 4, (j + KD) / 4);
       const int u = j % 4, d = j / 4;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
-      if constexpr (TAIL) {
-        o[d] = mfma32<BF>(vq[0], pb, o[d]);
-        if constexpr (WB)
-          o[d] = mfma32<BF>(vq[0], __builtin_bit_cast(s16x8, u32x4{pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]}), o[d]);
+      if constexpr (WB) {
+        o[d] = mfma32<1>(vq[0], pb, o[d]);
+        o[d] = mfma32<1>(vq[0], __builtin_bit_cast(s16x8, u32x4{pl[4 * u], pl[4 * u + 1], pl[4 * u + 2], pl[4 * u + 3]}), o[d]);
       } else {
         t[d % 2] = mfma32<0>(vq[0], pb, u == 0 ? f32x16{} : t[d % 2]);
         if (d > 0) {
@@ -1149,7 +1162,7 @@ k_kv8_chunk(Kv8Args A) {
       vq[KD - 1] = vn;
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (!TAIL) {
+    if constexpr (!WB) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[ND - 1][r] = __builtin_fmaf(t[(ND - 1) % 2][r], vd, o[ND - 1][r]);
     }
@@ -1223,7 +1236,7 @@ k_kv8_chunk(Kv8Args A) {
 
   float la = lrun, lb = lrun;
   xswap32(la, lb);
-  const float sum = la + lb, mul = active > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+  const float sum = (la + lb) * (1.f / LIFT2), mul = active > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   float zero[4] = {sum * 0.f};
   const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = A.rows * A.heads;
   auto leave = [&](auto obf) __attribute__((always_inline)) {

@@ -3,7 +3,10 @@
 //   o[i, h] = sum_{j <= i} p_j v[j, h / g] / sum_{j <= i} p_j,  p_j = 2^(scale log2(e) q[i, h].k[j, h / g] - m)
 // in one pass over the keys with m a running reference (the row's running max, which it may lag by
 // MAX_SLACK; sums and rescales in fp32, p rounded to the inputs' 16 bits for the second product: half
-// a step of a weight, as much as the output's own rounding).
+// a step of a weight, as much as the output's own rounding).  fp16 has no weight under 2^-24, which many
+// small ones beside one that takes nearly all would be, so m lies F16_LIFT under the reference: weights reach
+// 2^(F16_LIFT + MAX_SLACK) of fp16's 2^16, and what is lost is under 2^-32 of a row's largest (a key of no
+// value with 0.999 of the weight before 5,000 others, fp16 rows: 2.1e-4 off, unlifted 3.8e-2).
 //
 // A workgroup takes TT tokens of one sequence times the HH query heads of one key/value head: 128
 // rows, 32 a wave, row r being token r / HH and head r % HH.  The heads of a group so share every
@@ -28,6 +31,7 @@ namespace exn {
 
 #define PK 64            // keys a tile
 #define MAX_SLACK 8.f    // log2 units the running max may lag the true max by
+#define F16_LIFT 7.f     // log2 units that fp16 weights are held higher
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -119,6 +123,7 @@ k_attend_packed(PackedArgs A) {
   constexpr int DI = PK / RI / 4;                   // DMA instructions a wave and tile
   constexpr int NS = HD / 16;                       // k-steps of the S product
   constexpr int ND = HD / 32;                       // 32-dim blocks of O
+  constexpr float LIFT = BF ? 0.f : F16_LIFT;
   // K stage s at s STAGE, V stage s at (2 + s) STAGE, in two rings one tile apart: step t reads K of
   // tile t+1 and V of tile t.  K rows: 16-byte chunk c at c ^ (row % 16) (HD 64: c ^ (row / 2 % 8)),
   // so that 32 rows' same chunk meets every bank once; V rows: c ^ 4 (row % 4) (HD 64: c ^ 4 (row / 2
@@ -229,7 +234,7 @@ k_attend_packed(PackedArgs A) {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[b][r] = __builtin_fmaf(sc[b][r], A.scale, -mrun);
+      for (int r = 0; r < 16; ++r) sc[b][r] = __builtin_fmaf(sc[b][r], A.scale, LIFT - mrun);
     if (k0 + PK - 1 > minlim) {   // some key of this tile is hidden from some row
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -250,9 +255,9 @@ k_attend_packed(PackedArgs A) {
     }
     const float mx = pmax32(max3(max3(m4[0], m4[1], m4[2]), m4[3], m4[3]));
     // the first tile always sets the reference (its key 0 is visible to every row)
-    const bool move = t == 0 || mx > MAX_SLACK;
+    const bool move = t == 0 || mx > MAX_SLACK + LIFT;
     if (__ballot(move)) {
-      const float shift = move ? mx : 0.f;
+      const float shift = move ? mx - LIFT : 0.f;
       if (t > 0) {
         const float alpha = __builtin_amdgcn_exp2f(-shift);
         lrun *= alpha;
