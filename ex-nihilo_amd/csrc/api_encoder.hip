@@ -680,13 +680,18 @@ int exn_enc_cache_fork(exn_enc_cache* c, int from, int to) {
     FAIL(EXN_EINVAL, "encoder cache fork: sequence %d to %d of %d", from, to, c ? c->seqs : 0);
   if (from == to) return EXN_OK;
   TRY(use(c->e->ctx));
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIPCHK(hipStreamIsCapturing(c->e->ctx->stream, &cap));
+  if (cap != hipStreamCaptureStatusNone) FAIL(EXN_ESTATE, "encoder cache fork: not in a stream capture");
   TRY(exn_enc_cache_reset(c, to));   // it stays empty if a copy fails
-  // the tails of all layers: a strided copy of one sequence's share of each
+  // the tails of all layers: a strided copy of one sequence's share of each, done before TO has them (the
+  // next call may be ordered on another stream)
   if (c->lens[(size_t)from] % 64) {
     const size_t each = c->block * 2, pitch = each * (size_t)c->seqs;
     for (uint16_t* t : {c->tk, c->tv})
       HIPCHK(hipMemcpy2DAsync((char*)t + (size_t)to * each, pitch, (const char*)t + (size_t)from * each, pitch, each,
                               (size_t)c->e->layers, hipMemcpyDeviceToDevice, c->e->ctx->stream));
+    HIPCHK(hipStreamSynchronize(c->e->ctx->stream));
   }
   for (int b = 0; b < c->cols; ++b) {
     const int32_t p = c->table[(size_t)from * c->cols + b];

@@ -505,7 +505,8 @@ int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s,
  * goes on from the sequence's tokens so far; the picture's rows as in exn_enc_states, among the new
  * rows; OUT the new rows' states.  A full block is seen in 8 bits, by the tokens that filled it too.
  * exn_enc_cache_fork: sequence TO becomes FROM as it stands, sharing the pages of its full blocks (a
- * template and a picture's rows encoded once, continued by several instructions).  A refused call
+ * template and a picture's rows encoded once, continued by several instructions), and is done on return;
+ * like extend, it is refused in a stream capture (EXN_ESTATE).  A refused call
  * changes nothing; one that fails on the GPU, or for want of memory in its pass, empties the sequences it
  * was to extend (a fork, TO).  An encoder is destroyed after its caches (EXN_ESTATE before). */
 typedef struct exn_enc_cache exn_enc_cache;
