@@ -33,6 +33,13 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return __builtin_bit_cast(uint32_t, v);
 }
 
+// A mean of fp16 values, or 127 steps of the scale of a block of them, is past fp16's largest by its own
+// rounding alone (at most 2^-11 of it): finite values stay finite, infinities and NaN as they are
+__device__ __forceinline__ float in_f16(float x) {
+  return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x;
+}
+__device__ __forceinline__ uint32_t pack_f16x2_in(float a, float b) { return pack_f16x2(in_f16(a), in_f16(b)); }
+
 __device__ __forceinline__ float f16_lo(uint32_t u) {
   return (float)__builtin_bit_cast(f16x2, u)[0];
 }

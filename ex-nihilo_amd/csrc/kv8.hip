@@ -224,7 +224,7 @@ k_kv8_read(Kv8 c, const SeqTile* __restrict__ seqs, uint16_t* __restrict__ k, in
         for (int e = 0; e < E; e += 2) {
           const float a = d * (float)(int8_t)(code[i][e / 4] >> (8 * (e % 4)));
           const float z = d * (float)(int8_t)(code[i][e / 4] >> (8 * (e % 4) + 8));
-          r[i].w[e / 2] = c.bf16 ? pack_bf16x2(a, z) : pack_f16x2(a, z);
+          r[i].w[e / 2] = c.bf16 ? pack_bf16x2(a, z) : pack_f16x2_in(a, z);
         }
     }
   } else {
@@ -310,6 +310,11 @@ __device__ __forceinline__ float sum_groups(float v) {
   a = b = a + b;
   xswap32(a, b);
   return a + b;
+}
+
+// results of a cache of type BF (bf16's may well be past fp16's range)
+__device__ __forceinline__ uint32_t pack_out(float a, float b, int bf, int obf) {
+  return obf ? pack_bf16x2(a, b) : bf ? pack_f16x2(a, b) : pack_f16x2_in(a, b);
 }
 
 struct Kv8Args {
@@ -790,7 +795,7 @@ k_kv8_few(Kv8Args A) {
           for (int e = 0; e < E; e += 2) x[e / 2] = pack_bf16x2(y[e], y[e + 1]);
         } else {
 #pragma unroll
-          for (int e = 0; e < E; e += 2) x[e / 2] = pack_f16x2(y[e], y[e + 1]);
+          for (int e = 0; e < E; e += 2) x[e / 2] = pack_out(y[e], y[e + 1], BF, 0);
         }
         uint16_t* po = A.out + (int64_t)(T.row0 + tok) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + d0;
         if constexpr (E == 8)
@@ -849,8 +854,7 @@ k_kv8_join_few(Kv8Args A) {
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* po = A.out + (int64_t)(T.row0 + tok) * A.ldo + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + d;
-  *(u32x2*)po = A.obf ? u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)}
-                      : u32x2{pack_f16x2(y[0] * inv, y[1] * inv), pack_f16x2(y[2] * inv, y[3] * inv)};
+  *(u32x2*)po = u32x2{pack_out(y[0] * inv, y[1] * inv, A.c.bf16, A.obf), pack_out(y[2] * inv, y[3] * inv, A.c.bf16, A.obf)};
 }
 
 // --- many rows: 128 a workgroup -------------------------------------------------------------------
@@ -1258,7 +1262,7 @@ k_kv8_chunk(Kv8Args A) {
         else if constexpr (decltype(obf)::value == 1)
           *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
         else
-          *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3])};
+          *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack_out(y[0], y[1], BF, 0), pack_out(y[2], y[3], BF, 0)};
       }
   };
   if (active > 1) {
@@ -1283,7 +1287,7 @@ k_kv8_chunk(Kv8Args A) {
       if (active > 1)
         A.part[slot * HD + z * 64 + lane] = w;
       else
-        A.out[at * A.ldo + rh * HD + z * 64 + lane] = (uint16_t)(A.obf ? pack_bf16x2(w, 0.f) : pack_f16x2(w, 0.f));
+        A.out[at * A.ldo + rh * HD + z * 64 + lane] = (uint16_t)pack_out(w, 0.f, BF, A.obf);
     }
     if (active > 1 && lane == 0) *(f32x2*)(A.part + A.splits * n * HD + slot * 2) = f32x2{m, l};
   }
@@ -1341,8 +1345,7 @@ k_kv8_join(Kv8Args A) {
   if ((int)blockIdx.y * RW + r >= live * A.heads) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* po = A.out + (rowhead / A.heads) * A.ldo + (rowhead % A.heads) * HD + d;
-  *(u32x2*)po = A.obf ? u32x2{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)}
-                      : u32x2{pack_f16x2(y[0] * inv, y[1] * inv), pack_f16x2(y[2] * inv, y[3] * inv)};
+  *(u32x2*)po = u32x2{pack_out(y[0] * inv, y[1] * inv, A.c.bf16, A.obf), pack_out(y[2] * inv, y[3] * inv, A.c.bf16, A.obf)};
 }
 
 namespace {

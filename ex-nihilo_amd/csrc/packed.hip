@@ -43,6 +43,11 @@ __device__ __forceinline__ float ld16(const uint16_t* p) {
   return BF ? bf16_to_f32(*p) : f16_to_f32(*p);
 }
 __device__ __forceinline__ uint32_t pack16(float a, float b, int bf) { return bf ? pack_bf16x2(a, b) : pack_f16x2(a, b); }
+// results of inputs of type BF (bf16's may well be past fp16's range)
+template <int BF>
+__device__ __forceinline__ uint32_t pack_out(float a, float b, int obf) {
+  return obf ? pack_bf16x2(a, b) : BF ? pack_f16x2(a, b) : pack_f16x2_in(a, b);
+}
 
 template <int BF>
 __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
@@ -96,7 +101,7 @@ __device__ void packed_row(const uint16_t* __restrict__ q, const uint16_t* __res
         o[e] = (c == 0 ? o[e] * a : o[e]) + pc * ld16<BF>(v + (int64_t)(j0 + c) * ldv + e * 64 + lane);
     }
   }
-  for (int e = 0; e < HD / 64; ++e) out[e * 64 + lane] = (uint16_t)pack16(o[e] / l, 0.f, obf);
+  for (int e = 0; e < HD / 64; ++e) out[e * 64 + lane] = (uint16_t)pack_out<BF>(o[e] / l, 0.f, obf);
 }
 
 struct PackedArgs {
@@ -375,8 +380,8 @@ k_attend_packed(PackedArgs A) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) zero[e] = __builtin_fmaf(o[d][4 * r4 + e], 0.f, zero[e]);
         *(u32x2*)(mem + lo * ROWB + ((c ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4) + 8 * hi) =
-            u32x2{pack16(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, decltype(obf)::value),
-                  pack16(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv, decltype(obf)::value)};
+            u32x2{pack_out<BF>(o[d][4 * r4] * inv, o[d][4 * r4 + 1] * inv, decltype(obf)::value),
+                  pack_out<BF>(o[d][4 * r4 + 2] * inv, o[d][4 * r4 + 3] * inv, decltype(obf)::value)};
       }
   };
   if (A.obf)

@@ -226,7 +226,7 @@ int exn_kv8_attend(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, int heads,
                    float scale, void* out, int odt, int64_t ldo, float* part, int64_t part_cap);
 int exn_kv8_attend_part(const exn_seqs* s, int heads, int kv_heads, int head_dim, int cols, int64_t* floats);
 /* the plan's rows as the cache holds them after exn_kv8_append, into K and V (DT; code x scale,
- * rounded once; zeros where nothing is kept) */
+ * rounded once, in fp16 to 65504 at most; zeros where nothing is kept) */
 int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int64_t ldk, void* v, int64_t ldv);
 /* LENS += the plan's lengths, on the device: the step's last call */
 int exn_kv8_advance(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s);
