@@ -135,6 +135,14 @@ int check_kv8(const exn_kv8* c, const exn_seqs* s) {
   return EXN_OK;
 }
 
+// what a launch returned: the sizes it has no grid for are the caller's
+int launched(const char* what, hipError_t e) {
+  if (e == hipErrorInvalidConfiguration)
+    FAIL(EXN_EINVAL, "%s: more than 2^24 - 1 workgroups (fewer sequences or key/value heads)", what);
+  if (e != hipSuccess) FAIL(e == hipErrorOutOfMemory ? EXN_ENOMEM : EXN_EHIP, "%s: %s", what, hipGetErrorString(e));
+  return EXN_OK;
+}
+
 Kv8 kv8_of(const exn_kv8* c) {
   Kv8 k;
   k.bf16 = c->dt == EXN_DT_BF16;
@@ -164,10 +172,10 @@ int exn_attend_packed(exn_ctx* ctx, const exn_seqs* s, int dt, int heads, int kv
   TRY(check_rows("attend_packed out", out, ldo, (int64_t)heads * head_dim));
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
-  HIPCHK(attend_packed(ctx->stream, s->tiles, s->ntiles, dt == EXN_DT_BF16, heads, kv_heads, head_dim,
-                       (const uint16_t*)q, ldq, (const uint16_t*)k, ldk, (const uint16_t*)v, ldv, scale, (uint16_t*)out,
-                       odt == EXN_DT_BF16, ldo));
-  return EXN_OK;
+  return launched("attend_packed",
+                  attend_packed(ctx->stream, s->tiles, s->ntiles, dt == EXN_DT_BF16, heads, kv_heads, head_dim,
+                                (const uint16_t*)q, ldq, (const uint16_t*)k, ldk, (const uint16_t*)v, ldv, scale,
+                                (uint16_t*)out, odt == EXN_DT_BF16, ldo));
 }
 
 int exn_kv8_append(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const void* k, int64_t ldk, const void* v,
@@ -178,8 +186,8 @@ int exn_kv8_append(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const void
   if (s->longest > kNewMax) FAIL(EXN_EINVAL, "kv8_append: %d new tokens of a sequence (at most %d)", s->longest, kNewMax);
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
-  HIPCHK(kv8_append(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (const uint16_t*)k, ldk, (const uint16_t*)v, ldv));
-  return EXN_OK;
+  return launched("kv8_append", kv8_append(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (const uint16_t*)k,
+                                           ldk, (const uint16_t*)v, ldv));
 }
 
 int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int64_t ldk, void* v, int64_t ldv) {
@@ -189,8 +197,8 @@ int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int
   if (s->longest > kNewMax) FAIL(EXN_EINVAL, "kv8_read: %d new tokens of a sequence (at most %d)", s->longest, kNewMax);
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
-  HIPCHK(kv8_read(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (uint16_t*)k, ldk, (uint16_t*)v, ldv));
-  return EXN_OK;
+  return launched("kv8_read", kv8_read(ctx->stream, kv8_of(c), s->whole, s->seqs, s->longest, (uint16_t*)k, ldk,
+                                       (uint16_t*)v, ldv));
 }
 
 int exn_kv8_advance(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s) {
@@ -219,7 +227,7 @@ int exn_kv8_attend(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, int heads,
     FAIL(EXN_EINVAL, "kv8_attend: %lld floats of scratch at %p", (long long)part_cap, (const void*)part);
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
-  HIPCHK(kv8_attend(ctx->stream, kv8_of(c), s->tiles, s->ntiles, s->rows, s->longest, heads,
-                    (const uint16_t*)q, ldq, scale, (uint16_t*)out, odt == EXN_DT_BF16, ldo, part, part_cap));
-  return EXN_OK;
+  return launched("kv8_attend",
+                  kv8_attend(ctx->stream, kv8_of(c), s->tiles, s->ntiles, s->rows, s->longest, heads, (const uint16_t*)q,
+                             ldq, scale, (uint16_t*)out, odt == EXN_DT_BF16, ldo, part, part_cap));
 }

@@ -294,9 +294,12 @@ hipError_t attend(hipStream_t s, const uint16_t* q, const uint16_t* k, const uin
 // tokens t0 .. t0 + tt - 1 (as far as len) of sequence seq, whose rows begin at row0 and are len
 #define SEQ_TT0 8   // tokens a tile of the first list; list i has SEQ_TT0 << i
 #define SEQ_TTS 5
+// workgroups of 256 threads on a grid's first axis: a launch counts that axis' threads in 32 bits
+#define WG256_MAX ((int64_t)0xFFFFFFFF / 256)
 struct SeqTile {
   int32_t row0, len, t0, seq;
 };
+// the launches below return hipErrorInvalidConfiguration where they would be of more than WG256_MAX workgroups
 hipError_t attend_packed(hipStream_t s, const SeqTile* const* tiles, const int64_t* ntiles, int bf16, int heads,
                          int kv_heads, int head_dim, const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk,
                          const uint16_t* v, int64_t ldv, float scale, uint16_t* out, int obf, int64_t ldo);

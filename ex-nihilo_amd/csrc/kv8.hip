@@ -156,6 +156,7 @@ k_kv8_append(Kv8 c, const SeqTile* __restrict__ seqs, const uint16_t* __restrict
 hipError_t kv8_append(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, int longest, const uint16_t* k,
                       int64_t ldk, const uint16_t* v, int64_t ldv) {
   if (n == 0 || longest == 0) return hipSuccess;
+  if ((int64_t)n * c.kv_heads > WG256_MAX) return hipErrorInvalidConfiguration;
   const dim3 grid(n * c.kv_heads, (62 + longest) / 64 + 1, 2);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv); };
   if (c.head_dim == 128)
@@ -243,6 +244,7 @@ k_kv8_read(Kv8 c, const SeqTile* __restrict__ seqs, uint16_t* __restrict__ k, in
 hipError_t kv8_read(hipStream_t s, const Kv8& c, const SeqTile* seqs, int n, int longest, uint16_t* k, int64_t ldk,
                     uint16_t* v, int64_t ldv) {
   if (n == 0 || longest == 0) return hipSuccess;
+  if ((int64_t)n * c.kv_heads > WG256_MAX) return hipErrorInvalidConfiguration;
   const dim3 grid(n * c.kv_heads, (62 + longest) / 64 + 1, 2);
   if (c.head_dim == 128)
     hipLaunchKernelGGL(k_kv8_read<128>, grid, dim3(256), 0, s, c, seqs, k, ldk, v, ldv);
@@ -1443,7 +1445,7 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   a.rows = rows;
   const int64_t groups = (w.rt && w.splits ? w.splits : ntiles[w.z]) * w.chunks * c.kv_heads;
   const int64_t joins = ntiles[w.z] * w.chunks * c.kv_heads;
-  if (groups > INT32_MAX || joins > INT32_MAX) return hipErrorInvalidValue;
+  if (groups > WG256_MAX || (w.splits > 1 && joins > WG256_MAX)) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)groups, w.rt ? 1 : w.splits);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {

@@ -433,7 +433,7 @@ hipError_t attend_packed(hipStream_t s, const SeqTile* const* tiles, const int64
   a.tiles = tiles[z];
   a.obf = obf;
   const int64_t groups = ntiles[z] * a.chunks * kv_heads;
-  if (groups > INT32_MAX) return hipErrorInvalidValue;
+  if (groups > WG256_MAX) return hipErrorInvalidConfiguration;
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, s, a); };
   if (bf16 && obf)
     head_dim == 128 ? go(k_attend_packed<1, 128, 0>) : go(k_attend_packed<1, 64, 0>);

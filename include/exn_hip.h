@@ -178,7 +178,10 @@ int exn_euler(exn_ctx* ctx, int64_t count, float* z, const float* v, float ds);
  * reference counterpart: illatio runs one prompt at a time, src/encoder.lisp:143-183) ------------ */
 
 /* SEQS sequences of LENS tokens (host memory; 0 is allowed), packed one after the other in rows 0 ..
- * sum - 1: the plan that the calls below take.  At most 2^16 sequences and 2^22 rows.  Made outside
+ * sum - 1: the plan that the calls below take.  At most 2^16 sequences and 2^22 rows (and no more of
+ * them, with a call's heads, than fit in 2^24 - 1 workgroups: EXN_EINVAL; exn_kv8_append and read take a
+ * workgroup for each sequence and key/value head, the attention at most one for each 8 tokens begun and
+ * head).  Made outside
  * stream capture; freed when no work that reads it is left (exn_seqs_free waits for the device). */
 typedef struct exn_seqs exn_seqs;
 int exn_seqs_create(exn_ctx* ctx, const int32_t* lens, int seqs, exn_seqs** out);
