@@ -800,6 +800,16 @@ def load_encoder(tensors=None, *, device: int = 0, layers: int = 36, seed: int |
     return e
 
 
+def _picture(merged, deep):
+    """A picture's rows for the library, which reads m x 4096 floats of MERGED and 3 m x 4096 of DEEP."""
+    mg = np.ascontiguousarray(merged, dtype=np.float32)
+    dp = None if deep is None else np.ascontiguousarray(deep, dtype=np.float32)
+    if mg.ndim != 2 or mg.shape[1] != WIDTH or (dp is not None and dp.size != 3 * mg.size):
+        raise ExnError(EINVAL, "picture rows of %s, deep %s: not (m, %d) and (3, m, %d)"
+                       % (mg.shape, None if dp is None else dp.shape, WIDTH, WIDTH))
+    return mg, dp
+
+
 def encoder_states(e: Encoder, ids, pos=None, picture=None):
     """encoder-states (src/encoder.lisp:143-183): every token's state after the last block,
     before the final norm, (n, 4096).  POS: (n, 3) (t, h, w) positions or None (text 0..n-1);
@@ -812,8 +822,7 @@ def encoder_states(e: Encoder, ids, pos=None, picture=None):
         call("exn_enc_states", e.h, ptr(ids), n, None if p is None else ptr(p), 0, 0, None, None, ptr(out))
     else:
         a0, merged, deep = picture
-        mg = np.ascontiguousarray(merged, dtype=np.float32)
-        dp = None if deep is None else np.ascontiguousarray(deep, dtype=np.float32)
+        mg, dp = _picture(merged, deep)
         call("exn_enc_states", e.h, ptr(ids), n, None if p is None else ptr(p), a0, len(mg), ptr(mg),
              None if dp is None else ptr(dp), ptr(out))
     return out
@@ -864,10 +873,9 @@ class EncoderCache:
         pic = (0, 0, None, None)
         if picture is not None:
             s, a0, merged, deep = picture
-            mg = np.ascontiguousarray(merged, dtype=np.float32)
-            dp = None if deep is None else np.ascontiguousarray(deep, dtype=np.float32)
-            if a0 < 0 or a0 + len(mg) > lens[s]:
-                raise ExnError(EINVAL, "picture rows %d at %d of %d new tokens" % (len(mg), a0, lens[s]))
+            mg, dp = _picture(merged, deep)
+            if s not in new or a0 < 0 or a0 + len(mg) > lens[s]:
+                raise ExnError(EINVAL, "picture rows %d at %d of sequence %s, new tokens %s" % (len(mg), a0, s, lens.tolist()))
             pic = (int(starts[s]) + a0, len(mg), ptr(mg), None if dp is None else ptr(dp))
         call("exn_enc_cache_extend", self.h, ptr(ids), ptr(lens), self.seqs, None if p is None else ptr(p), *pic, ptr(out))
         return {s: out[starts[s]:starts[s + 1]] for s in new}

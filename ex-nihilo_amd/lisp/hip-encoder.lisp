@@ -213,6 +213,8 @@
     (unless (and (= n (length ids)) (or (null pos) (= (length pv) (* 3 n))))
       (error "sequences ~S of a cache of ~D, positions of ~D tokens" (mapcar #'car new) (encoder-cache-seqs cache)
              (length pos)))
+    (unless (and (zerop (mod (length merged) 4096)) (or (null deep) (= (length deep) (* 3 (length merged)))))
+      (error "picture rows of ~D floats, deep of ~D: not 4096 M and 3 x 4096 M" (length merged) (length deep)))
     (sb-sys:with-pinned-objects (ids lv out pv merged deep)
       (flet ((sap (v) (if v (sb-sys:vector-sap v) (sb-sys:int-sap 0))))
         (exn-check (%exn-enc-cache-extend (encoder-cache-handle cache) (sap ids) (sap lv) (length lens) (sap pv)
