@@ -893,9 +893,17 @@ class EncoderCache:
         return a
 
     def destroy(self):
-        if self.h:
+        if getattr(self, "h", None):
             call("exn_enc_cache_destroy", self.h)
             self.h = None
+
+    def __del__(self):
+        # its encoder can not be destroyed before it; with the context closed there is nothing to free
+        try:
+            if self.e.ctx.h:
+                self.destroy()
+        except Exception:
+            pass
 
 
 def enc_rope_table(n: int, pos=None, base: float = ENC_ROPE_BASE):
