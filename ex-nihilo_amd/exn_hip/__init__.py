@@ -858,8 +858,10 @@ class EncoderCache:
 
     def extend(self, new, pos=None, picture=None):
         """NEW: {sequence: token ids}; the new tokens' states, {sequence: (n, 4096)}.  POS:
-        {sequence: (n, 3)} or None (text, on from the sequence's tokens); PICTURE: (sequence, a0, merged,
-        deep or None), the picture's rows from that sequence's new row a0 on."""
+        {sequence: (n, 3)} or None (text, on from the sequence's count of tokens); PICTURE: (sequence, a0,
+        merged, deep or None), the picture's rows from that sequence's new row a0 on.  A picture's rows, and
+        the tokens after them in this call and later ones, do not stand where None has them
+        (src/encoder.lisp:125-129): give POS."""
         if any(s < 0 or s >= self.seqs for s in new):
             raise ExnError(EINVAL, "sequences %s of %d" % (sorted(new), self.seqs))
         ids, lens = _packed([new.get(s, ()) for s in range(self.seqs)], 0, np.int32)

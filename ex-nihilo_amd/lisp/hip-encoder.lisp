@@ -199,8 +199,9 @@
 (defun encoder-cache-extend (cache new &key pos picture)
   "NEW: a list of (sequence . ids), each sequence at most once; their new tokens' states, a list of
    (sequence . states) by sequence.  POS: the new tokens' (t h w), one list for all in the sequences'
-   order, or NIL (text, on from each sequence's tokens).  PICTURE: (row merged deep), the picture's
-   rows from new row ROW on (DEEP a list of three, or NIL), or NIL."
+   order, or NIL (text, on from each sequence's count of tokens).  PICTURE: (row merged deep), the
+   picture's rows from new row ROW on (DEEP a list of three, or NIL), or NIL; its rows and what follows
+   them, here and in later calls, need POS (src/encoder.lisp:125-129)."
   (gpu-encoder (encoder-cache-model cache))
   (let* ((new (sort (copy-list new) #'< :key #'car))
          (lens (loop for s below (encoder-cache-seqs cache) collect (length (cdr (assoc s new)))))

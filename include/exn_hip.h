@@ -505,7 +505,8 @@ int exn_enc_states_packed_dev(exn_enc* e, const int32_t* ids, const exn_seqs* s,
  * TOKENS tokens (rounded up to 64) through every layer, as exn_kv8 holds them, 74 kB a token at 36
  * layers (147 kB in 16 bits) and 9.4 MB of tails a sequence.  exn_enc_cache_extend: LENS new tokens of
  * each sequence (SEQS lengths, 0 for those that wait), packed as in exn_enc_states_packed; POS NULL
- * goes on from the sequence's tokens so far; the picture's rows as in exn_enc_states, among the new
+ * counts on from the sequence's tokens so far (text: neither a picture's rows nor what follows them stand
+ * there, src/encoder.lisp:125-129; give both theirs); the picture's rows as in exn_enc_states, among the new
  * rows; OUT the new rows' states.  A full block is seen in 8 bits, by the tokens that filled it too.
  * exn_enc_cache_fork: sequence TO becomes FROM as it stands, sharing the pages of its full blocks (a
  * template and a picture's rows encoded once, continued by several instructions), and is done on return;
