@@ -357,7 +357,7 @@ __device__ __forceinline__ int kv8_blocks(const Kv8& c, const SeqTile& t) {
 // How k_kv8_few's workgroups share the blocks of all tiles, one after the other (a wave finds it out).
 // SHARE consecutive ones each; or, where there is a workgroup for every tile and the longest is at most
 // 16 blocks over an even share, a tile each: then nothing is left to be joined (64 x 1000..2000 tokens
-// 43.7 us, shared 46.3; 4 x 1000..2000 13.0 shared, 24.7 a tile each).
+// 42.1 us, shared 46.3; 4 x 1000..2000 12.9 shared, 23.8 a tile each).
 struct Kv8Share {
   int all, share;   // share 0: a tile each
   int own;          // the blocks of the lane's tile of the first 64
@@ -1359,7 +1359,12 @@ struct Kv8Way {
   int64_t floats;          // of scratch that the splits take
 };
 // Splits go as far as the caller's scratch.  Times below are of 8 key/value heads of 128 and groups of 4,
-// fp16, in us, unless said.
+// fp16, in us a call by the host's clock over 40 calls (short ones come out up to 3 above the kernels' own
+// figures), unless said; the other side of each rule was built and timed with it.
+// The lengths are on the device, so the rules go by COLS: the tables timed are as wide as their longest
+// sequence, and one that is wider may pay for splits that its sequences have no use for (4 x 1 over
+// 270..333 in a table of 25 blocks 12.2, of 6 9.5).  So do sequences of one new token beside one of
+// many, which decides for all of a plan (64 x 1 over 700..8191, bf16: 79, with one of 76 among them 239).
 Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim, int cols, const int64_t* ntiles,
                int64_t part_cap) {
   Kv8Way w;
@@ -1369,26 +1374,26 @@ Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim,
   w.splits = 0;
   w.floats = 0;
   // Few rows: k_kv8_few, which reads codes into registers (64 x 1 token over 700..8191, bf16: 81, with
-  // k_kv8_chunk 231).  Two row tiles are one workgroup a CU, whose start and end short tables do not make
-  // up for: 17 to 32 rows take k_kv8_chunk up to 32 columns (1 x 8 tokens over 1100 13.4, with k_kv8_few
-  // 15.7; 64 x 8 over 700..2000 71, 92) and k_kv8_few past them (16 x 8 over 4000 51, 54; 64 x 8 over
-  // 700..8191, bf16, 138, 232).
+  // k_kv8_chunk 220).  Two row tiles are one workgroup a CU, whose start and end short tables do not make
+  // up for: 17 to 32 rows take k_kv8_chunk up to 32 columns (1 x 8 tokens over 1100 14.0, with k_kv8_few
+  // 15.3; 64 x 8 over 700..2000 69, 74) and k_kv8_few past them (16 x 8 over 4000 45, 54; 64 x 8 over
+  // 700..8191, bf16, 119, 221).
   if (longest * w.hh <= (cols > 32 ? 32 : 16)) {
     w.rt = longest * w.hh <= 16 ? 1 : 2;
     while ((SEQ_TT0 << w.z) < longest) ++w.z;
     w.chunks = (group + w.hh - 1) / w.hh;
     const int per = kv_heads * w.chunks;
-    // as many workgroups as the chip holds at once (64 x 1 over 700..8191: half of them 94, twice 92,
-    // these 83; 1 x 1 over 131071: 54.6, 58.0, 53.5)
+    // as many workgroups as the chip holds at once (64 x 1 over 700..8191, bf16: half of them 89, twice 89,
+    // these 81; 1 x 1 over 131071: 53.1, 56.3, 52.4)
     const int slots = 256 * (w.rt == 1 ? (head_dim == 64 ? 4 : 2) : (head_dim == 64 ? 2 : 1));
     int64_t s = slots / per > 0 ? slots / per : 1;
     const int64_t each = (int64_t)per * 32 * w.rt * (head_dim + 2), parts = 2 * ntiles[w.z] * per;
     if (s * each + parts > part_cap) s = (part_cap - parts) / each;
-    w.least = 2;   // 4 x 1 over 1100..4000: 15.1, with 4 blocks 16.6, with 16 23.0
+    w.least = 2;   // 4 x 1 over 1100..4000: 14.2, with 4 blocks 16.1, with 16 20.2
     // Tables of up to 16 blocks a workgroup a sequence: the sharing's own steps and the join cost more
-    // than it evens out (4 x 1 over 270..333 9.3, shared 15.4; 64 x 1 over 600..1000 26.9, 35.8).  So
-    // do many sequences even themselves out (200 x 1 over 700..4000 152, shared 145; 300 x 1 over
-    // 300..4000 174, 191).
+    // than it evens out (4 x 1 over 270..333 9.6, shared 11.9; 64 x 1 over 600..1000 25.4, 27.6; past it, 4
+    // x 1 over 1100..4000 shared 14.2, else 29.2).  Many sequences nearly even themselves out (300 x 1 over
+    // 300..4000 173, shared 167): past 4 tiles a place nothing is shared.
     if (cols > 16 && s > 1 && ntiles[w.z] * per <= 4 * slots && ntiles[w.z] * cols <= INT32_MAX) {
       w.splits = (int)s;
       w.floats = s * each + parts;
@@ -1398,12 +1403,12 @@ Kv8Way kv8_way(int64_t rows, int longest, int heads, int kv_heads, int head_dim,
   w.rt = 0;
   w.hh = group < 8 ? group : 8;   // as attend_packed
   while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
-  w.least = 2;   // 1 x 76 over 1100 19.1, with 1 or 4 blocks 21.8
+  w.least = 2;   // 1 x 76 over 1100 21.0, with 1 block 26.6, with 4 20.9
   w.chunks = (group + w.hh - 1) / w.hh;
   const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, most = (cols + w.least - 1) / w.least;
   const int64_t each = rows * heads * (head_dim + 2);
-  // two workgroups a CU: 4 x 512 over 2500..4001 (2 heads of 64, groups of 8, bf16) 65, with 256 in all
-  // 86, with 1024 69; 1 x 64 over 16000 40.4, 43.5, 54.4
+  // two workgroups a CU: 4 x 512 over 2500..4001 (2 heads of 64, groups of 8, bf16) 63, with 256 in all
+  // 79, with 1024 70; 1 x 64 over 16000 41.5, 43.6, 53.1
   int64_t s = groups > 0 ? 512 / groups : 1;
   if (s > most) s = most;
   if (each > 0 && s * each > part_cap) s = part_cap / each;
@@ -1464,7 +1469,7 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || w.splits < 2) return e;
   if (w.rt) {
-    // a row a workgroup where a tile has many parts (1 x 1 over 131071 53.0, else 57.7), or two shares
+    // a row a workgroup where a tile has many parts (1 x 1 over 131071 52.4, else 56.9), or two shares
     // and four rows (64-wide: eight)
     const bool few = ntiles[w.z] * 8 <= w.splits;
     const int rw = few ? 1 : 512 / c.head_dim;
@@ -1482,8 +1487,8 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   }
   const int th = c.head_dim / 4, most = (a.tt < longest ? a.tt : longest) * heads;   // a tile's rows and heads
   // The splits in as many shares as leave a row a workgroup, in half as many, or in one: 1 x 64 over 16000
-  // (32 splits) 40.7, 42.8, 47.4; 1 x 76 over 1100 (10) 18.8, 17.8, 19.3; 4 x 512 over 2500..4001 (64-wide, 2
-  // splits) 100, -, 65
+  // (32 splits) 41.5, 45.5, 50.2; 1 x 76 over 1100 (9) 21.6, 20.9, 21.4; 4 x 512 over 2500..4001 (64-wide, 2
+  // splits) 99, -, 63
   const int rw = w.splits > 16 ? 1 : w.splits > 4 ? 2 : 256 / th;
   const dim3 jg((unsigned)ntiles[w.z], (most + rw - 1) / rw);
   auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jg, dim3(256), 0, s, a); };

@@ -18,11 +18,11 @@
 // [key][dim]; gfx950's transposing LDS read hands each lane four keys of its dim.
 //
 // Matrix instructions bound it for long prompts: 2 x 8192 tokens (32 heads of 128, 8 of keys and values,
-// bf16) 998 us, 1,100 TFLOP/s where a large library product reaches 1,210 (matrix units busy 57% of the
+// bf16) 1,005 us, 1,090 TFLOP/s where a large library product reaches 1,210 (matrix units busy 57% of the
 // cycles at a clock that power holds at 1.6 to 1.9 GHz).  Two waves of a SIMD alternate between products
 // and exp2; 64 rows a wave took 1.21 ms, eight waves in two fixed phases 1.06 ms.  Short ones are bound
-// by the start and end of a workgroup: 4 x 1100..1180 57 us (740 TFLOP/s), 16 x 21..257 11.7 us, 1 x 24
-// 6.9 us; 24 x 5..4001 (16 heads of 64, 2 of keys and values) 91 us (820 TFLOP/s).
+// by the start and end of a workgroup: 4 x 1100..1180 58 us (735 TFLOP/s), 16 x 21..257 11.4 us, 1 x 24
+// 6.9 us; 24 x 5..4001 (16 heads of 64, 2 of keys and values) 89.5 us (830 TFLOP/s).
 #include "exn_common.h"
 
 #include <type_traits>
@@ -118,7 +118,7 @@ struct PackedArgs {
 
 // grid: tiles x chunks x kv_heads, the heads fastest; block 256.  LO: weights as two bf16 parts, where
 // bf16 inputs give fp16 rows: one part's half step, 2^-9, would be eight of the output's (4 x 1100..1180
-// tokens 73 us where bf16 rows take 56; 2.2e-4 from the exact values, in one part 1.2e-3).
+// tokens 75 us where bf16 rows take 58; 2.2e-4 from the exact values, in one part 1.2e-3).
 template <int BF, int HD, int LO>
 __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2)
 k_attend_packed(PackedArgs A) {
