@@ -191,8 +191,9 @@ int exn_seqs_free(exn_seqs* s);
  * heads of HEAD_DIM, 64 or 128) sees rows 0 .. i of its sequence in K and V (KV_HEADS heads, a
  * divisor of HEADS; head h reads h / (HEADS / KV_HEADS)), softmax of SCALE q.k in fp32.  Q, K and V
  * are EXN_DT_F16 or EXN_DT_BF16 (DT; the softmax's weights are rounded to that type for the second
- * product, from bf16 to fp16 rows in two parts; sums are fp32), OUT either (ODT).  All four 16-byte aligned, strides multiples of 8:
- * they may be parts of one row (q | k | v).  OUT overlaps none of them. */
+ * product, from bf16 to fp16 rows in two parts; sums are fp32, of weights up to 2^8: a row's keys times its
+ * largest |v| are to stay under 2^120, which fp16 always does), OUT either (ODT).  All four 16-byte
+ * aligned, strides multiples of 8: they may be parts of one row (q | k | v).  OUT overlaps none of them. */
 int exn_attend_packed(exn_ctx* ctx, const exn_seqs* s, int dt, int heads, int kv_heads, int head_dim, const void* q,
                       int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, float scale, void* out,
                       int odt, int64_t ldo);

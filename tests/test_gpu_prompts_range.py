@@ -1,12 +1,13 @@
 """Values at the end of fp16's range in the prompt side's attention: a block's scale is rounded up to 12
 significant bits, so that 127 of its steps may be up to 2^-11 more than the block's largest value, past
-where fp16 rounds to infinity.  What is finite is read as finite, and so are means of it.  Needs an MI355X."""
+where fp16 rounds to infinity.  What is finite is read as finite, and so are means of it.  And values near
+the end of fp32's.  Needs an MI355X."""
 import numpy as np
 import pytest
 
 import exn_hip as X
 import prompts_model as pm
-from test_gpu_prompts import cache_of, ctx, normal, say  # noqa: F401
+from test_gpu_prompts import attended, cache_of, ctx, filled, normal, off, say  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 TOP = 65504.0
@@ -59,3 +60,26 @@ def test_packed_largest_values(ctx, hd):  # noqa: F811
     X.attend_packed(ctx, X.Seqs(ctx, [n]), X.DT_F16, heads, 1, hd, dq.h, heads * hd, dk.h, hd, dv.h, hd, hd ** -0.5, o.h,
                     X.DT_F16, heads * hd)
     assert (abs(pm.value(o.get(), "fp16") - sign) <= 32).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 3, 20])
+def test_cache_of_very_large_values(ctx, new, hd):  # noqa: F811
+    """bf16 values of 2^112 in an unfinished block whose keys' weights are 2^7 of the blocks before it, so
+    that a reference lags by 7: the sums of values under weights that are held 2^7 higher still are past
+    fp32's largest (2^14 x 4 keys x 2^112), under the weights themselves 2^121."""
+    rng = np.random.default_rng([new, hd])
+    say("very large values", new, hd)
+    kv, heads, n = 2, 2, 256 + 4
+    m, d = filled(ctx, "bf16", [n - new], kv, hd, 6, rng)
+    qb = np.zeros((new, heads, hd), np.uint16)
+    qb[:, :, 0] = pm.bits(np.float32(16), "bf16")
+    q = pm.value(qb, "bf16")
+    m.k[:, :, :, 0] = 0
+    m.tk[:, :, :, 0] = pm.bits(np.float32(2.421875), "bf16")       # 16 x 2.42 x 0.125 = 4.84 = 7 ln 2
+    vb, _ = normal(rng, m.tv.shape, "bf16")
+    m.tv[:] = pm.bits(pm.rounded((2.0 ** 112 * (1.5 + 0.4 * np.sign(pm.value(vb, "bf16")))).astype(np.float32), "bf16"), "bf16")
+    for x in ("k", "tk", "tv"):
+        d.b[x].upload(getattr(m, x))
+    want, tol = m.attend(q, [new], 0.125, "bf16")
+    assert off(attended(ctx, d, qb, [new], heads, "bf16", 0.125), want, tol) <= 1
