@@ -4,7 +4,7 @@ rope_rows: rows of queries and keys as an attention takes them, each head RMS-no
 by its position, in one pass: both layouts of the pairs, all of a head or its first dims, positions on one
 or several axes or counted on from a cache's lengths, frequencies as they are or scaled for long contexts.
 
-kv8_attend_shared: attention over the cache in 8 bits of sequences that begin alike, on the same pages:
+attend_shared: attention over the cache in 8 bits of sequences that begin alike, on the same pages:
 what kv8_attend answers, with the keys and values of a common beginning read once for all of them.
 
 The cache, as the library lays it out: a page is a block of 64 tokens; codes of keys
@@ -273,7 +273,7 @@ def prepare(case, seed):
         st["cache"] = X.Kv8(DT[c["dt"]](X), kv, hd, pages, n, cols, st["k8"].data_ptr(), st["v8"].data_ptr(),
                             st["scales"].data_ptr(), st["tk"].data_ptr(), st["tv"].data_ptr(), st["table"].data_ptr(),
                             st["lens"].data_ptr())
-        floats = X.kv8_attend_shared_part(st["seqs"], st["prefixes"], c["heads"], kv, hd, cols)
+        floats = X.attend_shared_part(st["seqs"], st["prefixes"], c["heads"], kv, hd, cols)
         st["part"] = torch.empty(max(floats, 4), device=DEV)
     return st
 
@@ -303,7 +303,7 @@ def _own(st):
     X, ctx, c = _x(), _ctx(), st["c"]
     h, kv, hd = c["heads"], c["kv_heads"], c["dim"]
     if c["kind"] == "shared":
-        X.kv8_attend_shared(ctx, st["cache"], st["seqs"], st["prefixes"], h, st["q"].data_ptr(), h * hd, st["scale"],
+        X.attend_shared(ctx, st["cache"], st["seqs"], st["prefixes"], h, st["q"].data_ptr(), h * hd, st["scale"],
                             st["out"].data_ptr(), DT[c["odt"]](X), h * hd, st["part"].data_ptr(), st["part"].numel())
         return st["out"]
     wq, wk = (st[x].data_ptr() if c["norm"] else None for x in ("wq", "wk"))
