@@ -76,6 +76,23 @@ struct exn_seqs {
   const SeqTile* tiles[SEQ_TTS] = {};     // the sequences' tiles of SEQ_TT0 << i tokens, the costliest (causal) first
   int64_t ntiles[SEQ_TTS] = {};
   const SeqTile* whole = nullptr;         // one entry a sequence, in order
+  uint64_t id = 0;                        // no other plan's of this process
+};
+
+// sequences of a plan that begin alike (api_prefixes.hip)
+struct exn_prefixes {
+  int device = 0;
+  uint64_t plan = 0;    // the plan's id
+  void* mem = nullptr;
+  Kv8Shared sh = {};
+};
+
+// a rotary's frequencies (api_rope.hip)
+struct exn_rope {
+  int device = 0;
+  int pairs = 0, layout = 0, axes = 1;
+  float amp = 1.f;
+  void* mem = nullptr;   // the turns, then the axes
 };
 
 struct Buf {

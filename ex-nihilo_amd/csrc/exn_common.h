@@ -345,6 +345,42 @@ int64_t kv8_attend_part(int64_t rows, const int64_t* ntiles, int longest, int he
 hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles, int64_t rows,
                       int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out, int obf,
                       int64_t ldo, float* part, int64_t part_cap);
+// a plan's prefixes as the kernels take them: the tiles of each one's rows (row0 the first of them in ENTRY, seq the
+// prefix); pairs {row, sequence} in ENTRY, {first sequence, blocks} in PRE, {prefix or -1, first of its rows in
+// ENTRY} of each sequence in OF
+struct Kv8Shared {
+  const SeqTile* tiles[SEQ_TTS];
+  int64_t ntiles[SEQ_TTS], rows;
+  int most, blocks;   // the most rows of a prefix; the most blocks
+  const int32_t *entry, *pre, *of;
+};
+int64_t kv8_shared_part(int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
+                        int cols, const int64_t* ntiles);
+hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles,
+                             int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, const uint16_t* q,
+                             int64_t ldq, float scale, uint16_t* out, int obf, int64_t ldo, float* part, int64_t part_cap);
+
+// rows of heads normed and turned by their positions (rope.hip), q's and k's: heads 0 for none, w null for
+// no norm.  TURNS: each pair's frequency in 2^-64 turns; POS [row][axes], or null: from LENS (or 0) on in each sequence
+struct RopeSide {
+  const void* x;
+  int64_t ldx;
+  const float* w;
+  void* y;
+  int64_t ldy;
+  int heads;
+};
+struct RopeArgs {
+  const SeqTile* tiles;   // of 8 tokens
+  const uint64_t* turns;
+  const int32_t *axis, *pos, *lens;
+  int pairs, axes, hd;
+  float amp, eps;
+  RopeSide t[2];
+  uint64_t magic, pair_magic;   // 2^32 over the heads, over the pairs, rounded up: set by rope_rows
+  float per;
+};
+hipError_t rope_rows(hipStream_t s, const RopeArgs& args, int xt, int yt, int halves, int64_t ntiles, int longest);
 
 // the VAE decoder (vae.hip).  vae_conv's outputs: fp32 (+ bias, + res when given), bf16 (+ bias,
 // + res when given), fp32 (+ bias) clamped to -1 .. 1, fp32 (+ bias, + DupUp3D of keep: kcin

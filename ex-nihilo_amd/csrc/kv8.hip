@@ -340,7 +340,16 @@ struct Kv8Args {
   // k_kv8_chunk: [split][row][head][dim], [split][row][head][2]
   float* part;
   int64_t rows;
+  // the passes of attend_shared: pairs {row, sequence} of each prefix's rows, {first sequence, blocks} of each
+  // prefix, {prefix or -1, first of its rows there} of each sequence; the sums' references and weights
+  // [split][row][head][2] beside part's [split][row][head][dim]; rows times heads of them; the blocks that each
+  // sequence leaves to its prefix
+  const int32_t *entry, *pre, *of;
+  float* ml;
+  int64_t n;
+  int32_t* runs;
 };
+enum { ALONE = 0, PREFIX = 1, OWN = 2 };   // all of a sequence's keys; a prefix's, for all its rows; a sequence's others
 
 // the blocks of a tile's NB that split I of S takes: [*lo, *hi); the number of splits with any
 __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* lo, int* hi) {
@@ -348,6 +357,66 @@ __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* l
   *lo = min(nb, i * per);
   *hi = min(nb, (i + 1) * per);
   return (nb + per - 1) / per;
+}
+
+// The first blocks of a sequence that its prefix's pass takes for it: those full before the step whose pages
+// its table names as FIRST's does, at most NB (a wave finds it out)
+__device__ __forceinline__ int kv8_alike(const Kv8& c, int seq, int first, int nb) {
+  nb = min(nb, kv8_base(c, seq) / 64);
+  int run = nb;
+  const int32_t *mine = c.table + (int64_t)seq * c.cols, *its = c.table + (int64_t)first * c.cols;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < nb; i += 64)
+    if (mine[i] != its[i]) run = min(run, i);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) run = min(run, __shfl_xor(run, o, 64));
+  return __builtin_amdgcn_readfirstlane(run);
+}
+__device__ __forceinline__ int kv8_own_from(const Kv8Args& A, int seq) {
+  const int p = A.of[2 * seq];
+  return p < 0 ? 0 : kv8_alike(A.c, seq, A.pre[2 * p], min(A.pre[2 * p + 1], A.c.cols));
+}
+// The rows of a prefix's tile, N at most, and the blocks of the prefix that each may see (kv8_alike's, for a
+// workgroup's rows at once); RUN is the first row's of each sequence in each 64 rows, HEAD names that row
+template <int N>
+struct PrefixRows {
+  int row[N], seq[N], head[N], run[N];
+};
+template <int N>
+__device__ __forceinline__ void prefix_rows(const Kv8Args& A, const SeqTile& T, int n, int nb, PrefixRows<N>& R) {
+  const Kv8& c = A.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (tid < n) {
+    const int64_t e = 2 * ((int64_t)T.row0 + T.t0 + tid);
+    const int seq = A.entry[e + 1], before = __shfl_up(seq, 1, 64);
+    const uint64_t heads = __ballot(lane == 0 || seq != before);
+    R.row[tid] = A.entry[e];
+    R.seq[tid] = seq;
+    R.head[tid] = tid - lane + 63 - __builtin_clzll(heads & (~0ull >> (63 - lane)));
+    R.run[tid] = min(nb, kv8_base(c, seq) / 64);
+  }
+  __syncthreads();
+  const int32_t* its = c.table + (int64_t)A.pre[2 * T.seq] * c.cols;
+  for (int t = 4 * wave; t < n; t += 16) {   // four rows at a time
+    int at[4];
+    const int32_t* mine[4];
+    bool old = t % 64 > 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      at[j] = min(t + j, n - 1);
+      mine[j] = c.table + (int64_t)R.seq[at[j]] * c.cols;
+      old = old && R.head[at[j]] < t;
+    }
+    if (old) continue;
+#pragma unroll 2
+    for (int i = lane; i < nb; i += 64) {
+      const int x = its[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (mine[j][i] != x) atomicMin(&R.run[at[j]], i);
+    }
+  }
+  __syncthreads();
 }
 
 // a sequence's blocks after its new tokens
@@ -415,7 +484,7 @@ __device__ __forceinline__ uint32_t* kv8_parts(const Kv8Args& A, int per, int rt
 // 131071, fp16, 52.5 us, 5.0 and 5.1 TB/s, a copy's rate; 4 over 270..333 9.3 us, which is latency.
 //
 // Grid: workgroups x kv_heads x chunks, the heads fastest.
-template <int BF, int HD, int RT>
+template <int BF, int HD, int RT, int MODE>
 __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
 k_kv8_few(Kv8Args A) {
   constexpr int WV = 4;                       // waves
@@ -437,7 +506,7 @@ k_kv8_few(Kv8Args A) {
 
   // this workgroup's share: blocks [from, to) of the run of all tiles' blocks; tile I's begin at AT
   int i = w, at = 0, from = 0, to = 0x7FFFFFFF;
-  const Kv8Share sh = A.splits ? kv8_share(A) : Kv8Share{0, 0, 0};
+  const Kv8Share sh = MODE == ALONE && A.splits ? kv8_share(A) : Kv8Share{0, 0, 0};
   if (i >= A.ntiles && sh.share == 0) return;
   if (sh.share) {
     from = w * sh.share;
@@ -464,20 +533,35 @@ k_kv8_few(Kv8Args A) {
     }
   }
 
-  // a tile's part of the share
+  // a tile's part of the share; of a prefix, a split of its blocks; of a sequence's own, a split of those
   struct Seg {
     SeqTile T;
-    int base, total, nfull, nb, lo, hi, its;
+    int seq, base, total, nfull, nb, lo, hi, its;
   };
+  __shared__ PrefixRows<MODE == PREFIX ? 16 * RT : 1> pfx;
   auto segment = [&](int i, int at) __attribute__((always_inline)) {
     Seg s;
     s.T = A.tiles[i];
-    s.base = kv8_base(c, s.T.seq);
-    s.total = kv8_total(c, s.base, s.T.len);
+    s.seq = s.T.seq;
+    if constexpr (MODE == PREFIX) {
+      s.seq = A.pre[2 * s.T.seq];
+      s.base = s.total = min(A.pre[2 * s.T.seq + 1], c.cols) * 64;
+    } else {
+      s.base = kv8_base(c, s.T.seq);
+      s.total = kv8_total(c, s.base, s.T.len);
+    }
     s.nfull = s.total / 64;
     s.nb = (s.total + 63) / 64;
-    s.lo = max(0, from - at);
-    s.hi = min(s.nb, to - at);
+    if constexpr (MODE == ALONE) {
+      s.lo = max(0, from - at);
+      s.hi = min(s.nb, to - at);
+    } else {
+      const int run = MODE == OWN ? kv8_own_from(A, s.seq) : 0;
+      if (MODE == OWN && blockIdx.y == 0 && hc == 0 && tid == 0) A.runs[s.seq] = run;
+      kv8_split(max(0, s.nb - run), A.splits, A.least, blockIdx.y, &s.lo, &s.hi);
+      s.lo += run;
+      s.hi += run;
+    }
     s.its = (min(s.hi, s.nfull) - s.lo - wave + WV - 1) / WV;   // full blocks lo + wave + WV it of this wave
     return s;
   };
@@ -486,7 +570,7 @@ k_kv8_few(Kv8Args A) {
   // 64 of the wave's blocks' pages and scales, a lane each
   auto look = [&](const Seg& s, int it) __attribute__((always_inline)) {
     const int b = s.lo + wave + WV * (it + lane);
-    int64_t p = b < min(s.hi, s.nfull) ? kv8_page(c, s.T.seq, b) : -1;
+    int64_t p = b < min(s.hi, s.nfull) ? kv8_page(c, s.seq, b) : -1;
     pages = (int)p;
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
@@ -533,19 +617,27 @@ k_kv8_few(Kv8Args A) {
   };
 
   Seg S = segment(i, at);
+  if (MODE != ALONE && S.lo >= S.hi) return;
   begin(S);
+  if constexpr (MODE == PREFIX) prefix_rows(A, S.T, S.T.len, S.nb, pfx);
   for (;;) {
     const SeqTile T = S.T;
-    const int live = T.len, base = S.base;
-    int lim[RT];
+    const int live = T.len;
+    int lim[RT], base = S.base;
     s16x8 qf[RT][NS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = rt * 16 + col, tok = min((int)(r * A.magic >> 16), live - 1);
       const int head = min(r - (int)(r * A.magic >> 16) * A.hh, heads - 1);
-      lim[rt] = min(base + tok, S.total - 1);
+      lim[rt] = MODE == PREFIX ? pfx.run[pfx.head[tok]] * 64 - 1 : min(S.base + tok, S.total - 1);
+      if constexpr (MODE == PREFIX) {   // BASE: what every row sees all keys before
+        int least = lim[rt] + 1;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
+        base = min(base, __builtin_amdgcn_readfirstlane(least));
+      }
       // dims of k-step s: 16 g + 8 (s % 2) + 64 (s / 2) .., as the 16 bytes of codes a lane loads
-      const uint16_t* qr = A.q + (int64_t)(T.row0 + tok) * A.ldq + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
+      const uint16_t* qr = A.q + (int64_t)(MODE == PREFIX ? pfx.row[tok] : T.row0 + tok) * A.ldq + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
 #pragma unroll
       for (int s = 0; s < NS; ++s) qf[rt][s] = *(const s16x8*)(qr + 8 * (s % 2) + 64 * (s / 2));
     }
@@ -625,7 +717,7 @@ k_kv8_few(Kv8Args A) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         vdl[rt] = page >= 0 && k0 <= lim[rt] ? vd : 0.f;
-        if (page < 0 || k0 + 63 > base) {
+        if (page < 0 || k0 + (MODE == PREFIX ? 64 : 63) > base) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if (page < 0 || k0 + 16 * g + e > lim[rt]) s[rt][e] = -INFINITY;
@@ -647,7 +739,7 @@ k_kv8_few(Kv8Args A) {
     }
 
     // the tail, in 16 bits, by the wave whose turn it is
-    if (has_tail(S)) {
+    if (MODE != PREFIX && has_tail(S)) {
       const int left = S.total - S.nfull * 64, t0 = S.nfull * 64;
       int l = lane;
       asm volatile("" : "+v"(l));   // its addresses are made here, not kept through the loop above
@@ -739,11 +831,13 @@ k_kv8_few(Kv8Args A) {
     int mt = tid;
     asm volatile("" : "+v"(mt));   // as above
     // the next tile's first loads, then this one's sums meet: 16 threads a row, all waves' sums of it
-    const bool whole = S.lo == 0 && S.hi == S.nb, more = sh.share && at + S.nb < to;
+    const bool whole = MODE == ALONE && S.lo == 0 && S.hi == S.nb, more = sh.share && at + S.nb < to;
     const int nb = S.nb, lo = S.lo;
-    if (A.splits && lo == 0 && tid == 0)
-      *(u32x2*)(kv8_parts(A, per, RT, HD) + 2 * ((int64_t)i * per + hc)) =
-          u32x2{(uint32_t)w, (uint32_t)(sh.share ? (at + nb - 1) / sh.share : w)};
+    if constexpr (MODE == ALONE) {
+      if (A.splits && lo == 0 && tid == 0)
+        *(u32x2*)(kv8_parts(A, per, RT, HD) + 2 * ((int64_t)i * per + hc)) =
+            u32x2{(uint32_t)w, (uint32_t)(sh.share ? (at + nb - 1) / sh.share : w)};
+    }
     if (more) {
       at += nb;
       ++i;
@@ -785,7 +879,12 @@ k_kv8_few(Kv8Args A) {
           if (wt[k] > 0.f) y[e] = __builtin_fmaf(wt[k], obuf[k][rr][d0 + e], y[e]);
         y[e] *= inv;
       }
-      if (!whole) {   // the share's own first part (0) or the one begun in it (1)
+      if constexpr (MODE != ALONE) {
+        const int64_t slot = blockIdx.y * A.n + (int64_t)(T.row0 + tok) * A.heads + kvh * A.group + chunk * A.hh + head;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + slot * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        if ((mt & 15) == 0) *(f32x2*)(A.ml + slot * 2) = f32x2{m, sum};
+      } else if (!whole) {   // the share's own first part (0) or the one begun in it (1)
         const int64_t slot = ((int64_t)blockIdx.x * 2 + (lo == 0)) * 16 * RT + r;
 #pragma unroll
         for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + slot * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
@@ -925,7 +1024,7 @@ __device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int tota
   *l_ = l;
 }
 
-template <int BF, int HD>
+template <int BF, int HD, int MODE>
 __global__ void __launch_bounds__(256, 2)
 k_kv8_chunk(Kv8Args A) {
   constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
@@ -942,17 +1041,41 @@ k_kv8_chunk(Kv8Args A) {
   const int hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, lo = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len), nfull = total / 64;
+  const int seq = MODE == PREFIX ? A.pre[2 * T.seq] : T.seq;
+  const int base = MODE == PREFIX ? min(A.pre[2 * T.seq + 1], c.cols) * 64 : kv8_base(c, seq);
+  const int total = MODE == PREFIX ? base : kv8_total(c, base, T.len), nfull = total / 64;
   const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
-  int b0, b1;   // the blocks taken here
-  const int active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, blockIdx.y, &b0, &b1));
+  int b0, b1, active;   // the blocks taken here; the splits
+  if constexpr (MODE == PREFIX) {
+    active = kv8_split(nfull, A.splits, A.least, blockIdx.y, &b0, &b1);
+  } else if constexpr (MODE == OWN) {
+    const int run = kv8_own_from(A, seq);
+    if (blockIdx.y == 0 && hc == 0 && tid == 0) A.runs[seq] = run;
+    active = kv8_split(max(0, (min(base + T.t0 + live, total) + 63) / 64 - run), A.splits, A.least, blockIdx.y, &b0, &b1);
+    b0 += run;
+    b1 += run;
+  } else {
+    active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, blockIdx.y, &b0, &b1));
+  }
   if ((int)blockIdx.y >= active) return;
   const int row = wave * 32 + lo, tok = (int)(row * A.magic >> 16), head = row - tok * A.hh;
   const bool mine = tok < live && head < heads;
   const int ctok = min(tok, live - 1), chead = kvh * A.group + chunk * A.hh + min(head, heads - 1);
-  const int lim = min(base + T.t0 + ctok, total - 1);
-  const int minlim = min(base + T.t0 + min((int)(wave * 32 * A.magic >> 16), live - 1), total - 1);
-  const uint16_t* qr = A.q + (int64_t)(T.row0 + T.t0 + ctok) * A.ldq + (int64_t)chead * HD;
+  int lim, minlim;
+  __shared__ PrefixRows<MODE == PREFIX ? 128 : 1> pfx;
+  if constexpr (MODE == PREFIX) {
+    prefix_rows(A, T, live, nfull, pfx);
+    lim = minlim = pfx.run[pfx.head[ctok]] * 64 - 1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
+    minlim = __builtin_amdgcn_readfirstlane(minlim);
+  } else {
+    lim = min(base + T.t0 + ctok, total - 1);
+    minlim = min(base + T.t0 + min((int)(wave * 32 * A.magic >> 16), live - 1), total - 1);
+  }
+  // waves without a row do their part of each block's way into LDS only
+  const bool idle = MODE != ALONE && (int)(wave * 32 * A.magic >> 16) >= live;
+  const uint16_t* qr = A.q + (int64_t)(MODE == PREFIX ? pfx.row[ctok] : T.row0 + T.t0 + ctok) * A.ldq + (int64_t)chead * HD;
   s16x8 qf[NS];   // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
 #pragma unroll
   for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s + 8 * hi);
@@ -961,7 +1084,7 @@ k_kv8_chunk(Kv8Args A) {
   int pages = 0;
   float kds = 1.f, vds = 1.f;
   auto look = [&](int b) __attribute__((always_inline)) {
-    int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, T.seq, b + lane) : -1;
+    int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, seq, b + lane) : -1;
     pages = (int)p;
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
@@ -990,7 +1113,7 @@ k_kv8_chunk(Kv8Args A) {
     for (int i = 0; i < CI; ++i) x.w[i] = *(const u32x4*)(p + (tid + 256 * i) * 16);
     return x;
   };
-  const int64_t th = ((int64_t)T.seq * c.kv_heads + kvh) * 64 * HD;
+  const int64_t th = ((int64_t)seq * c.kv_heads + kvh) * 64 * HD;
   // the tail's 64 rows by DMA; those past its last token hold anything
   auto tail = [&](const uint16_t* all, uint8_t* p, auto swizzle) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -1191,10 +1314,12 @@ k_kv8_chunk(Kv8Args A) {
   barrier(b0 == nfull);
   sc[0] = f32x16{};
   sc[1] = f32x16{};
+  if (!idle) {
 #pragma unroll
-  for (int i = 0; i < 2 * NS; ++i) {
-    sc[i % 2] = mfma32<BF>(kfrag(i), qf[i / 2], sc[i % 2]);
-    if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < 2 * NS; ++i) {
+      sc[i % 2] = mfma32<BF>(kfrag(i), qf[i / 2], sc[i % 2]);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
   }
   fill_v(b0, 0, vc);
   if (b0 + 1 < b1) {
@@ -1221,7 +1346,7 @@ k_kv8_chunk(Kv8Args A) {
       F3 = facts(b + 3);
       kc = fetch(c.k, F3.page);
     }
-    step(std::integral_constant<bool, false>(), std::integral_constant<bool, false>(), b, F0);
+    if (!idle) step(std::integral_constant<bool, false>(), std::integral_constant<bool, false>(), b, F0);
     F0 = F1;
     F1 = F2;
     F2 = F3;
@@ -1231,20 +1356,23 @@ k_kv8_chunk(Kv8Args A) {
     for (int u = 0; u < 4; ++u) vofs[u] ^= STAGE;
   }
   barrier(b == nfull);
-  if (b < nfull) {
-    step(std::integral_constant<bool, true>(), std::integral_constant<bool, false>(), b, F0);
+  if (MODE == PREFIX || b < nfull) {
+    if (!idle) step(std::integral_constant<bool, true>(), std::integral_constant<bool, false>(), b, F0);
   } else {
     uint8_t* p = smem + (2 + ((b - b0) & 1)) * STAGE;   // V's rows past the last token: zeros
     for (int e = (total - b * 64) * (HD / 8) + tid; e < 64 * HD / 8; e += 256) *(u32x4*)(p + e * 16) = u32x4{};
     barrier(false);
-    step(std::integral_constant<bool, true>(), std::integral_constant<bool, true>(), b, F0);
+    if (!idle) step(std::integral_constant<bool, true>(), std::integral_constant<bool, true>(), b, F0);
   }
+  if (idle) return;
 
   float la = lrun, lb = lrun;
   xswap32(la, lb);
-  const float sum = (la + lb) * (1.f / LIFT2), mul = active > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+  const bool parts = MODE != ALONE || active > 1;
+  const float sum = (la + lb) * (1.f / LIFT2), mul = parts ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   float zero[4] = {sum * 0.f};
-  const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = A.rows * A.heads;
+  const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = MODE == ALONE ? A.rows * A.heads : A.n;
+  float* ml = MODE == ALONE ? A.part + A.splits * n * HD : A.ml;
   auto leave = [&](auto obf) __attribute__((always_inline)) {
     uint16_t* po = A.out + (int64_t)(T.row0 + T.t0 + tok) * A.ldo + (int64_t)chead * HD + 4 * hi;
     float* pp = A.part + ((int64_t)blockIdx.y * n + rowhead) * HD + 4 * hi;
@@ -1267,10 +1395,9 @@ k_kv8_chunk(Kv8Args A) {
           *(u32x2*)(po + 32 * d + 8 * r4) = u32x2{pack_out(y[0], y[1], BF, 0), pack_out(y[2], y[3], BF, 0)};
       }
   };
-  if (active > 1) {
+  if (parts) {
     leave(std::integral_constant<int, 2>());
-    if (mine && hi == 0)
-      *(f32x2*)(A.part + A.splits * n * HD + ((int64_t)blockIdx.y * n + rowhead) * 2) = f32x2{set ? mrun : -INFINITY, sum};
+    if (mine && hi == 0) *(f32x2*)(ml + ((int64_t)blockIdx.y * n + rowhead) * 2) = f32x2{set ? mrun : -INFINITY, sum};
   } else if (A.obf) {
     leave(std::integral_constant<int, 1>());
   } else {
@@ -1282,16 +1409,18 @@ k_kv8_chunk(Kv8Args A) {
     const int r = wave * 32 + __builtin_ctz(rows), rt = (int)(r * A.magic >> 16);
     const int64_t rh = kvh * A.group + chunk * A.hh + r - rt * A.hh, at = T.row0 + T.t0 + rt;
     float m, l, y[HD / 64];
-    kv8_row<BF, HD>(c, T.seq, kvh, b0, b1, total, min(base + T.t0 + rt, total - 1), A.q + at * A.ldq + rh * HD, A.scale, &m, &l, y);
+    const int64_t qrow = MODE == PREFIX ? pfx.row[rt] : at;
+    const int sees = MODE == PREFIX ? pfx.run[pfx.head[rt]] * 64 - 1 : min(base + T.t0 + rt, total - 1);
+    kv8_row<BF, HD>(c, seq, kvh, b0, b1, total, sees, A.q + qrow * A.ldq + rh * HD, A.scale, &m, &l, y);
     const int64_t slot = (int64_t)blockIdx.y * n + at * A.heads + rh;
     for (int z = 0; z < HD / 64; ++z) {
-      const float w = active > 1 ? y[z] : l == 0.f ? 0.f : y[z] / l;
-      if (active > 1)
+      const float w = parts ? y[z] : l == 0.f ? 0.f : y[z] / l;
+      if (parts)
         A.part[slot * HD + z * 64 + lane] = w;
       else
         A.out[at * A.ldo + rh * HD + z * 64 + lane] = (uint16_t)pack_out(w, 0.f, BF, A.obf);
     }
-    if (active > 1 && lane == 0) *(f32x2*)(A.part + A.splits * n * HD + slot * 2) = f32x2{m, l};
+    if (parts && lane == 0) *(f32x2*)(ml + slot * 2) = f32x2{m, l};
   }
 }
 
@@ -1455,8 +1584,8 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-    if (w.rt == 0) return go(k_kv8_chunk<BF, HD>);
-    w.rt == 2 ? go(k_kv8_few<BF, HD, 2>) : go(k_kv8_few<BF, HD, 1>);
+    if (w.rt == 0) return go(k_kv8_chunk<BF, HD, ALONE>);
+    w.rt == 2 ? go(k_kv8_few<BF, HD, 2, ALONE>) : go(k_kv8_few<BF, HD, 1, ALONE>);
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
@@ -1496,6 +1625,225 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
     rw == 1 ? join(k_kv8_join<128, 8>) : rw == 2 ? join(k_kv8_join<128, 4>) : join(k_kv8_join<128, 1>);
   else
     rw == 1 ? join(k_kv8_join<64, 16>) : rw == 2 ? join(k_kv8_join<64, 8>) : join(k_kv8_join<64, 1>);
+  return hipGetLastError();
+}
+
+// --- attention of sequences that begin alike --------------------------------------------------------
+//
+// A prefix's blocks are read once for the rows of all its sequences (PREFIX: its rows are one tile's, or
+// several's, whatever sequence each is of), each sequence's other blocks as ever (OWN); both leave sums
+// relative to a reference of their own, which meet here:
+//   m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m) / l.
+// Which blocks those are is found out on the device (kv8_alike): the plan of prefixes is a hint, and what
+// comes out is kv8_attend's answer whatever the tables hold.
+
+struct Kv8Meet {
+  Kv8Args own;
+  const float *part, *ml;   // the prefixes' sums
+  int64_t n;
+  int splits, least;
+};
+template <int HD, int SH>
+__global__ void __launch_bounds__(256)
+k_kv8_meet(Kv8Meet M) {
+  constexpr int TH = HD / 4, RW = 256 / TH / SH;   // threads a row and share; rows a workgroup
+  __shared__ __align__(16) float ys[256 / TH][HD];
+  __shared__ float ss[256 / TH], ms[256 / TH];
+  const Kv8Args& A = M.own;
+  const Kv8& c = A.c;
+  const SeqTile T = A.tiles[blockIdx.x];
+  const int live = min(A.tt, T.len - T.t0);
+  if ((int)blockIdx.y * RW >= live * A.heads) return;
+  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len);
+  const int run = A.runs[T.seq], p = A.of[2 * T.seq];
+  int lo, hi;
+  const int owns = kv8_split(max(0, (min(base + T.t0 + live, total) + 63) / 64 - run), A.splits, A.least, 0, &lo, &hi);
+  const int all = owns + (run > 0 ? kv8_split(min(A.pre[2 * p + 1], c.cols), M.splits, M.least, 0, &lo, &hi) : 0);
+  const int tid = threadIdx.x, sh = tid / TH % SH, r = tid / TH / SH, d = tid % TH * 4;
+  const int i = min((int)blockIdx.y * RW + r, live * A.heads - 1);
+  const int64_t mine = (int64_t)(T.row0 + T.t0) * A.heads + i;
+  const int64_t theirs = p < 0 ? 0 : ((int64_t)A.of[2 * T.seq + 1] + T.t0) * A.heads + i;
+  auto slot = [&](int z) { return z < owns ? A.ml + (z * A.n + mine) * 2 : M.ml + ((z - owns) * M.n + theirs) * 2; };
+  auto sums = [&](int z) { return z < owns ? A.part + (z * A.n + mine) * HD : M.part + ((z - owns) * M.n + theirs) * HD; };
+  float m = -INFINITY;
+  for (int z = sh; z < all; z += SH) m = fmaxf(m, *slot(z));
+  if constexpr (SH > 1) {
+    if (d == 0) ms[tid / TH] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < SH; ++k) m = fmaxf(m, ms[r * SH + k]);
+  }
+  float sum = 0.f;
+  f32x4 y = {};
+#pragma unroll 4
+  for (int z = sh; z < all; z += SH) {
+    const f32x2 ml = *(const f32x2*)slot(z);
+    const f32x4 x = *(const f32x4*)(sums(z) + d);
+    const float w = ml[0] == -INFINITY ? 0.f : ml[0] == m ? 1.f : __builtin_amdgcn_exp2f(ml[0] - m);
+    sum += ml[0] == -INFINITY ? ml[1] : w * ml[1];   // no reference: 0, or NaN
+    if (w > 0.f) y += w * x;
+  }
+  if constexpr (SH > 1) {
+    *(f32x4*)&ys[tid / TH][d] = y;
+    if (d == 0) ss[tid / TH] = sum;
+    __syncthreads();
+    if (sh) return;
+#pragma unroll
+    for (int k = 1; k < SH; ++k) {
+      y += *(const f32x4*)&ys[r * SH + k][d];
+      sum += ss[r * SH + k];
+    }
+  }
+  if ((int)blockIdx.y * RW + r >= live * A.heads) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* po = A.out + (mine / A.heads) * A.ldo + (mine % A.heads) * HD + d;
+  *(u32x2*)po = u32x2{pack_out(y[0] * inv, y[1] * inv, c.bf16, A.obf), pack_out(y[2] * inv, y[3] * inv, c.bf16, A.obf)};
+}
+
+namespace {
+
+// one of attend_shared's passes: how its rows are taken, and into how many splits their blocks
+struct PassWay {
+  int rt, z, hh, chunks, splits, least;
+};
+PassWay pass_way(int most, int heads, int kv_heads, int head_dim, int blocks, const int64_t* ntiles) {
+  PassWay w;
+  const int group = heads / kv_heads;
+  w.z = 0;
+  w.least = 2;
+  w.hh = group < 16 ? group : 16;
+  int64_t slots;
+  if ((int64_t)most * w.hh <= 32) {
+    w.rt = most * w.hh <= 16 ? 1 : 2;
+    while ((SEQ_TT0 << w.z) < most) ++w.z;
+    slots = 256 * (w.rt == 1 ? (head_dim == 64 ? 4 : 2) : (head_dim == 64 ? 2 : 1));
+  } else {
+    w.rt = 0;
+    w.hh = group < 8 ? group : 8;
+    while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
+    slots = 512;
+  }
+  w.chunks = (group + w.hh - 1) / w.hh;
+  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, pays = (blocks + w.least - 1) / w.least;
+  const int64_t s = groups > 0 ? slots / groups : 1;
+  w.splits = (int)(s > pays ? pays : s);
+  if (w.splits < 1) w.splits = 1;
+  return w;
+}
+struct SharedWay {
+  PassWay pre, own;
+  int64_t pre_each, own_each, floats;   // of a split of either; in all, with the runs
+};
+SharedWay shared_way(int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
+                     int cols, const int64_t* ntiles) {
+  SharedWay w;
+  w.pre = pass_way(sh.most, heads, kv_heads, head_dim, sh.blocks < cols ? sh.blocks : cols, sh.ntiles);
+  w.own = pass_way(longest, heads, kv_heads, head_dim, cols, ntiles);
+  w.pre_each = sh.rows * heads * (head_dim + 2);
+  w.own_each = rows * heads * (head_dim + 2);
+  w.floats = w.pre.splits * w.pre_each + w.own.splits * w.own_each + seqs;
+  return w;
+}
+
+}  // namespace
+
+int64_t kv8_shared_part(int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
+                        int cols, const int64_t* ntiles) {
+  const int64_t alone = kv8_attend_part(rows, ntiles, longest, heads, kv_heads, head_dim, cols);
+  if (sh.rows == 0) return alone;
+  const int64_t n = shared_way(rows, longest, seqs, sh, heads, kv_heads, head_dim, cols, ntiles).floats;
+  return n > alone ? n : alone;
+}
+
+hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles,
+                             int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, const uint16_t* q,
+                             int64_t ldq, float scale, uint16_t* out, int obf, int64_t ldo, float* part, int64_t part_cap) {
+  if (ntiles[0] == 0) return hipSuccess;
+  SharedWay w = shared_way(rows, longest, seqs, sh, heads, c.kv_heads, c.head_dim, c.cols, ntiles);
+  // less scratch: fewer splits, the prefixes' first to keep theirs; without room for one of each, nothing is shared
+  const int64_t spare = part_cap - seqs - w.pre_each - w.own_each;
+  if (sh.rows == 0 || spare < 0)
+    return kv8_attend(s, c, tiles, ntiles, rows, longest, heads, q, ldq, scale, out, obf, ldo, part, part_cap);
+  if (w.floats > part_cap) {
+    const int64_t p = 1 + spare / w.pre_each;
+    if (p < w.pre.splits) w.pre.splits = (int)p;
+    const int64_t o = 1 + (spare - (w.pre.splits - 1) * w.pre_each) / w.own_each;
+    if (o < w.own.splits) w.own.splits = (int)o;
+  }
+  Kv8Args a;
+  a.c = c;
+  a.q = q;
+  a.out = out;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.scale = scale * 1.4426950408889634f;
+  a.heads = heads;
+  a.group = heads / c.kv_heads;
+  a.obf = obf;
+  a.rows = rows;
+  a.entry = sh.entry;
+  a.pre = sh.pre;
+  a.of = sh.of;
+  Kv8Args b = a;   // a: the prefixes' pass, b: the sequences' own
+  a.tiles = sh.tiles[w.pre.z];
+  a.ntiles = (int)sh.ntiles[w.pre.z];
+  a.n = sh.rows * heads;
+  b.tiles = tiles[w.own.z];
+  b.ntiles = (int)ntiles[w.own.z];
+  b.n = rows * heads;
+  auto fill = [&](Kv8Args& x, const PassWay& p) {
+    x.tt = SEQ_TT0 << p.z;
+    x.hh = p.hh;
+    x.chunks = p.chunks;
+    x.magic = (65536 + p.hh - 1) / p.hh;
+    x.splits = p.splits;
+    x.least = p.least;
+    return (int64_t)x.ntiles * p.chunks * c.kv_heads;
+  };
+  const int64_t ga = fill(a, w.pre), gb = fill(b, w.own);
+  a.part = part;
+  b.part = a.part + a.splits * a.n * c.head_dim;
+  a.ml = b.part + b.splits * b.n * c.head_dim;
+  b.ml = a.ml + a.splits * a.n * 2;
+  a.runs = b.runs = (int32_t*)(b.ml + b.splits * b.n * 2);
+  if (ga > WG256_MAX || gb > WG256_MAX) return hipErrorInvalidConfiguration;
+  typedef std::integral_constant<int, 0> I0;
+  typedef std::integral_constant<int, 1> I1;
+  typedef std::integral_constant<int, 64> I64;
+  typedef std::integral_constant<int, 128> I128;
+  auto pass = [&](auto mode_c, const Kv8Args& x, int rt, int64_t groups) {
+    constexpr int MODE = decltype(mode_c)::value;
+    const dim3 grid((unsigned)groups, x.splits);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, x); };
+    auto rts = [&](auto bf, auto hd) {
+      constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
+      if (rt == 0) return go(k_kv8_chunk<BF, HD, MODE>);
+      rt == 2 ? go(k_kv8_few<BF, HD, 2, MODE>) : go(k_kv8_few<BF, HD, 1, MODE>);
+    };
+    if (c.head_dim == 128)
+      c.bf16 ? rts(I1(), I128()) : rts(I0(), I128());
+    else
+      c.bf16 ? rts(I1(), I64()) : rts(I0(), I64());
+    return hipGetLastError();
+  };
+  hipError_t e = pass(std::integral_constant<int, PREFIX>(), a, w.pre.rt, ga);
+  if (e == hipSuccess) e = pass(std::integral_constant<int, OWN>(), b, w.own.rt, gb);
+  if (e != hipSuccess) return e;
+  Kv8Meet m;
+  m.own = b;
+  m.part = a.part;
+  m.ml = a.ml;
+  m.n = a.n;
+  m.splits = a.splits;
+  m.least = a.least;
+  const int th = c.head_dim / 4, most = (b.tt < longest ? b.tt : longest) * heads;   // a tile's rows and heads
+  const int rw = a.splits + b.splits > 16 ? 1 : a.splits + b.splits > 4 ? 2 : 256 / th;
+  const dim3 jg((unsigned)ntiles[w.own.z], (most + rw - 1) / rw);
+  auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jg, dim3(256), 0, s, m); };
+  if (c.head_dim == 128)
+    rw == 1 ? join(k_kv8_meet<128, 8>) : rw == 2 ? join(k_kv8_meet<128, 4>) : join(k_kv8_meet<128, 1>);
+  else
+    rw == 1 ? join(k_kv8_meet<64, 16>) : rw == 2 ? join(k_kv8_meet<64, 8>) : join(k_kv8_meet<64, 1>);
   return hipGetLastError();
 }
 

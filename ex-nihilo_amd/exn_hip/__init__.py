@@ -29,6 +29,8 @@ LIB_PATH = os.environ.get("EXN_HIP_LIB") or os.path.join(os.path.dirname(HERE), 
 OK, ENODEV, EINVAL, ENOMEM, EHIP, ESTATE = 0, 1, 2, 3, 4, 5
 Q8_0, F32, BF16, F16 = 8, 0, 30, 1
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_TURNS, ROPE_INDEX = 0, 1, 2, 3, 4
+ROPE_HALF, ROPE_PAIRS = 0, 1
 WIDTH, HEADS, HEAD_DIM, FFN, LATENT = 4096, 32, 128, 12288, 64
 # Qwen-Image-2.1-Turbo's schedule (src/generate.lisp:7-9)
 TURBO_SIGMAS = (1.0, 0.978453, 0.95418, 0.926626, 0.89508, 0.845148, 0.704534, 0.414568, 0.0)
@@ -92,6 +94,15 @@ SIGNATURES = {
     "exn_kv8_attend_part": (c_int, [vp, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
     "exn_kv8_read": (c_int, [vp, vp, vp, vp, c_int64, vp, c_int64]),
     "exn_kv8_advance": (c_int, [vp, vp, vp]),
+    "exn_prefixes_create": (c_int, [vp, vp, vp, vp, c_int, POINTER(vp)]),
+    "exn_prefixes_free": (c_int, [vp]),
+    "exn_attend_shared": (c_int, [vp, vp, vp, vp, c_int, vp, c_int64, c_float, vp, c_int, c_int64, vp, c_int64]),
+    "exn_attend_shared_part": (c_int, [vp, vp, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
+    "exn_rope_freqs": (c_int, [c_int, c_double, c_int, c_double, c_double, c_double, c_double, vp]),
+    "exn_rope_create": (c_int, [vp, vp, c_int, c_int, vp, c_int, c_float, POINTER(vp)]),
+    "exn_rope_free": (c_int, [vp]),
+    "exn_rope_rows": (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_float, c_int, vp, c_int64, vp, vp, c_int64,
+                              c_int, vp, c_int64, vp, vp, c_int64]),
     "exn_euler": (c_int, [vp, c_int64, vp, vp, c_float]),
     "exn_dit_create": (c_int, [vp, c_int, POINTER(vp)]),
     "exn_dit_set": (c_int, [vp, c_char_p, c_int, vp, c_int64, c_int64]),
@@ -400,6 +411,87 @@ def kv8_read(ctx: Context, cache: Kv8, seqs: Seqs, k, ldk, v, ldv):
 def kv8_advance(ctx: Context, cache: Kv8, seqs: Seqs):
     """The step's tokens counted into the cache's lengths (exn_kv8_advance)."""
     call("exn_kv8_advance", ctx.h, cache.ref, seqs.h)
+
+
+class Prefixes:
+    """Sequences of a plan that begin alike (exn_prefixes_create): OF, each sequence's prefix or -1; BLOCKS, each
+    prefix's full blocks of 64 tokens."""
+
+    def __init__(self, ctx: Context, seqs: Seqs, of, blocks):
+        o, b = (np.ascontiguousarray(x, dtype=np.int32).reshape(-1) for x in (of, blocks))
+        if len(o) != seqs.seqs:
+            raise ExnError(EINVAL, "prefixes of %d sequences for a plan of %d" % (len(o), seqs.seqs))
+        h = vp()
+        call("exn_prefixes_create", ctx.h, seqs.h, ptr(o), ptr(b), len(b), ctypes.byref(h))
+        self.ctx, self.h = ctx, h
+
+    def free(self):
+        if getattr(self, "h", None):
+            call("exn_prefixes_free", self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def attend_shared_part(seqs: Seqs, prefixes: Prefixes, heads, kv_heads, head_dim, cols) -> int:
+    """The floats of scratch that attend_shared has a use for (exn_attend_shared_part)."""
+    n = c_int64()
+    call("exn_attend_shared_part", seqs.h, prefixes.h, heads, kv_heads, head_dim, cols, ctypes.byref(n))
+    return n.value
+
+
+def attend_shared(ctx: Context, cache: Kv8, seqs: Seqs, prefixes: Prefixes, heads, q, ldq, scale, out, odt, ldo,
+                  part=None, part_cap=0):
+    """kv8_attend with the blocks of each of PREFIXES read once for all its sequences (exn_attend_shared)."""
+    call("exn_attend_shared", ctx.h, cache.ref, seqs.h, prefixes.h, heads, q, ldq, scale, out, odt, ldo, part, part_cap)
+
+
+# --- rotary positions -----------------------------------------------------------------------
+
+
+def rope_freqs(dims, base, scaling=ROPE_PLAIN, factor=1.0, kept=1.0, low=0.0, high=1.0):
+    """A rotary's frequencies, as they are or for texts FACTOR times as long as KEPT tokens (exn_rope_freqs):
+    dims / 2 doubles."""
+    f = np.empty(max(0, dims // 2), np.float64)
+    call("exn_rope_freqs", dims, base, scaling, factor, kept, low, high, ptr(f))
+    return f
+
+
+class Rope:
+    """A rotary (exn_rope_create): FREQS radians a token, of dims j and j + pairs (ROPE_HALF) or 2j and 2j + 1
+    (ROPE_PAIRS); AXIS, the position that each pair turns by, or None for one of them; AMP, a factor of all."""
+
+    def __init__(self, ctx: Context, freqs, layout=ROPE_HALF, axis=None, amp=1.0):
+        f = np.ascontiguousarray(freqs, dtype=np.float64).reshape(-1)
+        a = None if axis is None else np.ascontiguousarray(axis, dtype=np.int32).reshape(-1)
+        if a is not None and len(a) != len(f):
+            raise ExnError(EINVAL, "rotary: %d axes for %d pairs" % (len(a), len(f)))
+        axes = 1 if a is None or not len(a) else int(a.max()) + 1
+        h = vp()
+        call("exn_rope_create", ctx.h, ptr(f), len(f), layout, None if a is None else ptr(a), axes, amp, ctypes.byref(h))
+        self.ctx, self.h, self.pairs, self.axes = ctx, h, len(f), axes
+
+    def free(self):
+        if getattr(self, "h", None):
+            call("exn_rope_free", self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def rope_rows(ctx: Context, rope: Rope, seqs: Seqs, head_dim, dt, odt, q, k=(0, None, 0, None, None, 0), eps=0.0,
+              pos=None, lens=None):
+    """Rows of queries and keys normed and turned in one pass (exn_rope_rows), on device addresses.  Q and K:
+    (heads, rows, their stride, the norm's weights or None, rows out, their stride)."""
+    call("exn_rope_rows", ctx.h, rope.h, seqs.h, pos, lens, head_dim, dt, odt, eps, *q, *k)
 
 
 # --- the backend trio (src/cuda-dit.lisp) -------------------------------------------------

@@ -48,7 +48,7 @@ extern "C" {
 /* activation dtypes of the op-level entry points */
 #define EXN_DT_F32 0
 #define EXN_DT_BF16 1
-#define EXN_DT_F16 2 /* outputs of exn_mm only */
+#define EXN_DT_F16 2
 
 typedef struct exn_ctx exn_ctx; /* a device and its stream (il::open-cuda / exn-device, src/cuda-dit.lisp:25-40) */
 typedef struct exn_w exn_w;     /* a weight matrix on the device (the gdit-w entries, src/cuda-dit.lisp:46) */
@@ -234,6 +234,63 @@ int exn_kv8_attend_part(const exn_seqs* s, int heads, int kv_heads, int head_dim
 int exn_kv8_read(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, void* k, int64_t ldk, void* v, int64_t ldv);
 /* LENS += the plan's lengths, on the device: the step's last call */
 int exn_kv8_advance(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s);
+
+/* Sequences of a plan that begin alike: sequence i has prefix OF[i] (0 .. PREFIXES - 1, or -1: none), whose BLOCKS[.]
+ * first blocks its table shares with the prefix's other sequences (host memory, both).  A hint of what to read
+ * once: which pages are the same is found out on the device in each call, so that a table that changes, or was
+ * never alike, costs time only.  Made for one plan, outside stream capture; freed when no work that reads it is
+ * left (exn_prefixes_free waits for the device). */
+typedef struct exn_prefixes exn_prefixes;
+int exn_prefixes_create(exn_ctx* ctx, const exn_seqs* s, const int32_t* of, const int32_t* blocks, int prefixes,
+                        exn_prefixes** out);
+int exn_prefixes_free(exn_prefixes* p);
+/* exn_kv8_attend with the blocks of each prefix read once for the rows of all its sequences: the same arguments and
+ * answer (not bit for bit: sums over a prefix and over the rest meet at the end).  Blocks are shared as far as a
+ * sequence's table begins with the pages of its prefix's first sequence (the lowest that has rows), full before the
+ * step.  PART is needed for it: with room for less than one split nothing is shared.  exn_attend_shared_part (needs
+ * no GPU): how many floats are of use. */
+int exn_attend_shared(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const exn_prefixes* p, int heads, const void* q,
+                      int64_t ldq, float scale, void* out, int odt, int64_t ldo, float* part, int64_t part_cap);
+int exn_attend_shared_part(const exn_seqs* s, const exn_prefixes* p, int heads, int kv_heads, int head_dim, int cols,
+                           int64_t* floats);
+
+/* --- rotary positions: what turns a product's rows into the attention's (x_qk_norm_rope, src/cuda/dit.cu:43-58, and
+ * illatio's for the text model, for any number and width of heads) --------------------------------------- */
+
+/* The frequencies of a rotary of DIMS dims (even), radians a token, into FREQ (DIMS / 2 doubles), on the host, no GPU
+ * needed: f_j = BASE^(-2j / DIMS), SCALING for texts FACTOR times as long as KEPT tokens, on which the model was trained:
+ * PLAIN  f_j (the rest unused)
+ * LINEAR f_j / FACTOR
+ * BASE   of the base BASE FACTOR^(DIMS / (DIMS - 2))
+ * TURNS  r f_j + (1 - r) f_j / FACTOR, r from 0 to 1 as a pair turns LOW to HIGH times over KEPT tokens
+ * INDEX  the same, r from 1 to 0 as j goes from floor(i(HIGH)) to ceil(i(LOW)) (within 0 .. DIMS - 1), i(n) =
+ *        DIMS ln(KEPT / 2 pi n) / (2 ln BASE), the pair that turns n times over KEPT tokens */
+#define EXN_ROPE_PLAIN 0
+#define EXN_ROPE_LINEAR 1
+#define EXN_ROPE_BASE 2
+#define EXN_ROPE_TURNS 3
+#define EXN_ROPE_INDEX 4
+int exn_rope_freqs(int dims, double base, int scaling, double factor, double kept, double low, double high, double* freq);
+/* A rotary: PAIRS frequencies FREQ (exn_rope_freqs' or any others), of dims j and j + PAIRS of a head (HALF) or 2j and
+ * 2j + 1 (PAIRS); AXIS (PAIRS of 0 .. AXES - 1, or null: all 0), the position that each turns by; AMP a factor of
+ * cosines and sines.  Made outside stream capture; freed when no work that reads it is left. */
+typedef struct exn_rope exn_rope;
+#define EXN_ROPE_HALF 0
+#define EXN_ROPE_PAIRS 1
+int exn_rope_create(exn_ctx* ctx, const double* freq, int pairs, int layout, const int32_t* axis, int axes, float amp,
+                    exn_rope** out);
+int exn_rope_free(exn_rope* r);
+/* The plan's rows of queries and keys normed and turned in one pass: each head x of HEAD_DIM (a multiple of 8, at most
+ * 256) of Q (HEADS) and K (KV_HEADS) becomes w x / sqrt(mean(x^2) + EPS) where its norm's weights WQ, WK (HEAD_DIM
+ * fp32) are given, then its first 2 PAIRS dims turn by the row's positions; all in fp32, rounded once.  Positions: POS
+ * [row][axes] (device), or, POS null and one axis, LENS[sequence] + i for row i of a sequence (a cache's tokens
+ * before the step; null: i), of any sign and size.  X of type DT into Y of ODT (any of the three), rows LD values
+ * apart, 16-byte aligned, strides multiples of 8; Y may be X itself (the same type and stride), else they do not
+ * overlap.  KV_HEADS 0: Q alone. */
+int exn_rope_rows(exn_ctx* ctx, const exn_rope* r, const exn_seqs* s, const int32_t* pos, const int32_t* lens,
+                  int head_dim, int dt, int odt, float eps, int heads, const void* q, int64_t ldq, const float* wq,
+                  void* qo, int64_t ldqo, int kv_heads, const void* k, int64_t ldk, const float* wk, void* ko,
+                  int64_t ldko);
 
 /* --- the model: the backend trio ----------------------------------------------------------------- */
 
