@@ -34,40 +34,47 @@ int exn_prefixes_create(exn_ctx* ctx, const exn_seqs* s, const int32_t* of, cons
         if (seqs[g]++ == 0) first[g] = i;
       }
     auto shared = [&](int g) { return g >= 0 && seqs[(size_t)g] > 1 && blocks[g] > 0; };
-    std::vector<int32_t> at((size_t)prefixes, 0), words;
     Kv8Shared& sh = p->sh;
-    std::vector<SeqTile> tiles;
-    size_t lists[SEQ_TTS];
+    std::vector<int32_t> at((size_t)prefixes, 0), words;
     for (int g = 0; g < prefixes; ++g)
       if (shared(g)) {
         at[(size_t)g] = (int32_t)sh.rows;
         sh.rows += rows[(size_t)g];
         sh.most = std::max(sh.most, (int)rows[(size_t)g]);
+        sh.seqs = std::max(sh.seqs, seqs[(size_t)g]);
         sh.blocks = std::max(sh.blocks, blocks[g]);
+        sh.saved += (int64_t)(seqs[(size_t)g] - 1) * blocks[g];
       }
+    sh.fewest = sh.blocks;
+    for (int i = 0; i < s->seqs; ++i)
+      if (s->lens[(size_t)i] > 0) sh.fewest = std::min(sh.fewest, shared(of[i]) ? blocks[of[i]] : 0);
+    // each list's tiles; then their blocks; of each sequence; the rows
+    std::vector<SeqTile> tiles;
+    size_t lists[SEQ_TTS];
     for (int z = 0; z < SEQ_TTS; ++z) {
       lists[z] = tiles.size();
       const int tt = SEQ_TT0 << z;
       for (int g = 0; g < prefixes; ++g)
-        for (int64_t t0 = 0; shared(g) && t0 < rows[(size_t)g]; t0 += tt)
-          tiles.push_back(SeqTile{at[(size_t)g], (int32_t)rows[(size_t)g], (int32_t)t0, g});
+        for (int64_t t0 = 0; shared(g) && t0 < rows[(size_t)g]; t0 += tt) {
+          tiles.push_back(SeqTile{at[(size_t)g], (int32_t)rows[(size_t)g], (int32_t)t0, first[(size_t)g]});
+          words.push_back(blocks[g]);
+        }
       sh.ntiles[z] = (int64_t)(tiles.size() - lists[z]);
     }
-    // entry, pre, of
-    words.assign((size_t)(2 * (sh.rows + prefixes + s->seqs)), 0);
-    int32_t *entry = words.data(), *pre = entry + 2 * sh.rows, *mine = pre + 2 * prefixes;
-    for (int g = 0; g < prefixes; ++g) {
-      pre[2 * g] = shared(g) ? first[(size_t)g] : 0;
-      pre[2 * g + 1] = shared(g) ? blocks[g] : 0;
-    }
+    words.resize((words.size() + 3) / 4 * 4);   // of each sequence: 16 bytes
+    const size_t of0 = words.size(), entry0 = of0 + 4 * (size_t)s->seqs;
+    words.resize(entry0 + 2 * (size_t)sh.rows);
     for (int i = 0, r = 0; i < s->seqs; r += s->lens[(size_t)i++]) {
-      mine[2 * i] = shared(of[i]) ? of[i] : -1;
+      int32_t* mine = &words[of0 + 4 * (size_t)i];
+      mine[0] = -1;
       if (!shared(of[i])) continue;
       int32_t& e = at[(size_t)of[i]];
-      mine[2 * i + 1] = e;
+      mine[0] = first[(size_t)of[i]];
+      mine[1] = blocks[of[i]];
+      mine[2] = e;
       for (int k = 0; k < s->lens[(size_t)i]; ++k, ++e) {
-        entry[2 * e] = r + k;
-        entry[2 * e + 1] = i;
+        words[entry0 + 2 * (size_t)e] = r + k;
+        words[entry0 + 2 * (size_t)e + 1] = i;
       }
     }
     const size_t tb = tiles.size() * sizeof(SeqTile), wb = words.size() * sizeof(int32_t);
@@ -87,10 +94,13 @@ int exn_prefixes_create(exn_ctx* ctx, const exn_seqs* s, const int32_t* of, cons
       delete p;
       return r;
     }
-    for (int z = 0; z < SEQ_TTS; ++z) sh.tiles[z] = (const SeqTile*)p->mem + lists[z];
-    sh.entry = (const int32_t*)((const char*)p->mem + tb);
-    sh.pre = sh.entry + 2 * sh.rows;
-    sh.of = sh.pre + 2 * prefixes;
+    const int32_t* w = (const int32_t*)((const char*)p->mem + tb);
+    for (int z = 0; z < SEQ_TTS; ++z) {
+      sh.tiles[z] = (const SeqTile*)p->mem + lists[z];
+      sh.tile_blocks[z] = w + lists[z];
+    }
+    sh.of = w + of0;
+    sh.entry = w + entry0;
   } catch (const std::bad_alloc&) {
     delete p;
     FAIL(EXN_ENOMEM, "prefixes: host memory");
@@ -124,7 +134,7 @@ int exn_attend_shared_part(const exn_seqs* s, const exn_prefixes* p, int heads, 
   TRY(check_prefixes(s, p));
   TRY(check_heads(EXN_DT_F16, EXN_DT_F16, heads, kv_heads, head_dim));
   if (cols < 1 || cols > (1 << 20)) FAIL(EXN_EINVAL, "attend_shared_part: %d columns", cols);
-  *floats = s->rows == 0 ? 0 : kv8_shared_part(s->rows, s->longest, s->seqs, p->sh, heads, kv_heads, head_dim, cols, s->ntiles);
+  *floats = s->rows == 0 ? 0 : kv8_shared_part(s->rows, s->longest, p->sh, heads, kv_heads, head_dim, cols, s->ntiles);
   return EXN_OK;
 }
 
@@ -140,7 +150,7 @@ int exn_attend_shared(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const e
   TRY(check_seqs(ctx, s));
   TRY(use(ctx));
   return launched("attend_shared",
-                  kv8_attend_shared(ctx->stream, kv8_of(c), s->tiles, s->ntiles, s->rows, s->longest, s->seqs, p->sh,
+                  kv8_attend_shared(ctx->stream, kv8_of(c), s->tiles, s->ntiles, s->rows, s->longest, p->sh,
                                     heads, (const uint16_t*)q, ldq, scale, (uint16_t*)out, odt == EXN_DT_BF16, ldo, part,
                                     part_cap));
 }

@@ -345,19 +345,23 @@ int64_t kv8_attend_part(int64_t rows, const int64_t* ntiles, int longest, int he
 hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles, int64_t rows,
                       int longest, int heads, const uint16_t* q, int64_t ldq, float scale, uint16_t* out, int obf,
                       int64_t ldo, float* part, int64_t part_cap);
-// a plan's prefixes as the kernels take them: the tiles of each one's rows (row0 the first of them in ENTRY, seq the
-// prefix); pairs {row, sequence} in ENTRY, {first sequence, blocks} in PRE, {prefix or -1, first of its rows in
-// ENTRY} of each sequence in OF
+// a plan's prefixes as the kernels take them: the tiles of each one's rows (row0 the first of them in ENTRY, seq its
+// first sequence) with its blocks; pairs {row, sequence} in ENTRY; in OF, of each sequence, {the first of its prefix or
+// -1, blocks, first of its rows in ENTRY, 0}
 struct Kv8Shared {
   const SeqTile* tiles[SEQ_TTS];
+  const int32_t* tile_blocks[SEQ_TTS];
   int64_t ntiles[SEQ_TTS], rows;
-  int most, blocks;   // the most rows of a prefix; the most blocks
-  const int32_t *entry, *pre, *of;
+  // the most rows and sequences of a prefix; the most blocks; the fewest of a sequence's with rows (0: one has none);
+  // the blocks that need not be read again
+  int most, seqs, blocks, fewest;
+  int64_t saved;
+  const int32_t *of, *entry;
 };
-int64_t kv8_shared_part(int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
+int64_t kv8_shared_part(int64_t rows, int longest, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
                         int cols, const int64_t* ntiles);
 hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles,
-                             int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, const uint16_t* q,
+                             int64_t rows, int longest, const Kv8Shared& sh, int heads, const uint16_t* q,
                              int64_t ldq, float scale, uint16_t* out, int obf, int64_t ldo, float* part, int64_t part_cap);
 
 // rows of heads normed and turned by their positions (rope.hip), q's and k's: heads 0 for none, w null for

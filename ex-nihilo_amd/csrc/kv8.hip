@@ -9,6 +9,7 @@
 // NaN has the scale NaN: what is read of it is NaN.
 #include "exn_common.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace exn {
@@ -340,14 +341,17 @@ struct Kv8Args {
   // k_kv8_chunk: [split][row][head][dim], [split][row][head][2]
   float* part;
   int64_t rows;
-  // the passes of attend_shared: pairs {row, sequence} of each prefix's rows, {first sequence, blocks} of each
-  // prefix, {prefix or -1, first of its rows there} of each sequence; the sums' references and weights
-  // [split][row][head][2] beside part's [split][row][head][dim]; rows times heads of them; the blocks that each
-  // sequence leaves to its prefix
-  const int32_t *entry, *pre, *of;
+  // the passes of attend_shared: pairs {row, sequence} of each prefix's rows, each tile's prefix's blocks, {first
+  // sequence of its prefix or -1, blocks, first of its rows in ENTRY} of each sequence (Kv8Shared); the sums'
+  // references and weights [split][row][head][2] beside part's [split][row][head][dim]; rows times heads of
+  // them; the prefix pass's splits; for the join, of each of a sequence's tiles: its splits, all with the
+  // prefix's, and the first of its rows there
+  const int32_t *entry, *blocks;
+  const int32x4* of;
   float* ml;
   int64_t n;
-  int32_t* runs;
+  int psplits, pleast;
+  int32x4* notes;
 };
 enum { ALONE = 0, PREFIX = 1, OWN = 2 };   // all of a sequence's keys; a prefix's, for all its rows; a sequence's others
 
@@ -359,64 +363,109 @@ __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* l
   return (nb + per - 1) / per;
 }
 
-// The first blocks of a sequence that its prefix's pass takes for it: those full before the step whose pages
-// its table names as FIRST's does, at most NB (a wave finds it out)
-__device__ __forceinline__ int kv8_alike(const Kv8& c, int seq, int first, int nb) {
-  nb = min(nb, kv8_base(c, seq) / 64);
-  int run = nb;
-  const int32_t *mine = c.table + (int64_t)seq * c.cols, *its = c.table + (int64_t)first * c.cols;
-#pragma unroll 4
-  for (int i = threadIdx.x & 63; i < nb; i += 64)
-    if (mine[i] != its[i]) run = min(run, i);
+// Which blocks a prefix's pass takes of a sequence: of each of the pass's splits, from its first block on, those full
+// before the step whose pages the sequence's table names as that of FIRST, the prefix's first sequence, does, up to
+// the first that is another.  Found out on the device in every call, by a split's workgroups for its own blocks and by
+// the sequence's for all of them.
+struct Kv8Own {
+  int first, nb, per;   // blocks below NB may be the pass's, in splits of PER
+};
+// page P of block B, or -1 where it is taken.  A wave's lanes take the same steps whatever their blocks: a loop that
+// each leaves at its own mismatch lost P, in this compiler's hands, where a lane did
+__device__ __forceinline__ int kv8_untaken(const Kv8& c, int seq, const Kv8Own& w, int b, int p) {
+  const int32_t *mine = c.table + (int64_t)seq * c.cols, *its = c.table + (int64_t)w.first * c.cols;
+  const int at = min(b, w.nb - 1), first = at / w.per * w.per;
+  int differ = b < w.nb ? 0 : 1;
+#pragma unroll 1
+  for (int k = 0; k < w.per; ++k) {
+    const int i = max(at - k, first);
+    differ |= mine[i] ^ its[i];
+  }
+  return differ ? p : -1;
+}
+__device__ __forceinline__ Kv8Own kv8_own(const Kv8Args& A, const int32x4& of, int base) {
+  if (of[0] < 0) return Kv8Own{0, 0, 1};
+  const int all = min(of[1], A.c.cols);
+  return Kv8Own{of[0], min(all, base / 64), max(A.pleast, (all + A.psplits - 1) / A.psplits)};
+}
+// the first block of a sequence that is not taken (a wave finds it out)
+__device__ __forceinline__ int kv8_own_from(const Kv8& c, int seq, const Kv8Own& w) {
+  const int32_t *mine = c.table + (int64_t)seq * c.cols, *its = c.table + (int64_t)w.first * c.cols;
+  int run = w.nb;
+#pragma unroll 8
+  for (int i = threadIdx.x & 63; i < w.nb; i += 64) run = min(run, mine[i] != its[i] ? i : run);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) run = min(run, __shfl_xor(run, o, 64));
   return __builtin_amdgcn_readfirstlane(run);
 }
-__device__ __forceinline__ int kv8_own_from(const Kv8Args& A, int seq) {
-  const int p = A.of[2 * seq];
-  return p < 0 ? 0 : kv8_alike(A.c, seq, A.pre[2 * p], min(A.pre[2 * p + 1], A.c.cols));
+// split I of a sequence's own blocks, FROM .. NB - 1 (taken ones among them are left out one by one): [*lo, *hi); the
+// splits with any
+__device__ __forceinline__ int kv8_own_split(const Kv8Args& A, int from, int nb, int i, int* lo, int* hi) {
+  const int n = kv8_split(max(0, nb - from), A.splits, A.least, i, lo, hi);
+  *lo += from;
+  *hi += from;
+  return n;
 }
-// The rows of a prefix's tile, N at most, and the blocks of the prefix that each may see (kv8_alike's, for a
-// workgroup's rows at once); RUN is the first row's of each sequence in each 64 rows, HEAD names that row
+// for the join: tile TILE's own splits, and where its rows are in the prefixes' pass
+__device__ __forceinline__ void kv8_note(const Kv8Args& A, const int32x4& of, int tile, int t0, int own) {
+  int a, b;
+  const int theirs = of[0] < 0 ? 0 : kv8_split(min(of[1], A.c.cols), A.psplits, A.pleast, 0, &a, &b);
+  A.notes[tile] = int32x4{own, own + theirs, of[2] + t0, 0};
+}
+// For the N rows of a prefix's tile: where the blocks [B0, B1) that each sees end.  RUN is of the first row of each
+// sequence in each 64 rows, which HEAD names.
 template <int N>
 struct PrefixRows {
-  int row[N], seq[N], head[N], run[N];
+  int seq[N], head[N], run[N];
 };
+__device__ __forceinline__ void lds_barrier() {   // with loads from memory in flight
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// in two steps, the first blocks' loads asked for between them
 template <int N>
-__device__ __forceinline__ void prefix_rows(const Kv8Args& A, const SeqTile& T, int n, int nb, PrefixRows<N>& R) {
+__device__ __forceinline__ void prefix_rows(const Kv8Args& A, const SeqTile& T, int n, int b1, PrefixRows<N>& R) {
   const Kv8& c = A.c;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63;
   if (tid < n) {
-    const int64_t e = 2 * ((int64_t)T.row0 + T.t0 + tid);
-    const int seq = A.entry[e + 1], before = __shfl_up(seq, 1, 64);
+    const int seq = A.entry[2 * ((int64_t)T.row0 + T.t0 + tid) + 1], before = __shfl_up(seq, 1, 64);
     const uint64_t heads = __ballot(lane == 0 || seq != before);
-    R.row[tid] = A.entry[e];
     R.seq[tid] = seq;
     R.head[tid] = tid - lane + 63 - __builtin_clzll(heads & (~0ull >> (63 - lane)));
-    R.run[tid] = min(nb, kv8_base(c, seq) / 64);
+    R.run[tid] = min(b1, kv8_base(c, seq) / 64);
   }
-  __syncthreads();
-  const int32_t* its = c.table + (int64_t)A.pre[2 * T.seq] * c.cols;
+}
+template <int N>
+__device__ __forceinline__ void prefix_ends(const Kv8Args& A, const SeqTile& T, int n, int b0, int b1, PrefixRows<N>& R) {
+  const Kv8& c = A.c;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_barrier();
+  const int32_t* its = c.table + (int64_t)T.seq * c.cols;
   for (int t = 4 * wave; t < n; t += 16) {   // four rows at a time
-    int at[4];
+    int at[4], end[4];
     const int32_t* mine[4];
     bool old = t % 64 > 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       at[j] = min(t + j, n - 1);
+      end[j] = b1;
       mine[j] = c.table + (int64_t)R.seq[at[j]] * c.cols;
       old = old && R.head[at[j]] < t;
     }
     if (old) continue;
 #pragma unroll 2
-    for (int i = lane; i < nb; i += 64) {
+    for (int i = b0 + lane; i < b1; i += 64) {
       const int x = its[i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (mine[j][i] != x) atomicMin(&R.run[at[j]], i);
+      for (int j = 0; j < 4; ++j) end[j] = min(end[j], mine[j][i] != x ? i : b1);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (end[j] < b1) atomicMin(&R.run[at[j]], end[j]);
   }
-  __syncthreads();
+  lds_barrier();
 }
 
 // a sequence's blocks after its new tokens
@@ -484,19 +533,27 @@ __device__ __forceinline__ uint32_t* kv8_parts(const Kv8Args& A, int per, int rt
 // 131071, fp16, 52.5 us, 5.0 and 5.1 TB/s, a copy's rate; 4 over 270..333 9.3 us, which is latency.
 //
 // Grid: workgroups x kv_heads x chunks, the heads fastest.
+template <int HD, int RT, int MODE>
+struct FewLds {
+  alignas(1024) uint8_t tbuf[2][MODE == PREFIX ? 1 : 64 * HD * 2];   // the tail's K and V
+  alignas(16) float obuf[4][16][HD + 4];
+  float mbuf[4][16], lbuf[4][16], pbuf[MODE == PREFIX ? 1 : 64][17];
+  PrefixRows<MODE == PREFIX ? 16 * RT : 1> pfx;
+};
 template <int BF, int HD, int RT, int MODE>
-__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
-k_kv8_few(Kv8Args A) {
+__device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>& lds, const int bx, const int by) {
   constexpr int WV = 4;                       // waves
   constexpr int NS = HD / 32, ND = HD / 16;   // k-steps of a score; 16-dim tiles of O
   constexpr int KL = HD / 64;                 // 16-byte loads a lane, key tile and block of K
-  constexpr int LD = HD + 4, ROWB = HD * 2, CH = HD / 8;
-  __shared__ __align__(16) float obuf[WV][16][LD];
-  __shared__ __align__(1024) uint8_t tbuf[2][64 * ROWB];   // the tail's K and V
-  __shared__ float mbuf[WV][16], lbuf[WV][16], pbuf[64][17];
+  constexpr int ROWB = HD * 2, CH = HD / 8;
+  auto &obuf = lds.obuf;
+  auto &tbuf = lds.tbuf;
+  auto &mbuf = lds.mbuf, &lbuf = lds.lbuf;
+  auto &pbuf = lds.pbuf;
+  auto &pfx = lds.pfx;
   const Kv8& c = A.c;
   const int per = c.kv_heads * A.chunks;
-  const int w = blockIdx.x / per, hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
+  const int w = bx / per, hc = bx % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = min(A.hh, A.group - chunk * A.hh);
@@ -536,16 +593,23 @@ k_kv8_few(Kv8Args A) {
   // a tile's part of the share; of a prefix, a split of its blocks; of a sequence's own, a split of those
   struct Seg {
     SeqTile T;
-    int seq, base, total, nfull, nb, lo, hi, its;
+    int base, total, nfull, nb, lo, hi, its;
+    int ahead;   // OWN: a lane's first page
   };
-  __shared__ PrefixRows<MODE == PREFIX ? 16 * RT : 1> pfx;
+  Kv8Own own;   // OWN: what the sequence's prefix takes
+  auto page_at = [&](const Seg& s, int it) __attribute__((always_inline)) {
+    const int b = s.lo + wave + WV * (it + lane);
+    int p = b < min(s.hi, s.nfull) ? (int)kv8_page(c, s.T.seq, b) : -1;
+    if (MODE == OWN && s.lo < own.nb) p = kv8_untaken(c, s.T.seq, own, b, p);
+    return p;
+  };
   auto segment = [&](int i, int at) __attribute__((always_inline)) {
     Seg s;
     s.T = A.tiles[i];
-    s.seq = s.T.seq;
+    int32x4 of;
+    if constexpr (MODE == OWN) of = A.of[s.T.seq];
     if constexpr (MODE == PREFIX) {
-      s.seq = A.pre[2 * s.T.seq];
-      s.base = s.total = min(A.pre[2 * s.T.seq + 1], c.cols) * 64;
+      s.base = s.total = min(A.blocks[i], c.cols) * 64;
     } else {
       s.base = kv8_base(c, s.T.seq);
       s.total = kv8_total(c, s.base, s.T.len);
@@ -555,12 +619,20 @@ k_kv8_few(Kv8Args A) {
     if constexpr (MODE == ALONE) {
       s.lo = max(0, from - at);
       s.hi = min(s.nb, to - at);
+    } else if constexpr (MODE == PREFIX) {
+      kv8_split(s.nb, A.splits, A.least, by, &s.lo, &s.hi);
     } else {
-      const int run = MODE == OWN ? kv8_own_from(A, s.seq) : 0;
-      if (MODE == OWN && blockIdx.y == 0 && hc == 0 && tid == 0) A.runs[s.seq] = run;
-      kv8_split(max(0, s.nb - run), A.splits, A.least, blockIdx.y, &s.lo, &s.hi);
-      s.lo += run;
-      s.hi += run;
+      // its first pages are asked for as if all that may be taken were, while that is found out
+      own = kv8_own(A, of, s.base);
+      int n = kv8_own_split(A, own.nb, s.nb, by, &s.lo, &s.hi);
+      const int b = s.lo + wave + WV * lane;
+      s.ahead = b < min(s.hi, s.nfull) ? (int)kv8_page(c, s.T.seq, b) : -1;
+      const int run = kv8_own_from(c, s.T.seq, own);
+      if (run != own.nb) {
+        n = kv8_own_split(A, run, s.nb, by, &s.lo, &s.hi);
+        s.ahead = page_at(s, 0);
+      }
+      if (by == 0 && hc == 0 && tid == 0) kv8_note(A, of, i, s.T.t0, n);
     }
     s.its = (min(s.hi, s.nfull) - s.lo - wave + WV - 1) / WV;   // full blocks lo + wave + WV it of this wave
     return s;
@@ -569,10 +641,8 @@ k_kv8_few(Kv8Args A) {
   float kds = 0.f, vds = 0.f;
   // 64 of the wave's blocks' pages and scales, a lane each
   auto look = [&](const Seg& s, int it) __attribute__((always_inline)) {
-    const int b = s.lo + wave + WV * (it + lane);
-    int64_t p = b < min(s.hi, s.nfull) ? kv8_page(c, s.seq, b) : -1;
-    pages = (int)p;
-    p = p < 0 ? 0 : p;
+    pages = MODE == OWN && it == 0 ? s.ahead : page_at(s, it);
+    const int64_t p = max(pages, 0);
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
     kds = d[0];
     vds = d[1] * (1.f / LIFT2);
@@ -602,7 +672,7 @@ k_kv8_few(Kv8Args A) {
       load_k(__builtin_amdgcn_readlane(pages, 0));
       load_v(__builtin_amdgcn_readlane(pages, 0));
     }
-    if (has_tail(s)) {
+    if (MODE != PREFIX && has_tail(s)) {
       const int64_t th = ((int64_t)s.T.seq * c.kv_heads + kvh) * 64 * HD;
 #pragma unroll 1
       for (int e = 0; e < CH; ++e) {
@@ -618,8 +688,9 @@ k_kv8_few(Kv8Args A) {
 
   Seg S = segment(i, at);
   if (MODE != ALONE && S.lo >= S.hi) return;
+  if constexpr (MODE == PREFIX) prefix_rows(A, S.T, S.T.len, S.hi, pfx);
   begin(S);
-  if constexpr (MODE == PREFIX) prefix_rows(A, S.T, S.T.len, S.nb, pfx);
+  if constexpr (MODE == PREFIX) prefix_ends(A, S.T, S.T.len, S.lo, S.hi, pfx);
   for (;;) {
     const SeqTile T = S.T;
     const int live = T.len;
@@ -637,7 +708,7 @@ k_kv8_few(Kv8Args A) {
         base = min(base, __builtin_amdgcn_readfirstlane(least));
       }
       // dims of k-step s: 16 g + 8 (s % 2) + 64 (s / 2) .., as the 16 bytes of codes a lane loads
-      const uint16_t* qr = A.q + (int64_t)(MODE == PREFIX ? pfx.row[tok] : T.row0 + tok) * A.ldq + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
+      const uint16_t* qr = A.q + (int64_t)(MODE == PREFIX ? A.entry[2 * ((int64_t)T.row0 + tok)] : T.row0 + tok) * A.ldq + (int64_t)(kvh * A.group + chunk * A.hh + head) * HD + 16 * g;
 #pragma unroll
       for (int s = 0; s < NS; ++s) qf[rt][s] = *(const s16x8*)(qr + 8 * (s % 2) + 64 * (s / 2));
     }
@@ -687,12 +758,14 @@ k_kv8_few(Kv8Args A) {
       return __builtin_bit_cast(s16x8, u32x4{pk[rt][4 * u], pk[rt][4 * u + 1], pk[rt][4 * u + 2], pk[rt][4 * u + 3]});
     };
 
-    for (int it = 0; it < S.its; ++it) {
+    // MORE: another block follows (true, false), or the lambda is to find out
+    auto block = [&](auto more_c, int it) __attribute__((always_inline)) {
+      const bool more = decltype(more_c)::value == 2 ? it + 1 < S.its : decltype(more_c)::value;
       const int page = __builtin_amdgcn_readlane(pages, it & 63);
       const float kd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, kds), it & 63)) * A.scale;
       const float vd = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vds), it & 63));
-      if ((it & 63) == 63 && it + 1 < S.its) look(S, it + 1);
-      const int next = it + 1 < S.its ? __builtin_amdgcn_readlane(pages, (it + 1) & 63) : 0;
+      if ((it & 63) == 63 && more) look(S, it + 1);
+      const int next = more ? __builtin_amdgcn_readlane(pages, (it + 1) & 63) : 0;
       const int k0 = (S.lo + wave + WV * it) * 64;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -710,9 +783,9 @@ k_kv8_few(Kv8Args A) {
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[rt][4 * t + e] = a[rt][e] * kd;
-        __builtin_amdgcn_sched_barrier(0);
+        if (RT == 1) __builtin_amdgcn_sched_barrier(0);
       }
-      if (it + 1 < S.its) load_k(next);
+      if (more) load_k(next);
       float vdl[RT];   // a row that sees nothing of the block takes nothing of its scale, which may be NaN
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
@@ -733,9 +806,16 @@ k_kv8_few(Kv8Args A) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[rt][d][e] = __builtin_fmaf(a[e], vdl[rt], o[rt][d][e]);
         }
-        if (d % 2) __builtin_amdgcn_sched_barrier(0);
+        if (RT == 1 && d % 2) __builtin_amdgcn_sched_barrier(0);
       }
-      if (it + 1 < S.its) load_v(next);
+      if (more) load_v(next);
+    };
+    if constexpr (MODE == ALONE) {
+      for (int it = 0; it < S.its; ++it) block(std::integral_constant<int, 2>(), it);
+    } else {
+      // the last one apart: where loads always follow, the wait for a block's K leaves its V's in flight
+      for (int it = 0; it + 1 < S.its; ++it) block(std::integral_constant<int, 1>(), it);
+      if (S.its > 0) block(std::integral_constant<int, 0>(), S.its - 1);
     }
 
     // the tail, in 16 bits, by the wave whose turn it is
@@ -880,12 +960,12 @@ k_kv8_few(Kv8Args A) {
         y[e] *= inv;
       }
       if constexpr (MODE != ALONE) {
-        const int64_t slot = blockIdx.y * A.n + (int64_t)(T.row0 + tok) * A.heads + kvh * A.group + chunk * A.hh + head;
+        const int64_t slot = by * A.n + (int64_t)(T.row0 + tok) * A.heads + kvh * A.group + chunk * A.hh + head;
 #pragma unroll
         for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + slot * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
         if ((mt & 15) == 0) *(f32x2*)(A.ml + slot * 2) = f32x2{m, sum};
       } else if (!whole) {   // the share's own first part (0) or the one begun in it (1)
-        const int64_t slot = ((int64_t)blockIdx.x * 2 + (lo == 0)) * 16 * RT + r;
+        const int64_t slot = ((int64_t)bx * 2 + (lo == 0)) * 16 * RT + r;
 #pragma unroll
         for (int e = 0; e < E; e += 4) *(f32x4*)(A.part + slot * HD + d0 + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
         if ((mt & 15) == 0) *(f32x2*)(A.part + (int64_t)A.splits * per * 32 * RT * HD + slot * 2) = f32x2{m, sum};
@@ -907,6 +987,13 @@ k_kv8_few(Kv8Args A) {
     }
     if (!more) return;
   }
+}
+
+template <int BF, int HD, int RT>
+__global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
+k_kv8_few(Kv8Args A) {
+  __shared__ FewLds<HD, RT, ALONE> lds;
+  few_rows<BF, HD, RT, ALONE>(A, lds, blockIdx.x, 0);
 }
 
 // The sums of k_kv8_few's workgroups of each tile that more than one had a part of, in a fixed order:
@@ -1024,67 +1111,71 @@ __device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int tota
   *l_ = l;
 }
 
-template <int BF, int HD, int MODE>
-__global__ void __launch_bounds__(256, 2)
-k_kv8_chunk(Kv8Args A) {
-  constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
-  constexpr int NS = HD / 16, ND = HD / 32;
-  constexpr int CI = HD / 64;                       // 16-byte loads of codes a thread and block
+template <int HD, int MODE>
+struct ChunkLds {
   // K stage s at s STAGE: rows of keys, 16-byte chunk c at c ^ (key % 16) (HD 64: c ^ (key / 2 % 8)).
   // V^T stage s at (2 + s) STAGE: rows of dims of 128 bytes, chunk c at c ^ (dim / 2 % 8); a row's
   // keys in vt_pos's order, the one in which a lane's weights lie.  The tail's V is as in memory, rows
   // of keys, chunk c at c ^ 4 (key % 4) (HD 64: c ^ 4 (key / 2 % 2)), and is turned when it is read.
-  __shared__ __align__(1024) uint8_t smem[4 * STAGE];
+  alignas(1024) uint8_t smem[4 * 64 * HD * 2];
+  PrefixRows<MODE == PREFIX ? 128 : 1> pfx;
+};
+template <int BF, int HD, int MODE, int KG>
+__device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>& lds, const int bx, const int by) {
+  constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
+  constexpr int NS = HD / 16, ND = HD / 32;
+  // a wave's halves of a block of keys: both, or, in tiles of 64 rows, one (waves 2 and 3 take the second's)
+  constexpr int NH = 2 / KG, NU = 2 * NH;
+  constexpr int CI = HD / 64;                       // 16-byte loads of codes a thread and block
+  uint8_t* const smem = lds.smem;
+  auto& pfx = lds.pfx;
   const Kv8& c = A.c;
   const int per = c.kv_heads * A.chunks;
-  const SeqTile T = A.tiles[blockIdx.x / per];
-  const int hc = blockIdx.x % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
+  const SeqTile T = A.tiles[bx / per];
+  const int hc = bx % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, lo = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int seq = MODE == PREFIX ? A.pre[2 * T.seq] : T.seq;
-  const int base = MODE == PREFIX ? min(A.pre[2 * T.seq + 1], c.cols) * 64 : kv8_base(c, seq);
+  const int base = MODE == PREFIX ? min(A.blocks[bx / per], c.cols) * 64 : kv8_base(c, T.seq);
   const int total = MODE == PREFIX ? base : kv8_total(c, base, T.len), nfull = total / 64;
   const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
   int b0, b1, active;   // the blocks taken here; the splits
   if constexpr (MODE == PREFIX) {
-    active = kv8_split(nfull, A.splits, A.least, blockIdx.y, &b0, &b1);
-  } else if constexpr (MODE == OWN) {
-    const int run = kv8_own_from(A, seq);
-    if (blockIdx.y == 0 && hc == 0 && tid == 0) A.runs[seq] = run;
-    active = kv8_split(max(0, (min(base + T.t0 + live, total) + 63) / 64 - run), A.splits, A.least, blockIdx.y, &b0, &b1);
-    b0 += run;
-    b1 += run;
+    active = kv8_split(nfull, A.splits, A.least, by, &b0, &b1);
   } else {
-    active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, blockIdx.y, &b0, &b1));
+    active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, by, &b0, &b1));
   }
-  if ((int)blockIdx.y >= active) return;
-  const int row = wave * 32 + lo, tok = (int)(row * A.magic >> 16), head = row - tok * A.hh;
+  if (by >= active) return;
+  const int rw = wave % (4 / KG), kg = wave / (4 / KG);
+  const int row = rw * 32 + lo, tok = (int)(row * A.magic >> 16), head = row - tok * A.hh;
   const bool mine = tok < live && head < heads;
   const int ctok = min(tok, live - 1), chead = kvh * A.group + chunk * A.hh + min(head, heads - 1);
-  int lim, minlim;
-  __shared__ PrefixRows<MODE == PREFIX ? 128 : 1> pfx;
-  if constexpr (MODE == PREFIX) {
-    prefix_rows(A, T, live, nfull, pfx);
-    lim = minlim = pfx.run[pfx.head[ctok]] * 64 - 1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
-    minlim = __builtin_amdgcn_readfirstlane(minlim);
-  } else {
-    lim = min(base + T.t0 + ctok, total - 1);
-    minlim = min(base + T.t0 + min((int)(wave * 32 * A.magic >> 16), live - 1), total - 1);
-  }
   // waves without a row do their part of each block's way into LDS only
-  const bool idle = MODE != ALONE && (int)(wave * 32 * A.magic >> 16) >= live;
-  const uint16_t* qr = A.q + (int64_t)(MODE == PREFIX ? pfx.row[ctok] : T.row0 + T.t0 + ctok) * A.ldq + (int64_t)chead * HD;
+  const bool idle = MODE == PREFIX && (int)(rw * 32 * A.magic >> 16) >= live;
+  int lim, minlim;
   s16x8 qf[NS];   // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
+  auto rows_here = [&]() __attribute__((always_inline)) {
+    const int64_t qrow = MODE == PREFIX ? A.entry[2 * ((int64_t)T.row0 + T.t0 + ctok)] : T.row0 + T.t0 + ctok;
+    const uint16_t* qr = A.q + qrow * A.ldq + (int64_t)chead * HD;
 #pragma unroll
-  for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s + 8 * hi);
+    for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s + 8 * hi);
+    if constexpr (MODE == PREFIX) {
+      prefix_ends(A, T, live, b0, b1, pfx);
+      lim = minlim = pfx.run[pfx.head[ctok]] * 64 - 1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
+      minlim = __builtin_amdgcn_readfirstlane(minlim);
+    } else {
+      lim = min(base + T.t0 + ctok, total - 1);
+      minlim = min(base + T.t0 + min((int)(rw * 32 * A.magic >> 16), live - 1), total - 1);
+    }
+  };
+  if constexpr (MODE != PREFIX) rows_here();
 
   // 64 blocks' pages and scales from block B on, a lane each
   int pages = 0;
   float kds = 1.f, vds = 1.f;
   auto look = [&](int b) __attribute__((always_inline)) {
-    int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, seq, b + lane) : -1;
+    int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, T.seq, b + lane) : -1;
     pages = (int)p;
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
@@ -1113,7 +1204,7 @@ k_kv8_chunk(Kv8Args A) {
     for (int i = 0; i < CI; ++i) x.w[i] = *(const u32x4*)(p + (tid + 256 * i) * 16);
     return x;
   };
-  const int64_t th = ((int64_t)seq * c.kv_heads + kvh) * 64 * HD;
+  const int64_t th = ((int64_t)T.seq * c.kv_heads + kvh) * 64 * HD;
   // the tail's 64 rows by DMA; those past its last token hold anything
   auto tail = [&](const uint16_t* all, uint8_t* p, auto swizzle) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -1151,17 +1242,17 @@ k_kv8_chunk(Kv8Args A) {
       tail(c.tv, p, [&](int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); });
     }
   };
-  int kofs[NS], vofs[4];   // K row lo, chunk 2s + hi; V^T row lo, chunk 2u + hi
+  int kofs[NS], vofs[NU];   // K row lo (of the wave's half), chunk 2s + hi; V^T row lo, chunk 2u + hi
 #pragma unroll
-  for (int s = 0; s < NS; ++s) kofs[s] = lo * ROWB + (((2 * s + hi) ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4);
+  for (int s = 0; s < NS; ++s) kofs[s] = (32 * kg + lo) * ROWB + (((2 * s + hi) ^ (HD == 128 ? lo & 15 : (lo >> 1) & 7)) << 4);
 #pragma unroll
-  for (int u = 0; u < 4; ++u) vofs[u] = 2 * STAGE + lo * 128 + (((2 * u + hi) ^ ((lo >> 1) & 7)) << 4);
-  auto kfrag = [&](int i) { return *(const s16x8*)(smem + kofs[i / 2] + (i % 2) * 32 * ROWB); };
+  for (int u = 0; u < NU; ++u) vofs[u] = 2 * STAGE + lo * 128 + (((2 * (u + 2 * kg) + hi) ^ ((lo >> 1) & 7)) << 4);
+  auto kfrag = [&](int i) { return *(const s16x8*)(smem + kofs[i / NH] + (i % NH) * 32 * ROWB); };
   auto vfrag = [&](auto tail_c, int u, int d) __attribute__((always_inline)) {
     if constexpr (decltype(tail_c)::value) {
       typedef __attribute__((address_space(3))) s16x4 lds_s4;
       const int r = 4 * hi + ((lane & 15) >> 2), x = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      uint8_t* p = smem + ((vofs[0] & ~(STAGE - 1)) + (16 * u + r) * ROWB +
+      uint8_t* p = smem + ((vofs[0] & ~(STAGE - 1)) + (16 * (u + 2 * kg) + r) * ROWB +
                            ((x ^ (HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))) << 4) + 8 * (lane & 1));
       return __builtin_shufflevector(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p),
                                      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 8 * ROWB)), 0, 1, 2, 3, 4, 5, 6, 7);
@@ -1170,7 +1261,7 @@ k_kv8_chunk(Kv8Args A) {
     }
   };
 
-  f32x16 o[ND], sc[2];
+  f32x16 o[ND], sc[NH];
   float mrun = 0.f, lrun = 0.f;
   bool set = false;          // the row has a reference
 #pragma unroll
@@ -1192,28 +1283,30 @@ k_kv8_chunk(Kv8Args A) {
     const float factor = F.kd * A.scale;
     const bool gone = F.page < 0 && b < nfull;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[h][r] = __builtin_fmaf(sc[h][r], factor, UP - mrun);
     if (gone || k0 + 63 > minlim) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * h + 8 * (r >> 2) + 4 * hi + (r & 3);
+          const int key = k0 + 32 * (h + kg) + 8 * (r >> 2) + 4 * hi + (r & 3);
           if (gone || key > lim) sc[h][r] = -INFINITY;
         }
     }
-    float m4[4];
+    float m4[2 * NH];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 2 * NH; ++q) {
       const int h = q / 2, r0 = (q % 2) * 8;
       float m = max3(sc[h][r0], sc[h][r0 + 1], sc[h][r0 + 2]);
       m = max3(m, sc[h][r0 + 3], sc[h][r0 + 4]);
       m = max3(m, sc[h][r0 + 5], sc[h][r0 + 6]);
       m4[q] = fmaxf(m, sc[h][r0 + 7]);
     }
-    float ma = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), mb = ma;
+    float ma = fmaxf(m4[0], m4[1]);
+    if constexpr (NH == 2) ma = fmaxf(ma, fmaxf(m4[2], m4[3]));
+    float mb = ma;
     xswap32(ma, mb);
     const float mx = fmaxf(ma, mb);
     const bool move = set ? mx > MAX_SLACK + UP : mx > -INFINITY;
@@ -1227,19 +1320,19 @@ k_kv8_chunk(Kv8Args A) {
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
       mrun += shift;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[h][r] -= shift;
       set = set || move;
     }
-    constexpr int KD = 3, NI = 2 * NS, PS = 16 / NI;
-    f32x16 sn[2];
-    uint32_t pk[16], pl[WB ? 16 : 1];
+    constexpr int KD = 3, NI = NH * NS, PS = 8 / NS;
+    f32x16 sn[NH];
+    uint32_t pk[8 * NH], pl[WB ? 8 * NH : 1];
     float ls[2] = {lrun, 0.f};
     s16x8 kq[KD], vq[KD];
     if constexpr (!LAST) {
-      sn[0] = f32x16{};
-      sn[1] = f32x16{};
+#pragma unroll
+      for (int h = 0; h < NH; ++h) sn[h] = f32x16{};
 #pragma unroll
       for (int i = 0; i < KD; ++i) kq[i] = kfrag(i);
     }
@@ -1248,12 +1341,12 @@ k_kv8_chunk(Kv8Args A) {
       if constexpr (!LAST) {
         s16x8 kn = {};
         if (i + KD < NI) kn = kfrag(i + KD);
-        sn[i % 2] = mfma32<BF>(kq[0], qf[i / 2], sn[i % 2]);
+        sn[i % NH] = mfma32<BF>(kq[0], qf[i / NH], sn[i % NH]);
 #pragma unroll
         for (int d = 0; d + 1 < KD; ++d) kq[d] = kq[d + 1];
         kq[KD - 1] = kn;
       }
-      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(tail_c, (i - (NI - KD)) % 4, (i - (NI - KD)) / 4);
+      if (i >= NI - KD) vq[i - (NI - KD)] = vfrag(tail_c, (i - (NI - KD)) % NU, (i - (NI - KD)) / NU);
 #pragma unroll
       for (int z = 0; z < PS; ++z) {
         const int pi = PS * i + z, h = pi / 8, r = 2 * (pi % 8);
@@ -1271,10 +1364,10 @@ k_kv8_chunk(Kv8Args A) {
     const float vd = gone || k0 > lim ? 0.f : (TAIL ? 1.f : F.vd) * (1.f / LIFT2);
     f32x16 t[2];
 #pragma unroll
-    for (int j = 0; j < 4 * ND; ++j) {
+    for (int j = 0; j < NU * ND; ++j) {
       s16x8 vn = {};
-      if (j + KD < 4 * ND) vn = vfrag(tail_c, (j + KD) % 4, (j + KD) / 4);
-      const int u = j % 4, d = j / 4;
+      if (j + KD < NU * ND) vn = vfrag(tail_c, (j + KD) % NU, (j + KD) / NU);
+      const int u = j % NU, d = j / NU;
       const s16x8 pb = __builtin_bit_cast(s16x8, u32x4{pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]});
       if constexpr (WB) {
         o[d] = mfma32<1>(vq[0], pb, o[d]);
@@ -1283,7 +1376,7 @@ k_kv8_chunk(Kv8Args A) {
         t[d % 2] = mfma32<0>(vq[0], pb, u == 0 ? f32x16{} : t[d % 2]);
         if (d > 0) {
 #pragma unroll
-          for (int r = 4 * u; r < 4 * u + 4; ++r) o[d - 1][r] = __builtin_fmaf(t[(d - 1) % 2][r], vd, o[d - 1][r]);
+          for (int r = 16 / NU * u; r < 16 / NU * (u + 1); ++r) o[d - 1][r] = __builtin_fmaf(t[(d - 1) % 2][r], vd, o[d - 1][r]);
         }
       }
 #pragma unroll
@@ -1296,28 +1389,30 @@ k_kv8_chunk(Kv8Args A) {
       for (int r = 0; r < 16; ++r) o[ND - 1][r] = __builtin_fmaf(t[(ND - 1) % 2][r], vd, o[ND - 1][r]);
     }
     if constexpr (!LAST) {
-      sc[0] = sn[0];
-      sc[1] = sn[1];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) sc[h] = sn[h];
     }
     asm volatile("" : "+v"(lrun));
   };
 
   // block b's K is filled two steps ahead of its softmax, its V one; codes are asked for one step
   // before they are filled
+  if constexpr (MODE == PREFIX) prefix_rows(A, T, live, b1, pfx);
   Facts F0 = facts(b0), F1 = F0, F2 = F0;
   Codes kc = fetch(c.k, F0.page), vc = fetch(c.v, F0.page), kn = kc;
   if (b0 + 1 < b1) {
     F1 = facts(b0 + 1);
     kn = fetch(c.k, F1.page);
   }
+  if constexpr (MODE == PREFIX) rows_here();   // while the first codes are on their way
   fill_k(b0, 0, kc);
   barrier(b0 == nfull);
-  sc[0] = f32x16{};
-  sc[1] = f32x16{};
+#pragma unroll
+  for (int h = 0; h < NH; ++h) sc[h] = f32x16{};
   if (!idle) {
 #pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) {
-      sc[i % 2] = mfma32<BF>(kfrag(i), qf[i / 2], sc[i % 2]);
+    for (int i = 0; i < NH * NS; ++i) {
+      sc[i % NH] = mfma32<BF>(kfrag(i), qf[i / NH], sc[i % NH]);
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -1353,7 +1448,7 @@ k_kv8_chunk(Kv8Args A) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) kofs[s] ^= STAGE;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) vofs[u] ^= STAGE;
+    for (int u = 0; u < NU; ++u) vofs[u] ^= STAGE;
   }
   barrier(b == nfull);
   if (MODE == PREFIX || b < nfull) {
@@ -1364,18 +1459,47 @@ k_kv8_chunk(Kv8Args A) {
     barrier(false);
     if (!idle) step(std::integral_constant<bool, true>(), std::integral_constant<bool, true>(), b, F0);
   }
+  if constexpr (KG == 2) {   // the second half's sums to the first's wave
+    constexpr int N = 16 * ND + 2;
+    float* buf = (float*)smem + rw * N * 64 + lane;
+    barrier(false);   // all reads of the blocks are done
+    if (kg && !idle) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) buf[(16 * d + r) * 64] = o[d][r];
+      buf[16 * ND * 64] = set ? mrun : -INFINITY;
+      buf[(16 * ND + 1) * 64] = lrun;
+    }
+    barrier(false);
+    if (kg || idle) return;
+    const float m = buf[16 * ND * 64], l = buf[(16 * ND + 1) * 64];
+    if (m == -INFINITY) {
+      lrun += l;   // 0, or NaN
+    } else {
+      const float mn = set ? fmaxf(mrun, m) : m;
+      const float a = set ? __builtin_amdgcn_exp2f(mrun - mn) : 1.f, w = __builtin_amdgcn_exp2f(m - mn);
+      lrun = lrun * a + l * w;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = __builtin_fmaf(w, buf[(16 * d + r) * 64], o[d][r] * a);
+      mrun = mn;
+      set = true;
+    }
+  }
   if (idle) return;
 
   float la = lrun, lb = lrun;
   xswap32(la, lb);
-  const bool parts = MODE != ALONE || active > 1;
+  const bool parts = MODE == PREFIX || active > 1;
   const float sum = (la + lb) * (1.f / LIFT2), mul = parts ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   float zero[4] = {sum * 0.f};
   const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = MODE == ALONE ? A.rows * A.heads : A.n;
   float* ml = MODE == ALONE ? A.part + A.splits * n * HD : A.ml;
   auto leave = [&](auto obf) __attribute__((always_inline)) {
     uint16_t* po = A.out + (int64_t)(T.row0 + T.t0 + tok) * A.ldo + (int64_t)chead * HD + 4 * hi;
-    float* pp = A.part + ((int64_t)blockIdx.y * n + rowhead) * HD + 4 * hi;
+    float* pp = A.part + ((int64_t)by * n + rowhead) * HD + 4 * hi;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1397,7 +1521,7 @@ k_kv8_chunk(Kv8Args A) {
   };
   if (parts) {
     leave(std::integral_constant<int, 2>());
-    if (mine && hi == 0) *(f32x2*)(ml + ((int64_t)blockIdx.y * n + rowhead) * 2) = f32x2{set ? mrun : -INFINITY, sum};
+    if (mine && hi == 0) *(f32x2*)(ml + ((int64_t)by * n + rowhead) * 2) = f32x2{set ? mrun : -INFINITY, sum};
   } else if (A.obf) {
     leave(std::integral_constant<int, 1>());
   } else {
@@ -1406,13 +1530,13 @@ k_kv8_chunk(Kv8Args A) {
   const uint64_t redo = __ballot(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.f) && mine);
 #pragma unroll 1
   for (uint32_t rows = (uint32_t)(redo | redo >> 32); rows; rows &= rows - 1) {
-    const int r = wave * 32 + __builtin_ctz(rows), rt = (int)(r * A.magic >> 16);
+    const int r = rw * 32 + __builtin_ctz(rows), rt = (int)(r * A.magic >> 16);
     const int64_t rh = kvh * A.group + chunk * A.hh + r - rt * A.hh, at = T.row0 + T.t0 + rt;
     float m, l, y[HD / 64];
-    const int64_t qrow = MODE == PREFIX ? pfx.row[rt] : at;
+    const int64_t qrow = MODE == PREFIX ? A.entry[2 * at] : at;
     const int sees = MODE == PREFIX ? pfx.run[pfx.head[rt]] * 64 - 1 : min(base + T.t0 + rt, total - 1);
-    kv8_row<BF, HD>(c, seq, kvh, b0, b1, total, sees, A.q + qrow * A.ldq + rh * HD, A.scale, &m, &l, y);
-    const int64_t slot = (int64_t)blockIdx.y * n + at * A.heads + rh;
+    kv8_row<BF, HD>(c, T.seq, kvh, b0, b1, total, sees, A.q + qrow * A.ldq + rh * HD, A.scale, &m, &l, y);
+    const int64_t slot = (int64_t)by * n + at * A.heads + rh;
     for (int z = 0; z < HD / 64; ++z) {
       const float w = parts ? y[z] : l == 0.f ? 0.f : y[z] / l;
       if (parts)
@@ -1422,6 +1546,13 @@ k_kv8_chunk(Kv8Args A) {
     }
     if (parts && lane == 0) *(f32x2*)(ml + slot * 2) = f32x2{m, l};
   }
+}
+
+template <int BF, int HD>
+__global__ void __launch_bounds__(256, 2)
+k_kv8_chunk(Kv8Args A) {
+  __shared__ ChunkLds<HD, ALONE> lds;
+  chunk_rows<BF, HD, ALONE, 1>(A, lds, blockIdx.x, blockIdx.y);
 }
 
 // The splits' sums of each row and head, in a fixed order: HD / 4 threads take one's dims in each of SH
@@ -1584,8 +1715,8 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a); };
   auto rts = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-    if (w.rt == 0) return go(k_kv8_chunk<BF, HD, ALONE>);
-    w.rt == 2 ? go(k_kv8_few<BF, HD, 2, ALONE>) : go(k_kv8_few<BF, HD, 1, ALONE>);
+    if (w.rt == 0) return go(k_kv8_chunk<BF, HD>);
+    w.rt == 2 ? go(k_kv8_few<BF, HD, 2>) : go(k_kv8_few<BF, HD, 1>);
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
@@ -1637,11 +1768,35 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
 // Which blocks those are is found out on the device (kv8_alike): the plan of prefixes is a hint, and what
 // comes out is kv8_attend's answer whatever the tables hold.
 
+// Both passes in one launch: PW workgroups of the prefixes', which take their rows as WAY says (0, 3: chunk_rows, tiles
+// of 64 and 128 rows; 1, 2: few_rows with as many row tiles), then the sequences' own
+template <int HD, int WAY>
+struct PrefixLds : FewLds<HD, WAY, PREFIX> {};
+template <int HD>
+struct PrefixLds<HD, 0> : ChunkLds<HD, PREFIX> {};
+template <int HD>
+struct PrefixLds<HD, 3> : ChunkLds<HD, PREFIX> {};
+template <int BF, int HD, int WAY>
+__global__ void __launch_bounds__(256, WAY == 2 ? 1 : 2)
+k_kv8_shared(Kv8Args P, Kv8Args O, uint32_t pw, uint32_t pgroups, uint32_t ogroups) {
+  __shared__ union Lds {
+    PrefixLds<HD, WAY> p;
+    FewLds<HD, 1, OWN> o;
+  } lds;
+  if (blockIdx.x >= pw) {
+    const uint32_t i = blockIdx.x - pw;
+    few_rows<BF, HD, 1, OWN>(O, lds.o, i % ogroups, i / ogroups);
+  } else if constexpr (WAY % 3 == 0) {
+    chunk_rows<BF, HD, PREFIX, WAY == 0 ? 2 : 1>(P, lds.p, blockIdx.x % pgroups, blockIdx.x / pgroups);
+  } else {
+    few_rows<BF, HD, WAY, PREFIX>(P, lds.p, blockIdx.x % pgroups, blockIdx.x / pgroups);
+  }
+}
+
 struct Kv8Meet {
   Kv8Args own;
   const float *part, *ml;   // the prefixes' sums
   int64_t n;
-  int splits, least;
 };
 template <int HD, int SH>
 __global__ void __launch_bounds__(256)
@@ -1652,36 +1807,44 @@ k_kv8_meet(Kv8Meet M) {
   const Kv8Args& A = M.own;
   const Kv8& c = A.c;
   const SeqTile T = A.tiles[blockIdx.x];
+  const int32x4 note = A.notes[blockIdx.x];
   const int live = min(A.tt, T.len - T.t0);
   if ((int)blockIdx.y * RW >= live * A.heads) return;
-  const int base = kv8_base(c, T.seq), total = kv8_total(c, base, T.len);
-  const int run = A.runs[T.seq], p = A.of[2 * T.seq];
-  int lo, hi;
-  const int owns = kv8_split(max(0, (min(base + T.t0 + live, total) + 63) / 64 - run), A.splits, A.least, 0, &lo, &hi);
-  const int all = owns + (run > 0 ? kv8_split(min(A.pre[2 * p + 1], c.cols), M.splits, M.least, 0, &lo, &hi) : 0);
+  const int owns = note[0], all = note[1];
   const int tid = threadIdx.x, sh = tid / TH % SH, r = tid / TH / SH, d = tid % TH * 4;
   const int i = min((int)blockIdx.y * RW + r, live * A.heads - 1);
-  const int64_t mine = (int64_t)(T.row0 + T.t0) * A.heads + i;
-  const int64_t theirs = p < 0 ? 0 : ((int64_t)A.of[2 * T.seq + 1] + T.t0) * A.heads + i;
-  auto slot = [&](int z) { return z < owns ? A.ml + (z * A.n + mine) * 2 : M.ml + ((z - owns) * M.n + theirs) * 2; };
-  auto sums = [&](int z) { return z < owns ? A.part + (z * A.n + mine) * HD : M.part + ((z - owns) * M.n + theirs) * HD; };
-  float m = -INFINITY;
-  for (int z = sh; z < all; z += SH) m = fmaxf(m, *slot(z));
-  if constexpr (SH > 1) {
-    if (d == 0) ms[tid / TH] = m;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < SH; ++k) m = fmaxf(m, ms[r * SH + k]);
-  }
-  float sum = 0.f;
+  const int64_t mine = (int64_t)(T.row0 + T.t0) * A.heads + i, theirs = (int64_t)note[2] * A.heads + i;
+  auto slot = [&](int z) { return z < owns ? z * A.n + mine : (z - owns) * M.n + theirs; };
+  // a share's sums as they come, under the largest reference so far
+  float m = -INFINITY, sum = 0.f;
   f32x4 y = {};
 #pragma unroll 4
   for (int z = sh; z < all; z += SH) {
-    const f32x2 ml = *(const f32x2*)slot(z);
-    const f32x4 x = *(const f32x4*)(sums(z) + d);
-    const float w = ml[0] == -INFINITY ? 0.f : ml[0] == m ? 1.f : __builtin_amdgcn_exp2f(ml[0] - m);
-    sum += ml[0] == -INFINITY ? ml[1] : w * ml[1];   // no reference: 0, or NaN
+    const int64_t at = slot(z);
+    const f32x2 ml = *(const f32x2*)((z < owns ? A.ml : M.ml) + at * 2);
+    const f32x4 x = *(const f32x4*)((z < owns ? A.part : M.part) + at * HD + d);
+    if (ml[0] == -INFINITY) {   // no reference: a weight of 0, or NaN
+      sum += ml[1];
+      continue;
+    }
+    const float mn = fmaxf(m, ml[0]);
+    const float a = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn), w = ml[0] == mn ? 1.f : __builtin_amdgcn_exp2f(ml[0] - mn);
+    sum = sum * a + w * ml[1];
+    y *= a;
     if (w > 0.f) y += w * x;
+    m = mn;
+  }
+  if constexpr (SH > 1) {
+    if (d == 0) ms[tid / TH] = m;
+    __syncthreads();
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < SH; ++k) top = fmaxf(top, ms[r * SH + k]);
+    if (m != top) {
+      const float a = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      sum *= a;
+      y *= a;
+    }
   }
   if constexpr (SH > 1) {
     *(f32x4*)&ys[tid / TH][d] = y;
@@ -1702,70 +1865,90 @@ k_kv8_meet(Kv8Meet M) {
 
 namespace {
 
-// one of attend_shared's passes: how its rows are taken, and into how many splits their blocks
+// one of attend_shared's passes: how its rows are taken (k_kv8_shared), and into how many splits their blocks
 struct PassWay {
-  int rt, z, hh, chunks, splits, least;
+  int way, z, hh, chunks, splits, least;
+  int64_t groups;   // workgroups a split
 };
-PassWay pass_way(int most, int heads, int kv_heads, int head_dim, int blocks, const int64_t* ntiles) {
-  PassWay w;
-  const int group = heads / kv_heads;
-  w.z = 0;
-  w.least = 2;
-  w.hh = group < 16 ? group : 16;
-  int64_t slots;
-  if ((int64_t)most * w.hh <= 32) {
-    w.rt = most * w.hh <= 16 ? 1 : 2;
-    while ((SEQ_TT0 << w.z) < most) ++w.z;
-    slots = 256 * (w.rt == 1 ? (head_dim == 64 ? 4 : 2) : (head_dim == 64 ? 2 : 1));
-  } else {
-    w.rt = 0;
-    w.hh = group < 8 ? group : 8;
-    while (w.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.z + 1)) * w.hh <= 128) ++w.z;
-    slots = 512;
-  }
-  w.chunks = (group + w.hh - 1) / w.hh;
-  const int64_t groups = ntiles[w.z] * w.chunks * kv_heads, pays = (blocks + w.least - 1) / w.least;
-  const int64_t s = groups > 0 ? slots / groups : 1;
-  w.splits = (int)(s > pays ? pays : s);
-  if (w.splits < 1) w.splits = 1;
-  return w;
+// as many splits as SLOTS workgroups are, none of less than LEAST blocks
+void split_pass(PassWay& w, double slots, int blocks, int least) {
+  w.least = least;
+  const int64_t s = w.groups > 0 ? (int64_t)(slots / w.groups) : 1, pays = (blocks + least - 1) / least;
+  w.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(s, pays), 128));
 }
 struct SharedWay {
   PassWay pre, own;
-  int64_t pre_each, own_each, floats;   // of a split of either; in all, with the runs
+  bool pays;
+  int64_t pre_each, own_each, notes, floats;   // of a split of either; of the notes; in all
 };
-SharedWay shared_way(int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
-                     int cols, const int64_t* ntiles) {
+SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, int kv_heads, int head_dim, int cols,
+                     const int64_t* ntiles) {
   SharedWay w;
-  w.pre = pass_way(sh.most, heads, kv_heads, head_dim, sh.blocks < cols ? sh.blocks : cols, sh.ntiles);
-  w.own = pass_way(longest, heads, kv_heads, head_dim, cols, ntiles);
+  const int group = heads / kv_heads, blocks = sh.blocks < cols ? sh.blocks : cols;
+  w.pays = sh.rows > 0 && longest * (group < 16 ? group : 16) <= 16 && blocks > 16 &&
+           sh.saved >= (sh.seqs < 4 ? 384 : 112);
+  if (!w.pays) return w;
+  auto rows_way = [&](PassWay& p, int hh, int tile, const int64_t* n) {
+    p.hh = hh;
+    while ((SEQ_TT0 << p.z) * hh < tile && p.z + 1 < SEQ_TTS) ++p.z;
+    p.chunks = (group + hh - 1) / hh;
+    p.groups = n[p.z] * p.chunks * kv_heads;
+  };
+  const int hh = group < 16 ? group : 16;
+  w.own.way = 1;
+  w.own.z = w.pre.z = 0;
+  rows_way(w.own, hh, longest * hh, ntiles);
+  const int64_t most = (int64_t)sh.most * hh;
+  if (most <= 32) {
+    w.pre.way = most <= 16 ? 1 : 2;
+    const bool two = w.pre.way == 2 && sh.most <= 16 && blocks < 1000;
+    if (two) w.pre.way = 1;
+    rows_way(w.pre, two ? 16 / sh.most : hh, sh.most * (two ? 16 / sh.most : hh), sh.ntiles);
+  } else {
+    const int h8 = group < 8 ? group : 8;
+    w.pre.way = (int64_t)sh.most * h8 <= 64 ? 0 : 3;
+    while (w.pre.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.pre.z + 1)) * h8 <= (w.pre.way ? 128 : 64)) ++w.pre.z;
+    rows_way(w.pre, h8, 0, sh.ntiles);
+  }
+  const int own = cols > sh.fewest ? cols - sh.fewest : 1;
+  const int places = 256 * (head_dim == 64 ? 4 : 2);   // of few_rows with one row tile that the chip holds
+  split_pass(w.own, places, own, 8);
+  double slots;
+  if (w.pre.way % 3) {
+    const int all = w.pre.way == 1 ? places : places / 2;
+    slots = std::max<double>(all - w.own.groups, all / 2);
+  } else {
+    // of the time that each pass would take with all CUs: 1.5 us a block of a prefix's tile, and a quarter of the own
+    // blocks that there may be at 5 TB/s
+    const double units = w.pre.groups * (double)blocks;
+    const double a = units * 1.5 / 256, b = w.own.groups * (double)own / 4 * (head_dim * 128) / 5e6;
+    slots = a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1;
+  }
+  split_pass(w.pre, slots, blocks, w.pre.way % 3 ? 4 : 2);
   w.pre_each = sh.rows * heads * (head_dim + 2);
   w.own_each = rows * heads * (head_dim + 2);
-  w.floats = w.pre.splits * w.pre_each + w.own.splits * w.own_each + seqs;
+  w.notes = 4 * ntiles[w.own.z];
+  w.floats = w.pre.splits * w.pre_each + w.own.splits * w.own_each + w.notes;
   return w;
 }
 
 }  // namespace
 
-int64_t kv8_shared_part(int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
+int64_t kv8_shared_part(int64_t rows, int longest, const Kv8Shared& sh, int heads, int kv_heads, int head_dim,
                         int cols, const int64_t* ntiles) {
-  const int64_t alone = kv8_attend_part(rows, ntiles, longest, heads, kv_heads, head_dim, cols);
-  if (sh.rows == 0) return alone;
-  const int64_t n = shared_way(rows, longest, seqs, sh, heads, kv_heads, head_dim, cols, ntiles).floats;
-  return n > alone ? n : alone;
+  const SharedWay w = shared_way(rows, longest, sh, heads, kv_heads, head_dim, cols, ntiles);
+  return w.pays ? w.floats : kv8_attend_part(rows, ntiles, longest, heads, kv_heads, head_dim, cols);
 }
 
 hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, const int64_t* ntiles,
-                             int64_t rows, int longest, int seqs, const Kv8Shared& sh, int heads, const uint16_t* q,
+                             int64_t rows, int longest, const Kv8Shared& sh, int heads, const uint16_t* q,
                              int64_t ldq, float scale, uint16_t* out, int obf, int64_t ldo, float* part, int64_t part_cap) {
   if (ntiles[0] == 0) return hipSuccess;
-  SharedWay w = shared_way(rows, longest, seqs, sh, heads, c.kv_heads, c.head_dim, c.cols, ntiles);
-  // less scratch: fewer splits, the prefixes' first to keep theirs; without room for one of each, nothing is shared
-  const int64_t spare = part_cap - seqs - w.pre_each - w.own_each;
-  if (sh.rows == 0 || spare < 0)
+  SharedWay w = shared_way(rows, longest, sh, heads, c.kv_heads, c.head_dim, c.cols, ntiles);
+  if (!w.pays || part_cap < w.notes + w.pre_each + w.own_each)
     return kv8_attend(s, c, tiles, ntiles, rows, longest, heads, q, ldq, scale, out, obf, ldo, part, part_cap);
-  if (w.floats > part_cap) {
-    const int64_t p = 1 + spare / w.pre_each;
+  if (w.floats > part_cap) {   // fewer splits, the prefixes' first to keep theirs
+    const int64_t spare = part_cap - w.notes - w.pre_each - w.own_each, p = 1 + spare / w.pre_each;
     if (p < w.pre.splits) w.pre.splits = (int)p;
     const int64_t o = 1 + (spare - (w.pre.splits - 1) * w.pre_each) / w.own_each;
     if (o < w.own.splits) w.own.splits = (int)o;
@@ -1782,8 +1965,8 @@ hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* 
   a.obf = obf;
   a.rows = rows;
   a.entry = sh.entry;
-  a.pre = sh.pre;
-  a.of = sh.of;
+  a.blocks = sh.tile_blocks[w.pre.z];
+  a.of = (const int32x4*)sh.of;
   Kv8Args b = a;   // a: the prefixes' pass, b: the sequences' own
   a.tiles = sh.tiles[w.pre.z];
   a.ntiles = (int)sh.ntiles[w.pre.z];
@@ -1798,44 +1981,45 @@ hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* 
     x.magic = (65536 + p.hh - 1) / p.hh;
     x.splits = p.splits;
     x.least = p.least;
-    return (int64_t)x.ntiles * p.chunks * c.kv_heads;
   };
-  const int64_t ga = fill(a, w.pre), gb = fill(b, w.own);
+  fill(a, w.pre);
+  fill(b, w.own);
   a.part = part;
   b.part = a.part + a.splits * a.n * c.head_dim;
-  a.ml = b.part + b.splits * b.n * c.head_dim;
+  b.notes = (int32x4*)(b.part + b.splits * b.n * c.head_dim);
+  a.ml = (float*)(b.notes + b.ntiles);
   b.ml = a.ml + a.splits * a.n * 2;
-  a.runs = b.runs = (int32_t*)(b.ml + b.splits * b.n * 2);
-  if (ga > WG256_MAX || gb > WG256_MAX) return hipErrorInvalidConfiguration;
+  a.notes = nullptr;
+  b.psplits = a.splits;
+  b.pleast = a.least;
+  const int64_t pw = w.pre.groups * a.splits, all = pw + w.own.groups * b.splits;
+  if (all > WG256_MAX) return hipErrorInvalidConfiguration;
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
   typedef std::integral_constant<int, 64> I64;
   typedef std::integral_constant<int, 128> I128;
-  auto pass = [&](auto mode_c, const Kv8Args& x, int rt, int64_t groups) {
-    constexpr int MODE = decltype(mode_c)::value;
-    const dim3 grid((unsigned)groups, x.splits);
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, x); };
-    auto rts = [&](auto bf, auto hd) {
-      constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
-      if (rt == 0) return go(k_kv8_chunk<BF, HD, MODE>);
-      rt == 2 ? go(k_kv8_few<BF, HD, 2, MODE>) : go(k_kv8_few<BF, HD, 1, MODE>);
-    };
-    if (c.head_dim == 128)
-      c.bf16 ? rts(I1(), I128()) : rts(I0(), I128());
-    else
-      c.bf16 ? rts(I1(), I64()) : rts(I0(), I64());
-    return hipGetLastError();
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)all), dim3(256), 0, s, a, b, (uint32_t)pw, (uint32_t)w.pre.groups,
+                       (uint32_t)w.own.groups);
   };
-  hipError_t e = pass(std::integral_constant<int, PREFIX>(), a, w.pre.rt, ga);
-  if (e == hipSuccess) e = pass(std::integral_constant<int, OWN>(), b, w.own.rt, gb);
+  auto ways = [&](auto bf, auto hd) {
+    constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;
+    w.pre.way == 0   ? go(k_kv8_shared<BF, HD, 0>)
+    : w.pre.way == 1 ? go(k_kv8_shared<BF, HD, 1>)
+    : w.pre.way == 2 ? go(k_kv8_shared<BF, HD, 2>)
+                     : go(k_kv8_shared<BF, HD, 3>);
+  };
+  if (c.head_dim == 128)
+    c.bf16 ? ways(I1(), I128()) : ways(I0(), I128());
+  else
+    c.bf16 ? ways(I1(), I64()) : ways(I0(), I64());
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   Kv8Meet m;
   m.own = b;
   m.part = a.part;
   m.ml = a.ml;
   m.n = a.n;
-  m.splits = a.splits;
-  m.least = a.least;
   const int th = c.head_dim / 4, most = (b.tt < longest ? b.tt : longest) * heads;   // a tile's rows and heads
   const int rw = a.splits + b.splits > 16 ? 1 : a.splits + b.splits > 4 ? 2 : 256 / th;
   const dim3 jg((unsigned)ntiles[w.own.z], (most + rw - 1) / rw);

@@ -8,7 +8,6 @@ static std::string g_err, g_log;
 static exn_ctx g_ctx;
 static int g_capturing = 0, g_no_memory = 0;
 static Kv8Shared g_shared;
-static int g_seqs = 0, g_prefixes = 0;
 static RopeArgs g_rope;
 
 namespace exn {
@@ -41,13 +40,11 @@ hipError_t kv8_attend(hipStream_t, const Kv8&, const SeqTile* const*, const int6
                       const uint16_t*, int64_t, float, uint16_t*, int, int64_t, float*, int64_t) {
   return note("attend");
 }
-int64_t kv8_shared_part(int64_t, int, int, const Kv8Shared&, int, int, int, int, const int64_t*) { return 34; }
-hipError_t kv8_attend_shared(hipStream_t, const Kv8&, const SeqTile* const*, const int64_t*, int64_t, int, int seqs,
+int64_t kv8_shared_part(int64_t, int, const Kv8Shared&, int, int, int, int, const int64_t*) { return 34; }
+hipError_t kv8_attend_shared(hipStream_t, const Kv8&, const SeqTile* const*, const int64_t*, int64_t, int,
                              const Kv8Shared& sh, int, const uint16_t*, int64_t, float, uint16_t*, int, int64_t, float*,
                              int64_t) {
   g_shared = sh;
-  g_seqs = seqs;
-  g_prefixes = (int)(sh.of - sh.pre) / 2;
   return note("shared");
 }
 hipError_t rope_rows(hipStream_t, const RopeArgs& a, int, int, int, int64_t, int) {
@@ -91,21 +88,21 @@ const char* ph_log() {
   g_log.clear();
   return l.c_str();
 }
-// what the last attend_shared got: {rows, most, blocks, prefixes, sequences}; then entry, pre, of; then each list's
-// tiles after (-1, tokens a tile, 0, 0)
-int ph_shared(int32_t* out) {
+// what the last attend_shared got: {rows, most, blocks}; the SEQS sequences' {first, blocks, row, 0}; the rows' {row,
+// sequence}; then each list's tiles with their blocks after (-1, tokens a tile, 0, 0, 0)
+int ph_shared(int32_t* out, int seqs) {
   int32_t* o = out;
-  for (int64_t v : {g_shared.rows, (int64_t)g_shared.most, (int64_t)g_shared.blocks, (int64_t)g_prefixes, (int64_t)g_seqs})
-    *o++ = (int32_t)v;
-  const size_t words = 2 * (size_t)(g_shared.rows + g_prefixes + g_seqs);
-  memcpy(o, g_shared.entry, 4 * words);
-  o += words;
-  for (int z = 0; z < SEQ_TTS; ++z) {
-    const SeqTile head{-1, SEQ_TT0 << z, 0, 0};
-    memcpy(o, &head, sizeof head);
-    memcpy(o + 4, g_shared.tiles[z], sizeof(SeqTile) * (size_t)g_shared.ntiles[z]);
-    o += 4 + 4 * g_shared.ntiles[z];
-  }
+  for (int64_t v : {g_shared.rows, (int64_t)g_shared.most, (int64_t)g_shared.blocks}) *o++ = (int32_t)v;
+  memcpy(o, g_shared.of, 16 * (size_t)seqs);
+  o += 4 * seqs;
+  memcpy(o, g_shared.entry, 8 * (size_t)g_shared.rows);
+  o += 2 * g_shared.rows;
+  for (int z = 0; z < SEQ_TTS; ++z)
+    for (int64_t i = -1; i < g_shared.ntiles[z]; ++i, o += 5) {
+      const SeqTile t = i < 0 ? SeqTile{-1, SEQ_TT0 << z, 0, 0} : g_shared.tiles[z][i];
+      memcpy(o, &t, sizeof t);
+      o[4] = i < 0 ? 0 : g_shared.tile_blocks[z][i];
+    }
   return (int)(o - out);
 }
 // the turns and axes of the last rope_rows

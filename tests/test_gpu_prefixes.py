@@ -102,6 +102,76 @@ def test_shared(ctx, shape, heads, kv, hd, dt, odt):
         assert r <= 1
 
 
+# as above, with prefixes long enough, and of enough sequences, that their blocks are read once for all (the plan decides by
+# both): rows of a prefix that fill one tile of 16, two, half a tile of 128, several
+LONG = {
+    "eight": ([0] * 8, [17], [5, 60, 0, 63, 64, 127, 1, 300], [1] * 8),
+    "new blocks": ([0] * 9, [18], [63] * 4 + [126] * 5, [1] * 9),
+    "two prefixes and some alone": ([i % 3 - 1 for i in range(24)], [17, 29], [(31 * i) % 200 for i in range(24)], [1] * 24),
+    "waiting": ([0] * 12, [20], [(17 * i) % 70 for i in range(12)], [i % 2 for i in range(12)]),
+    "three tokens": ([0] * 10 + [-1], [19], [(41 * i) % 150 for i in range(10)] + [700], [3, 1, 2, 3, 0, 3, 2, 2, 1, 3, 3]),
+    "sixteen": ([0] * 16, [21], [(13 * i) % 130 for i in range(16)], [1] * 16),
+    "forty": ([0] * 40, [17], [(7 * i) % 90 for i in range(40)], [1] * 40),
+    "long tails": ([0] * 8, [17], [1200, 3, 900, 0, 2000, 640, 64, 63], [1] * 8),
+    "a long and a short": ([0, 0, 0, 0, 1, 1, 1, 1], [50, 1], [3, 70, 64, 0, 9, 500, 64, 1], [1] * 8),
+}
+
+
+@pytest.mark.parametrize("dt,odt", [("fp16", "bf16"), ("bf16", "fp16"), ("bf16", "bf16"), ("fp16", "fp16")])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 1, 64), (3, 3, 128), (4, 2, 64), (5, 1, 128), (16, 1, 64), (2, 2, 64)])
+@pytest.mark.parametrize("shape", LONG)
+def test_long_shared(ctx, shape, heads, kv, hd, dt, odt):
+    of, blocks, own, new = LONG[shape]
+    rng = np.random.default_rng([len(of), heads, hd])
+    say("long shared", shape, heads, kv, hd, dt, odt)
+    before = [n + 64 * (blocks[g] if g >= 0 else 0) for n, g in zip(own, of)]
+    m, d = alike(ctx, dt, kv, hd, of, blocks, before, rng)
+    for _ in range(2):
+        r = step(ctx, m, d, of, blocks, new, heads, odt, rng)
+        say("worst", r)
+        assert r <= 1
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("heads,kv,hd,seqs,tokens", [(2, 1, 64, 2, 30000), (4, 1, 64, 8, 70000), (4, 1, 128, 8, 66000),
+                                                     (4, 2, 128, 3, 14000), (8, 1, 128, 8, 20000), (8, 1, 64, 30, 9000)])
+def test_very_long_prefixes(ctx, heads, kv, hd, seqs, tokens, dt):
+    """Tens of thousands of keys: two tiles of rows a workgroup, few sequences, 128 splits."""
+    rng = np.random.default_rng([32, seqs])
+    of, blocks = [0] * seqs, [tokens // 64]
+    say("very long", heads, kv, hd, seqs, tokens, dt)
+    m, d = alike(ctx, dt, kv, hd, of, blocks, [blocks[0] * 64 + (37 * i) % 400 for i in range(seqs)], rng)
+    assert step(ctx, m, d, of, blocks, [1] * seqs, heads, "bf16", rng) <= 1
+
+
+def test_long_tables_that_are_not_alike(ctx):
+    """Tables that part at a split's first block, within one, at the last, at several; that meet again; lengths under the
+    prefix; pages that are none, alike and not; the first sequence's own table and length odd."""
+    rng = np.random.default_rng(33)
+    say("long not alike")
+    for heads, kv, hd, n in ((2, 2, 64, 12), (4, 2, 128, 12), (4, 1, 64, 30), (4, 1, 128, 14)):
+        of, blocks, b = [0] * n, [30], 30
+        before = [b * 64 + (29 * i) % 150 for i in range(n)]
+        before[3], before[5], before[7] = 100, 0, 64 * 17 + 63
+        m, d = alike(ctx, "fp16", kv, hd, of, blocks, before, rng, cols=36)
+        other = lambda i, j: m.table[i, 35 - j % 3]
+        m.table[1, 0] = other(1, 0)
+        m.table[2, 29] = other(2, 1)
+        m.table[4, [7, 8, 20]] = [other(4, 0), other(4, 1), -1]
+        m.table[6, 2:30:3] = [other(6, j) for j in range(10)]
+        m.table[8, 10:] = m.table[9, 10:][::-1]
+        m.table[[0, 9, 10], 16] = 1 << 30          # no page, in some and in the first's
+        m.table[11, 12] = -7
+        d.b["table"].upload(m.table)
+        for blocks in ([30], [20], [36], [1 << 20]):
+            r = step(ctx, m, d, of, blocks, [1] * n, heads, "bf16", rng)
+            say(blocks, "worst", r)
+            assert r <= 1
+        m.lens[0] = 0                              # the first sequence begins anew: its table is what counts
+        d.b["lens"].upload(m.lens)
+        assert step(ctx, m, d, of, [30], [1] * n, heads, "fp16", rng) <= 1
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("cap", [None, 0.5, 0.2, 0.05, 0], ids=str)
 def test_scratch(ctx, cap, hd):
@@ -149,6 +219,10 @@ def test_full_tables(ctx):
     """A sequence whose table is full keeps no new token; with all its blocks shared it has none of its own."""
     rng = np.random.default_rng(24)
     say("full tables")
+    for new in (1, 2):
+        n = 9
+        m, d = alike(ctx, "bf16", 2, 128, [0] * n, [18], [18 * 64] * 4 + [18 * 64 - 1, 18 * 64 - 64] + [1 << 30, -5, 1], rng, cols=18)
+        assert step(ctx, m, d, [0] * n, [18], [new] * n, 4, "bf16", rng) <= 1
     for new in ([1, 1, 1], [20, 3, 70]):
         m, d = alike(ctx, "bf16", 2, 128, [0] * 3, [4], [256, 256, 250], rng, cols=4)
         assert step(ctx, m, d, [0] * 3, [4], new, 4, "bf16", rng) <= 1
@@ -205,11 +279,51 @@ def test_blocks_that_are_not_finite(ctx, dt, bad, new):
     assert (abs(got - want)[same] <= tol[same]).all()
 
 
+@pytest.mark.parametrize("heads", [2, 4, 8])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, "scale"])
+def test_long_prefix_with_a_block_that_is_not_finite(ctx, bad, heads):
+    """A spoilt block of the prefix is seen by the sequences that share it, and by none whose table has parted before it; a
+    sequence's own spoilt block by itself alone; infinite scores in the prefix as in a sequence's own."""
+    rng = np.random.default_rng(34)
+    say("long not finite", bad, heads)
+    kv, hd, n, of, blocks = 2, 128, 14, [0] * 14, [24]
+    m, d = alike(ctx, "bf16", kv, hd, of, blocks, [24 * 64 + 70 + 5 * i for i in range(n)], rng)
+    m.table[3, 2] = m.table[3, -1]
+    m.table[4, 11] = m.table[4, -1]
+    value = np.nan if bad == "scale" else bad
+    m.scales[m.table[0, 11], 1, 1] = value                  # values of the second head's twelfth block
+    m.scales[m.table[6, 24], 0, 0] = np.nan                 # a sequence's own keys
+    d.b["table"].upload(m.table)
+    d.b["scales"].upload(m.scales)
+    s = X.Seqs(ctx, [1] * n)
+    p = X.Prefixes(ctx, s, of, blocks)
+    qb, q = normal(rng, (n, heads, hd), "bf16")
+    dq, o = X.DevBuf.of(ctx, qb), X.DevBuf(ctx, (n, heads, hd), np.uint16)
+    floats = X.attend_shared_part(s, p, heads, kv, hd, m.cols)
+    part = X.DevBuf(ctx, (floats,), np.float32)
+    X.attend_shared(ctx, d.h, s, p, heads, dq.h, heads * hd, 0.09, o.h, X.DT_BF16, heads * hd, part.h, floats)
+    got = pm.value(o.get(), "bf16")
+    half = heads // 2
+    sees = [i for i in range(n) if i != 4]                  # the fourth has parted there and only there
+    assert not np.isfinite(got[sees][:, half:]).any() and np.isnan(got[6, :half]).all()
+    m.scales[~np.isfinite(m.scales)] = 0.03
+    want, tol = m.attend(q, [1] * n, 0.09, "bf16")
+    same = np.zeros(got.shape, bool)
+    same[:, :half] = True
+    same[4] = True
+    same[6, :half] = False
+    assert (abs(got - want)[same] <= tol[same]).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, 3.0, 1e-4])
 def test_sharp_and_flat(ctx, scale):
     """Scores of hundreds, in the prefix or outside of it, and of nothing."""
     rng = np.random.default_rng(26)
     say("scale", scale)
+    for heads, kv in ((2, 2), (4, 2), (4, 1)):
+        of, blocks = [0] * 12, [19]
+        m, d = alike(ctx, "fp16", kv, 128, of, blocks, [19 * 64 + 51 * i for i in range(12)], rng)
+        assert step(ctx, m, d, of, blocks, [1] * 12, heads, "bf16", rng, scale=scale) <= 1
     for new in (1, 40):
         of, blocks = [0] * 4, [7]
         m, d = alike(ctx, "bf16", 2, 128, of, blocks, [448, 460, 500, 700], rng)
@@ -221,6 +335,14 @@ def test_large_values_meet_small_ones(ctx):
     rng = np.random.default_rng(27)
     say("sizes")
     for at in (0, 1):
+        for heads, kv in ((2, 2), (4, 2), (4, 1)):
+            of, blocks, n = [0] * 16, [20], 16
+            m, d = alike(ctx, "bf16", kv, 128, of, blocks, [1280 + 33 * i for i in range(n)], rng)
+            shared = m.table[0, :20]
+            rest = np.setdiff1d(np.arange(m.pages), shared)
+            m.scales[shared if at == 0 else rest, :, 1] *= np.float32(2.0 ** 17)
+            d.b["scales"].upload(m.scales)
+            assert step(ctx, m, d, of, blocks, [1] * n, heads, "bf16", rng) <= 1
         of, blocks = [0] * 3, [3]
         m, d = alike(ctx, "bf16", 1, 128, of, blocks, [250, 330, 200], rng)
         shared = m.table[0, :3]
@@ -303,10 +425,10 @@ def test_captured_steps_with_tables_that_change(ctx):
     hip = ctypes.CDLL("libamdhip64.so")
     vp = ctypes.c_void_p
     rng = np.random.default_rng(31)
-    heads, kv, hd, n = 8, 2, 128, 5
-    of, blocks, new = [0, 0, 0, 1, 1], [3, 2], [1] * 5
+    heads, kv, hd, n = 8, 2, 128, 12
+    of, blocks, new = [0] * 8 + [1] * 4, [18, 17], [1] * 12
     say("captured")
-    m, d = alike(ctx, "fp16", kv, hd, of, blocks, [192 + 60, 192 + 63, 192, 128 + 5, 128 + 70], rng)
+    m, d = alike(ctx, "fp16", kv, hd, of, blocks, [64 * blocks[g] + (60 + 3 * i) % 90 for i, g in enumerate(of)], rng)
     s = X.Seqs(ctx, new)
     p = X.Prefixes(ctx, s, of, blocks)
     freqs = X.rope_freqs(hd, 5e6)

@@ -90,34 +90,32 @@ def test_plans(L, lens, of, blocks):
     assert r == X.OK
     assert shared(L, s, p, len(lens)) == X.OK and L.ph_log() == b"shared "
     out = np.zeros(1 << 16, np.int32)
-    n = L.ph_shared(out.ctypes.data_as(vp))
-    rows, most, top, groups, count = out[:5].tolist()
-    assert (groups, count) == (len(blocks), len(lens))
-    who = {g: [i for i in range(len(lens)) if of[i] == g and lens[i]] for g in range(groups)}
+    count, groups = len(lens), len(blocks)
+    n = L.ph_shared(out.ctypes.data_as(vp), count)
+    rows, most, top = out[:3].tolist()
+    who = {g: [i for i in range(count) if of[i] == g and lens[i]] for g in range(groups)}
     live = [g for g in who if len(who[g]) > 1 and blocks[g] > 0]
     size = {g: sum(lens[i] for i in who[g]) for g in live}
     assert rows == sum(size.values()) and most == max(size.values(), default=0)
     assert top == max((blocks[g] for g in live), default=0)
-    entry, pre, mine = (out[5 + a:5 + b].reshape(-1, 2).tolist() for a, b in
-                        ((0, 2 * rows), (2 * rows, 2 * (rows + groups)), (2 * (rows + groups), 2 * (rows + groups + count))))
+    mine = out[3:3 + 4 * count].reshape(-1, 4).tolist()
+    entry = out[3 + 4 * count:3 + 4 * count + 2 * rows].reshape(-1, 2).tolist()
     starts = np.concatenate([[0], np.cumsum(lens)])
     first = dict(zip(live, np.concatenate([[0], np.cumsum([size[g] for g in live])])))
-    for g in range(groups):
-        assert pre[g] == ([who[g][0], blocks[g]] if g in live else [0, 0])
     for i in range(count):
         if of[i] not in live:
             assert mine[i][0] == -1
             continue
-        assert mine[i][0] == of[i]
+        assert mine[i][:2] == [who[of[i]][0], blocks[of[i]]]
         for k in range(lens[i]):
-            assert entry[mine[i][1] + k] == [starts[i] + k, i]
+            assert entry[mine[i][2] + k] == [starts[i] + k, i]
     assert sorted(e[0] for e in entry) == sorted(int(starts[i]) + k for g in live for i in who[g] for k in range(lens[i]))
-    rest = out[5 + 2 * (rows + groups + count):n].reshape(-1, 4)
+    rest = out[3 + 4 * count + 2 * rows:n].reshape(-1, 5)
     heads = np.flatnonzero(rest[:, 0] == -1)
     assert list(rest[heads, 1]) == [8, 16, 32, 64, 128]
     for a, b in zip(heads, [*heads[1:], len(rest)]):
         tt = int(rest[a, 1])
-        want = [(int(first[g]), size[g], t0, g) for g in live for t0 in range(0, size[g], tt)]
+        want = [(int(first[g]), size[g], t0, who[g][0], blocks[g]) for g in live for t0 in range(0, size[g], tt)]
         assert list(map(tuple, rest[a + 1:b].tolist())) == want
     assert L.exn_prefixes_free(p) == X.OK and L.exn_seqs_free(s) == X.OK
 
