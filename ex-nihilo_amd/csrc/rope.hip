@@ -81,11 +81,11 @@ enum { PAIRED = 0, HALVES = 1, HALVES_ANY = 2 };   // pairs (2j, 2j + 1); (j, j 
 
 // One workgroup a tile of at most 8 tokens (and a share of their heads, blockIdx.y): the tile's cosines and
 // sines into LDS once for all heads, then G lanes a head, 8 dims each, as many heads at a time as 256 threads
-// hold and U of them in flight.  Bytes are what it costs: each value is read and written once.
+// hold, the next ones' loads ahead of the work.  Bytes are what it costs: each value is read and written once.
 template <int XT, int YT, int G, int WAY>
 __global__ void __launch_bounds__(256)
 k_rope_rows(RopeArgs A) {
-  constexpr int SLOTS = 256 / G, U = 2;
+  constexpr int SLOTS = 256 / G;
   __shared__ f32x2 cs[8][128];
   __shared__ float buf[WAY == HALVES_ANY ? 256 : 1][8];   // a lane's normed values
   const SeqTile T = A.tiles[blockIdx.x];
@@ -105,16 +105,15 @@ k_rope_rows(RopeArgs A) {
   }
   // unit u: row u / H of the tile, head u % H of q's and k's
   const int step = SLOTS * gridDim.y;
-  Eight<XT> x[U];
-  auto load = [&](int u, Eight<XT>& r) __attribute__((always_inline)) {
+  Eight<XT> x;
+  auto load = [&](int u) __attribute__((always_inline)) {
     if (u >= units || !has) return;
     const int i = over(u, A.magic), h = u - i * H;
     const RopeSide& t = A.t[h >= A.t[0].heads];
-    eight_load<XT>(r, t.x, (row0 + i) * t.ldx + (int64_t)(h >= A.t[0].heads ? h - A.t[0].heads : h) * A.hd + 8 * l);
+    eight_load<XT>(x, t.x, (row0 + i) * t.ldx + (int64_t)(h >= A.t[0].heads ? h - A.t[0].heads : h) * A.hd + 8 * l);
   };
   int u = blockIdx.y * SLOTS + slot;
-#pragma unroll
-  for (int k = 0; k < U; ++k) load(u + k * step, x[k]);
+  load(u);
   for (int z = tid; z < live * A.pairs; z += 256) {
     const int i = over(z, A.pair_magic), j = z - i * A.pairs;
     const int64_t p = A.pos ? A.pos[(row0 + i) * A.axes + A.axis[j]] : (int64_t)(A.lens ? A.lens[T.seq] : 0) + T.t0 + i;
@@ -122,74 +121,71 @@ k_rope_rows(RopeArgs A) {
   }
   __syncthreads();
   const int P = A.pairs;
-  for (int base = blockIdx.y * SLOTS; base < units; base += U * step) {
+  for (int base = blockIdx.y * SLOTS; base < units; base += step, u += step) {
+    const int at = min(u, units - 1), i = over(at, A.magic), h = at - i * H, side = h >= A.t[0].heads;
+    const RopeSide& t = A.t[side];
+    float f[8] = {};
+    if (has) eight_get<XT>(x, f);
+    load(u + step);
+    if (t.w) {
+      float ss = 0.f;
 #pragma unroll
-    for (int k = 0; k < U; ++k, u += step) {
-      const int at = min(u, units - 1), i = over(at, A.magic), h = at - i * H, side = h >= A.t[0].heads;
-      const RopeSide& t = A.t[side];
-      float f[8] = {};
-      if (has) eight_get<XT>(x[k], f);
-      load(u + U * step, x[k]);
-      if (t.w) {
-        float ss = 0.f;
+      for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+      ss = head_sum<G>(ss);
+      float eps = A.eps;
+      // squares past fp32's range, or under it with nothing else in the root: of values 2^96 times as small or large
+      const float by = ss >= 0x1p120f ? 0x1p-96f : ss < 0x1p-100f && eps < 0x1p-100f ? 0x1p96f : 1.f;
+      if (__ballot(by != 1.f)) {
+        ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+        for (int e = 0; e < 8; ++e) {
+          f[e] *= by;
+          ss += f[e] * f[e];
+        }
         ss = head_sum<G>(ss);
-        float eps = A.eps;
-        // squares past fp32's range, or under it with nothing else in the root: of values 2^96 times as small or large
-        const float by = ss >= 0x1p120f ? 0x1p-96f : ss < 0x1p-100f && eps < 0x1p-100f ? 0x1p96f : 1.f;
-        if (__ballot(by != 1.f)) {
-          ss = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] *= by;
-            ss += f[e] * f[e];
-          }
-          ss = head_sum<G>(ss);
-          eps = eps * by * by;
-        }
-        const float inv = rsqrtf(ss * A.per + eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= inv * (side ? wk[e] : wq[e]);
+        eps = eps * by * by;
       }
-      float y[8];
-      if constexpr (WAY == PAIRED) {
+      const float inv = rsqrtf(ss * A.per + eps);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x2 r = cs[i][min(4 * l + e, 127)];
-          const bool turn = 4 * l + e < P;
-          y[2 * e] = turn ? f[2 * e] * r[0] - f[2 * e + 1] * r[1] : f[2 * e];
-          y[2 * e + 1] = turn ? f[2 * e] * r[1] + f[2 * e + 1] * r[0] : f[2 * e + 1];
-        }
-      } else if constexpr (WAY == HALVES) {
-        const int lh = P / 8;
-        const bool second = l >= lh, turn = l < 2 * lh;
-        const int from = (tid & 63) + (!turn ? 0 : second ? -lh : lh), j0 = turn ? 8 * (second ? l - lh : l) : 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float o = __shfl(f[e], from, 64);
-          const f32x2 r = cs[i][j0 + e];
-          const float v = f[e] * r[0] + (second ? o : -o) * r[1];
-          y[e] = turn ? v : f[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) *(f32x4*)&buf[tid][e] = f32x4{f[e], f[e + 1], f[e + 2], f[e + 3]};
-        asm volatile("" ::: "memory");   // a head's lanes are one wave's, whose LDS accesses keep their order
-        const float* head = &buf[tid - l][0];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = 8 * l + e;
-          const bool second = d >= P, turn = d < 2 * P;
-          const float o = head[!turn ? d : second ? d - P : d + P];
-          const f32x2 r = cs[i][!turn ? 0 : second ? d - P : d];
-          y[e] = turn ? f[e] * r[0] + (second ? o : -o) * r[1] : f[e];
-        }
-        asm volatile("" ::: "memory");
-      }
-      if (u < units && has)
-        eight_store<YT>(t.y, (row0 + i) * t.ldy + (int64_t)(side ? h - A.t[0].heads : h) * A.hd + 8 * l, y);
+      for (int e = 0; e < 8; ++e) f[e] *= inv * (side ? wk[e] : wq[e]);
     }
+    float y[8];
+    if constexpr (WAY == PAIRED) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x2 r = cs[i][min(4 * l + e, 127)];
+        const bool turn = 4 * l + e < P;
+        y[2 * e] = turn ? f[2 * e] * r[0] - f[2 * e + 1] * r[1] : f[2 * e];
+        y[2 * e + 1] = turn ? f[2 * e] * r[1] + f[2 * e + 1] * r[0] : f[2 * e + 1];
+      }
+    } else if constexpr (WAY == HALVES) {
+      const int lh = P / 8;
+      const bool second = l >= lh, turn = l < 2 * lh;
+      const int from = (tid & 63) + (!turn ? 0 : second ? -lh : lh), j0 = turn ? 8 * (second ? l - lh : l) : 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float o = __shfl(f[e], from, 64);
+        const f32x2 r = cs[i][j0 + e];
+        const float v = f[e] * r[0] + (second ? o : -o) * r[1];
+        y[e] = turn ? v : f[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) *(f32x4*)&buf[tid][e] = f32x4{f[e], f[e + 1], f[e + 2], f[e + 3]};
+      asm volatile("" ::: "memory");   // a head's lanes are one wave's, whose LDS accesses keep their order
+      const float* head = &buf[tid - l][0];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = 8 * l + e;
+        const bool second = d >= P, turn = d < 2 * P;
+        const float o = head[!turn ? d : second ? d - P : d + P];
+        const f32x2 r = cs[i][!turn ? 0 : second ? d - P : d];
+        y[e] = turn ? f[e] * r[0] + (second ? o : -o) * r[1] : f[e];
+      }
+      asm volatile("" ::: "memory");
+    }
+    if (u < units && has)
+      eight_store<YT>(t.y, (row0 + i) * t.ldy + (int64_t)(side ? h - A.t[0].heads : h) * A.hd + 8 * l, y);
   }
 }
 
@@ -201,7 +197,7 @@ hipError_t rope_rows(hipStream_t s, const RopeArgs& args, int xt, int yt, int ha
   a.pair_magic = ((1ull << 32) + a.pairs - 1) / a.pairs;
   a.per = 1.f / a.hd;
   const int passes = ((longest < 8 ? longest : 8) * H + slots - 1) / slots;
-  int64_t y = 4096 / ntiles;
+  int64_t y = 2048 / ntiles;
   y = y < 1 ? 1 : y > passes ? passes : y;
   const dim3 grid((unsigned)ntiles, (unsigned)y);
   const int way = !halves ? PAIRED : a.pairs % 8 ? HALVES_ANY : HALVES;
