@@ -1777,7 +1777,7 @@ struct PrefixLds<HD, 0> : ChunkLds<HD, PREFIX> {};
 template <int HD>
 struct PrefixLds<HD, 3> : ChunkLds<HD, PREFIX> {};
 template <int BF, int HD, int WAY>
-__global__ void __launch_bounds__(256, WAY == 2 ? 1 : 2)
+__global__ void __launch_bounds__(256, 2)
 k_kv8_shared(Kv8Args P, Kv8Args O, uint32_t pw, uint32_t pgroups, uint32_t ogroups) {
   __shared__ union Lds {
     PrefixLds<HD, WAY> p;
@@ -1874,7 +1874,7 @@ struct PassWay {
 void split_pass(PassWay& w, double slots, int blocks, int least) {
   w.least = least;
   const int64_t s = w.groups > 0 ? (int64_t)(slots / w.groups) : 1, pays = (blocks + least - 1) / least;
-  w.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(s, pays), 128));
+  w.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(s, pays), 64));
 }
 struct SharedWay {
   PassWay pre, own;
@@ -1901,7 +1901,7 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
   const int64_t most = (int64_t)sh.most * hh;
   if (most <= 32) {
     w.pre.way = most <= 16 ? 1 : 2;
-    const bool two = w.pre.way == 2 && sh.most <= 16 && blocks < 1000;
+    const bool two = w.pre.way == 2 && sh.most <= 16 && blocks < 400;
     if (two) w.pre.way = 1;
     rows_way(w.pre, two ? 16 / sh.most : hh, sh.most * (two ? 16 / sh.most : hh), sh.ntiles);
   } else {
@@ -1915,8 +1915,7 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
   split_pass(w.own, places, own, 8);
   double slots;
   if (w.pre.way % 3) {
-    const int all = w.pre.way == 1 ? places : places / 2;
-    slots = std::max<double>(all - w.own.groups, all / 2);
+    slots = 256;
   } else {
     // of the time that each pass would take with all CUs: 1.5 us a block of a prefix's tile, and a quarter of the own
     // blocks that there may be at 5 TB/s
