@@ -463,14 +463,16 @@ def rope_freqs(dims, base, scaling=ROPE_PLAIN, factor=1.0, kept=1.0, low=0.0, hi
 
 class Rope:
     """A rotary (exn_rope_create): FREQS radians a token, of dims j and j + pairs (ROPE_HALF) or 2j and 2j + 1
-    (ROPE_PAIRS); AXIS, the position that each pair turns by, or None for one of them; AMP, a factor of all."""
+    (ROPE_PAIRS); AXIS, the position that each pair turns by, of AXES of them (as many as AXIS names), or None for
+    one; AMP, a factor of all."""
 
-    def __init__(self, ctx: Context, freqs, layout=ROPE_HALF, axis=None, amp=1.0):
+    def __init__(self, ctx: Context, freqs, layout=ROPE_HALF, axis=None, amp=1.0, axes=None):
         f = np.ascontiguousarray(freqs, dtype=np.float64).reshape(-1)
         a = None if axis is None else np.ascontiguousarray(axis, dtype=np.int32).reshape(-1)
         if a is not None and len(a) != len(f):
             raise ExnError(EINVAL, "rotary: %d axes for %d pairs" % (len(a), len(f)))
-        axes = 1 if a is None or not len(a) else int(a.max()) + 1
+        if axes is None:
+            axes = 1 if a is None or not len(a) else int(a.max()) + 1
         h = vp()
         call("exn_rope_create", ctx.h, ptr(f), len(f), layout, None if a is None else ptr(a), axes, amp, ctypes.byref(h))
         self.ctx, self.h, self.pairs, self.axes = ctx, h, len(f), axes
