@@ -239,7 +239,7 @@ def prepare(case, seed):
             freqs = X.rope_freqs(2 * c["pairs"], BASE, getattr(X, "ROPE_" + c["scaling"].upper()), FACTOR, KEPT, LOW, HIGH)
             st["seqs"] = X.Seqs(_ctx(), lens)
             st["rope"] = X.Rope(_ctx(), freqs, X.ROPE_PAIRS if c["layout"] == "pairs" else X.ROPE_HALF,
-                                _axis(c) if c["axes"] > 1 else None, _amp(c))
+                                _axis(c) if c["axes"] > 1 else None, _amp(c), c["axes"])
         return st
     new = c["new"]
     before, (tokens, of) = _before(c), _prefixes(c)
