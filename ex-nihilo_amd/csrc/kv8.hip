@@ -1765,8 +1765,14 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
 // several's, whatever sequence each is of), each sequence's other blocks as ever (OWN); both leave sums
 // relative to a reference of their own, which meet here:
 //   m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m) / l.
-// Which blocks those are is found out on the device (kv8_alike): the plan of prefixes is a hint, and what
-// comes out is kv8_attend's answer whatever the tables hold.
+// Which blocks those are is found out on the device (Kv8Own): the plan of prefixes is a hint, and what comes
+// out is kv8_attend's answer whatever the tables hold.
+//
+// 64 x 1 token, 60..2000 of their own after 8192 (8 heads of 128, groups of 4, bf16): 48.8 us, kv8_attend 134;
+// its bytes would take 18.7: the prefix's products and the own blocks take turns on the CUs, whose places (two
+// workgroups each) one launch's 128 prefix workgroups and 512 others fill unevenly.  8 x 1 after 131008, fp16:
+// 61 us (kernel 56, 4.9 TB/s; join 7), kv8_attend 288.  16 x 1 after 1088: 15.7 us, 19.2: five loads that wait for
+// each other, two blocks, the sums out and in again.
 
 // Both passes in one launch: PW workgroups of the prefixes', which take their rows as WAY says (0, 3: chunk_rows, tiles
 // of 64 and 128 rows; 1, 2: few_rows with as many row tiles), then the sequences' own
@@ -1798,6 +1804,8 @@ struct Kv8Meet {
   const float *part, *ml;   // the prefixes' sums
   int64_t n;
 };
+// The sums of a sequence's own splits and of its prefix's of each row and head, in a fixed order, one pass over them: HD / 4
+// threads take one's dims in each of SH shares of the splits, then the shares are summed
 template <int HD, int SH>
 __global__ void __launch_bounds__(256)
 k_kv8_meet(Kv8Meet M) {
@@ -1865,65 +1873,69 @@ k_kv8_meet(Kv8Meet M) {
 
 namespace {
 
-// one of attend_shared's passes: how its rows are taken (k_kv8_shared), and into how many splits their blocks
+// one of attend_shared's passes: how its rows are taken (k_kv8_shared's WAY), and into how many splits their blocks
 struct PassWay {
   int way, z, hh, chunks, splits, least;
   int64_t groups;   // workgroups a split
 };
-// as many splits as SLOTS workgroups are, none of less than LEAST blocks
-void split_pass(PassWay& w, double slots, int blocks, int least) {
+// HH heads a workgroup, in tiles that hold TOKENS (or in the largest)
+PassWay pass_rows(int way, int hh, int tokens, int group, int kv_heads, const int64_t* ntiles) {
+  PassWay w{way, 0, hh, (group + hh - 1) / hh, 1, 1, 0};
+  while ((SEQ_TT0 << w.z) < tokens && w.z + 1 < SEQ_TTS) ++w.z;
+  w.groups = ntiles[w.z] * w.chunks * kv_heads;
+  return w;
+}
+// As many splits as SLOTS workgroups are, none of less than LEAST blocks; at most 64, whose sums the join reads (2
+// x 1 after 32768, 16 heads over 1: 25.5, at most 128 32.9, 16 27.9; 4 x 1: 28.0, 30.7, 49.0)
+void pass_splits(PassWay& w, double slots, int blocks, int least) {
   w.least = least;
   const int64_t s = w.groups > 0 ? (int64_t)(slots / w.groups) : 1, pays = (blocks + least - 1) / least;
   w.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(s, pays), 64));
 }
 struct SharedWay {
-  PassWay pre, own;
   bool pays;
-  int64_t pre_each, own_each, notes, floats;   // of a split of either; of the notes; in all
+  PassWay pre, own;
+  int64_t pre_each, own_each, notes, floats;   // floats of a split of either, of the notes, in all
 };
+// The rules' times are as kv8_way's, of one new token a sequence in bf16 with 12 to 200 of its own, unless said.
 SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, int kv_heads, int head_dim, int cols,
                      const int64_t* ntiles) {
-  SharedWay w;
-  const int group = heads / kv_heads, blocks = sh.blocks < cols ? sh.blocks : cols;
-  w.pays = sh.rows > 0 && longest * (group < 16 ? group : 16) <= 16 && blocks > 16 &&
-           sh.saved >= (sh.seqs < 4 ? 384 : 112);
+  SharedWay w{};
+  const int group = heads / kv_heads, h16 = group < 16 ? group : 16, h8 = group < 8 ? group : 8;
+  const int blocks = sh.blocks < cols ? sh.blocks : cols, own = cols > sh.fewest ? cols - sh.fewest : 1;
+  // Where reading a prefix once saves more than a second pass and the join take: for sequences of at most 16 rows a
+  // key/value head (of more, each fills tiles of its own: 8 x 76 tokens after 1088 42, shared 56; 32 x 32 after 4096
+  // 105, 121), prefixes past 16 blocks (up to there kv8_attend is one launch: 64 x 1 after 640 19.5, shared 24.8), and
+  // so many blocks read again (8 x 1 after 1088, 119 of them: 17.2, shared 14.4; 4 after 2048, 96: 13.9, 15.4; 2
+  // after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0, 26.3)
+  w.pays = sh.rows > 0 && longest * h16 <= 16 && blocks > 16 && sh.saved >= (sh.seqs < 4 ? 384 : 112);
   if (!w.pays) return w;
-  auto rows_way = [&](PassWay& p, int hh, int tile, const int64_t* n) {
-    p.hh = hh;
-    while ((SEQ_TT0 << p.z) * hh < tile && p.z + 1 < SEQ_TTS) ++p.z;
-    p.chunks = (group + hh - 1) / hh;
-    p.groups = n[p.z] * p.chunks * kv_heads;
-  };
-  const int hh = group < 16 ? group : 16;
-  w.own.way = 1;
-  w.own.z = w.pre.z = 0;
-  rows_way(w.own, hh, longest * hh, ntiles);
-  const int64_t most = (int64_t)sh.most * hh;
-  if (most <= 32) {
-    w.pre.way = most <= 16 ? 1 : 2;
-    const bool two = w.pre.way == 2 && sh.most <= 16 && blocks < 400;
-    if (two) w.pre.way = 1;
-    rows_way(w.pre, two ? 16 / sh.most : hh, sh.most * (two ? 16 / sh.most : hh), sh.ntiles);
+  w.own = pass_rows(1, h16, longest, group, kv_heads, ntiles);
+  // a sequence's own blocks are split as far as there are places for the workgroups
+  pass_splits(w.own, 256 * (head_dim == 64 ? 4 : 2), own, 8);
+  if ((int64_t)sh.most * h16 <= 32) {
+    // The bytes are the cost: few_rows.  17 to 32 rows are two row tiles of a workgroup (8 x 1 after 131008 58.7), or
+    // in shorter prefixes workgroups of half the heads, whose blocks' second reading the L2 has (8 x 1 after 8192
+    // 17.2, two row tiles 20.1; after 32768 30.3, 27.9)
+    const bool half = sh.most * h16 > 16 && sh.most <= 16 && blocks < 400;
+    w.pre = pass_rows(sh.most * h16 <= 16 || half ? 1 : 2, half ? 16 / sh.most : h16, sh.most, group, kv_heads, sh.ntiles);
+    // one workgroup a CU, the other place is the sequences' (8 x 1 after 131008: 58.7, 192 in all 67.6, 320 74.3)
+    pass_splits(w.pre, 256, blocks, 4);
   } else {
-    const int h8 = group < 8 ? group : 8;
-    w.pre.way = (int64_t)sh.most * h8 <= 64 ? 0 : 3;
-    while (w.pre.z + 1 < SEQ_TTS && (SEQ_TT0 << (w.pre.z + 1)) * h8 <= (w.pre.way ? 128 : 64)) ++w.pre.z;
-    rows_way(w.pre, h8, 0, sh.ntiles);
-  }
-  const int own = cols > sh.fewest ? cols - sh.fewest : 1;
-  const int places = 256 * (head_dim == 64 ? 4 : 2);   // of few_rows with one row tile that the chip holds
-  split_pass(w.own, places, own, 8);
-  double slots;
-  if (w.pre.way % 3) {
-    slots = 256;
-  } else {
-    // of the time that each pass would take with all CUs: 1.5 us a block of a prefix's tile, and a quarter of the own
-    // blocks that there may be at 5 TB/s
+    // The products are: chunk_rows, tiles of 128 rows, up to 64 rows of 64 (a wave half of a block's keys: 16 x 1 after
+    // 131008 105, with half of the waves idle 121)
+    const int way = (int64_t)sh.most * h8 <= 64 ? 0 : 3;
+    int tokens = SEQ_TT0;
+    while (2 * tokens * h8 <= (way ? 128 : 64) && tokens < (SEQ_TT0 << (SEQ_TTS - 1))) tokens *= 2;
+    w.pre = pass_rows(way, h8, tokens, group, kv_heads, sh.ntiles);
+    // The share of the CUs, a workgroup each, that this pass is of both, where each would take so long with all of them:
+    // 1.5 us a block of a tile, a quarter of the own blocks that there may be at 5 TB/s (64 x 1 after 8192, 60..2000 of
+    // their own: 128 workgroups 48.4, 64 69.5, 256 53.1, 512 62.9; 12..200: 128 44, 256 33.5); two each for long ones (64
+    // x 1 after 65536: 106, one each 125)
     const double units = w.pre.groups * (double)blocks;
     const double a = units * 1.5 / 256, b = w.own.groups * (double)own / 4 * (head_dim * 128) / 5e6;
-    slots = a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1;
+    pass_splits(w.pre, a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1, blocks, 2);
   }
-  split_pass(w.pre, slots, blocks, w.pre.way % 3 ? 4 : 2);
   w.pre_each = sh.rows * heads * (head_dim + 2);
   w.own_each = rows * heads * (head_dim + 2);
   w.notes = 4 * ntiles[w.own.z];
@@ -1944,7 +1956,8 @@ hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* 
                              int64_t ldq, float scale, uint16_t* out, int obf, int64_t ldo, float* part, int64_t part_cap) {
   if (ntiles[0] == 0) return hipSuccess;
   SharedWay w = shared_way(rows, longest, sh, heads, c.kv_heads, c.head_dim, c.cols, ntiles);
-  if (!w.pays || part_cap < w.notes + w.pre_each + w.own_each)
+  if (!w.pays || part_cap < w.notes + w.pre_each + w.own_each ||
+      w.pre.groups * w.pre.splits + w.own.groups * w.own.splits > WG256_MAX)
     return kv8_attend(s, c, tiles, ntiles, rows, longest, heads, q, ldq, scale, out, obf, ldo, part, part_cap);
   if (w.floats > part_cap) {   // fewer splits, the prefixes' first to keep theirs
     const int64_t spare = part_cap - w.notes - w.pre_each - w.own_each, p = 1 + spare / w.pre_each;
@@ -1991,15 +2004,14 @@ hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* 
   a.notes = nullptr;
   b.psplits = a.splits;
   b.pleast = a.least;
-  const int64_t pw = w.pre.groups * a.splits, all = pw + w.own.groups * b.splits;
-  if (all > WG256_MAX) return hipErrorInvalidConfiguration;
+  const int64_t pw = w.pre.groups * a.splits;
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
   typedef std::integral_constant<int, 64> I64;
   typedef std::integral_constant<int, 128> I128;
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)all), dim3(256), 0, s, a, b, (uint32_t)pw, (uint32_t)w.pre.groups,
-                       (uint32_t)w.own.groups);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(pw + w.own.groups * b.splits)), dim3(256), 0, s, a, b, (uint32_t)pw,
+                       (uint32_t)w.pre.groups, (uint32_t)w.own.groups);
   };
   auto ways = [&](auto bf, auto hd) {
     constexpr int BF = decltype(bf)::value, HD = decltype(hd)::value;

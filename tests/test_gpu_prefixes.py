@@ -483,3 +483,52 @@ def test_captured_steps_with_tables_that_change(ctx):
         X.call("exn_set_stream", ctx.h, None)
         hip.hipStreamSynchronize(stream)
         hip.hipStreamDestroy(stream)
+
+
+def test_two_streams_at_once(ctx):
+    """One plan and its prefixes, one cache, in calls of two contexts that overlap: scratch and results of their own."""
+    rng = np.random.default_rng(35)
+    kv, hd, heads, n = 2, 128, 8, 24
+    of, blocks = [0] * n, [40]
+    m, d = alike(ctx, "fp16", kv, hd, of, blocks, [2560 + 17 * i for i in range(n)], rng)
+    say("two streams")
+    s = X.Seqs(ctx, [1] * n)
+    p = X.Prefixes(ctx, s, of, blocks)
+    floats = X.attend_shared_part(s, p, heads, kv, hd, m.cols)
+    with X.Context(0) as other:
+        runs = []
+        for c in (ctx, other):
+            qb, q = normal(rng, (n, heads, hd), "fp16")
+            runs.append((c, X.DevBuf.of(c, qb), X.DevBuf(c, (floats,), np.float32), X.DevBuf(c, (n, heads, hd), np.uint16), q))
+        for _ in range(20):
+            for c, dq, part, o, _q in runs:
+                X.attend_shared(c, d.h, s, p, heads, dq.h, heads * hd, 0.09, o.h, X.DT_BF16, heads * hd, part.h, floats)
+        for c, dq, part, o, q in runs:
+            want, tol = m.attend(q, [1] * n, 0.09, "bf16")
+            assert off(pm.value(o.get(), "bf16"), want, tol) <= 1
+        for b in runs[1][1:4]:
+            b.free()
+
+
+def test_the_same_page_many_times(ctx):
+    """Tables that name one page again and again, in the prefix and after it."""
+    rng = np.random.default_rng(36)
+    say("same page")
+    n, of, blocks = 9, [0] * 9, [20]
+    m, d = alike(ctx, "bf16", 2, 64, of, blocks, [20 * 64 + 1 + 64 * (i % 3) for i in range(n)], rng)
+    m.table[:, :20] = m.table[0, 0]
+    m.table[4, :22] = m.table[4, 21]
+    d.b["table"].upload(m.table)
+    assert step(ctx, m, d, of, blocks, [1] * n, 4, "bf16", rng) <= 1
+
+
+def test_plans_of_many_sequences(ctx):
+    """Thousands of sequences over one prefix, and as many prefixes as sequences allow."""
+    rng = np.random.default_rng(37)
+    say("many sequences")
+    n, kv, hd = 1500, 1, 64
+    of = [0] * 700 + [1 + i % 80 for i in range(n - 700)]
+    blocks = [17] + [18] * 80
+    before = [64 * blocks[g] + i % 5 for i, g in enumerate(of)]
+    m, d = alike(ctx, "fp16", kv, hd, of, blocks, before, rng, cols=20)
+    assert step(ctx, m, d, of, blocks, [1] * n, 1, "fp16", rng) <= 1
