@@ -22,8 +22,8 @@ int exn_rope_freqs(int dims, double base, int scaling, double factor, double kep
   double first = 0, last = 0;
   if (scaling == EXN_ROPE_INDEX) {
     auto at = [&](double turns) { return dims * std::log(kept / (2 * kPi * turns)) / (2 * std::log(base)); };
-    first = std::max(std::floor(at(high)), 0.0);
-    last = std::min(std::ceil(at(low)), dims - 1.0);
+    first = std::min(std::max(std::floor(at(high)), 0.0), dims - 1.0);
+    last = std::min(std::max(std::ceil(at(low)), 0.0), dims - 1.0);
     if (last == first) last += 1e-3;   // a step
   }
   for (int j = 0; j < dims / 2; ++j) {

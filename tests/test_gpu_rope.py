@@ -120,6 +120,21 @@ def test_axes_amplitude_and_heads(ctx, layout):
     assert run(ctx, [3, 9], 1024, 1024, 64, freqs[:32], layout, "fp16", "bf16", rng) <= 1
 
 
+def test_more_axes_than_are_named(ctx):
+    """Positions may have axes by which no pair turns: their rows are as far apart as the rotary says."""
+    rng = np.random.default_rng(47)
+    say("axes that no pair names")
+    pos = rng.integers(-50, 900, (21, 3)).astype(np.int32)
+    freqs = X.rope_freqs(8, 1e4)
+    for axis in (None, [1, 0, 1, 0]):
+        b, x = held(rng.standard_normal((21, 4, 64)), "fp16")
+        s, r = X.Seqs(ctx, [20, 1]), X.Rope(ctx, freqs, X.ROPE_HALF, axis, axes=3)
+        d, dp = X.DevBuf.of(ctx, b), X.DevBuf.of(ctx, pos)
+        X.rope_rows(ctx, r, s, 64, X.DT_F16, X.DT_F16, (4, d.h, 256, None, d.h, 256), pos=dp.h)
+        want, tol = pr.rope_rows(x, None, 0.0, pos, freqs, axis, 0, 1.0, "fp16")
+        assert off(pm.value(d.get(), "fp16"), want, tol) <= 1
+
+
 @pytest.mark.parametrize("far", [131071, 10 ** 6, (1 << 31) - 40, -(1 << 31)])
 def test_far_positions(ctx, far):
     """Angles of far positions, to fp32's own rounding."""

@@ -225,6 +225,13 @@ def test_frequencies_of_a_step(L):
     assert np.allclose(got, [f[0], *(x / 2 for x in f[1:])], rtol=1e-13)
 
 
+def test_frequencies_with_the_ramp_past_an_end(L):
+    """Every pair turns more than HIGH times, or fewer than LOW: all as they are, or all but the first divided."""
+    f = plain(64, 10.0)
+    assert np.allclose(X.rope_freqs(64, 10.0, X.ROPE_INDEX, 4.0, 1e6, 1.0, 32.0), f, rtol=1e-13)
+    assert np.allclose(X.rope_freqs(64, 10.0, X.ROPE_INDEX, 4.0, 1e-3, 1.0, 32.0), [f[0], *(x / 4 for x in f[1:])], rtol=1e-13)
+
+
 def test_frequency_refusals(L):
     f = np.zeros(128)
     p = f.ctypes.data_as(vp)
