@@ -82,6 +82,9 @@ enum { PAIRED = 0, HALVES = 1, HALVES_ANY = 2 };   // pairs (2j, 2j + 1); (j, j 
 // One workgroup a tile of at most 8 tokens (and a share of their heads, blockIdx.y): the tile's cosines and
 // sines into LDS once for all heads, then G lanes a head, 8 dims each, as many heads at a time as 256 threads
 // hold, the next ones' loads ahead of the work.  Bytes are what it costs: each value is read and written once.
+// 2 documents of 8192 tokens (40 heads of 128, bf16) 73.6 us, 4.6 TB/s of what a copy's 5.2 allow; 4 x 1100..1180 from
+// fp32 to fp16 32.1 us, 4.4 TB/s; one token of 4 sequences 3.8 us, a launch.  Two units ahead, or 4096 workgroups for 2048
+// of a short call (a tile's angles made once in each), took longer: 16 x 21..257 12.6 us, so 9.7.
 template <int XT, int YT, int G, int WAY>
 __global__ void __launch_bounds__(256)
 k_rope_rows(RopeArgs A) {
@@ -197,7 +200,7 @@ hipError_t rope_rows(hipStream_t s, const RopeArgs& args, int xt, int yt, int ha
   a.pair_magic = ((1ull << 32) + a.pairs - 1) / a.pairs;
   a.per = 1.f / a.hd;
   const int passes = ((longest < 8 ? longest : 8) * H + slots - 1) / slots;
-  int64_t y = 2048 / ntiles;
+  int64_t y = 2048 / ntiles;   // workgroups that share a tile's heads
   y = y < 1 ? 1 : y > passes ? passes : y;
   const dim3 grid((unsigned)ntiles, (unsigned)y);
   const int way = !halves ? PAIRED : a.pairs % 8 ? HALVES_ANY : HALVES;
