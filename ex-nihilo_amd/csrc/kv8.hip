@@ -1072,8 +1072,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // One row by a whole wave, blocks [lo, hi), nothing that it does not see multiplied: for rows whose
 // sums came out not finite (a hidden value of the tail that is not, times a weight of zero)
-template <int BF, int HD>
-__device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int total, int lim, const uint16_t* q,
+template <int BF, int HD, int MODE>
+__device__ void kv8_row(const Kv8& c, int seq, const Kv8Own& own, int kvh, int lo, int hi, int total, int lim, const uint16_t* q,
                         float scale, float* m_, float* l_, float* o) {
   const int lane = threadIdx.x & 63;
   float m = -INFINITY, l = 0.f;
@@ -1081,7 +1081,8 @@ __device__ void kv8_row(const Kv8& c, int seq, int kvh, int lo, int hi, int tota
 #pragma unroll 1
   for (int b = lo; b < hi && b * 64 <= lim; ++b) {
     const bool full = b * 64 + 64 <= total;
-    const int64_t page = full ? kv8_page(c, seq, b) : 0;
+    int64_t page = full ? kv8_page(c, seq, b) : 0;
+    if (MODE == OWN && b < own.nb) page = kv8_untaken(c, seq, own, b, (int)page);
     if (page < 0) continue;
     const int64_t ph = (page * c.kv_heads + kvh), th = ((int64_t)seq * c.kv_heads + kvh) * 64 * HD;
     const float kd = full ? c.scales[ph * 2] : 1.f, vd = full ? c.scales[ph * 2 + 1] : 1.f;
@@ -1139,8 +1140,14 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
   const int total = MODE == PREFIX ? base : kv8_total(c, base, T.len), nfull = total / 64;
   const int live = min(A.tt, T.len - T.t0), heads = min(A.hh, A.group - chunk * A.hh);
   int b0, b1, active;   // the blocks taken here; the splits
+  Kv8Own own{};         // OWN: what the sequence's prefix takes
   if constexpr (MODE == PREFIX) {
     active = kv8_split(nfull, A.splits, A.least, by, &b0, &b1);
+  } else if constexpr (MODE == OWN) {
+    const int32x4 of = A.of[T.seq];
+    own = kv8_own(A, of, base);
+    active = kv8_own_split(A, kv8_own_from(c, T.seq, own), (min(base + T.t0 + live, total) + 63) / 64, by, &b0, &b1);
+    if (by == 0 && hc == 0 && tid == 0) kv8_note(A, of, bx / per, T.t0, active);
   } else {
     active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, by, &b0, &b1));
   }
@@ -1150,7 +1157,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
   const bool mine = tok < live && head < heads;
   const int ctok = min(tok, live - 1), chead = kvh * A.group + chunk * A.hh + min(head, heads - 1);
   // waves without a row do their part of each block's way into LDS only
-  const bool idle = MODE == PREFIX && (int)(rw * 32 * A.magic >> 16) >= live;
+  const bool idle = MODE != ALONE && (int)(rw * 32 * A.magic >> 16) >= live;
   int lim, minlim;
   s16x8 qf[NS];   // Q^T as the B operand: this lane's row, dims 16s + 8 hi ..
   auto rows_here = [&]() __attribute__((always_inline)) {
@@ -1176,6 +1183,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
   float kds = 1.f, vds = 1.f;
   auto look = [&](int b) __attribute__((always_inline)) {
     int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, T.seq, b + lane) : -1;
+    if (MODE == OWN && b < own.nb) p = kv8_untaken(c, T.seq, own, b + lane, (int)p);
     pages = (int)p;
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
@@ -1492,7 +1500,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
 
   float la = lrun, lb = lrun;
   xswap32(la, lb);
-  const bool parts = MODE == PREFIX || active > 1;
+  const bool parts = MODE != ALONE || active > 1;
   const float sum = (la + lb) * (1.f / LIFT2), mul = parts ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   float zero[4] = {sum * 0.f};
   const int64_t rowhead = (int64_t)(T.row0 + T.t0 + tok) * A.heads + chead, n = MODE == ALONE ? A.rows * A.heads : A.n;
@@ -1535,7 +1543,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
     float m, l, y[HD / 64];
     const int64_t qrow = MODE == PREFIX ? A.entry[2 * at] : at;
     const int sees = MODE == PREFIX ? pfx.run[pfx.head[rt]] * 64 - 1 : min(base + T.t0 + rt, total - 1);
-    kv8_row<BF, HD>(c, T.seq, kvh, b0, b1, total, sees, A.q + qrow * A.ldq + rh * HD, A.scale, &m, &l, y);
+    kv8_row<BF, HD, MODE>(c, T.seq, own, kvh, b0, b1, total, sees, A.q + qrow * A.ldq + rh * HD, A.scale, &m, &l, y);
     const int64_t slot = (int64_t)by * n + at * A.heads + rh;
     for (int z = 0; z < HD / 64; ++z) {
       const float w = parts ? y[z] : l == 0.f ? 0.f : y[z] / l;
@@ -1772,27 +1780,37 @@ hipError_t kv8_attend(hipStream_t s, const Kv8& c, const SeqTile* const* tiles, 
 // its bytes would take 18.7: the prefix's products and the own blocks take turns on the CUs, whose places (two
 // workgroups each) one launch's 128 prefix workgroups and 512 others fill unevenly.  8 x 1 after 131008, fp16:
 // 61 us (kernel 56, 4.9 TB/s; join 7), kv8_attend 288.  16 x 1 after 1088: 15.7 us, 19.2: five loads that wait for
-// each other, two blocks, the sums out and in again.
+// each other, two blocks, the sums out and in again.  32 x 9 tokens, 12..200 of their own after 8192: 76 us, 164.
 
 // Both passes in one launch: PW workgroups of the prefixes', which take their rows as WAY says (0, 3: chunk_rows, tiles
-// of 64 and 128 rows; 1, 2: few_rows with as many row tiles), then the sequences' own
+// of 64 and 128 rows; 1, 2: few_rows with as many row tiles), then the sequences' own by few_rows; WAY 4: tiles of 128 rows
+// and of 64
 template <int HD, int WAY>
 struct PrefixLds : FewLds<HD, WAY, PREFIX> {};
 template <int HD>
 struct PrefixLds<HD, 0> : ChunkLds<HD, PREFIX> {};
 template <int HD>
 struct PrefixLds<HD, 3> : ChunkLds<HD, PREFIX> {};
+template <int HD>
+struct PrefixLds<HD, 4> : ChunkLds<HD, PREFIX> {};
+template <int HD, int WAY>
+struct OwnLds : FewLds<HD, 1, OWN> {};
+template <int HD>
+struct OwnLds<HD, 4> : ChunkLds<HD, OWN> {};
 template <int BF, int HD, int WAY>
 __global__ void __launch_bounds__(256, 2)
 k_kv8_shared(Kv8Args P, Kv8Args O, uint32_t pw, uint32_t pgroups, uint32_t ogroups) {
   __shared__ union Lds {
     PrefixLds<HD, WAY> p;
-    FewLds<HD, 1, OWN> o;
+    OwnLds<HD, WAY> o;
   } lds;
   if (blockIdx.x >= pw) {
     const uint32_t i = blockIdx.x - pw;
-    few_rows<BF, HD, 1, OWN>(O, lds.o, i % ogroups, i / ogroups);
-  } else if constexpr (WAY % 3 == 0) {
+    if constexpr (WAY == 4)
+      chunk_rows<BF, HD, OWN, 2>(O, lds.o, i % ogroups, i / ogroups);
+    else
+      few_rows<BF, HD, 1, OWN>(O, lds.o, i % ogroups, i / ogroups);
+  } else if constexpr (WAY == 0 || WAY > 2) {
     chunk_rows<BF, HD, PREFIX, WAY == 0 ? 2 : 1>(P, lds.p, blockIdx.x % pgroups, blockIdx.x / pgroups);
   } else {
     few_rows<BF, HD, WAY, PREFIX>(P, lds.p, blockIdx.x % pgroups, blockIdx.x / pgroups);
@@ -1903,17 +1921,25 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
   SharedWay w{};
   const int group = heads / kv_heads, h16 = group < 16 ? group : 16, h8 = group < 8 ? group : 8;
   const int blocks = sh.blocks < cols ? sh.blocks : cols, own = cols > sh.fewest ? cols - sh.fewest : 1;
-  // Where reading a prefix once saves more than a second pass and the join take: for sequences of at most 16 rows a
-  // key/value head (of more, each fills tiles of its own: 8 x 76 tokens after 1088 42, shared 56; 32 x 32 after 4096
-  // 105, 121), prefixes past 16 blocks (up to there kv8_attend is one launch: 64 x 1 after 640 19.5, shared 24.8), and
-  // so many blocks read again (8 x 1 after 1088, 119 of them: 17.2, shared 14.4; 4 after 2048, 96: 13.9, 15.4; 2
-  // after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0, 26.3)
-  w.pays = sh.rows > 0 && longest * h16 <= 16 && blocks > 16 && sh.saved >= (sh.seqs < 4 ? 384 : 112);
+  // Where reading a prefix once saves more than a second pass and the join take: prefixes past 16 blocks (up to there
+  // kv8_attend is one launch: 64 x 1 after 640 19.5, shared 24.8), and so many blocks read again (8 x 1 after 1088, 119 of
+  // them: 17.2, shared 14.4; 4 after 2048, 96: 13.9, 15.4; 2 after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0, 26.3).
+  // Sequences of 17 to 64 rows a key/value head leave tiles of their own half empty and need more (12..200 of their own:
+  // 4 x 8 after 4096, 192: 28.8, 25.6, 4 x 16: 30.8, 31.9; 4 x 16 after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968:
+  // 164, 76; where kv8_attend's workgroups fill the chip just so it is ahead still, 32 x 8 after 2048: 32.9, 37.6); more
+  // rows fill them (8 x 76 tokens after 1088 42, shared 56; 32 x 32 after 4096 105, 121)
+  const bool few = longest * h16 <= 16;
+  w.pays = sh.rows > 0 && longest * h8 <= 64 && blocks > 16 && sh.saved >= (!few || sh.seqs < 4 ? 384 : 112);
   if (!w.pays) return w;
-  w.own = pass_rows(1, h16, longest, group, kv_heads, ntiles);
+  auto tokens = [&](int rows) {   // that tiles of ROWS rows hold
+    int n = SEQ_TT0;
+    while (2 * n * h8 <= rows && n < (SEQ_TT0 << (SEQ_TTS - 1))) n *= 2;
+    return n;
+  };
+  w.own = few ? pass_rows(1, h16, longest, group, kv_heads, ntiles) : pass_rows(0, h8, tokens(64), group, kv_heads, ntiles);
   // a sequence's own blocks are split as far as there are places for the workgroups
   pass_splits(w.own, 256 * (head_dim == 64 ? 4 : 2), own, 8);
-  if ((int64_t)sh.most * h16 <= 32) {
+  if (few && (int64_t)sh.most * h16 <= 32) {
     // The bytes are the cost: few_rows.  17 to 32 rows are two row tiles of a workgroup (8 x 1 after 131008 58.7), or
     // in shorter prefixes workgroups of half the heads, whose blocks' second reading the L2 has (8 x 1 after 8192
     // 17.2, two row tiles 20.1; after 32768 30.3, 27.9)
@@ -1924,17 +1950,15 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
   } else {
     // The products are: chunk_rows, tiles of 128 rows, up to 64 rows of 64 (a wave half of a block's keys: 16 x 1 after
     // 131008 105, with half of the waves idle 121)
-    const int way = (int64_t)sh.most * h8 <= 64 ? 0 : 3;
-    int tokens = SEQ_TT0;
-    while (2 * tokens * h8 <= (way ? 128 : 64) && tokens < (SEQ_TT0 << (SEQ_TTS - 1))) tokens *= 2;
-    w.pre = pass_rows(way, h8, tokens, group, kv_heads, sh.ntiles);
+    const int way = !few ? 4 : (int64_t)sh.most * h8 <= 64 ? 0 : 3;
+    w.pre = pass_rows(way, h8, tokens(way ? 128 : 64), group, kv_heads, sh.ntiles);
     // The share of the CUs, a workgroup each, that this pass is of both, where each would take so long with all of them:
     // 1.5 us a block of a tile, a quarter of the own blocks that there may be at 5 TB/s (64 x 1 after 8192, 60..2000 of
     // their own: 128 workgroups 48.4, 64 69.5, 256 53.1, 512 62.9; 12..200: 128 44, 256 33.5); two each for long ones (64
     // x 1 after 65536: 106, one each 125)
     const double units = w.pre.groups * (double)blocks;
     const double a = units * 1.5 / 256, b = w.own.groups * (double)own / 4 * (head_dim * 128) / 5e6;
-    pass_splits(w.pre, a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1, blocks, 2);
+    pass_splits(w.pre, std::min(512., a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1), blocks, 2);
   }
   w.pre_each = sh.rows * heads * (head_dim + 2);
   w.own_each = rows * heads * (head_dim + 2);
@@ -2018,7 +2042,8 @@ hipError_t kv8_attend_shared(hipStream_t s, const Kv8& c, const SeqTile* const* 
     w.pre.way == 0   ? go(k_kv8_shared<BF, HD, 0>)
     : w.pre.way == 1 ? go(k_kv8_shared<BF, HD, 1>)
     : w.pre.way == 2 ? go(k_kv8_shared<BF, HD, 2>)
-                     : go(k_kv8_shared<BF, HD, 3>);
+    : w.pre.way == 3 ? go(k_kv8_shared<BF, HD, 3>)
+                     : go(k_kv8_shared<BF, HD, 4>);
   };
   if (c.head_dim == 128)
     c.bf16 ? ways(I1(), I128()) : ways(I0(), I128());

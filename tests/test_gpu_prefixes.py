@@ -532,3 +532,136 @@ def test_plans_of_many_sequences(ctx):
     before = [64 * blocks[g] + i % 5 for i, g in enumerate(of)]
     m, d = alike(ctx, "fp16", kv, hd, of, blocks, before, rng, cols=20)
     assert step(ctx, m, d, of, blocks, [1] * n, 1, "fp16", rng) <= 1
+
+
+# sequences of several tokens, of 17 to 64 rows a key/value head: new tokens, by the sequence's number
+STEPS = {
+    "even": lambda i, most: most,
+    "ragged": lambda i, most: 1 + (5 * i) % most if i else most,
+    "waiting": lambda i, most: [0, 1, most][i % 3],
+}
+
+
+@pytest.mark.parametrize("dt,odt", [("fp16", "bf16"), ("bf16", "fp16"), ("bf16", "bf16"), ("fp16", "fp16")])
+@pytest.mark.parametrize("heads,kv,hd,most", [(8, 2, 128, 16), (8, 2, 128, 5), (8, 1, 64, 8), (5, 1, 128, 12), (2, 2, 64, 64),
+                                              (2, 2, 128, 17), (16, 1, 64, 8), (32, 1, 128, 3), (3, 3, 128, 30), (7, 1, 64, 3)])
+@pytest.mark.parametrize("tokens", STEPS)
+def test_steps_of_several_tokens(ctx, tokens, heads, kv, hd, most, dt, odt):
+    rng = np.random.default_rng([37, heads, most])
+    of = [-1 if i % 7 == 6 else i % 9 // 8 for i in range(28)]
+    blocks = [33, 17]
+    own = [(37 * i) % 130 if i % 5 else 900 - i for i in range(28)]
+    new = [STEPS[tokens](i, most) for i in range(28)]
+    say("steps", tokens, heads, kv, hd, most, dt, odt)
+    m, d = alike(ctx, dt, kv, hd, of, blocks, [n + 64 * (blocks[g] if g >= 0 else 0) for n, g in zip(own, of)], rng)
+    for _ in range(2):
+        r = step(ctx, m, d, of, blocks, new, heads, odt, rng)
+        say("worst", r)
+        assert r <= 1
+
+
+@pytest.mark.parametrize("heads,kv,hd,seqs,most,tokens", [(8, 2, 128, 3, 8, 14000), (4, 1, 64, 9, 9, 20000), (4, 2, 128, 30, 10, 5000)])
+def test_steps_of_several_tokens_after_long_prefixes(ctx, heads, kv, hd, seqs, most, tokens):
+    rng = np.random.default_rng([38, seqs])
+    of, blocks = [0] * seqs, [tokens // 64]
+    say("steps, long", heads, kv, hd, seqs, most, tokens)
+    m, d = alike(ctx, "bf16", kv, hd, of, blocks, [blocks[0] * 64 + (37 * i) % 400 for i in range(seqs)], rng)
+    assert step(ctx, m, d, of, blocks, [most - i % 3 for i in range(seqs)], heads, "bf16", rng) <= 1
+
+
+def test_steps_whose_tables_are_not_alike(ctx):
+    """As for single tokens: tables that part and meet again, pages that are none, odd lengths and hints."""
+    rng = np.random.default_rng(39)
+    say("steps not alike")
+    for heads, kv, hd, n, most in ((8, 2, 128, 24, 5), (8, 1, 64, 20, 8), (2, 2, 64, 16, 40)):
+        of, b = [0] * n, 30
+        before = [b * 64 + (29 * i) % 150 for i in range(n)]
+        before[3], before[5], before[7] = 100, 0, 64 * 17 + 63
+        m, d = alike(ctx, "fp16", kv, hd, of, [b], before, rng, cols=36)
+        other = lambda i, j: m.table[i, 35 - j % 3]
+        m.table[1, 0] = other(1, 0)
+        m.table[2, 29] = other(2, 1)
+        m.table[4, [7, 8, 20]] = [other(4, 0), other(4, 1), -1]
+        m.table[6, 2:30:3] = [other(6, j) for j in range(10)]
+        m.table[8, 10:] = m.table[9, 10:][::-1]
+        m.table[[0, 9, 10], 16] = 1 << 30
+        m.table[11, 12] = -7
+        d.b["table"].upload(m.table)
+        new = [most - i % 4 for i in range(n)]
+        for blocks in ([30], [36], [1 << 20]):
+            r = step(ctx, m, d, of, blocks, new, heads, "bf16", rng)
+            say(blocks, "worst", r)
+            assert r <= 1
+        m.lens[0] = 0
+        d.b["lens"].upload(m.lens)
+        assert step(ctx, m, d, of, [30], new, heads, "fp16", rng) <= 1
+
+
+@pytest.mark.parametrize("cap", [0.5, 0.1, 0.02, 0], ids=str)
+def test_steps_and_scratch(ctx, cap):
+    rng = np.random.default_rng(40)
+    of, blocks, new = [0] * 18, [24], [5, 3, 8] * 6
+    say("steps, scratch", cap)
+    m, d = alike(ctx, "fp16", 2, 128, of, blocks, [24 * 64 + 23 * i for i in range(18)], rng)
+    assert step(ctx, m, d, of, blocks, new, 8, "fp16", rng, lambda n: int(n * cap) // 4 * 4) <= 1
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_steps_with_values_that_are_not_finite(ctx, bad, dt):
+    """A step's last token is not finite: those before it do not see it, also where its sequence's table parts from its
+    prefix and meets it again; a spoilt block of the prefix is not seen by the sequences that have parted there."""
+    rng = np.random.default_rng(41)
+    say("steps, not finite", bad, dt)
+    kv, hd, heads, n, most = 2, 128, 8, 20, 6
+    of, blocks, new = [0] * n, [24], [most] * n
+    m, d = alike(ctx, dt, kv, hd, of, blocks, [24 * 64 + 3 + 2 * i for i in range(n)], rng)
+    m.table[2, 5] = m.table[2, -1]
+    m.table[3, 11] = m.table[3, -1]
+    m.scales[m.table[0, 11], 1, 1] = bad
+    d.b["table"].upload(m.table)
+    d.b["scales"].upload(m.scales)
+    s = X.Seqs(ctx, new)
+    p = X.Prefixes(ctx, s, of, blocks)
+    kb, _ = normal(rng, (n * most, kv, hd), dt)
+    vb, _ = normal(rng, (n * most, kv, hd), dt)
+    qb, q = normal(rng, (n * most, heads, hd), dt)
+    spoilt = vb.reshape(n, most, kv, hd).copy()
+    spoilt[:, -1, 0, :] = pm.bits(np.float32(bad), dt)[()]
+    dq, dk, dv = (X.DevBuf.of(ctx, b) for b in (qb, kb, spoilt))
+    o = X.DevBuf(ctx, (n, most, heads, hd), np.uint16)
+    X.kv8_append(ctx, d.h, s, dk.h, kv * hd, dv.h, kv * hd)
+    floats = X.attend_shared_part(s, p, heads, kv, hd, m.cols)
+    assert floats != X.kv8_attend_part(s, heads, kv, hd, m.cols)
+    part = X.DevBuf(ctx, (floats,), np.float32)
+    X.attend_shared(ctx, d.h, s, p, heads, dq.h, heads * hd, 0.09, o.h, X.DT_BF16, heads * hd, part.h, floats)
+    got = pm.value(o.get(), "bf16")
+    m.append(kb, vb, new)
+    m.scales[~np.isfinite(m.scales)] = 0.03
+    want, tol = (x.reshape(got.shape) for x in m.attend(q, new, 0.09, "bf16"))
+    half = heads // 2
+    assert not np.isfinite(got[:, -1, :half]).any()
+    sees = [i for i in range(n) if i != 3]
+    assert not np.isfinite(got[sees][:, :, half:]).any()
+    assert (abs(got - want)[:, :-1, :half] <= tol[:, :-1, :half]).all()
+    assert (abs(got - want)[3, :, half:] <= tol[3, :, half:]).all()
+
+
+def test_two_runs_of_steps_are_bit_identical(ctx):
+    rng = np.random.default_rng(42)
+    kv, hd, heads, n = 8, 128, 32, 16
+    of, blocks = [0] * 12 + [1] * 4, [40, 17]
+    m, d = alike(ctx, "fp16", kv, hd, of, blocks, [64 * blocks[g] + 9 * i for i, g in enumerate(of)], rng)
+    say("steps twice")
+    new = [7, 12, 1, 5] * 4
+    s = X.Seqs(ctx, new)
+    p = X.Prefixes(ctx, s, of, blocks)
+    dq = X.DevBuf.of(ctx, normal(rng, (sum(new), heads, hd), "fp16")[0])
+    floats = X.attend_shared_part(s, p, heads, kv, hd, m.cols)
+    outs = []
+    for fill in (0.0, np.nan):
+        part = X.DevBuf.of(ctx, np.full(floats, fill, np.float32))
+        o = X.DevBuf(ctx, (sum(new), heads, hd), np.uint16)
+        X.attend_shared(ctx, d.h, s, p, heads, dq.h, heads * hd, 0.09, o.h, X.DT_BF16, heads * hd, part.h, floats)
+        outs.append(o.get())
+    assert np.array_equal(*outs)

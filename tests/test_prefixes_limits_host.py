@@ -43,8 +43,11 @@ def test_sizes(L):
     (8, 1, 32, 8, 128, 17, 16, False),          # of which the table holds less
     (6, 1, 32, 8, 128, 17, 20, False),          # little to save
     (2, 1, 32, 8, 128, 300, 303, False),
-    (64, 5, 32, 8, 128, 128, 160, False),       # sequences of more than 16 rows a head
-    (64, 2, 16, 1, 128, 128, 160, False),
+    (64, 5, 32, 8, 128, 128, 160, True), (64, 2, 16, 1, 128, 128, 160, True), (20, 16, 32, 8, 128, 21, 30, True),
+    (20, 64, 8, 8, 64, 21, 30, True),           # sequences of 17 to 64 rows a head
+    (19, 5, 32, 8, 128, 21, 30, False),         # little to save
+    (64, 17, 32, 8, 128, 128, 160, False),      # of more
+    (64, 9, 16, 1, 128, 128, 160, False),
 ])
 def test_scratch_and_what_is_shared(L, n, longest, heads, kv, hd, blocks, cols, pays):
     alone = ctypes.c_int64()
@@ -55,6 +58,9 @@ def test_scratch_and_what_is_shared(L, n, longest, heads, kv, hd, blocks, cols, 
     assert got != alone.value
     # a whole number of splits of at most 64 each, of the prefix's rows and of the sequences', and the tiles' notes
     each = n * longest * heads * (hd + 2)
-    tiles = n * -(-longest // 8)
+    tokens = 8
+    while 2 * tokens * min(8, heads // kv) <= 64 and longest * min(16, heads // kv) > 16:
+        tokens *= 2
+    tiles = n * -(-longest // tokens)
     splits, left = divmod(got - 4 * tiles, each)
     assert left == 0 and 2 <= splits <= 128
