@@ -1924,18 +1924,22 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
   // Where reading a prefix once saves more than a second pass and the join take: prefixes past 16 blocks (up to there
   // kv8_attend is one launch: 64 x 1 after 640 19.5, shared 24.8), and so many blocks read again (8 x 1 after 1088, 119 of
   // them: 17.2, shared 14.4; 4 after 2048, 96: 13.9, 15.4; 2 after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0, 26.3).
-  // Sequences of 17 to 64 rows a key/value head leave tiles of their own half empty and need more (12..200 of their own:
-  // 4 x 8 after 4096, 192: 28.8, 25.6, 4 x 16: 30.8, 31.9; 4 x 16 after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968:
-  // 164, 76; where kv8_attend's workgroups fill the chip just so it is ahead still, 32 x 8 after 2048: 32.9, 37.6); more
-  // rows fill them (8 x 76 tokens after 1088 42, shared 56; 32 x 32 after 4096 105, 121)
+  // Sequences of 17 rows a key/value head and more need more (12..200 of their own: 4 x 8 after 4096, 192: 28.8, 25.6, 4 x
+  // 16: 30.8, 31.9; 4 x 16 after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968: 164, 76; where kv8_attend's workgroups
+  // fill the chip just so it is ahead still, 32 x 8 after 2048: 32.9, 37.6), and those of more than 64 are shared where
+  // kv8_attend's tiles of 128 would be a good part empty, which is what a prefix's are not (20 of 32 tokens and less: 16 x
+  // 40 after 8192, 1920: 175, 126; 8 x 40 after 4096, 448: 61.8, 63.1; 16 x 24 after 4096, 960: 62.2, 65.5; 8 x 76 after
+  // 1088 45.9, 44.5; 32 x 32 after 4096 107, 116)
   const bool few = longest * h16 <= 16;
-  w.pays = sh.rows > 0 && longest * h8 <= 64 && blocks > 16 && sh.saved >= (!few || sh.seqs < 4 ? 384 : 112);
-  if (!w.pays) return w;
   auto tokens = [&](int rows) {   // that tiles of ROWS rows hold
     int n = SEQ_TT0;
     while (2 * n * h8 <= rows && n < (SEQ_TT0 << (SEQ_TTS - 1))) n *= 2;
     return n;
   };
+  const int64_t held = tokens(128), room = (longest + held - 1) / held * held;   // tokens of a sequence's tiles of 128 rows
+  const int64_t least = few ? (sh.seqs < 4 ? 384 : 112) : longest * h8 <= 64 ? 384 : 8ll * longest <= 5 * room ? 896 : INT64_MAX;
+  w.pays = sh.rows > 0 && blocks > 16 && sh.saved >= least;
+  if (!w.pays) return w;
   w.own = few ? pass_rows(1, h16, longest, group, kv_heads, ntiles) : pass_rows(0, h8, tokens(64), group, kv_heads, ntiles);
   // a sequence's own blocks are split as far as there are places for the workgroups
   pass_splits(w.own, 256 * (head_dim == 64 ? 4 : 2), own, 8);

@@ -569,6 +569,22 @@ def test_steps_of_several_tokens_after_long_prefixes(ctx, heads, kv, hd, seqs, m
     assert step(ctx, m, d, of, blocks, [most - i % 3 for i in range(seqs)], heads, "bf16", rng) <= 1
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("heads,kv,hd,most", [(8, 2, 128, 17), (4, 1, 64, 40), (2, 2, 64, 80), (8, 1, 128, 10), (1, 1, 128, 160)])
+def test_steps_of_many_tokens(ctx, heads, kv, hd, most, dt):
+    """More than 64 rows a key/value head and sequence, in several tiles each."""
+    rng = np.random.default_rng([43, heads, most])
+    of, blocks, n = [0] * 13 + [-1], [80], 14
+    say("many tokens", heads, kv, hd, most, dt)
+    m, d = alike(ctx, dt, kv, hd, of, blocks, [80 * 64 * (g == 0) + (37 * i) % 150 for i, g in enumerate(of)], rng)
+    m.table[5, 33] = m.table[5, -1]
+    d.b["table"].upload(m.table)
+    new = [most - (i % 3) * (most // 4) for i in range(n)]
+    s = X.Seqs(ctx, new)
+    assert X.attend_shared_part(s, X.Prefixes(ctx, s, of, blocks), heads, kv, hd, m.cols) != X.kv8_attend_part(s, heads, kv, hd, m.cols)
+    assert step(ctx, m, d, of, blocks, new, heads, "bf16", rng) <= 1
+
+
 def test_steps_whose_tables_are_not_alike(ctx):
     """As for single tokens: tables that part and meet again, pages that are none, odd lengths and hints."""
     rng = np.random.default_rng(39)

@@ -46,8 +46,11 @@ def test_sizes(L):
     (64, 5, 32, 8, 128, 128, 160, True), (64, 2, 16, 1, 128, 128, 160, True), (20, 16, 32, 8, 128, 21, 30, True),
     (20, 64, 8, 8, 64, 21, 30, True),           # sequences of 17 to 64 rows a head
     (19, 5, 32, 8, 128, 21, 30, False),         # little to save
-    (64, 17, 32, 8, 128, 128, 160, False),      # of more
-    (64, 9, 16, 1, 128, 128, 160, False),
+    (64, 17, 32, 8, 128, 128, 160, True), (64, 20, 32, 8, 128, 128, 160, True), (10, 40, 32, 8, 128, 100, 130, True),
+    (64, 9, 16, 1, 128, 128, 160, True), (16, 160, 8, 8, 128, 100, 130, True),   # of more, in tiles that they do not fill
+    (8, 40, 32, 8, 128, 100, 130, False),       # little to save
+    (64, 21, 32, 8, 128, 128, 160, False), (64, 76, 32, 8, 128, 128, 160, False), (64, 32, 32, 8, 128, 128, 160, False),
+    (64, 11, 16, 1, 128, 128, 160, False), (64, 32, 40, 8, 128, 128, 160, False),
 ])
 def test_scratch_and_what_is_shared(L, n, longest, heads, kv, hd, blocks, cols, pays):
     alone = ctypes.c_int64()
