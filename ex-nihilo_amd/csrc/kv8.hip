@@ -418,6 +418,16 @@ template <int N>
 struct PrefixRows {
   int seq[N], head[N], run[N];
 };
+// what a body keeps of that in LDS: nothing but in a prefix's pass
+template <int MODE, int N>
+struct RowsLds {
+  __device__ __forceinline__ PrefixRows<N>* rows() { return nullptr; }
+};
+template <int N>
+struct RowsLds<PREFIX, N> {
+  PrefixRows<N> pfx;
+  __device__ __forceinline__ PrefixRows<N>* rows() { return &pfx; }
+};
 __device__ __forceinline__ void lds_barrier() {   // with loads from memory in flight
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
@@ -533,13 +543,15 @@ __device__ __forceinline__ uint32_t* kv8_parts(const Kv8Args& A, int per, int rt
 // 131071, fp16, 52.5 us, 5.0 and 5.1 TB/s, a copy's rate; 4 over 270..333 9.3 us, which is latency.
 //
 // Grid: workgroups x kv_heads x chunks, the heads fastest.
-template <int HD, int RT, int MODE>
-struct FewLds {
-  alignas(1024) uint8_t tbuf[2][MODE == PREFIX ? 1 : 64 * HD * 2];   // the tail's K and V
-  alignas(16) float obuf[4][16][HD + 4];
+// LDS at a multiple of 1024 bytes; in ALONE no more than the tail and the sums
+template <int HD, int MODE>
+struct FewSums {
+  alignas(16) uint8_t tbuf[2][MODE == PREFIX ? 16 : 64 * HD * 2];   // the tail's K and V
+  float obuf[4][16][HD + 4];
   float mbuf[4][16], lbuf[4][16], pbuf[MODE == PREFIX ? 1 : 64][17];
-  PrefixRows<MODE == PREFIX ? 16 * RT : 1> pfx;
 };
+template <int HD, int RT, int MODE>
+struct FewLds : FewSums<HD, MODE>, RowsLds<MODE, 16 * RT> {};
 template <int BF, int HD, int RT, int MODE>
 __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>& lds, const int bx, const int by) {
   constexpr int WV = 4;                       // waves
@@ -550,7 +562,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
   auto &tbuf = lds.tbuf;
   auto &mbuf = lds.mbuf, &lbuf = lds.lbuf;
   auto &pbuf = lds.pbuf;
-  auto &pfx = lds.pfx;
+  PrefixRows<16 * RT>* const pfx = lds.rows();
   const Kv8& c = A.c;
   const int per = c.kv_heads * A.chunks;
   const int w = bx / per, hc = bx % per, kvh = hc % c.kv_heads, chunk = hc / c.kv_heads;
@@ -688,9 +700,9 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
 
   Seg S = segment(i, at);
   if (MODE != ALONE && S.lo >= S.hi) return;
-  if constexpr (MODE == PREFIX) prefix_rows(A, S.T, S.T.len, S.hi, pfx);
+  if constexpr (MODE == PREFIX) prefix_rows(A, S.T, S.T.len, S.hi, *pfx);
   begin(S);
-  if constexpr (MODE == PREFIX) prefix_ends(A, S.T, S.T.len, S.lo, S.hi, pfx);
+  if constexpr (MODE == PREFIX) prefix_ends(A, S.T, S.T.len, S.lo, S.hi, *pfx);
   for (;;) {
     const SeqTile T = S.T;
     const int live = T.len;
@@ -700,7 +712,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
     for (int rt = 0; rt < RT; ++rt) {
       const int r = rt * 16 + col, tok = min((int)(r * A.magic >> 16), live - 1);
       const int head = min(r - (int)(r * A.magic >> 16) * A.hh, heads - 1);
-      lim[rt] = MODE == PREFIX ? pfx.run[pfx.head[tok]] * 64 - 1 : min(S.base + tok, S.total - 1);
+      lim[rt] = MODE == PREFIX ? pfx->run[pfx->head[tok]] * 64 - 1 : min(S.base + tok, S.total - 1);
       if constexpr (MODE == PREFIX) {   // BASE: what every row sees all keys before
         int least = lim[rt] + 1;
 #pragma unroll
@@ -783,7 +795,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[rt][4 * t + e] = a[rt][e] * kd;
-        if (RT == 1) __builtin_amdgcn_sched_barrier(0);
+        if (RT == 1 || MODE == ALONE) __builtin_amdgcn_sched_barrier(0);
       }
       if (more) load_k(next);
       float vdl[RT];   // a row that sees nothing of the block takes nothing of its scale, which may be NaN
@@ -806,7 +818,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[rt][d][e] = __builtin_fmaf(a[e], vdl[rt], o[rt][d][e]);
         }
-        if (RT == 1 && d % 2) __builtin_amdgcn_sched_barrier(0);
+        if ((RT == 1 || MODE == ALONE) && d % 2) __builtin_amdgcn_sched_barrier(0);
       }
       if (more) load_v(next);
     };
@@ -992,7 +1004,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
 template <int BF, int HD, int RT>
 __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1)
 k_kv8_few(Kv8Args A) {
-  __shared__ FewLds<HD, RT, ALONE> lds;
+  __shared__ __align__(1024) FewLds<HD, RT, ALONE> lds;
   few_rows<BF, HD, RT, ALONE>(A, lds, blockIdx.x, 0);
 }
 
@@ -1112,15 +1124,16 @@ __device__ void kv8_row(const Kv8& c, int seq, const Kv8Own& own, int kvh, int l
   *l_ = l;
 }
 
-template <int HD, int MODE>
-struct ChunkLds {
+template <int HD>
+struct ChunkStages {
   // K stage s at s STAGE: rows of keys, 16-byte chunk c at c ^ (key % 16) (HD 64: c ^ (key / 2 % 8)).
   // V^T stage s at (2 + s) STAGE: rows of dims of 128 bytes, chunk c at c ^ (dim / 2 % 8); a row's
   // keys in vt_pos's order, the one in which a lane's weights lie.  The tail's V is as in memory, rows
   // of keys, chunk c at c ^ 4 (key % 4) (HD 64: c ^ 4 (key / 2 % 2)), and is turned when it is read.
-  alignas(1024) uint8_t smem[4 * 64 * HD * 2];
-  PrefixRows<MODE == PREFIX ? 128 : 1> pfx;
+  alignas(16) uint8_t smem[4 * 64 * HD * 2];
 };
+template <int HD, int MODE>
+struct ChunkLds : ChunkStages<HD>, RowsLds<MODE, 128> {};   // at a multiple of 1024 bytes
 template <int BF, int HD, int MODE, int KG>
 __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>& lds, const int bx, const int by) {
   constexpr int ROWB = HD * 2, STAGE = 64 * ROWB;   // bytes of a key's row; of a block's K or V^T
@@ -1129,7 +1142,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
   constexpr int NH = 2 / KG, NU = 2 * NH;
   constexpr int CI = HD / 64;                       // 16-byte loads of codes a thread and block
   uint8_t* const smem = lds.smem;
-  auto& pfx = lds.pfx;
+  PrefixRows<128>* const pfx = lds.rows();
   const Kv8& c = A.c;
   const int per = c.kv_heads * A.chunks;
   const SeqTile T = A.tiles[bx / per];
@@ -1166,8 +1179,8 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
 #pragma unroll
     for (int s = 0; s < NS; ++s) qf[s] = *(const s16x8*)(qr + 16 * s + 8 * hi);
     if constexpr (MODE == PREFIX) {
-      prefix_ends(A, T, live, b0, b1, pfx);
-      lim = minlim = pfx.run[pfx.head[ctok]] * 64 - 1;
+      prefix_ends(A, T, live, b0, b1, *pfx);
+      lim = minlim = pfx->run[pfx->head[ctok]] * 64 - 1;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) minlim = min(minlim, __shfl_xor(minlim, o, 64));
       minlim = __builtin_amdgcn_readfirstlane(minlim);
@@ -1405,7 +1418,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
 
   // block b's K is filled two steps ahead of its softmax, its V one; codes are asked for one step
   // before they are filled
-  if constexpr (MODE == PREFIX) prefix_rows(A, T, live, b1, pfx);
+  if constexpr (MODE == PREFIX) prefix_rows(A, T, live, b1, *pfx);
   Facts F0 = facts(b0), F1 = F0, F2 = F0;
   Codes kc = fetch(c.k, F0.page), vc = fetch(c.v, F0.page), kn = kc;
   if (b0 + 1 < b1) {
@@ -1542,7 +1555,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
     const int64_t rh = kvh * A.group + chunk * A.hh + r - rt * A.hh, at = T.row0 + T.t0 + rt;
     float m, l, y[HD / 64];
     const int64_t qrow = MODE == PREFIX ? A.entry[2 * at] : at;
-    const int sees = MODE == PREFIX ? pfx.run[pfx.head[rt]] * 64 - 1 : min(base + T.t0 + rt, total - 1);
+    const int sees = MODE == PREFIX ? pfx->run[pfx->head[rt]] * 64 - 1 : min(base + T.t0 + rt, total - 1);
     kv8_row<BF, HD, MODE>(c, T.seq, own, kvh, b0, b1, total, sees, A.q + qrow * A.ldq + rh * HD, A.scale, &m, &l, y);
     const int64_t slot = (int64_t)by * n + at * A.heads + rh;
     for (int z = 0; z < HD / 64; ++z) {
@@ -1559,7 +1572,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
 template <int BF, int HD>
 __global__ void __launch_bounds__(256, 2)
 k_kv8_chunk(Kv8Args A) {
-  __shared__ ChunkLds<HD, ALONE> lds;
+  __shared__ __align__(1024) ChunkLds<HD, ALONE> lds;
   chunk_rows<BF, HD, ALONE, 1>(A, lds, blockIdx.x, blockIdx.y);
 }
 
@@ -1800,7 +1813,7 @@ struct OwnLds<HD, 4> : ChunkLds<HD, OWN> {};
 template <int BF, int HD, int WAY>
 __global__ void __launch_bounds__(256, 2)
 k_kv8_shared(Kv8Args P, Kv8Args O, uint32_t pw, uint32_t pgroups, uint32_t ogroups) {
-  __shared__ union Lds {
+  __shared__ __align__(1024) union Lds {
     PrefixLds<HD, WAY> p;
     OwnLds<HD, WAY> o;
   } lds;
