@@ -369,24 +369,16 @@ __device__ __forceinline__ int kv8_split(int nb, int S, int least, int i, int* l
 // the sequence's for all of them.
 struct Kv8Own {
   int first, nb, per;   // blocks below NB may be the pass's, in splits of PER
+  const int* ends;      // where they part: of each split (64 at most), the first block that is not the pass's
 };
-// page P of block B, or -1 where it is taken.  A wave's lanes take the same steps whatever their blocks: a loop that
-// each leaves at its own mismatch lost P, in this compiler's hands, where a lane did
-__device__ __forceinline__ int kv8_untaken(const Kv8& c, int seq, const Kv8Own& w, int b, int p) {
-  const int32_t *mine = c.table + (int64_t)seq * c.cols, *its = c.table + (int64_t)w.first * c.cols;
-  const int at = min(b, w.nb - 1), first = at / w.per * w.per;
-  int differ = b < w.nb ? 0 : 1;
-#pragma unroll 1
-  for (int k = 0; k < w.per; ++k) {
-    const int i = max(at - k, first);
-    differ |= mine[i] ^ its[i];
-  }
-  return differ ? p : -1;
+// page P of block B, or -1 where it is taken
+__device__ __forceinline__ int kv8_untaken(const Kv8Own& w, int b, int p) {
+  return b < w.nb && b < w.ends[min(b, w.nb - 1) / w.per] ? -1 : p;
 }
 __device__ __forceinline__ Kv8Own kv8_own(const Kv8Args& A, const int32x4& of, int base) {
-  if (of[0] < 0) return Kv8Own{0, 0, 1};
+  if (of[0] < 0) return Kv8Own{0, 0, 1, nullptr};
   const int all = min(of[1], A.c.cols);
-  return Kv8Own{of[0], min(all, base / 64), max(A.pleast, (all + A.psplits - 1) / A.psplits)};
+  return Kv8Own{of[0], min(all, base / 64), max(A.pleast, (all + A.psplits - 1) / A.psplits), nullptr};
 }
 // the first block of a sequence that is not taken (a wave finds it out)
 __device__ __forceinline__ int kv8_own_from(const Kv8& c, int seq, const Kv8Own& w) {
@@ -397,6 +389,26 @@ __device__ __forceinline__ int kv8_own_from(const Kv8& c, int seq, const Kv8Own&
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) run = min(run, __shfl_xor(run, o, 64));
   return __builtin_amdgcn_readfirstlane(run);
+}
+// the ends of a sequence whose table parts at block RUN, a split a lane, 64 blocks' entries at a time.  Found once and
+// looked up: a walk back to the split's first block for each look-up costs the square of a long split (8 x 1 after 131008
+// with scratch for one, a table that parts half-way: 1495 us, so 1095)
+__device__ __forceinline__ void kv8_parted(const Kv8& c, int seq, Kv8Own& w, int run, int* ends) {
+  const int32_t *mine = c.table + (int64_t)seq * c.cols, *its = c.table + (int64_t)w.first * c.cols;
+  const int lane = threadIdx.x & 63, b0 = lane * w.per, b1 = b0 + w.per;
+  int end = b1;
+#pragma unroll 4
+  for (int at = run & ~63; at < w.nb; at += 64) {
+    const int i = min(at + lane, w.nb - 1), from = max(b0 - at, 0), to = min(b1 - at, 64);
+    uint64_t differ = __ballot(mine[i] != its[i]);
+    if (from < to) {
+      differ = differ >> from << from & ~0ull >> (64 - to);
+      if (differ) end = min(end, at + __builtin_ctzll(differ));
+    }
+  }
+  ends[lane] = end;
+  asm volatile("" ::: "memory");   // read by this wave alone, whose LDS accesses keep their order
+  w.ends = ends;
 }
 // split I of a sequence's own blocks, FROM .. NB - 1 (taken ones among them are left out one by one): [*lo, *hi); the
 // splits with any
@@ -427,6 +439,11 @@ template <int N>
 struct RowsLds<PREFIX, N> {
   PrefixRows<N> pfx;
   __device__ __forceinline__ PrefixRows<N>* rows() { return &pfx; }
+};
+template <int N>
+struct RowsLds<OWN, N> {
+  int ends[4][64];   // each wave's Kv8Own's
+  __device__ __forceinline__ PrefixRows<N>* rows() { return nullptr; }
 };
 __device__ __forceinline__ void lds_barrier() {   // with loads from memory in flight
   asm volatile("" ::: "memory");
@@ -612,7 +629,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
   auto page_at = [&](const Seg& s, int it) __attribute__((always_inline)) {
     const int b = s.lo + wave + WV * (it + lane);
     int p = b < min(s.hi, s.nfull) ? (int)kv8_page(c, s.T.seq, b) : -1;
-    if (MODE == OWN && s.lo < own.nb) p = kv8_untaken(c, s.T.seq, own, b, p);
+    if (MODE == OWN && s.lo < own.nb) p = kv8_untaken(own, b, p);
     return p;
   };
   auto segment = [&](int i, int at) __attribute__((always_inline)) {
@@ -641,6 +658,7 @@ __device__ __forceinline__ void few_rows(const Kv8Args& A, FewLds<HD, RT, MODE>&
       s.ahead = b < min(s.hi, s.nfull) ? (int)kv8_page(c, s.T.seq, b) : -1;
       const int run = kv8_own_from(c, s.T.seq, own);
       if (run != own.nb) {
+        kv8_parted(c, s.T.seq, own, run, lds.ends[wave]);
         n = kv8_own_split(A, run, s.nb, by, &s.lo, &s.hi);
         s.ahead = page_at(s, 0);
       }
@@ -1094,7 +1112,7 @@ __device__ void kv8_row(const Kv8& c, int seq, const Kv8Own& own, int kvh, int l
   for (int b = lo; b < hi && b * 64 <= lim; ++b) {
     const bool full = b * 64 + 64 <= total;
     int64_t page = full ? kv8_page(c, seq, b) : 0;
-    if (MODE == OWN && b < own.nb) page = kv8_untaken(c, seq, own, b, (int)page);
+    if (MODE == OWN && b < own.nb) page = kv8_untaken(own, b, (int)page);
     if (page < 0) continue;
     const int64_t ph = (page * c.kv_heads + kvh), th = ((int64_t)seq * c.kv_heads + kvh) * 64 * HD;
     const float kd = full ? c.scales[ph * 2] : 1.f, vd = full ? c.scales[ph * 2 + 1] : 1.f;
@@ -1159,7 +1177,9 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
   } else if constexpr (MODE == OWN) {
     const int32x4 of = A.of[T.seq];
     own = kv8_own(A, of, base);
-    active = kv8_own_split(A, kv8_own_from(c, T.seq, own), (min(base + T.t0 + live, total) + 63) / 64, by, &b0, &b1);
+    const int run = kv8_own_from(c, T.seq, own);
+    if (run != own.nb) kv8_parted(c, T.seq, own, run, lds.ends[wave]);
+    active = kv8_own_split(A, run, (min(base + T.t0 + live, total) + 63) / 64, by, &b0, &b1);
     if (by == 0 && hc == 0 && tid == 0) kv8_note(A, of, bx / per, T.t0, active);
   } else {
     active = max(1, kv8_split((min(base + T.t0 + live, total) + 63) / 64, A.splits, A.least, by, &b0, &b1));
@@ -1196,7 +1216,7 @@ __device__ __forceinline__ void chunk_rows(const Kv8Args& A, ChunkLds<HD, MODE>&
   float kds = 1.f, vds = 1.f;
   auto look = [&](int b) __attribute__((always_inline)) {
     int64_t p = b + lane < min(b1, nfull) ? kv8_page(c, T.seq, b + lane) : -1;
-    if (MODE == OWN && b < own.nb) p = kv8_untaken(c, T.seq, own, b + lane, (int)p);
+    if (MODE == OWN && b < own.nb) p = kv8_untaken(own, b + lane, (int)p);
     pages = (int)p;
     p = p < 0 ? 0 : p;
     const f32x2 d = *(const f32x2*)(c.scales + (p * c.kv_heads + kvh) * 2);
