@@ -1974,8 +1974,10 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
   w.pays = sh.rows > 0 && blocks > 16 && sh.saved >= least;
   if (!w.pays) return w;
   w.own = few ? pass_rows(1, h16, longest, group, kv_heads, ntiles) : pass_rows(0, h8, tokens(64), group, kv_heads, ntiles);
-  // a sequence's own blocks are split as far as there are places for the workgroups
-  pass_splits(w.own, 256 * (head_dim == 64 ? 4 : 2), own, 8);
+  // A sequence's own blocks are split as far as there are places for the workgroups, by all the table's: any may come to be
+  // its own, where its table parts from its prefix (4 x 1 after 32768, 2 heads of 64, one parted at its first: 26 us, split
+  // by the blocks past the shortest prefix 165; 8 x 1 after 131008: 187, 504)
+  pass_splits(w.own, 256 * (head_dim == 64 ? 4 : 2), cols, 8);
   if (few && (int64_t)sh.most * h16 <= 32) {
     // The bytes are the cost: few_rows.  17 to 32 rows are two row tiles of a workgroup (8 x 1 after 131008 58.7), or
     // in shorter prefixes workgroups of half the heads, whose blocks' second reading the L2 has (8 x 1 after 8192
