@@ -1948,21 +1948,39 @@ struct SharedWay {
   PassWay pre, own;
   int64_t pre_each, own_each, notes, floats;   // floats of a split of either, of the notes, in all
 };
+// Microseconds of a call of kv8_attend whose sequences have BLOCKS blocks in all of their prefixes, and of one in the two
+// passes W: lines through the times of 1726 calls, taken on either side (1 to 32 key/value heads of 64 and 128, groups of 1 to
+// 16, 2 to 256 sequences of 12..200 tokens of their own and 1 to 64 new ones, prefixes of 4 to 2000 blocks, bf16; root mean
+// square 16% and 15% off).  What they are to get right is which is the smaller: by them and the rule in shared_way 13 of those
+// calls run the slower side at a loss of more than 3%, 3.8 us at most (by counts of saved blocks alone 105, 16 us at most); of
+// 350 others, drawn at random, also of long sequences of their own, 31, by sharing 8 (7.9 us at most).
+double alone_us(int64_t rows, int longest, int64_t blocks, int heads, int kv_heads, int head_dim, int cols,
+                const int64_t* ntiles) {
+  const Kv8Way a = kv8_way(rows, longest, heads, kv_heads, head_dim, cols, ntiles, INT64_MAX);
+  const int64_t per = (int64_t)kv_heads * a.chunks, tiles = (longest + (SEQ_TT0 << a.z) - 1) / (SEQ_TT0 << a.z);
+  // those that one of 512 places takes, of a key/value head of 128
+  const double steps = (double)blocks * tiles * per * head_dim / 128 / 512;
+  if (a.rt == 0) return 13.6 + 2.94 * steps + (a.splits > 1 ? 0.18 * a.splits * rows * heads * head_dim / 128e3 : 0);
+  if (a.rt == 1) return (cols > 16 ? 16.3 : 8.9) + 1.45 * steps;   // one launch up to 16 columns
+  // two row tiles: workgroups of whole sequences where there are as many places (32 x 8 after 2048 35, 16 x 8 32, 64 x 8 82)
+  return (ntiles[a.z] * per == 256 * (head_dim == 64 ? 2 : 1) ? 12.5 : 22.6) + 1.16 * steps;
+}
+double shared_us(const SharedWay& w, int64_t rows, int heads, int head_dim, int blocks) {
+  const int way = w.pre.way, S = w.pre.splits;
+  const double sums = (double)rows * heads * head_dim / 128e3;   // a split's, in and out again, some us a thousand
+  // a workgroup's blocks one after the other
+  const double chain = (way == 4 ? 1.5 : way == 0 || way == 3 ? 1.9 : 0.38) * (head_dim == 64 ? 0.4 : 1) *
+                       std::max(w.pre.least, (blocks + S - 1) / S);
+  return (way == 4 ? 14.5 + 0.5 * sums : 10.1 + 2.3 * sums) + chain + 0.2 * sums * S + 0.045 * S +
+         0.085 * std::max(0, S - 32) + 0.2 * w.own.groups / 512;
+}
 // The rules' times are as kv8_way's, of one new token a sequence in bf16 with 12 to 200 of its own, unless said.
 SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, int kv_heads, int head_dim, int cols,
                      const int64_t* ntiles) {
   SharedWay w{};
   const int group = heads / kv_heads, h16 = group < 16 ? group : 16, h8 = group < 8 ? group : 8;
   const int blocks = sh.blocks < cols ? sh.blocks : cols, own = cols > sh.fewest ? cols - sh.fewest : 1;
-  // Where reading a prefix once saves more than a second pass and the join take: prefixes past 16 blocks (up to there
-  // kv8_attend is one launch: 64 x 1 after 640 19.5, shared 24.8), and so many blocks read again (8 x 1 after 1088, 119 of
-  // them: 17.2, shared 14.4; 4 after 2048, 96: 13.9, 15.4; 2 after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0, 26.3).
-  // Sequences of 17 rows a key/value head and more need more (12..200 of their own: 4 x 8 after 4096, 192: 28.8, 25.6, 4 x
-  // 16: 30.8, 31.9; 4 x 16 after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968: 164, 76; where kv8_attend's workgroups
-  // fill the chip just so it is ahead still, 32 x 8 after 2048: 32.9, 37.6), and those of more than 64 are shared where
-  // kv8_attend's tiles of 128 would be a good part empty, which is what a prefix's are not (20 of 32 tokens and less: 16 x
-  // 40 after 8192, 1920: 175, 126; 8 x 40 after 4096, 448: 61.8, 63.1; 16 x 24 after 4096, 960: 62.2, 65.5; 8 x 76 after
-  // 1088 45.9, 44.5; 32 x 32 after 4096 107, 116)
+  const int64_t saved = std::min(sh.saved, sh.rows * cols);   // a hint may say more than tables hold
   const bool few = longest * h16 <= 16;
   auto tokens = [&](int rows) {   // that tiles of ROWS rows hold
     int n = SEQ_TT0;
@@ -1970,9 +1988,18 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
     return n;
   };
   const int64_t held = tokens(128), room = (longest + held - 1) / held * held;   // tokens of a sequence's tiles of 128 rows
+  // Shared where enough blocks need not be read again, counted as of 8 key/value heads where there are more, and where the
+  // estimates above are for it: prefixes past 16 blocks (up to there kv8_attend is one launch, 64 x 1 after 640 19.5, shared 24.8, which
+  // 100 MB make up for: 64 x 1 after 1024, 32 heads, 529 MB, 98.9, 41.9; 16 x 1 after 512, 63 MB, 19.4, 22.4) and so many blocks
+  // (8 x 1 after 1088, 119: 17.2, 14.4; 4 after 2048, 96: 13.9, 15.4; 2 after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0,
+  // 26.3), of sequences of 17 rows a key/value head and more 384 (4 x 8 after 4096, 192: 28.8, 25.6, 4 x 16: 30.8, 31.9; 4 x 16
+  // after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968: 164, 76), of more than 64 where kv8_attend's tiles of 128 would be a
+  // good part empty, which is what a prefix's are not (20 of 32 tokens and less: 16 x 40 after 8192, 1920: 175, 126; 8 x 40
+  // after 4096, 448: 61.8, 63.1; 16 x 24 after 4096, 960: 62.2, 65.5; 32 x 32 after 4096 107, 116).
   const int64_t least = few ? (sh.seqs < 4 ? 384 : 112) : longest * h8 <= 64 ? 384 : 8ll * longest <= 5 * room ? 896 : INT64_MAX;
-  w.pays = sh.rows > 0 && blocks > 16 && sh.saved >= least;
-  if (!w.pays) return w;
+  const bool enough = blocks > 16 ? saved * std::max(kv_heads, 8) / 8 >= least
+                                  : few && saved * kv_heads * head_dim >= 100000000 / 128;
+  if (sh.rows == 0 || !enough) return w;
   w.own = few ? pass_rows(1, h16, longest, group, kv_heads, ntiles) : pass_rows(0, h8, tokens(64), group, kv_heads, ntiles);
   // A sequence's own blocks are split as far as there are places for the workgroups, by all the table's: any may come to be
   // its own, where its table parts from its prefix (4 x 1 after 32768, 2 heads of 64, one parted at its first: 26 us, split
@@ -1999,6 +2026,8 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
     const double a = units * 1.5 / 256, b = w.own.groups * (double)own / 4 * (head_dim * 128) / 5e6;
     pass_splits(w.pre, std::min(512., a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1), blocks, 2);
   }
+  w.pays = shared_us(w, rows, heads, head_dim, blocks) < alone_us(rows, longest, saved + blocks, heads, kv_heads, head_dim, cols, ntiles);
+  if (!w.pays) return w;
   w.pre_each = sh.rows * heads * (head_dim + 2);
   w.own_each = rows * heads * (head_dim + 2);
   w.notes = 4 * ntiles[w.own.z];

@@ -247,9 +247,12 @@ int exn_prefixes_free(exn_prefixes* p);
 /* exn_kv8_attend with the blocks of each prefix read once for the rows of all its sequences: the same arguments and
  * answer, within the same distance of the exact one (not bit for bit: sums over a prefix and over the rest meet at
  * the end).  Blocks are shared as far as a sequence's table names the pages that its prefix's first sequence's does
- * (the lowest that has rows), full before the step; and only where that is faster: by the plan, for prefixes of more
- * than 16 blocks and steps of at most 64 rows a key/value head and sequence (tokens times the heads of a group), or of
- * more that leave its tiles of 128 a good part empty; else this is exn_kv8_attend.  PART (as there) is needed for it: with room for less than a split nothing is shared.
+ * (the lowest that has rows), full before the step; and only where the library estimates that to be faster, by the plan
+ * and the table's width: for prefixes of more than 16 blocks, or shorter ones of very many sequences, and steps of at most 64
+ * rows a key/value head and sequence (tokens times the heads of a group), or of more that leave its tiles of 128 a good
+ * part empty; else this is exn_kv8_attend.  Tables that part from their prefix cost more than exn_kv8_attend takes (up to
+ * a quarter was measured, with all of PART).  PART (as there) is needed for it: with room for less than a split nothing is
+ * shared.
  * exn_attend_shared_part (needs no GPU): how many floats are of use. */
 int exn_attend_shared(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const exn_prefixes* p, int heads, const void* q,
                       int64_t ldq, float scale, void* out, int odt, int64_t ldo, float* part, int64_t part_cap);

@@ -88,7 +88,7 @@ PARTED = {"first block": {1: [0]}, "last block": {1: [299], 7: [298, 299]}, "mid
           "all": {i: list(range(300)) for i in range(8)}}
 
 
-@pytest.mark.parametrize("heads,kv,hd", [(2, 2, 64), (4, 1, 64), (4, 2, 128), (8, 1, 128)])
+@pytest.mark.parametrize("heads,kv,hd", [(2, 2, 64), (4, 1, 64), (4, 2, 128), (16, 2, 128)])
 @pytest.mark.parametrize("splits", [1, 2, 5, None], ids=str)
 @pytest.mark.parametrize("where", PARTED)
 def test_parted(ctx, where, splits, heads, kv, hd):

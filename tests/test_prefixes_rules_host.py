@@ -1,4 +1,4 @@
-"""attend_shared's rules, without a GPU: into how many splits its passes go.  tests/host/prefixes_limits_host.cpp calls
+"""attend_shared's rules, without a GPU: into how many splits its passes go, and where nothing is shared.  tests/host/prefixes_limits_host.cpp calls
 them (this build's own kv8.o)."""
 import ctypes
 import os
@@ -40,3 +40,34 @@ def test_own_blocks_are_split_by_the_whole_table(L, n, heads, kv, hd, blocks, co
     assert got != alone
     splits, left = divmod(got - 4 * n, n * heads * (hd + 2))
     assert left == 0 and splits == prefix + own
+
+
+@pytest.mark.parametrize("n,longest,heads,kv,hd,blocks,cols,shared", [
+    # each side's time on the card (us), unshared and shared
+    (32, 8, 32, 8, 128, 32, 36, False),      # 35.2, 37.8: a workgroup of kv8_attend for each sequence and head fits the chip
+    (32, 32, 8, 8, 128, 32, 36, False),      # 34.9, 39.6
+    (8, 32, 32, 32, 128, 32, 36, False),     # 35.1, 40.0
+    (2, 1, 16, 1, 128, 512, 516, False),     # 24.0, 26.0: few workgroups for the prefix
+    (4, 1, 16, 1, 128, 2000, 2004, False),   # 42.6, 55.5
+    (3, 1, 16, 1, 64, 2000, 2004, False),    # 31.1, 42.1
+    (4, 16, 4, 1, 128, 128, 132, False),     # 21.2, 26.2
+    (16, 1, 32, 32, 128, 8, 12, False),      # 19.4, 22.4: a short prefix, 63 MB
+    (64, 1, 32, 32, 128, 16, 20, True),      # 98.9, 41.9: 529 MB
+    (64, 1, 32, 32, 128, 8, 12, True),       # 59.8, 40.4
+    (256, 1, 32, 8, 128, 16, 20, True),      # 94.3, 47.2
+    (256, 1, 32, 8, 128, 8, 12, True),       # 59.1, 45.4
+    (2, 1, 32, 32, 128, 128, 132, True),     # 34.3, 25.2: many heads
+    (4, 24, 32, 32, 128, 64, 68, True),      # 46.4, 34.5
+    (16, 17, 32, 32, 128, 17, 21, True),     # 56.6, 35.9
+    (16, 1, 16, 1, 128, 512, 516, True),     # 40.4, 34.7
+    (4, 1, 16, 4, 64, 512, 516, True),       # 26.7, 17.7
+    (8, 1, 8, 1, 64, 32, 36, True),          # 13.7, 12.7
+])
+def test_the_faster_side_runs(L, n, longest, heads, kv, hd, blocks, cols, shared):
+    got, alone = part(L, n, longest, heads, kv, hd, blocks, cols)
+    assert (got != alone) == shared
+
+
+def test_a_hint_past_the_table_saves_no_more_than_the_table(L):
+    """A prefix said to be of a million blocks, in tables of 12: as one of 12."""
+    assert part(L, 8, 1, 32, 8, 128, 1 << 20, 12) == part(L, 8, 1, 32, 8, 128, 12, 12)
