@@ -150,7 +150,7 @@ k_rope_rows(RopeArgs A) {
       }
       const float inv = rsqrtf(ss * A.per + eps);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= inv * (side ? wk[e] : wq[e]);
+      for (int e = 0; e < 8; ++e) f[e] = f[e] * inv * (side ? wk[e] : wq[e]);   // weights of any size: the head first
     }
     float y[8];
     if constexpr (WAY == PAIRED) {
