@@ -211,6 +211,15 @@ def call(name, *args):
     return check(getattr(lib(), name)(*args))
 
 
+def int32s(what, a) -> np.ndarray:
+    """Whole numbers as the library takes them; refused where 32 bits do not hold them."""
+    x = np.asarray(a).reshape(-1)
+    if x.size and not (x.dtype.kind in "biuf" and np.isfinite(x).all() and (x == np.rint(x)).all() and
+                       x.min() >= -2 ** 31 and x.max() < 2 ** 31):
+        raise ExnError(EINVAL, "%s: whole numbers of 32 bits" % what)
+    return np.ascontiguousarray(x, dtype=np.int32)
+
+
 def ptr(a: np.ndarray):
     assert a.flags["C_CONTIGUOUS"]
     return a.ctypes.data_as(vp)
@@ -349,7 +358,7 @@ class Seqs:
     """A plan of packed sequences (exn_seqs_create): LENS tokens each, one after the other."""
 
     def __init__(self, ctx: Context, lens):
-        a = np.ascontiguousarray(lens, dtype=np.int32).reshape(-1)
+        a = int32s("sequences' lengths", lens)
         h = vp()
         call("exn_seqs_create", ctx.h, ptr(a), len(a), ctypes.byref(h))
         self.ctx, self.h = ctx, h
@@ -418,7 +427,7 @@ class Prefixes:
     prefix's full blocks of 64 tokens."""
 
     def __init__(self, ctx: Context, seqs: Seqs, of, blocks):
-        o, b = (np.ascontiguousarray(x, dtype=np.int32).reshape(-1) for x in (of, blocks))
+        o, b = int32s("sequences' prefixes", of), int32s("prefixes' blocks", blocks)
         if len(o) != seqs.seqs:
             raise ExnError(EINVAL, "prefixes of %d sequences for a plan of %d" % (len(o), seqs.seqs))
         h = vp()
@@ -468,7 +477,7 @@ class Rope:
 
     def __init__(self, ctx: Context, freqs, layout=ROPE_HALF, axis=None, amp=1.0, axes=None):
         f = np.ascontiguousarray(freqs, dtype=np.float64).reshape(-1)
-        a = None if axis is None else np.ascontiguousarray(axis, dtype=np.int32).reshape(-1)
+        a = None if axis is None else int32s("rotary: axes", axis)
         if a is not None and len(a) != len(f):
             raise ExnError(EINVAL, "rotary: %d axes for %d pairs" % (len(a), len(f)))
         if axes is None:
