@@ -250,8 +250,8 @@ int exn_prefixes_free(exn_prefixes* p);
  * (the lowest that has rows), full before the step; and only where the library estimates that to be faster, by the plan
  * and the table's width: for prefixes of more than 16 blocks, or shorter ones of very many sequences, and steps of at most 64
  * rows a key/value head and sequence (tokens times the heads of a group), or of more that leave its tiles of 128 a good
- * part empty; else this is exn_kv8_attend.  Tables that part from their prefix cost more than exn_kv8_attend takes (up to
- * a quarter was measured, with all of PART).  PART (as there) is needed for it: with room for less than a split nothing is
+ * part empty; else this is exn_kv8_attend.  Tables that part from their prefix may cost more than exn_kv8_attend does
+ * (up to 1.3 times, with all of PART).  PART (as there) is needed for it: with room for less than a split nothing is
  * shared.
  * exn_attend_shared_part (needs no GPU): how many floats are of use. */
 int exn_attend_shared(exn_ctx* ctx, const exn_kv8* c, const exn_seqs* s, const exn_prefixes* p, int heads, const void* q,
