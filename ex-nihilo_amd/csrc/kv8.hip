@@ -10,6 +10,7 @@
 #include "exn_common.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace exn {
@@ -1949,30 +1950,39 @@ struct SharedWay {
   int64_t pre_each, own_each, notes, floats;   // floats of a split of either, of the notes, in all
 };
 // Microseconds of a call of kv8_attend whose sequences have BLOCKS blocks in all of their prefixes, and of one in the two
-// passes W: lines through the times of 1726 calls, taken on either side (1 to 32 key/value heads of 64 and 128, groups of 1 to
-// 16, 2 to 256 sequences of 12..200 tokens of their own and 1 to 64 new ones, prefixes of 4 to 2000 blocks, bf16; root mean
-// square 16% and 15% off).  What they are to get right is which is the smaller: by them and the rule in shared_way 13 of those
-// calls run the slower side at a loss of more than 3%, 3.8 us at most (by counts of saved blocks alone 105, 16 us at most); of
-// 350 others, drawn at random, also of long sequences of their own, 31, by sharing 8 (7.9 us at most).
+// passes W: lines through the times of 3029 calls, taken on either side (1 to 32 key/value heads of 64 and 128, groups of 1 to
+// 16, 2 to 256 sequences of 12..200 tokens of their own and 1 to 160 new ones, prefixes of 4 to 2000 blocks, bf16), those of
+// MANY rows a head and sequence (past 64) by themselves; root mean square 15% off, of many rows 6%.  What they are to get
+// right is which is the smaller.  By them and the rule in shared_way 14 of the 1726 calls of up to 64 rows run the slower side
+// at a loss of more than 3%, 3.8 us at most (by counts of saved blocks alone 105, 16 us at most), and 63 of the 1303 of more,
+// 9 us at most (158, 32 us); of 350 others, drawn at random, also of long sequences of their own, 34, by sharing 10 of them,
+// 8.3 us at most.
 double alone_us(int64_t rows, int longest, int64_t blocks, int heads, int kv_heads, int head_dim, int cols,
-                const int64_t* ntiles) {
+                const int64_t* ntiles, bool many) {
   const Kv8Way a = kv8_way(rows, longest, heads, kv_heads, head_dim, cols, ntiles, INT64_MAX);
   const int64_t per = (int64_t)kv_heads * a.chunks, tiles = (longest + (SEQ_TT0 << a.z) - 1) / (SEQ_TT0 << a.z);
-  // those that one of 512 places takes, of a key/value head of 128
-  const double steps = (double)blocks * tiles * per * head_dim / 128 / 512;
-  if (a.rt == 0) return 13.6 + 2.94 * steps + (a.splits > 1 ? 0.18 * a.splits * rows * heads * head_dim / 128e3 : 0);
-  if (a.rt == 1) return (cols > 16 ? 16.3 : 8.9) + 1.45 * steps;   // one launch up to 16 columns
+  // those that one of 512 places takes, of a key/value head of 128; a split's sums, in and out again
+  const double steps = (double)blocks * tiles * per * head_dim / 128 / 512, sums = (double)rows * heads * head_dim / 128e3;
+  const double joined = a.splits > 1 ? sums * a.splits : 0;
+  if (many) return 12.3 + (head_dim == 64 ? 3.24 : 2.42) * steps + 0.283 * joined + 0.37 * sums;
+  if (a.rt == 0) return 13.8 + 2.95 * steps + 0.195 * joined;
+  if (a.rt == 1) return (cols > 16 ? 15.9 : 8) + 1.36 * steps;   // one launch up to 16 columns
   // two row tiles: workgroups of whole sequences where there are as many places (32 x 8 after 2048 35, 16 x 8 32, 64 x 8 82)
-  return (ntiles[a.z] * per == 256 * (head_dim == 64 ? 2 : 1) ? 12.5 : 22.6) + 1.16 * steps;
+  return (ntiles[a.z] * per == 256 * (head_dim == 64 ? 2 : 1) ? 14 : 22.5) + 1.21 * steps;
 }
-double shared_us(const SharedWay& w, int64_t rows, int heads, int head_dim, int blocks) {
-  const int way = w.pre.way, S = w.pre.splits;
-  const double sums = (double)rows * heads * head_dim / 128e3;   // a split's, in and out again, some us a thousand
-  // a workgroup's blocks one after the other
-  const double chain = (way == 4 ? 1.5 : way == 0 || way == 3 ? 1.9 : 0.38) * (head_dim == 64 ? 0.4 : 1) *
-                       std::max(w.pre.least, (blocks + S - 1) / S);
-  return (way == 4 ? 14.5 + 0.5 * sums : 10.1 + 2.3 * sums) + chain + 0.2 * sums * S + 0.045 * S +
-         0.085 * std::max(0, S - 32) + 0.2 * w.own.groups / 512;
+double shared_us(const SharedWay& w, int64_t rows, int heads, int head_dim, int blocks, bool many) {
+  // a workgroup's blocks one after the other; the splits with any
+  const int way = w.pre.way, chain = std::max(w.pre.least, (blocks + w.pre.splits - 1) / w.pre.splits);
+  const int S = (blocks + chain - 1) / chain;
+  const double sums = (double)rows * heads * head_dim / 128e3, own = w.own.groups / 512.;
+  if (many) {   // a prefix's workgroups past the places run in turns, and past half of them share the CUs
+    const double turns = (double)w.pre.groups * w.pre.splits / 512;
+    return 8.7 + (head_dim == 64 ? 1.18 : 1.75) * chain * (std::max(1., std::ceil(turns)) + 0.59 * std::max(0., turns - 0.5)) +
+           0.44 * sums * S + 0.07 * S + 6.7 * own;
+  }
+  const double step = (way == 4 ? 1.79 : way == 0 || way == 3 ? 1.82 : 0.37) * (head_dim == 64 ? 0.4 : 1);
+  return (way == 4 ? 14.25 + 0.3 * sums : 10 + 1.56 * sums) + step * chain + (way == 4 ? 0.21 : 0.225) * sums * S +
+         0.05 * S + 0.065 * std::max(0, S - 32) + 1.5 * own;
 }
 // The rules' times are as kv8_way's, of one new token a sequence in bf16 with 12 to 200 of its own, unless said.
 SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, int kv_heads, int head_dim, int cols,
@@ -1988,14 +1998,15 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
     return n;
   };
   const int64_t held = tokens(128), room = (longest + held - 1) / held * held;   // tokens of a sequence's tiles of 128 rows
-  // Shared where enough blocks need not be read again, counted as of 8 key/value heads where there are more, and where the
-  // estimates above are for it: prefixes past 16 blocks (up to there kv8_attend is one launch, 64 x 1 after 640 19.5, shared 24.8, which
-  // 100 MB make up for: 64 x 1 after 1024, 32 heads, 529 MB, 98.9, 41.9; 16 x 1 after 512, 63 MB, 19.4, 22.4) and so many blocks
-  // (8 x 1 after 1088, 119: 17.2, 14.4; 4 after 2048, 96: 13.9, 15.4; 2 after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0,
-  // 26.3), of sequences of 17 rows a key/value head and more 384 (4 x 8 after 4096, 192: 28.8, 25.6, 4 x 16: 30.8, 31.9; 4 x 16
-  // after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968: 164, 76), of more than 64 where kv8_attend's tiles of 128 would be a
-  // good part empty, which is what a prefix's are not (20 of 32 tokens and less: 16 x 40 after 8192, 1920: 175, 126; 8 x 40
-  // after 4096, 448: 61.8, 63.1; 16 x 24 after 4096, 960: 62.2, 65.5; 32 x 32 after 4096 107, 116).
+  // Shared where enough blocks need not be read again, counted as of 8 key/value heads where there are more, and
+  // where the estimates above are for it.  Enough: of prefixes past 16 blocks (up to there
+  // kv8_attend is one launch, 64 x 1 after 640 19.5, shared 24.8, which 100 MB make up for: 64 x 1 after 1024, 32 heads, 529
+  // MB, 98.9, 41.9; 16 x 1 after 512, 63 MB, 19.4, 22.4) so many (8 x 1 after 1088, 119: 17.2, 14.4; 4 after 2048, 96: 13.9,
+  // 15.4; 2 after 8192, 128: 18.3, 20.8, after 32768, 512: 33.0, 26.3); of sequences of 17 rows a key/value head and more 384
+  // (4 x 8 after 4096, 192: 28.8, 25.6, 4 x 16: 30.8, 31.9; 4 x 16 after 8192, 384: 38.9, 36.3; 32 x 9 after 8192, 3968: 164,
+  // 76); of more than 64 where kv8_attend's tiles of 128 would be a good part empty, which is what a prefix's are not (20 of
+  // 32 tokens and less: 16 x 40 after 8192, 1920: 175, 126; 8 x 40 after 4096, 448: 61.8, 63.1; 16 x 24 after 4096, 960: 62.2,
+  // 65.5; 32 x 32 after 4096 107, 116).
   const int64_t least = few ? (sh.seqs < 4 ? 384 : 112) : longest * h8 <= 64 ? 384 : 8ll * longest <= 5 * room ? 896 : INT64_MAX;
   const bool enough = blocks > 16 ? saved * std::max(kv_heads, 8) / 8 >= least
                                   : few && saved * kv_heads * head_dim >= 100000000 / 128;
@@ -2026,7 +2037,9 @@ SharedWay shared_way(int64_t rows, int longest, const Kv8Shared& sh, int heads, 
     const double a = units * 1.5 / 256, b = w.own.groups * (double)own / 4 * (head_dim * 128) / 5e6;
     pass_splits(w.pre, std::min(512., a / (a + b) * (units >= 16 * 512 ? 512 : 256) + w.pre.groups - 1), blocks, 2);
   }
-  w.pays = shared_us(w, rows, heads, head_dim, blocks) < alone_us(rows, longest, saved + blocks, heads, kv_heads, head_dim, cols, ntiles);
+  const bool many = longest * h8 > 64;
+  w.pays = shared_us(w, rows, heads, head_dim, blocks, many) <
+           alone_us(rows, longest, saved + blocks, heads, kv_heads, head_dim, cols, ntiles, many);
   if (!w.pays) return w;
   w.pre_each = sh.rows * heads * (head_dim + 2);
   w.own_each = rows * heads * (head_dim + 2);

@@ -62,6 +62,12 @@ def test_own_blocks_are_split_by_the_whole_table(L, n, heads, kv, hd, blocks, co
     (16, 1, 16, 1, 128, 512, 516, True),     # 40.4, 34.7
     (4, 1, 16, 4, 64, 512, 516, True),       # 26.7, 17.7
     (8, 1, 8, 1, 64, 32, 36, True),          # 13.7, 12.7
+    # more than 64 rows a head and sequence
+    (2, 9, 8, 1, 128, 2000, 2004, False),    # 47.9, 73.4
+    (2, 17, 16, 4, 64, 1000, 1004, False),   # 40.7, 52.3
+    (32, 160, 32, 32, 128, 17, 23, False),   # 236.8, 268.4
+    (16, 40, 32, 8, 128, 128, 132, True),    # 174, 125
+    (10, 40, 32, 8, 128, 100, 104, True),
 ])
 def test_the_faster_side_runs(L, n, longest, heads, kv, hd, blocks, cols, shared):
     got, alone = part(L, n, longest, heads, kv, hd, blocks, cols)
