@@ -119,3 +119,24 @@ def test_pages_past_4_gb(ctx, n, new, heads, blocks):
     m.append(kb, vb, new)
     want, tol = m.attend(q, new, 0.09, "fp16")
     assert off(got, want, tol) <= 1
+
+
+@pytest.mark.parametrize("n,heads,kv,hd,blocks", [(64, 32, 32, 128, 8), (96, 32, 32, 128, 3), (300, 16, 8, 128, 8)])
+def test_short_prefixes_of_many_sequences(ctx, n, heads, kv, hd, blocks):
+    """A few blocks, which many sequences of many heads read: shared all the same; one table has parted, one sequence is new."""
+    say("short prefixes", n, heads, kv, hd, blocks)
+
+    def part(m):
+        m.table[7, 1] = m.table[7, -1]
+        m.lens[9] = 0
+
+    rng = np.random.default_rng([75, n])
+    of, before = [0] * n, [64 * blocks + (11 * i) % 60 for i in range(n)]
+    m, d = alike(ctx, "bf16", kv, hd, of, [blocks], before, rng, cols=blocks + 2, spare=0)
+    part(m)
+    d.b["table"].upload(m.table)
+    d.b["lens"].upload(m.lens)
+    assert shares(ctx, of, [blocks], [1] * n, heads, kv, hd, m.cols)
+    r = step(ctx, m, d, of, [blocks], [1] * n, heads, "bf16", rng)
+    say("worst", r)
+    assert r <= 1
